@@ -13,7 +13,8 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libbgtq.so"
 
 OK, EINVAL, ECAPACITY, ENONFINITE, EBUSY, ELAYOUT, ETIMEOUT, ECUDA, ENOMEM = range(9)
-F16, F32 = 1, 2
+F16, F32, BF16 = 1, 2, 3
+PAGES_F16, PAGES_BF16, PAGES_INT8, PAGES_INT4 = 1, 2, 3, 4
 KEYS_PACKED, KEYS_FP16, KEYS_COMPRESSED = 1, 2, 3
 
 
@@ -61,6 +62,24 @@ class DecoderDesc(C.Structure):
         ("rms_eps", C.c_float)] + [(n, C.c_void_p) for n in (
             "inv_freq", "ln1", "qkv_bias", "ln2", "w_qkv", "w_o", "w_gate_up", "w_down", "final_norm", "lm_head",
             "embedding", "attention")] + [("ctas_per_sm", C.c_uint32)]
+
+
+class PagedCacheDesc(C.Structure):
+    """bgtq_paged_cache: pages of the caller's memory."""
+    _fields_ = [("device", C.c_int), ("format", C.c_int)] + [
+        (n, C.c_uint32) for n in ("kv_heads", "dim", "page_size", "pages")] + [
+        (n, C.c_void_p) for n in ("k", "v", "k_scales", "v_scales")]
+
+
+class PromptDesc(C.Structure):
+    """bgtq_prompt: a packed batch of prompts."""
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int)] + [
+        (n, C.c_uint32) for n in ("sequences", "q_heads", "kv_heads", "dim")] + [
+        (n, C.c_uint64) for n in ("q_tokens", "k_tokens")] + [(n, C.c_void_p) for n in ("q", "k", "v")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                 "v_token_stride", "v_head_stride")] + [
+        ("starts", C.c_void_p), ("key_starts", C.c_void_p), ("causal", C.c_int), ("scale", C.c_float),
+        ("out", C.c_void_p), ("lse", C.c_void_p)]
 
 
 # (name, restype, argtypes) for every exported symbol declared in include/bgtq.h
@@ -130,6 +149,11 @@ SIGNATURES = {
     "bgtq_keys_sync_lengths": (I32, [P]),
     "bgtq_values_sync_lengths": (I32, [P]),
     "bgtq_values_reset": (I32, [P, P]),
+    "bgtq_paged_write": (I32, [P, P, P, I32, U64, I64, I64, I64, I64, P, P]),
+    "bgtq_paged_read": (I32, [P, P, U64, P, P, I32, P]),
+    "bgtq_paged_attend_workspace": (I32, [P, U32, U32, P]),
+    "bgtq_paged_attend": (I32, [P, P, I32, U32, U32, I64, I64, P, I64, U32, P, C.c_float, P, P, P, SZ, P]),
+    "bgtq_prompt_attend": (I32, [P, P]),
 }
 
 _lib = None

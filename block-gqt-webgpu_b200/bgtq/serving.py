@@ -1,0 +1,215 @@
+"""Serving requests of different lengths: packed prompts and a paged, quantised K/V cache.
+
+    prompt_attention   a whole batch of prompts, packed one after the other, in one call
+    PagedCache         K and V of every request in the pages of one pool, in 16, 8 or 4 bits:
+                       ``write`` quantises new rows, ``read`` gives back what rows stand for,
+                       ``attend`` runs one new token of every request over its own pages
+
+No counterpart in the reference, whose stores hold one sequence each.  CUDA tensors in, CUDA
+tensors out, ordered on the current stream of the tensors' device; nothing synchronises.
+Indices that only the GPU sees (slots, page tables, lengths, starts) are checked there: what
+lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
+length or starts).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_DTYPE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+# format: (code, element type, elements of a row per dimension, dimensions per scale)
+_FORMATS = {"f16": (_lib.PAGES_F16, torch.float16), "bf16": (_lib.PAGES_BF16, torch.bfloat16),
+            "int8": (_lib.PAGES_INT8, torch.int8), "int4": (_lib.PAGES_INT4, torch.uint8)}
+
+
+def _refuse(message: str):
+    raise _lib.RangeError(_lib.EINVAL, message)
+
+
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class PagedCache:
+    """K and V rows of ``pages`` pages of ``page_size`` tokens for ``kv_heads`` heads.
+
+    format "f16" / "bf16" (rounded rows), "int8" (one BF16 scale a row) or "int4" (one BF16
+    scale for every 32 dimensions).  The memory is the tensors ``k``, ``v`` [pages, kv_heads,
+    page_size, row] and ``k_scales``, ``v_scales`` [pages, kv_heads, page_size, groups] (None
+    in 16 bits), allocated zeroed here or taken from ``storage`` (a dict of those four).  Which
+    page belongs to which request is the caller's business: rows are addressed by slots (page *
+    page_size + row), requests by rows of a page table."""
+
+    def __init__(self, kv_heads: int, dim: int, pages: int, page_size: int = 64, format: str = "int8",
+                 device: int = 0, storage: dict | None = None):
+        if format not in _FORMATS:
+            _refuse(f"Paged cache: format must be one of {sorted(_FORMATS)}")
+        if dim not in (64, 128):
+            _refuse("Paged cache: head dim must be 64 or 128")
+        if page_size not in (16, 32, 64, 128, 256):
+            _refuse("Paged cache: page size must be a power of two from 16 to 256")
+        if not 1 <= kv_heads <= 1024 or not 1 <= pages < 2**31:
+            _refuse("Paged cache: invalid head or page count")
+        code, dtype = _FORMATS[format]
+        groups = {"int8": 1, "int4": dim // 32}.get(format, 0)
+        want = dict(k=(dtype, dim // 2 if format == "int4" else dim), k_scales=(torch.bfloat16, groups))
+        want.update(v=want["k"], v_scales=want["k_scales"])
+        tensors = {}
+        for name, (dt, width) in want.items():
+            shape = (pages, kv_heads, page_size, width)
+            if not width:
+                t = None
+                if storage is not None and storage.get(name) is not None:
+                    _refuse(f"Paged cache: {format} pages have no {name}")
+            elif storage is None:
+                t = torch.zeros(shape, dtype=dt, device=torch.device("cuda", device))
+            else:
+                t = storage.get(name)
+                if t is None or not t.is_cuda or t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous():
+                    _refuse(f"Paged cache: {name} must be a contiguous CUDA tensor {list(shape)} of {dt}")
+            tensors[name] = t
+        self.k, self.v, self.k_scales, self.v_scales = (tensors[n] for n in ("k", "v", "k_scales", "v_scales"))
+        if any(t is not None and t.device != self.k.device for t in tensors.values()):
+            _refuse("Paged cache: all storage must be on one device")
+        self.kv_heads, self.dim, self.pages, self.page_size = int(kv_heads), int(dim), int(pages), int(page_size)
+        self.format, self.device = format, self.k.device.index
+        self._desc = _lib.PagedCacheDesc(self.device, code, kv_heads, dim, page_size, pages, self.k.data_ptr(),
+                                         self.v.data_ptr(), *(None if t is None else t.data_ptr()
+                                                              for t in (self.k_scales, self.v_scales)))
+        self._ref = C.byref(self._desc)
+        self._workspace = {}
+
+    def _slots(self, slots):
+        if (not slots.is_cuda or slots.device.index != self.device or slots.dtype != torch.int64 or slots.dim() != 1
+                or not slots.is_contiguous()):
+            _refuse("Paged cache: slots must be a contiguous one-dimensional int64 tensor on the cache's device")
+        return slots
+
+    def write(self, k, v, slots) -> None:
+        """Store rows k, v [tokens, kv_heads, dim] (float16, bfloat16 or float32; any strides with
+        a contiguous last dimension) at ``slots`` [tokens].  Negative slots are padding."""
+        slots = self._slots(slots)
+        shape = (slots.shape[0], self.kv_heads, self.dim)
+        if tuple(k.shape) != shape or tuple(v.shape) != shape:
+            _refuse("Paged write: K and V must be [tokens, kv_heads, dim] with one slot a token")
+        if k.dtype != v.dtype or k.dtype not in _DTYPE:
+            _refuse("Paged write: K and V must both be float16, bfloat16 or float32")
+        if not k.is_cuda or k.device != slots.device or v.device != slots.device:
+            _refuse("Paged write: K and V must be on the cache's device")
+        if k.stride(2) != 1 or v.stride(2) != 1:
+            _refuse("Paged write: the last dimension must be contiguous")
+        _lib.call("bgtq_paged_write", self._ref, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], shape[0], k.stride(0),
+                  k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), _stream(self.device))
+
+    def read(self, slots, dtype=None):
+        """(k, v) [tokens, kv_heads, dim]: the values that the rows at ``slots`` stand for, as
+        dtype (default: the pages' own type, bfloat16 for 8- and 4-bit pages); zeros for
+        negative slots."""
+        slots = self._slots(slots)
+        if dtype is None:
+            dtype = torch.float16 if self.format == "f16" else torch.bfloat16
+        if dtype not in _DTYPE:
+            _refuse("Paged read: dtype must be float16, bfloat16 or float32")
+        k = torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=dtype, device=slots.device)
+        v = torch.empty_like(k)
+        _lib.call("bgtq_paged_read", self._ref, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(),
+                  _DTYPE[dtype], _stream(self.device))
+        return k, v
+
+    def attend(self, q, table, lengths, scale: float | None = None, out=None, lse: bool = False):
+        """One new token of every request: q [batch, q_heads, dim] (float16 or bfloat16, the
+        pages' type over 16-bit pages) over the first ``lengths`` [batch] (int32) tokens of the
+        pages in ``table`` [batch, width] (int32).  Returns out [batch, q_heads, dim], with
+        ``lse`` also the log sums [batch, q_heads] (float32).  scale: 1 / sqrt(dim) if None."""
+        if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+            _refuse("Paged attention: Q must be [batch, q_heads, dim], q_heads a multiple of kv_heads")
+        batch, heads = q.shape[0], q.shape[1]
+        if q.dtype not in (torch.float16, torch.bfloat16) or self.format in ("f16", "bf16") and q.dtype != self.k.dtype:
+            _refuse("Paged attention: Q must be float16 or bfloat16, and of the type of 16-bit pages")
+        if not q.is_cuda or q.device.index != self.device or q.stride(2) != 1:
+            _refuse("Paged attention: Q must be on the cache's device with a contiguous last dimension")
+        if (table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32 or table.device != q.device
+                or (table.shape[1] > 1 and table.stride(1) != 1)):
+            _refuse("Paged attention: the table must be int32 [batch, width] on the cache's device")
+        if (lengths.dim() != 1 or lengths.shape[0] != batch or lengths.dtype != torch.int32
+                or lengths.device != q.device or (batch > 1 and lengths.stride(0) != 1)):
+            _refuse("Paged attention: lengths must be int32 [batch] on the cache's device")
+        if scale is not None and not 0.0 < scale < float("inf"):
+            _refuse("Paged attention: scale must be positive and finite")
+        if out is None:
+            out = torch.empty((batch, heads, self.dim), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            _refuse("Paged attention: out must be contiguous, of Q's shape, type and device")
+        sums = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if lse else None
+        st = _stream(self.device)
+        work = self._work(batch, heads, st)
+        _lib.call("bgtq_paged_attend", self._ref, q.data_ptr(), _DTYPE[q.dtype], batch, heads, q.stride(0), q.stride(1),
+                  table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+                  0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr(),
+                  None if work is None else work.data_ptr(), 0 if work is None else work.numel(), st)
+        return (out, sums) if lse else out
+
+    def _work(self, batch: int, heads: int, stream: int):
+        """The stream's own workspace (calls on different streams may overlap), grown on demand."""
+        need = C.c_size_t()
+        _lib.call("bgtq_paged_attend_workspace", self._ref, batch, heads, C.byref(need))
+        if not need.value:
+            return None
+        have = self._workspace.get(stream)
+        if have is None or have.numel() < need.value:
+            have = torch.zeros(need.value, dtype=torch.uint8, device=self.k.device)
+            self._workspace[stream] = have
+        return have
+
+
+def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scale: float | None = None, out=None,
+                     lse: bool = False):
+    """Attention of a packed batch of prompts: q [tokens, q_heads, dim], k and v [key tokens,
+    kv_heads, dim] (float16 or bfloat16, one type; q_heads a multiple of kv_heads).  Sequence s
+    is query rows starts[s] .. starts[s + 1] and key rows key_starts[s] .. key_starts[s + 1]
+    (int32 [sequences + 1]; key_starts None: the same as starts).  Causal rows see their
+    sequence's keys up to their own, counted from the end, so a chunk whose prefix is cached
+    passes more keys than queries.  Rows that see nothing are zeros.  Any strides with a
+    contiguous last dimension; a tensor whose strides or address are not multiples of 16
+    bytes is copied.  Returns out [tokens, q_heads, dim], with ``lse`` also the log sums
+    [tokens, q_heads] (float32)."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        _refuse("Prompt attention: Q must be [tokens, q_heads, dim], K and V [key tokens, kv_heads, dim]")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        _refuse("Prompt attention: Q, K and V must all be float16 or all bfloat16")
+    if not q.is_cuda or k.device != q.device or v.device != q.device:
+        _refuse("Prompt attention: Q, K and V must be CUDA tensors on one device")
+    if q.shape[2] not in (64, 128) or k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        _refuse("Prompt attention: head dim must be 64 or 128 and q_heads a multiple of kv_heads")
+    for s in (starts, key_starts):
+        if s is not None and (s.dim() != 1 or s.shape[0] != starts.shape[0] or s.shape[0] < 1 or s.dtype != torch.int32
+                              or s.device != q.device or not s.is_contiguous()):
+            _refuse("Prompt attention: starts must be int32 [sequences + 1] on Q's device")
+    if key_starts is None and k.shape[0] != q.shape[0]:
+        _refuse("Prompt attention: key_starts are needed when K has other tokens than Q")
+    if scale is not None and not 0.0 < scale < float("inf"):
+        _refuse("Prompt attention: scale must be positive and finite")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        _refuse("Prompt attention: out must be contiguous, of Q's shape, type and device")
+    sums = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if lse else None
+
+    def even(t):
+        # a stride of a dimension of one element is never used
+        steps = [t.stride(i) for i in (0, 1) if t.shape[i] > 1]
+        if t.stride(2) != 1 or any(s % 8 or s == 0 for s in steps) or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.stride(0) if t.shape[0] > 1 else 8, t.stride(1) if t.shape[1] > 1 else 8
+
+    (q, *sq), (k, *sk), (v, *sv) = even(q), even(k), even(v)
+    dev = q.device.index
+    p = _lib.PromptDesc(dev, _DTYPE[q.dtype], starts.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], q.shape[0],
+                        k.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), *sq, *sk, *sv, starts.data_ptr(),
+                        None if key_starts is None else key_starts.data_ptr(), int(bool(causal)),
+                        0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr())
+    _lib.call("bgtq_prompt_attend", C.byref(p), _stream(dev))
+    return (out, sums) if lse else out

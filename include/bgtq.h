@@ -57,7 +57,7 @@ enum {
     BGTQ_ENOMEM = 8       /* device or host allocation failed */
 };
 
-typedef enum { BGTQ_F16 = 1, BGTQ_F32 = 2 } bgtq_dtype;
+typedef enum { BGTQ_F16 = 1, BGTQ_F32 = 2, BGTQ_BF16 = 3 /* serving operators only */ } bgtq_dtype;
 typedef enum { BGTQ_KEYS_PACKED = 1, BGTQ_KEYS_FP16 = 2, BGTQ_KEYS_COMPRESSED = 3 } bgtq_keys_kind;
 
 typedef struct bgtq_tables bgtq_tables;
@@ -448,6 +448,93 @@ bgtq_status bgtq_decoder_trace(bgtq_decoder *dec, int on, uint64_t *out, uint32_
  * tables the append CTAs stage in shared memory (0: read from global memory).  Nullable. */
 bgtq_status bgtq_decoder_info(const bgtq_decoder *dec, uint32_t *ctas, uint32_t *smem_bytes, uint32_t *table_bytes);
 void bgtq_decoder_destroy(bgtq_decoder *dec);
+
+/* ---- serving operators ------------------------------------------------------------- */
+
+/* Requests of different lengths (no counterpart in the reference, whose stores hold one
+ * sequence): prompts are attended as one packed batch, keys and values live in the pages of
+ * a shared cache, in 16, 8 or 4 bits, and every new token attends over its request's own
+ * pages.  All pointers are device memory, all work is stream-ordered, nothing is allocated;
+ * head dims are 64 and 128.
+ *
+ * A cache is memory of the caller's, described by this struct.  Token row t of page p of KV
+ * head h is row (p * kv_heads + h) * page_size + t of `k` and of `v`:
+ *   BGTQ_PAGES_F16 / BF16  dim elements
+ *   BGTQ_PAGES_INT8        dim signed codes; one scale a row
+ *   BGTQ_PAGES_INT4        dim / 2 bytes, even dimension in the low nibble, code + 8; one
+ *                          scale for every 32 dimensions
+ * Scales are BF16, at the same row index (times dim / 32 in 4 bits); a stored value is
+ * code * scale.  `k` and `v` are 16-byte aligned, the scales 8-byte. */
+typedef enum { BGTQ_PAGES_F16 = 1, BGTQ_PAGES_BF16 = 2, BGTQ_PAGES_INT8 = 3, BGTQ_PAGES_INT4 = 4 } bgtq_page_format;
+typedef struct bgtq_paged_cache {
+    int device;
+    bgtq_page_format format;
+    uint32_t kv_heads, dim;
+    uint32_t page_size;  /* tokens a page: a power of two, 16 to 256 */
+    uint32_t pages;
+    void *k, *v;
+    uint16_t *k_scales, *v_scales; /* null for the 16-bit formats */
+} bgtq_paged_cache;
+
+/* Quantise and store `tokens` rows of every KV head.  Source element (t, h, i) is at
+ * k[t * k_token_stride + h * k_head_stride + i] (elements of dtype F16, BF16 or F32), v the
+ * same.  slots[t] = page * page_size + row; a negative slot is padding and is not stored.
+ * Slots of one call are distinct.  A slot past the last page is not stored and sets a bit of
+ * the device status word.  A scale is max|x| / 127 (8 bits) or / 7 (4 bits) rounded to BF16,
+ * a code is x / scale rounded to the nearest, ties to even; rows (groups) with an infinity
+ * or a NaN in them read back as NaN. */
+bgtq_status bgtq_paged_write(const bgtq_paged_cache *c, const void *k, const void *v, bgtq_dtype dtype,
+                             uint64_t tokens, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                             int64_t v_head_stride, const int64_t *slots, void *stream);
+/* Read rows back as the values that they stand for: k_out, v_out dense [tokens][kv_heads][dim]
+ * of dtype (F16, BF16, F32).  Negative slots, and slots past the last page (which also set
+ * the status bit), give zeros. */
+bgtq_status bgtq_paged_read(const bgtq_paged_cache *c, const int64_t *slots, uint64_t tokens, void *k_out,
+                            void *v_out, bgtq_dtype dtype, void *stream);
+/* Bytes of workspace that bgtq_paged_attend needs for these sizes (a multiple of 16). */
+bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t batch, uint32_t q_heads, size_t *bytes);
+/* One new token per request: out[b][h] = sum over t < lengths[b] of softmax(scale q.k_t) v_t.
+ *   q        element (b, h, i) at q[b * q_batch_stride + h * q_head_stride + i], dtype F16 or
+ *            BF16; over 16-bit pages the pages' own type.  Query head h uses KV head
+ *            h / (q_heads / kv_heads)
+ *   table    [batch] rows of table_width page indices, table_stride apart; entries past a
+ *            request's length are not read
+ *   lengths  [batch] int32 tokens; 0 gives zeros.  A length past table_width pages is cut
+ *            there and sets a status bit; tokens of a page index past the last page are left
+ *            out and set one
+ *   scale    of the logits, positive (0: 1 / sqrt(dim))
+ *   out      dense [batch][q_heads][dim] of dtype; lse [batch][q_heads] FP32 natural log of
+ *            the sum of exponentials (-inf for length 0), or null
+ *   workspace  zero-filled before its first use; every call leaves it ready for the next.
+ *            Calls that may overlap on the GPU need workspaces of their own. */
+bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dtype dtype, uint32_t batch,
+                              uint32_t q_heads, int64_t q_batch_stride, int64_t q_head_stride, const int32_t *table,
+                              int64_t table_stride, uint32_t table_width, const int32_t *lengths, float scale,
+                              void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Packed prompts: queries q_tokens x q_heads x dim, keys and values k_tokens x kv_heads x
+ * dim, all of dtype (F16 or BF16), element (t, h, i) at t * token_stride + h * head_stride
+ * + i.  Sequence s holds query rows starts[s] .. starts[s + 1] and key rows key_starts[s] ..
+ * key_starts[s + 1] (device int32, ascending; null: the same as starts).  Causal: row i of a
+ * sequence sees its keys j <= i + (keys - queries), so prompts whose earlier tokens are
+ * cached pass more keys than queries.  Rows that see nothing give zeros and -inf; query rows
+ * that no sequence holds are not written.  Starts that fall or pass the token counts set a
+ * status bit and their sequence is skipped.
+ * Pointers are 16-byte aligned, strides positive multiples of 8 elements; q_heads / kv_heads <= 128. */
+typedef struct bgtq_prompt {
+    int device;
+    bgtq_dtype dtype;
+    uint32_t sequences, q_heads, kv_heads, dim;
+    uint64_t q_tokens, k_tokens;
+    const void *q, *k, *v;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int32_t *starts, *key_starts;
+    int causal;
+    float scale;  /* of the logits, positive (0: 1 / sqrt(dim)) */
+    void *out;    /* dense [q_tokens][q_heads][dim] of dtype */
+    float *lse;   /* [q_tokens][q_heads] FP32, or null */
+} bgtq_prompt;
+bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream);
 
 /* Device status word written by kernels (0 = fine); reading it synchronises. */
 bgtq_status bgtq_device_status(int device, uint32_t *status_out);
