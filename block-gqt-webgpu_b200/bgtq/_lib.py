@@ -151,7 +151,7 @@ SIGNATURES = {
     "bgtq_values_reset": (I32, [P, P]),
     "bgtq_paged_write": (I32, [P, P, P, I32, U64, I64, I64, I64, I64, P, P]),
     "bgtq_paged_read": (I32, [P, P, U64, P, P, I32, P]),
-    "bgtq_paged_attend_workspace": (I32, [P, U32, U32, P]),
+    "bgtq_paged_attend_workspace": (I32, [P, U32, P]),
     "bgtq_paged_attend": (I32, [P, P, I32, U32, U32, I64, I64, P, I64, U32, P, C.c_float, P, P, P, SZ, P]),
     "bgtq_prompt_attend": (I32, [P, P]),
 }

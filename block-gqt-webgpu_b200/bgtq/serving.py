@@ -145,23 +145,21 @@ class PagedCache:
             _refuse("Paged attention: out must be contiguous, of Q's shape, type and device")
         sums = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if lse else None
         st = _stream(self.device)
-        work = self._work(batch, heads, st)
+        work = self._work(heads, st)
         _lib.call("bgtq_paged_attend", self._ref, q.data_ptr(), _DTYPE[q.dtype], batch, heads, q.stride(0), q.stride(1),
                   table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
                   0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr(),
-                  None if work is None else work.data_ptr(), 0 if work is None else work.numel(), st)
+                  work.data_ptr(), work.numel(), st)
         return (out, sums) if lse else out
 
-    def _work(self, batch: int, heads: int, stream: int):
-        """The stream's own workspace (calls on different streams may overlap), grown on demand."""
-        need = C.c_size_t()
-        _lib.call("bgtq_paged_attend_workspace", self._ref, batch, heads, C.byref(need))
-        if not need.value:
-            return None
-        have = self._workspace.get(stream)
-        if have is None or have.numel() < need.value:
+    def _work(self, heads: int, stream: int):
+        """The stream's own workspace (calls on different streams may overlap)."""
+        have = self._workspace.get((stream, heads))
+        if have is None:
+            need = C.c_size_t()
+            _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
             have = torch.zeros(need.value, dtype=torch.uint8, device=self.k.device)
-            self._workspace[stream] = have
+            self._workspace[stream, heads] = have
         return have
 
 

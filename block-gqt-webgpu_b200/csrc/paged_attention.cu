@@ -1,7 +1,32 @@
 // Attention of one new token per request over the pages of a cache:
-//     out = sum_t softmax_t(scale q.k_t) v_t  over the request's first `length` tokens,
-// with a running maximum and sum (FP32).  A request of length 0 gives zeros and a log sum of
-// minus infinity.
+//     out = sum_t softmax_t(scale q.k_t) v_t  over the request's first `length` tokens.
+//
+// What bounds it is the one pass over K and V: 2 row_bytes a token and KV head, against 2 D
+// multiply-adds for each query head, so the work is laid out for the memory system.
+//   * The (request, KV head, block of query heads) pairs are cut into units of kTokens tokens,
+//     and the units, in order, are dealt to the CTAs in equal ranges, whatever the lengths
+//     are: a range covers the end of one pair, whole pairs, and the start of another.  The
+//     deal is computed on the device from the lengths, so a recorded launch stays balanced
+//     while the requests grow.  A pair that lies in one range is written at once; parts of a
+//     pair go to the workspace and the CTA that finishes last joins them, in order.
+//   * A warp takes every fourth unit of its CTA's range, through a ring of its own in shared
+//     memory filled by cp.async (rows past the length arrive as zeros), which runs ahead
+//     across pair boundaries.  Nothing but the join of four warps at the end of a pair
+//     synchronises the CTA.
+//   * Products run on the tensor cores with the tokens as the long side: S^T = K Q^T (16
+//     tokens x 8 heads), O^T = V^T P^T (16 dimensions x 8 heads), so the 8 columns hold the
+//     query heads of a KV head and no row is padding.  8- and 4-bit codes become FP16
+//     integers in registers (exactly); the dimensions and tokens inside a product are taken
+//     in the order in which the loaded words hold them.
+//   * Softmax statistics and outputs are FP32.  The probabilities are rounded to 16 bits for
+//     the second product: FP16 (times 2^12, which keeps 2^-26 of the largest normal) or, over
+//     BF16 pages, BF16.
+//   * 8-bit pages: a key's scale multiplies its logit, a value's scale its probability before
+//     the rounding.  4-bit pages: the logit is the sum of scale x partial product over groups
+//     of 32 dimensions; the values are multiplied in registers (code x scale has 11 bits, so
+//     FP16 holds it exactly).  Value scales are taken relative to a running power of two of
+//     the largest seen, and queries to one of their row's largest, so that FP16's exponent
+//     range holds any BF16 scale or query that matters beside the largest.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -11,85 +36,734 @@ namespace bgtq {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
+enum { F_F16, F_BF16, F_INT8, F_INT4 };
+constexpr int kLeastExp = -100;  // value scales below 2^-100 count as that in the running power of two
 
-template <int D>
-__device__ __forceinline__ void load_row(const unsigned char *p, const uint16_t *sc, bgtq_page_format f, uint32_t lane,
-                                         float (&x)[D / 32]) {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const uint32_t d = 32 * i + lane;
-        switch (f) {
-            case BGTQ_PAGES_F16: x[i] = __half2float(reinterpret_cast<const __half *>(p)[d]); break;
-            case BGTQ_PAGES_BF16: x[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[d]); break;
-            case BGTQ_PAGES_INT8:
-                x[i] = (float)(signed char)p[d] * __bfloat162float(__ushort_as_bfloat16(sc[0]));
-                break;
-            default:
-                x[i] = (float)((int)(p[d / 2] >> (4 * (d & 1u)) & 15u) - 8) *
-                       __bfloat162float(__ushort_as_bfloat16(sc[i]));
-        }
+template <int F, int D, int NT>
+struct Shape {
+    static constexpr int kRow = F == F_INT4 ? D / 2 : F == F_INT8 ? D : 2 * D;  // bytes
+    static constexpr int kGroups = F == F_INT4 ? D / 32 : F == F_INT8 ? 1 : 0;
+    static constexpr int kTokens = kRow >= 256 ? 16 : kRow >= 128 ? 32 : 64;  // of a unit: 8 KB, or 4 KB
+    static constexpr int kStages = kRow >= 64 ? 3 : 4;
+    static constexpr int kPart = kTokens * kRow;                 // K or V rows of a unit
+    static constexpr int kScale = kTokens * kGroups * 2;         // K or V scales of a unit
+    static constexpr int kStage = 2 * (kPart + kScale);
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kHeads = 8 * NT;
+    static constexpr int kJoin = kHeads * (D + 2) * 4;           // one warp's part: O, m, l
+    static constexpr int kSmem = kWarps * (kRing + kJoin) + 128;
+};
+
+// 16-byte chunk `c` of row r in a ring slot.  Rows share 128-byte lines; the chunks of a line
+// are permuted so that ldmatrix (8 rows, one chunk), the key loads (8 rows x 4 threads) and
+// the value loads (4 rows two apart x 8 threads) all spread over the 32 banks.
+template <int R>
+__device__ __forceinline__ uint32_t place(uint32_t r, uint32_t c) {
+    if constexpr (R >= 128) {
+        const uint32_t x = ((r ^ (r >> 1)) & 1u) << 2 | (r >> 2 & 1u) << 1 | (r >> 1 & 1u);
+        return r * R + ((c ^ x) << 4);
+    } else {
+        constexpr uint32_t per = 128 / R, chunks = R / 16;
+        const uint32_t line = r / per, u = (r % per) * chunks + c;
+        const uint32_t x = R == 64 ? ((line & 3u) ^ (line & 3u) << 1) : (line & 1u) * 3u;
+        return line * 128 + ((u ^ (x & 7u)) << 4);
     }
 }
 
-// One warp per (request, query head), its lanes over the head's dimensions.
-template <int D>
-__global__ void __launch_bounds__(32) attend_kernel(const PagedAttendArgs a) {
-    constexpr int N = D / 32;
-    const uint32_t h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x, kh = h / a.group;
-    int32_t len = a.lengths[b];
-    if (len < 0 || (uint64_t)len > (uint64_t)a.width << a.c.page_shift) {
-        if (lane == 0) atomicOr(a.status, kStatusBadExtent);
-        len = len < 0 ? 0 : (int32_t)(a.width << a.c.page_shift);
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ uint32_t turn(uint32_t x) {  // an 8 x 8 matrix of 16-bit values, transposed
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <bool BF>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
     }
-    float q[N], o[N] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int64_t at = (int64_t)b * a.q_batch + (int64_t)h * a.q_head + 32 * i + lane;
-        q[i] = a.dtype == BGTQ_F16 ? __half2float(static_cast<const __half *>(a.q)[at])
-                                   : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at]);
-    }
-    for (int32_t t = 0; t < len; ++t) {
-        const int32_t page = a.table[(int64_t)b * a.table_stride + (t >> a.c.page_shift)];
-        if ((uint32_t)page >= a.c.pages) {
-            if (lane == 0) atomicOr(a.status, kStatusBadSlot);
-            continue;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float from_bf16(uint32_t bits) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// Bytes as FP16: 1024 + byte is 0x6400 | byte.  Signed codes come in with their sign bit
+// flipped, so 1024 + 128 goes off again.
+__device__ __forceinline__ uint32_t bytes_to_half(uint32_t w, uint32_t sel) {
+    return sub2(__byte_perm(w, 0x64646464u, sel), 0x64806480u);
+}
+// Nibbles 0 of both halves (1024 + code + 8), and nibbles 1 of both halves (64 + code + 8).
+__device__ __forceinline__ uint32_t nibble0(uint32_t w) { return sub2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
+__device__ __forceinline__ uint32_t nibble1(uint32_t w) { return sub2((w & 0x00f000f0u) | 0x54005400u, 0x54805480u); }
+
+// Where a warp's next unit is: request b, pair p of it, units [at, end) of the pair left in this
+// segment; `u` is the flat index of the segment's first unit.
+struct Cursor {
+    uint32_t b, pair, units, at, end;
+    int32_t len;
+    uint64_t u;
+};
+
+template <int F, int D, int NT>
+__global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs a) {
+    using S = Shape<F, D, NT>;
+    constexpr bool BF = F == F_BF16;
+    constexpr int T = S::kTokens, C16 = T / 16, KS = D / 16;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row4 = lane >> 2, col4 = lane & 3u;
+    unsigned char *ring = smem + warp * S::kRing;
+    const uint32_t ring_at = smem_addr(ring);
+    float *join = reinterpret_cast<float *>(smem + kWarps * S::kRing);
+    uint32_t *flags = reinterpret_cast<uint32_t *>(smem + kWarps * (S::kRing + S::kJoin));
+    const uint32_t blocks = (a.group + S::kHeads - 1) / S::kHeads, pairs = a.c.heads * blocks;
+    const uint32_t shift = a.c.page_shift, H = a.c.heads;
+
+    auto length = [&](uint32_t b) -> int32_t {
+        const int32_t n = __ldg(a.lengths + b);
+        return n < 0 ? 0 : (int32_t)min((uint32_t)n, a.width << shift);
+    };
+    // ---- the deal: all units, this CTA's range of them ----
+    uint64_t total = 0;
+    {
+        uint32_t *sums = reinterpret_cast<uint32_t *>(join);
+        uint64_t mine = 0;
+        for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
+            const int32_t n = length(b);
+            if (n != __ldg(a.lengths + b) && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
+            mine += (uint32_t)(n + T - 1) / T;
         }
-        const uint64_t r = ((uint64_t)page * a.c.heads + kh) * a.c.page_size + (t & (a.c.page_size - 1));
-        float k[N], v[N], s = 0.0f;
-        load_row<D>(a.c.k + r * a.c.row_bytes, a.c.ks + r * a.c.groups, a.c.format, lane, k);
-        load_row<D>(a.c.v + r * a.c.row_bytes, a.c.vs + r * a.c.groups, a.c.format, lane, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(q[i], k[i], s);
+        for (int w = 16; w; w >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
+        uint64_t *part = reinterpret_cast<uint64_t *>(sums);
+        if (lane == 0) part[warp] = mine;
+        __syncthreads();
 #pragma unroll
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.scale;
-        const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-        const float old = exp2f(m - ref), p = exp2f(s - ref);
-        m = mn;
-        l = fmaf(l, old, p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(p, v[i], o[i] * old);
+        for (uint32_t w = 0; w < kWarps; ++w) total += part[w];
+        __syncthreads();
+        total *= pairs;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const uint64_t row = (uint64_t)b * a.q_heads + h;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint64_t at = row * D + 32 * i + lane;
-        if (a.dtype == BGTQ_F16) static_cast<__half *>(a.out)[at] = __float2half_rn(o[i] * inv);
-        else static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(o[i] * inv);
+    // a request without tokens: zeros
+    for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        if (length(b) != 0) continue;
+        uint16_t *o = static_cast<uint16_t *>(a.out) + (uint64_t)b * a.q_heads * D;
+        for (uint32_t i = threadIdx.x; i < a.q_heads * D; i += kThreads) o[i] = 0;
+        if (a.lse)
+            for (uint32_t i = threadIdx.x; i < a.q_heads; i += kThreads) a.lse[(uint64_t)b * a.q_heads + i] = -INFINITY;
     }
-    if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    const uint64_t most = (total + kWarps - 1) / kWarps;
+    const uint64_t ctas = most < gridDim.x ? most : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    const uint64_t first = (uint64_t)blockIdx.x * total / ctas, last = (uint64_t)(blockIdx.x + 1) * total / ctas;
+    Cursor cur;
+    {
+        uint64_t base = 0;
+        cur.b = 0;
+        for (uint32_t b0 = 0;; b0 += 32) {  // ends: first < total
+            const uint32_t n = b0 + lane < a.batch ? (uint32_t)(length(b0 + lane) + T - 1) / T : 0u;
+            uint64_t sum = (uint64_t)n * pairs;
+#pragma unroll
+            for (int w = 1; w < 32; w <<= 1) {
+                const uint64_t o = __shfl_up_sync(0xffffffffu, sum, w);
+                if (lane >= (uint32_t)w) sum += o;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, base + sum > first);
+            if (past || b0 + 32 >= a.batch) {
+                const uint32_t l = past ? __ffs(past) - 1 : 31u;
+                base += __shfl_sync(0xffffffffu, sum, l) - (uint64_t)__shfl_sync(0xffffffffu, n, l) * pairs;
+                cur.b = b0 + l;
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        cur.len = length(cur.b);
+        cur.units = (uint32_t)(cur.len + T - 1) / T;
+        cur.pair = (uint32_t)((first - base) / cur.units);
+        cur.at = (uint32_t)((first - base) % cur.units);
+        cur.u = first;
+        cur.end = (uint32_t)min((uint64_t)cur.units, cur.at + (last - first));
+    }
+    // the segment after this one; false past the range's end
+    auto next_segment = [&](Cursor &c, uint32_t start) {
+        c.u += c.end - start;
+        if (c.u >= last) return false;
+        if (++c.pair == pairs) {
+            c.pair = 0;
+            do {
+                if (++c.b >= a.batch) return false;
+                c.len = length(c.b);
+            } while (c.len == 0);
+            c.units = (uint32_t)(c.len + T - 1) / T;
+        }
+        c.at = 0;
+        c.end = (uint32_t)min((uint64_t)c.units, last - c.u);
+        return true;
+    };
+
+    // ---- filling the ring ----
+    Cursor pre = cur;
+    uint32_t pre_start = pre.at;
+    bool more = true;
+    pre.at += warp;
+    int32_t page_reg = -1;
+    auto settle = [&]() {  // moves `pre` to the warp's next unit, if there is one, and loads its page indices
+        while (more && pre.at >= pre.end) {
+            more = next_segment(pre, pre_start);
+            pre_start = 0;
+            if (more) pre.at = warp;
+        }
+        if (more) {
+            const uint32_t t = pre.at * T + (lane << shift);
+            page_reg = t < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T)
+                           ? __ldg(a.table + (int64_t)pre.b * a.table_stride + (t >> shift)) : -1;
+        }
+    };
+    settle();
+    auto fill = [&](uint32_t stage) {
+        if (more) {
+            const uint32_t t0 = pre.at * T, kh = pre.pair / blocks;
+            const int32_t page = page_reg;
+            const bool wrong = (uint32_t)page >= a.c.pages;
+            const bool asked = t0 + (lane << shift) < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T);
+            const uint32_t bad = __ballot_sync(0xffffffffu, wrong && asked);
+            if (bad && lane == 0) atomicOr(a.status, kStatusBadSlot);
+            if (lane == 0) flags[warp * 4 + stage] = bad;
+            const uint32_t dst = ring_at + stage * S::kStage;
+            constexpr uint32_t CH = S::kRow / 16;
+#pragma unroll
+            for (uint32_t i = 0; i < T * CH / 32; ++i) {
+                const uint32_t idx = i * 32 + lane, r = idx / CH, c = idx % CH;
+                const uint32_t pi = r >> shift;
+                const int32_t pg = __shfl_sync(0xffffffffu, page, pi);
+                const bool ok = t0 + r < (uint32_t)pre.len && !(bad >> pi & 1u);
+                const uint64_t at = ((uint64_t)(ok ? (uint32_t)pg : 0u) * H + kh << shift) + ((t0 + r) & ((1u << shift) - 1));
+                const uint64_t off = ok ? at * S::kRow + c * 16 : 0;
+                const uint32_t to = place<S::kRow>(r, c);
+                copy16(dst + to, a.c.k + off, ok ? 16u : 0u);
+                copy16(dst + S::kPart + to, a.c.v + off, ok ? 16u : 0u);
+            }
+            if constexpr (S::kGroups != 0) {
+                constexpr uint32_t N = S::kScale / 16, PER = 8 / S::kGroups;  // 16-byte chunks, tokens in one
+#pragma unroll
+                for (uint32_t i = 0; i < (N + 31) / 32; ++i) {
+                    const uint32_t idx = i * 32 + lane, r = idx * PER, pi = min(r >> shift, 31u);
+                    const int32_t pg = __shfl_sync(0xffffffffu, page, pi);
+                    const int32_t left = pre.len - (int32_t)(t0 + r);
+                    const bool ok = left > 0 && !(bad >> pi & 1u);
+                    const uint64_t at = ((uint64_t)(ok ? (uint32_t)pg : 0u) * H + kh << shift) + ((t0 + r) & ((1u << shift) - 1));
+                    const uint64_t off = ok ? at * S::kGroups : 0;
+                    const uint32_t bytes = ok ? min(16u, (uint32_t)left * S::kGroups * 2u) : 0u;
+                    if (N % 32 == 0 || idx < N) {
+                        copy16(dst + 2 * S::kPart + idx * 16, a.c.ks + off, bytes);
+                        copy16(dst + 2 * S::kPart + S::kScale + idx * 16, a.c.vs + off, bytes);
+                    }
+                }
+            }
+            pre.at += kWarps;
+            settle();
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (uint32_t s = 0; s < (uint32_t)S::kStages - 1; ++s) fill(s);
+
+    uint32_t stage = 0;
+    for (;;) {
+        // ---- a segment: units [cur.at, cur.end) of one pair ----
+        const uint32_t start = cur.at, kh = cur.pair / blocks, block = cur.pair % blocks;
+        const uint32_t head0 = kh * a.group + block * S::kHeads;
+        const uint32_t heads = min((uint32_t)S::kHeads, a.group - block * S::kHeads);
+        uint32_t q[KS][NT][2];
+        float qs[NT][2];  // what a logit of this thread's heads is multiplied by
+        {
+            float x[NT][KS][4];
+            float big[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t h = n * 8 + row4;
+                const int64_t at = (int64_t)cur.b * a.q_batch + (int64_t)(head0 + h) * a.q_head;
+                big[n] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        int d;  // the dimension in slot (s, e) of this thread, in the order of the key words
+                        if constexpr (F == F_INT8) d = 64 * (s / 4) + 16 * col4 + 4 * (s % 4) + e;
+                        else if constexpr (F == F_INT4)
+                            d = 32 * (s / 2) + 8 * col4 + 2 * (s % 2) + (e & 1) * 4 + (e >> 1);
+                        else d = 16 * s + 2 * col4 + (e & 1) + 8 * (e >> 1);
+                        float v = 0.0f;
+                        if (h < heads)
+                            v = a.dtype == BGTQ_F16
+                                    ? __half2float(static_cast<const __half *>(a.q)[at + d])
+                                    : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at + d]);
+                        x[n][s][e] = v;
+                        big[n] = fmaxf(big[n], fabsf(v));
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f = 1.0f;
+                if constexpr (F >= F_INT8) {
+                    // the row's largest value to [2^13, 2^14): what FP16 then drops is 2^-38 of it
+                    float m = big[n];
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const int e = (int)(__float_as_uint(m) >> 23) - 127;  // m = 0, tiny: -127; inf, NaN: 128
+                    const int up = min(max(13 - e, -126), 126);
+                    f = __uint_as_float((uint32_t)(127 - up) << 23);
+                    const float g = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[n][s][k] *= g;
+                }
+                f *= a.scale;
+                qs[n][0] = __shfl_sync(0xffffffffu, f, col4 * 8);
+                qs[n][1] = __shfl_sync(0xffffffffu, f, col4 * 8 + 4);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    q[s][n][0] = pack<BF>(x[n][s][0], x[n][s][1]);
+                    q[s][n][1] = pack<BF>(x[n][s][2], x[n][s][3]);
+                }
+            }
+        }
+        float o[KS][NT][4] = {};
+        float m[NT][2], l[NT][2] = {};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
+        int vexp = kLeastExp;  // 2^vexp: the running power of two of the value scales
+
+        for (uint32_t unit = start + warp; unit < cur.end; unit += kWarps) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+            __syncwarp();
+            const unsigned char *buf = ring + stage * S::kStage;
+            const uint32_t buf_at = ring_at + stage * S::kStage;
+            const uint16_t *ksc = reinterpret_cast<const uint16_t *>(buf + 2 * S::kPart);
+            const uint16_t *vsc = ksc + S::kScale / 2;
+            const uint32_t bad = flags[warp * 4 + stage];
+            const int32_t left = cur.len - (int32_t)(unit * T);  // tokens of the unit that exist
+            // ---- S^T = K Q^T ----
+            float s[C16][NT][4];
+#pragma unroll
+            for (int c = 0; c < C16; ++c) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[c][n][0] = s[c][n][1] = s[c][n][2] = s[c][n][3] = 0.0f;
+                const uint32_t r0 = 16 * c + row4;
+                if constexpr (F <= F_BF16) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        uint32_t f[4];
+                        ldsm4(f, buf_at + place<S::kRow>(16 * c + (lane & 15u), 2 * k + (lane >> 4)));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<BF>(s[c][n], f, q[k][n][0], q[k][n][1]);
+                    }
+                } else if constexpr (F == F_INT8) {
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        uint4 lo = *reinterpret_cast<const uint4 *>(buf + place<S::kRow>(r0, 4 * j + col4));
+                        uint4 hi = *reinterpret_cast<const uint4 *>(buf + place<S::kRow>(r0 + 8, 4 * j + col4));
+                        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t x = wl[i] ^ 0x80808080u, y = wh[i] ^ 0x80808080u;
+                            const uint32_t f[4] = {bytes_to_half(x, 0x4140), bytes_to_half(y, 0x4140),
+                                                   bytes_to_half(x, 0x4342), bytes_to_half(y, 0x4342)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma<false>(s[c][n], f, q[4 * j + i][n][0], q[4 * j + i][n][1]);
+                        }
+                    }
+                    const float k0 = from_bf16(ksc[r0]), k1 = from_bf16(ksc[r0 + 8]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        s[c][n][0] *= k0;
+                        s[c][n][1] *= k0;
+                        s[c][n][2] *= k1;
+                        s[c][n][3] *= k1;
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < D / 32; ++g) {
+                        uint32_t x = *reinterpret_cast<const uint32_t *>(buf + place<S::kRow>(r0, g) + 4 * col4);
+                        uint32_t y = *reinterpret_cast<const uint32_t *>(buf + place<S::kRow>(r0 + 8, g) + 4 * col4);
+                        float p[NT][4] = {};
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t f[4] = {nibble0(x), nibble0(y), nibble1(x), nibble1(y)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma<false>(p[n], f, q[2 * g + i][n][0], q[2 * g + i][n][1]);
+                            x >>= 8;
+                            y >>= 8;
+                        }
+                        const float k0 = from_bf16(ksc[r0 * S::kGroups + g]);
+                        const float k1 = from_bf16(ksc[(r0 + 8) * S::kGroups + g]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            s[c][n][0] = fmaf(p[n][0], k0, s[c][n][0]);
+                            s[c][n][1] = fmaf(p[n][1], k0, s[c][n][1]);
+                            s[c][n][2] = fmaf(p[n][2], k1, s[c][n][2]);
+                            s[c][n][3] = fmaf(p[n][3], k1, s[c][n][3]);
+                        }
+                    }
+                }
+            }
+            // ---- logits in log2 units, masked; the running maximum ----
+            float top[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < C16; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int32_t t = 16 * c + row4 + 8 * e;
+                    const bool in = t < left && !(bad && bad >> (t >> shift) & 1u);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float &x = s[c][n][2 * e + h];
+                            x = in ? x * qs[n][h] : -INFINITY;
+                            top[n][h] = fmaxf(top[n][h], x);
+                        }
+                }
+            bool moved = false;
+            float alpha[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = top[n][h];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float now = fmaxf(m[n][h], x);
+                    moved |= now > m[n][h];
+                    alpha[n][h] = now == -INFINITY ? 1.0f : ex2(m[n][h] - now);
+                    m[n][h] = now;
+                }
+            // ---- value scales: the running power of two ----
+            float vmul = 4096.0f;  // of a probability (FP16 and 8-bit pages) or a value scale (4 bits)
+            if constexpr (F >= F_INT8) {
+                uint32_t big = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < (T * S::kGroups + 31) / 32; ++i) {
+                    const uint32_t x = vsc[i * 32 + lane];
+                    big = max(big, x < 0x7f80u ? x : 0u);
+                }
+                big = __reduce_max_sync(0xffffffffu, big);
+                const int e = min((int)(big >> 7) - 127, 126);
+                if (e > vexp) {
+                    const float f = __uint_as_float((uint32_t)max(vexp - e + 127, 0) << 23);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < KS; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[i][n][k] *= f;
+                    vexp = e;
+                }
+                vmul = __uint_as_float((uint32_t)(127 - vexp) << 23);  // 2^-vexp
+                vmul *= F == F_INT8 ? 4096.0f : 128.0f;
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    l[n][0] *= alpha[n][0];
+                    l[n][1] *= alpha[n][1];
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        o[i][n][0] *= alpha[n][0];
+                        o[i][n][1] *= alpha[n][1];
+                        o[i][n][2] *= alpha[n][0];
+                        o[i][n][3] *= alpha[n][1];
+                    }
+                }
+            }
+            // ---- probabilities, O^T += V^T P^T ----
+#pragma unroll
+            for (int c = 0; c < C16; ++c) {
+                uint32_t p[NT][2];
+                float w0 = vmul, w1 = vmul;
+                if constexpr (F == F_BF16) w0 = w1 = 1.0f;
+                if constexpr (F == F_INT4) w0 = w1 = 4096.0f;
+                if constexpr (F == F_INT8) {
+                    w0 = from_bf16(vsc[16 * c + row4]) * vmul;
+                    w1 = from_bf16(vsc[16 * c + row4 + 8]) * vmul;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float r0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+                    const float e0 = ex2(s[c][n][0] - r0), e1 = ex2(s[c][n][1] - r1);
+                    const float e2 = ex2(s[c][n][2] - r0), e3 = ex2(s[c][n][3] - r1);
+                    l[n][0] += e0 + e2;
+                    l[n][1] += e1 + e3;
+                    p[n][0] = turn(pack<BF>(e0 * w0, e1 * w0));
+                    p[n][1] = turn(pack<BF>(e2 * w1, e3 * w1));
+                }
+                if constexpr (F <= F_BF16) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        uint32_t f[4];
+                        ldsm4_t(f, buf_at + S::kPart + place<S::kRow>(16 * c + (lane & 7u) + (lane >> 4) * 8, 2 * i + (lane >> 3 & 1u)));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<BF>(o[i][n], f, p[n][0], p[n][1]);
+                    }
+                } else {
+                    // this thread's words: tokens 2c, 2c + 1, 2c + 8, 2c + 9, dimensions D/8 * row4 ..
+                    constexpr int W = F == F_INT8 ? D / 32 : D / 64;  // 32-bit words of D / 8 dimensions
+                    uint32_t w[4][W];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t r = 16 * c + 2 * col4 + (e & 1) + 8 * (e >> 1), byte = row4 * W * 4;
+                        const unsigned char *at = buf + S::kPart + place<S::kRow>(r, byte >> 4) + (byte & 15u);
+                        if constexpr (W == 4) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(at);
+                            w[e][0] = x.x, w[e][1] = x.y, w[e][2] = x.z, w[e][3] = x.w;
+                        } else if constexpr (W == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+                            w[e][0] = x.x, w[e][1] = x.y;
+                        } else w[e][0] = *reinterpret_cast<const uint32_t *>(at);
+                    }
+                    if constexpr (F == F_INT8) {
+#pragma unroll
+                        for (int i = 0; i < W; ++i) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e][i] ^= 0x80808080u;
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {  // two dimensions of both token pairs
+                                const uint32_t y = __byte_perm(w[0][i], w[1][i], k ? 0x7362 : 0x5140);
+                                const uint32_t z = __byte_perm(w[2][i], w[3][i], k ? 0x7362 : 0x5140);
+                                const uint32_t f[4] = {bytes_to_half(y, 0x4140), bytes_to_half(y, 0x4342),
+                                                       bytes_to_half(z, 0x4140), bytes_to_half(z, 0x4342)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma<false>(o[2 * i + k][n], f, p[n][0], p[n][1]);
+                            }
+                        }
+                    } else {
+                        // D / 8 dimensions lie in one group: scales of the four tokens as two FP16 pairs
+                        const uint32_t g = row4 * (D / 8) / 32, t = 16 * c + 2 * col4;
+                        const float f0 = from_bf16(vsc[t * S::kGroups + g]) * vmul;
+                        const float f1 = from_bf16(vsc[(t + 1) * S::kGroups + g]) * vmul;
+                        const float f2 = from_bf16(vsc[(t + 8) * S::kGroups + g]) * vmul;
+                        const float f3 = from_bf16(vsc[(t + 9) * S::kGroups + g]) * vmul;
+                        const uint32_t sa = pack<false>(f0, f1), sb = pack<false>(f2, f3);
+#pragma unroll
+                        for (int i = 0; i < W; ++i)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                uint32_t y = __byte_perm(w[0][i], w[1][i], half ? 0x7632 : 0x5410);
+                                uint32_t z = __byte_perm(w[2][i], w[3][i], half ? 0x7632 : 0x5410);
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    const uint32_t f[4] = {mul2(nibble0(y), sa), mul2(nibble1(y), sa),
+                                                           mul2(nibble0(z), sb), mul2(nibble1(z), sb)};
+#pragma unroll
+                                    for (int n = 0; n < NT; ++n)
+                                        mma<false>(o[4 * i + 2 * half + k][n], f, p[n][0], p[n][1]);
+                                    y >>= 8;
+                                    z >>= 8;
+                                }
+                            }
+                    }
+                }
+            }
+            __syncwarp();  // the slot that the next fill takes was read in the round before this one
+            fill(stage == 0 ? S::kStages - 1 : stage - 1);
+            stage = stage + 1 == (uint32_t)S::kStages ? 0 : stage + 1;
+        }
+
+        // ---- the four warps' parts, joined through shared memory ----
+        {
+            float unit_out = 1.0f;
+            if constexpr (F != F_BF16) unit_out = 1.0f / 4096.0f;
+            if constexpr (F == F_INT4) unit_out *= 1.0f / 128.0f;
+            if constexpr (F >= F_INT8) unit_out *= __uint_as_float((uint32_t)(vexp + 127) << 23);
+            float *mine = join + warp * S::kHeads * (D + 2);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = l[n][h];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    const uint32_t head = n * 8 + 2 * col4 + h;
+                    if (row4 == 0) {
+                        mine[S::kHeads * D + head] = m[n][h];
+                        mine[S::kHeads * (D + 1) + head] = x;
+                    }
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t d = F <= F_BF16 ? 16 * i + row4 + 8 * e : (D / 8) * row4 + 2 * i + e;
+                            mine[head * D + d] = o[i][n][2 * e + h] * unit_out;
+                        }
+                }
+        }
+        __syncthreads();
+        const uint64_t pair_first = cur.u - start, pair_last = pair_first + cur.units - 1;
+        const bool whole = start == 0 && cur.end == cur.units;
+        const uint64_t c_first = ((pair_first + 1) * ctas - 1) / total, c_last = ((pair_last + 1) * ctas - 1) / total;
+        // at most one pair that is not whole begins in a CTA's range: its counter is that CTA's
+        uint32_t *counter = static_cast<uint32_t *>(a.workspace) + c_first;
+        float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters);
+        constexpr uint32_t kPartFloats = S::kHeads * (D + 2);
+        auto write_out = [&](uint32_t head, uint32_t d, float x, float y, float big, float sum) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const uint64_t row = (uint64_t)cur.b * a.q_heads + head0 + head;
+            uint32_t *out = static_cast<uint32_t *>(a.out) + (row * D + d) / 2;
+            *out = a.dtype == BGTQ_F16 ? pack<false>(x * inv, y * inv) : pack<true>(x * inv, y * inv);
+            if (a.lse && d == 0) a.lse[row] = sum == 0.0f ? -INFINITY : (big + __log2f(sum)) * kLn2;
+        };
+        // this CTA's slot for the segment: its range begins in the pair (first slot) or the pair in it (second)
+        float *slot = parts + (2ull * blockIdx.x + (start == 0 ? 1 : 0)) * kPartFloats;
+        for (uint32_t i = threadIdx.x; i < heads * (D / 2); i += kThreads) {
+            const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
+            float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) big = fmaxf(big, join[w * kPartFloats + S::kHeads * D + head]);
+            const float ref = big == -INFINITY ? 0.0f : big;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float *p = join + w * kPartFloats;
+                const float f = ex2(p[S::kHeads * D + head] - ref);
+                sum = fmaf(f, p[S::kHeads * (D + 1) + head], sum);
+                x = fmaf(f, p[head * D + d], x);
+                y = fmaf(f, p[head * D + d + 1], y);
+            }
+            if (whole) write_out(head, d, x, y, big, sum);
+            else {
+                *reinterpret_cast<float2 *>(slot + head * D + d) = make_float2(x, y);
+                if (d == 0) {
+                    slot[S::kHeads * D + head] = big;
+                    slot[S::kHeads * (D + 1) + head] = sum;
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const uint32_t n = atomicAdd(counter, 1u);
+                flags[kWarps * 4] = n == (uint32_t)(c_last - c_first);
+                if (n == (uint32_t)(c_last - c_first)) *counter = 0;
+            }
+            __syncthreads();
+            if (flags[kWarps * 4]) {
+                __threadfence();
+                for (uint32_t i = threadIdx.x; i < heads * (D / 2); i += kThreads) {
+                    const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
+                    float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+                    for (uint64_t c = c_first; c <= c_last; ++c) {
+                        const float *p = parts + (2 * c + (c == c_first ? 1 : 0)) * kPartFloats;
+                        const float pm = __ldcg(p + S::kHeads * D + head), pl = __ldcg(p + S::kHeads * (D + 1) + head);
+                        const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + head * D + d));
+                        const float now = fmaxf(big, pm), ref = now == -INFINITY ? 0.0f : now;
+                        const float f = ex2(big - ref), g = ex2(pm - ref);
+                        big = now;
+                        sum = sum * f + pl * g;
+                        x = x * f + v.x * g;
+                        y = y * f + v.y * g;
+                    }
+                    write_out(head, d, x, y, big, sum);
+                }
+            }
+        }
+        if (!next_segment(cur, start)) break;
+        __syncthreads();
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// CTAs of a launch at most: the workspace holds two parts of each.
+uint32_t most_ctas() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return (uint32_t)sms * 4;
+}
+uint32_t counter_bytes() { return (most_ctas() * 4 + 15) / 16 * 16; }
+
+template <int F, int D, int NT>
+cudaError_t run(const PagedAttendArgs &a, cudaStream_t s) {
+    using S = Shape<F, D, NT>;
+    auto kernel = attend_kernel<F, D, NT>;
+    static int resident[64] = {};  // CTAs an SM holds, by device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    if (!resident[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return e;
+        int n = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, S::kSmem);
+        if (e != cudaSuccess) return e;
+        resident[dev] = n < 1 ? 1 : n > 4 ? 4 : n;
+    }
+    int sms = 0;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    PagedAttendArgs b = a;
+    b.counters = counter_bytes();
+    kernel<<<(uint32_t)(sms * resident[dev]), kThreads, S::kSmem, s>>>(b);
+    return cudaGetLastError();
+}
+
+template <int F>
+cudaError_t by_shape(const PagedAttendArgs &a, cudaStream_t s) {
+    if (a.c.dim == 64) return a.group <= 8 ? run<F, 64, 1>(a, s) : run<F, 64, 2>(a, s);
+    return a.group <= 8 ? run<F, 128, 1>(a, s) : run<F, 128, 2>(a, s);
 }
 
 }  // namespace
 
-size_t paged_attend_workspace(uint32_t, uint32_t, uint32_t, uint32_t) { return 0; }
+size_t paged_attend_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t dim) {
+    return counter_bytes() + 2ull * most_ctas() * (q_heads / kv_heads <= 8 ? 8u : 16u) * (dim + 2) * 4;
+}
 
 cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t s) {
-    const dim3 grid(a.q_heads, a.batch);
-    if (a.c.dim == 64) attend_kernel<64><<<grid, 32, 0, s>>>(a);
-    else attend_kernel<128><<<grid, 32, 0, s>>>(a);
-    return cudaGetLastError();
+    switch (a.c.format) {
+        case BGTQ_PAGES_F16: return by_shape<F_F16>(a, s);
+        case BGTQ_PAGES_BF16: return by_shape<F_BF16>(a, s);
+        case BGTQ_PAGES_INT8: return by_shape<F_INT8>(a, s);
+        default: return by_shape<F_INT4>(a, s);
+    }
 }
 
 }  // namespace bgtq

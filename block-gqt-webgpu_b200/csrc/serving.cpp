@@ -49,8 +49,8 @@ bgtq_status view(const bgtq_paged_cache *c, PageView &v) {
     const bool scaled = c->format == BGTQ_PAGES_INT8 || c->format == BGTQ_PAGES_INT4;
     if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16))
         return refuse("Paged cache: pages must be 16-byte aligned device memory");
-    if (scaled && (!c->k_scales || !c->v_scales || !aligned(c->k_scales, 8) || !aligned(c->v_scales, 8)))
-        return refuse("Paged cache: scales must be 8-byte aligned device memory");
+    if (scaled && (!c->k_scales || !c->v_scales || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16)))
+        return refuse("Paged cache: scales must be 16-byte aligned device memory");
     v.k = static_cast<unsigned char *>(c->k);
     v.v = static_cast<unsigned char *>(c->v);
     v.ks = scaled ? c->k_scales : nullptr;
@@ -125,13 +125,13 @@ bgtq_status bgtq_paged_read(const bgtq_paged_cache *c, const int64_t *slots, uin
     return launched(launch_paged_read(a, static_cast<cudaStream_t>(stream)), "Paged read");
 }
 
-bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t batch, uint32_t q_heads, size_t *bytes) {
+bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t q_heads, size_t *bytes) {
     PageView v{};
     if (bgtq_status s = view(c, v)) return s;
     if (!bytes || !q_heads || q_heads % c->kv_heads) return refuse("Paged attention: invalid head count");
     OnDevice on(c->device);
     if (!on.ok) return launched(cudaErrorInvalidDevice, "Paged attention");
-    *bytes = paged_attend_workspace(batch, q_heads, c->kv_heads, c->dim);
+    *bytes = paged_attend_workspace(q_heads, c->kv_heads, c->dim);
     return BGTQ_OK;
 }
 
@@ -156,7 +156,7 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
     OnDevice on(c->device);
     a.status = on.ok ? device_status_word(c->device) : nullptr;
     if (!a.status) return launched(cudaErrorInvalidDevice, "Paged attention");
-    const size_t need = paged_attend_workspace(batch, q_heads, c->kv_heads, c->dim);
+    const size_t need = paged_attend_workspace(q_heads, c->kv_heads, c->dim);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return refuse("Paged attention: the workspace is too small or misaligned");
     a.q = q;

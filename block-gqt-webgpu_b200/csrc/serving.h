@@ -56,6 +56,7 @@ struct PagedAttendArgs {
     float *lse;  // nullable
     void *workspace;
     uint32_t batch, q_heads, group, width;
+    uint32_t counters;  // bytes of the workspace's counters (the launcher's)
     float scale;  // of the logits, times log2(e)
     bgtq_dtype dtype;
     uint32_t *status;
@@ -78,7 +79,7 @@ struct PromptArgs {
 cudaError_t launch_paged_write(const PagedWriteArgs &a, cudaStream_t s);
 cudaError_t launch_paged_read(const PagedReadArgs &a, cudaStream_t s);
 // Bytes of the workspace that launch_paged_attend needs (counters first, zero between calls).
-size_t paged_attend_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t dim);
+size_t paged_attend_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t dim);
 cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t s);
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s);
 

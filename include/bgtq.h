@@ -464,7 +464,7 @@ void bgtq_decoder_destroy(bgtq_decoder *dec);
  *   BGTQ_PAGES_INT4        dim / 2 bytes, even dimension in the low nibble, code + 8; one
  *                          scale for every 32 dimensions
  * Scales are BF16, at the same row index (times dim / 32 in 4 bits); a stored value is
- * code * scale.  `k` and `v` are 16-byte aligned, the scales 8-byte. */
+ * code * scale.  All four are 16-byte aligned. */
 typedef enum { BGTQ_PAGES_F16 = 1, BGTQ_PAGES_BF16 = 2, BGTQ_PAGES_INT8 = 3, BGTQ_PAGES_INT4 = 4 } bgtq_page_format;
 typedef struct bgtq_paged_cache {
     int device;
@@ -491,8 +491,8 @@ bgtq_status bgtq_paged_write(const bgtq_paged_cache *c, const void *k, const voi
  * the status bit), give zeros. */
 bgtq_status bgtq_paged_read(const bgtq_paged_cache *c, const int64_t *slots, uint64_t tokens, void *k_out,
                             void *v_out, bgtq_dtype dtype, void *stream);
-/* Bytes of workspace that bgtq_paged_attend needs for these sizes (a multiple of 16). */
-bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t batch, uint32_t q_heads, size_t *bytes);
+/* Bytes of workspace that bgtq_paged_attend needs for this head count, whatever the batch. */
+bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t q_heads, size_t *bytes);
 /* One new token per request: out[b][h] = sum over t < lengths[b] of softmax(scale q.k_t) v_t.
  *   q        element (b, h, i) at q[b * q_batch_stride + h * q_head_stride + i], dtype F16 or
  *            BF16; over 16-bit pages the pages' own type.  Query head h uses KV head

@@ -40,12 +40,12 @@ def attend(c, q=GOOD, dtype=_lib.F16, batch=2, heads=4, table=GOOD, width=4, len
     (dict(page_size=24), "page size"), (dict(page_size=8), "page size"), (dict(page_size=512), "page size"),
     (dict(kv_heads=0), "head or page count"), (dict(kv_heads=1025), "head or page count"),
     (dict(pages=0), "head or page count"), (dict(pages=1 << 31), "head or page count"), (dict(k=None), "16-byte"),
-    (dict(v=GOOD + 8), "16-byte"), (dict(k_scales=None), "scales"), (dict(v_scales=GOOD + 2), "scales")])
+    (dict(v=GOOD + 8), "16-byte"), (dict(k_scales=None), "scales"), (dict(v_scales=GOOD + 8), "scales")])
 def test_every_call_refuses_a_wrong_cache(change, message):
     c = cache(**change)
     for call in (write(c), read(c), attend(c)):
         refused(message, *call)
-    refused(message, "bgtq_paged_attend_workspace", C.byref(c), 1, 2, C.byref(C.c_size_t()))
+    refused(message, "bgtq_paged_attend_workspace", C.byref(c), 2, C.byref(C.c_size_t()))
 
 
 def test_null_cache():
