@@ -51,8 +51,9 @@ struct Shape {
     static constexpr int kStage = 2 * (kPart + kScale);
     static constexpr int kRing = kStages * kStage;
     static constexpr int kHeads = 8 * NT;
-    static constexpr int kJoin = kHeads * (D + 2) * 4;           // one warp's part: O, m, l
-    static constexpr int kSmem = kWarps * (kRing + kJoin) + 128;
+    static constexpr int kPartFloats = kHeads * (D + 2);         // a part in the workspace: O, m, l
+    static constexpr int kSmem = kWarps * kRing + kWarps * kHeads * 8 + 128;
+    static_assert(kStage >= kHeads * D * 4, "a warp's outputs are joined in the ring slot that it read last");
 };
 
 // 16-byte chunk `c` of row r in a ring slot.  Rows share 128-byte lines; the chunks of a line
@@ -132,16 +133,20 @@ __device__ __forceinline__ uint32_t bytes_to_half(uint32_t w, uint32_t sel) {
 __device__ __forceinline__ uint32_t nibble0(uint32_t w) { return sub2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
 __device__ __forceinline__ uint32_t nibble1(uint32_t w) { return sub2((w & 0x00f000f0u) | 0x54005400u, 0x54805480u); }
 
-// Where a warp's next unit is: request b, pair p of it, units [at, end) of the pair left in this
-// segment; `u` is the flat index of the segment's first unit.
+// One item of the deal: a pair (request, KV head, block of query heads), which may be cut between
+// CTAs, or, of a short request, four pairs side by side, a whole one for each warp.
 struct Cursor {
-    uint32_t b, pair, units, at, end;
+    uint32_t b, item, items, units, weight;
     int32_t len;
-    uint64_t u;
+    bool quad;
+    uint64_t base;     // where the item begins in the deal
+    uint32_t at, end;  // the units of it that are this CTA's (quads: all or none)
 };
+// What an item costs beside its units, in units: its queries, the join of the warps, its output.
+constexpr uint32_t kItemCost = 6;
 
 template <int F, int D, int NT>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendArgs a) {
     using S = Shape<F, D, NT>;
     constexpr bool BF = F == F_BF16;
     constexpr int T = S::kTokens, C16 = T / 16, KS = D / 16;
@@ -149,8 +154,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row4 = lane >> 2, col4 = lane & 3u;
     unsigned char *ring = smem + warp * S::kRing;
     const uint32_t ring_at = smem_addr(ring);
-    float *join = reinterpret_cast<float *>(smem + kWarps * S::kRing);
-    uint32_t *flags = reinterpret_cast<uint32_t *>(smem + kWarps * (S::kRing + S::kJoin));
+    float2 *sums = reinterpret_cast<float2 *>(smem + kWarps * S::kRing);  // [warp][head]: maximum, sum
+    uint32_t *flags = reinterpret_cast<uint32_t *>(sums + kWarps * S::kHeads);
     const uint32_t blocks = (a.group + S::kHeads - 1) / S::kHeads, pairs = a.c.heads * blocks;
     const uint32_t shift = a.c.page_shift, H = a.c.heads;
 
@@ -158,26 +163,41 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
         const int32_t n = __ldg(a.lengths + b);
         return n < 0 ? 0 : (int32_t)min((uint32_t)n, a.width << shift);
     };
-    // ---- the deal: all units, this CTA's range of them ----
-    uint64_t total = 0;
-    {
-        uint32_t *sums = reinterpret_cast<uint32_t *>(join);
-        uint64_t mine = 0;
-        for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
-            const int32_t n = length(b);
-            if (n != __ldg(a.lengths + b) && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
-            mine += (uint32_t)(n + T - 1) / T;
-        }
+    // ---- the deal ----
+    auto block_sum = [&](uint64_t x) {
+        uint64_t *part = reinterpret_cast<uint64_t *>(sums), all = 0;
 #pragma unroll
-        for (int w = 16; w; w >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
-        uint64_t *part = reinterpret_cast<uint64_t *>(sums);
-        if (lane == 0) part[warp] = mine;
+        for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+        if (lane == 0) part[warp] = x;
         __syncthreads();
 #pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) total += part[w];
+        for (uint32_t w = 0; w < kWarps; ++w) all += part[w];
         __syncthreads();
-        total *= pairs;
+        return all;
+    };
+    uint64_t mine = 0;
+    for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
+        const int32_t n = length(b);
+        if (n != __ldg(a.lengths + b) && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
+        mine += (uint32_t)(n + T - 1) / T;
     }
+    const uint64_t all_units = block_sum(mine) * pairs;
+    // a request whose quad of pairs is within a CTA's share of the units goes by quads
+    const uint64_t share = all_units / gridDim.x;
+    auto plan = [&](Cursor &c) {  // from c.b and c.len
+        c.units = (uint32_t)(c.len + T - 1) / T;
+        c.quad = pairs > 1 && 4ull * c.units <= share;
+        c.items = c.len == 0 ? 0 : c.quad ? (pairs + 3) / 4 : pairs;
+        c.weight = (c.quad ? 4 * c.units : c.units) + kItemCost;
+    };
+    mine = 0;
+    for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
+        Cursor c;
+        c.len = length(b);
+        plan(c);
+        mine += (uint64_t)c.items * c.weight;
+    }
+    const uint64_t total = block_sum(mine);
     // a request without tokens: zeros
     for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (length(b) != 0) continue;
@@ -186,69 +206,85 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
         if (a.lse)
             for (uint32_t i = threadIdx.x; i < a.q_heads; i += kThreads) a.lse[(uint64_t)b * a.q_heads + i] = -INFINITY;
     }
-    const uint64_t most = (total + kWarps - 1) / kWarps;
+    const uint64_t most = (all_units + kWarps - 1) / kWarps;
     const uint64_t ctas = most < gridDim.x ? most : gridDim.x;
     if (blockIdx.x >= ctas) return;
     const uint64_t first = (uint64_t)blockIdx.x * total / ctas, last = (uint64_t)(blockIdx.x + 1) * total / ctas;
+    // this CTA's share of the item: a unit, or a quad, belongs to the CTA whose range holds its place
+    auto take = [&](Cursor &c) {
+        if (c.quad) {
+            c.at = 0;
+            c.end = c.base >= first && c.base < last ? c.units : 0;
+        } else {
+            const uint64_t from = c.base + kItemCost;
+            c.at = first <= from ? 0u : (uint32_t)min((uint64_t)c.units, first - from);
+            c.end = last <= from ? 0u : (uint32_t)min((uint64_t)c.units, last - from);
+        }
+    };
+    // the next item with units of this CTA's; false past the range's end
+    auto next_item = [&](Cursor &c) {
+        do {
+            c.base += c.weight;
+            if (c.base >= last) return false;
+            if (++c.item == c.items) {
+                c.item = 0;
+                do {
+                    if (++c.b >= a.batch) return false;
+                    c.len = length(c.b);
+                } while (c.len == 0);
+                plan(c);
+            }
+            take(c);
+        } while (c.at >= c.end);
+        return true;
+    };
     Cursor cur;
     {
         uint64_t base = 0;
-        cur.b = 0;
         for (uint32_t b0 = 0;; b0 += 32) {  // ends: first < total
-            const uint32_t n = b0 + lane < a.batch ? (uint32_t)(length(b0 + lane) + T - 1) / T : 0u;
-            uint64_t sum = (uint64_t)n * pairs;
+            cur.len = b0 + lane < a.batch ? length(b0 + lane) : 0;
+            plan(cur);
+            const uint64_t own = (uint64_t)cur.items * cur.weight;
+            uint64_t sum = own;
 #pragma unroll
             for (int w = 1; w < 32; w <<= 1) {
                 const uint64_t o = __shfl_up_sync(0xffffffffu, sum, w);
                 if (lane >= (uint32_t)w) sum += o;
             }
             const uint32_t past = __ballot_sync(0xffffffffu, base + sum > first);
-            if (past || b0 + 32 >= a.batch) {
-                const uint32_t l = past ? __ffs(past) - 1 : 31u;
-                base += __shfl_sync(0xffffffffu, sum, l) - (uint64_t)__shfl_sync(0xffffffffu, n, l) * pairs;
+            if (past) {
+                const uint32_t l = __ffs(past) - 1;
+                base += __shfl_sync(0xffffffffu, sum - own, l);
                 cur.b = b0 + l;
                 break;
             }
+            if (b0 + 32 >= a.batch) return;
             base += __shfl_sync(0xffffffffu, sum, 31);
         }
         cur.len = length(cur.b);
-        cur.units = (uint32_t)(cur.len + T - 1) / T;
-        cur.pair = (uint32_t)((first - base) / cur.units);
-        cur.at = (uint32_t)((first - base) % cur.units);
-        cur.u = first;
-        cur.end = (uint32_t)min((uint64_t)cur.units, cur.at + (last - first));
+        plan(cur);
+        cur.item = (uint32_t)((first - base) / cur.weight);
+        cur.base = base + (uint64_t)cur.item * cur.weight;
+        take(cur);
+        if (cur.at >= cur.end && !next_item(cur)) return;
     }
-    // the segment after this one; false past the range's end
-    auto next_segment = [&](Cursor &c, uint32_t start) {
-        c.u += c.end - start;
-        if (c.u >= last) return false;
-        if (++c.pair == pairs) {
-            c.pair = 0;
-            do {
-                if (++c.b >= a.batch) return false;
-                c.len = length(c.b);
-            } while (c.len == 0);
-            c.units = (uint32_t)(c.len + T - 1) / T;
-        }
-        c.at = 0;
-        c.end = (uint32_t)min((uint64_t)c.units, last - c.u);
-        return true;
-    };
+    // a warp's first unit of an item, its step, and its pair
+    auto unit0 = [&](const Cursor &c) { return c.quad ? (c.item * 4 + warp < pairs ? 0u : c.end) : c.at + warp; };
+    auto step_of = [](const Cursor &c) { return c.quad ? 1u : kWarps; };
+    auto pair_of = [&](const Cursor &c) { return c.quad ? c.item * 4 + warp : c.item; };
 
     // ---- filling the ring ----
     Cursor pre = cur;
-    uint32_t pre_start = pre.at;
+    uint32_t pre_unit = unit0(pre);
     bool more = true;
-    pre.at += warp;
     int32_t page_reg = -1;
     auto settle = [&]() {  // moves `pre` to the warp's next unit, if there is one, and loads its page indices
-        while (more && pre.at >= pre.end) {
-            more = next_segment(pre, pre_start);
-            pre_start = 0;
-            if (more) pre.at = warp;
+        while (more && pre_unit >= pre.end) {
+            more = next_item(pre);
+            if (more) pre_unit = unit0(pre);
         }
         if (more) {
-            const uint32_t t = pre.at * T + (lane << shift);
+            const uint32_t t = pre_unit * T + (lane << shift);
             page_reg = t < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T)
                            ? __ldg(a.table + (int64_t)pre.b * a.table_stride + (t >> shift)) : -1;
         }
@@ -256,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
     settle();
     auto fill = [&](uint32_t stage) {
         if (more) {
-            const uint32_t t0 = pre.at * T, kh = pre.pair / blocks;
+            const uint32_t t0 = pre_unit * T, kh = pair_of(pre) / blocks;
             const int32_t page = page_reg;
             const bool wrong = (uint32_t)page >= a.c.pages;
             const bool asked = t0 + (lane << shift) < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T);
@@ -294,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
                     }
                 }
             }
-            pre.at += kWarps;
+            pre_unit += step_of(pre);
             settle();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -304,8 +340,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
 
     uint32_t stage = 0;
     for (;;) {
-        // ---- a segment: units [cur.at, cur.end) of one pair ----
-        const uint32_t start = cur.at, kh = cur.pair / blocks, block = cur.pair % blocks;
+        // ---- an item: this warp's units of its pair ----
+        const uint32_t pair = min(pair_of(cur), pairs - 1), kh = pair / blocks, block = pair % blocks;
         const uint32_t head0 = kh * a.group + block * S::kHeads;
         const uint32_t heads = min((uint32_t)S::kHeads, a.group - block * S::kHeads);
         uint32_t q[KS][NT][2];
@@ -369,7 +405,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
         int vexp = kLeastExp;  // 2^vexp: the running power of two of the value scales
 
-        for (uint32_t unit = start + warp; unit < cur.end; unit += kWarps) {
+        for (uint32_t unit = unit0(cur); unit < cur.end; unit += step_of(cur)) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
             __syncwarp();
             const unsigned char *buf = ring + stage * S::kStage;
@@ -607,13 +643,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
             stage = stage + 1 == (uint32_t)S::kStages ? 0 : stage + 1;
         }
 
-        // ---- the four warps' parts, joined through shared memory ----
+        // ---- the warp's part, in the ring slot that it read last (the next fill comes after a unit more) ----
+        float *mine_o = reinterpret_cast<float *>(ring + (stage == 0 ? S::kStages - 1 : stage - 1) * S::kStage);
         {
             float unit_out = 1.0f;
             if constexpr (F != F_BF16) unit_out = 1.0f / 4096.0f;
             if constexpr (F == F_INT4) unit_out *= 1.0f / 128.0f;
             if constexpr (F >= F_INT8) unit_out *= __uint_as_float((uint32_t)(vexp + 127) << 23);
-            float *mine = join + warp * S::kHeads * (D + 2);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -623,27 +659,16 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);
                     const uint32_t head = n * 8 + 2 * col4 + h;
-                    if (row4 == 0) {
-                        mine[S::kHeads * D + head] = m[n][h];
-                        mine[S::kHeads * (D + 1) + head] = x;
-                    }
+                    if (row4 == 0) sums[warp * S::kHeads + head] = make_float2(m[n][h], x);
 #pragma unroll
                     for (int i = 0; i < KS; ++i)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const uint32_t d = F <= F_BF16 ? 16 * i + row4 + 8 * e : (D / 8) * row4 + 2 * i + e;
-                            mine[head * D + d] = o[i][n][2 * e + h] * unit_out;
+                            mine_o[head * D + d] = o[i][n][2 * e + h] * unit_out;
                         }
                 }
         }
-        __syncthreads();
-        const uint64_t pair_first = cur.u - start, pair_last = pair_first + cur.units - 1;
-        const bool whole = start == 0 && cur.end == cur.units;
-        const uint64_t c_first = ((pair_first + 1) * ctas - 1) / total, c_last = ((pair_last + 1) * ctas - 1) / total;
-        // at most one pair that is not whole begins in a CTA's range: its counter is that CTA's
-        uint32_t *counter = static_cast<uint32_t *>(a.workspace) + c_first;
-        float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters);
-        constexpr uint32_t kPartFloats = S::kHeads * (D + 2);
         auto write_out = [&](uint32_t head, uint32_t d, float x, float y, float big, float sum) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const uint64_t row = (uint64_t)cur.b * a.q_heads + head0 + head;
@@ -651,29 +676,51 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
             *out = a.dtype == BGTQ_F16 ? pack<false>(x * inv, y * inv) : pack<true>(x * inv, y * inv);
             if (a.lse && d == 0) a.lse[row] = sum == 0.0f ? -INFINITY : (big + __log2f(sum)) * kLn2;
         };
-        // this CTA's slot for the segment: its range begins in the pair (first slot) or the pair in it (second)
-        float *slot = parts + (2ull * blockIdx.x + (start == 0 ? 1 : 0)) * kPartFloats;
+        if (cur.quad) {
+            __syncwarp();
+            if (pair_of(cur) < pairs)
+                for (uint32_t i = lane; i < heads * (D / 2); i += 32) {
+                    const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
+                    const float2 ml = sums[warp * S::kHeads + head], v = *reinterpret_cast<float2 *>(mine_o + head * D + d);
+                    write_out(head, d, v.x, v.y, ml.x, ml.y);
+                }
+            __syncwarp();
+            if (!next_item(cur)) break;
+            if (!cur.quad) __syncthreads();
+            continue;
+        }
+        if (lane == 0) flags[kWarps * 4 + 1 + warp] = (uint32_t)(reinterpret_cast<unsigned char *>(mine_o) - smem);
+        __syncthreads();
+        const bool whole = cur.at == 0 && cur.end == cur.units;
+        // the CTAs that hold its first and its last unit
+        const uint64_t from = cur.base + kItemCost;
+        const uint64_t c_first = ((from + 1) * ctas - 1) / total, c_last = ((from + cur.units) * ctas - 1) / total;
+        // at most one pair that is not whole begins in a CTA's range: its counter is that CTA's
+        uint32_t *counter = static_cast<uint32_t *>(a.workspace) + c_first;
+        float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters);
+        // this CTA's slot for the part: the pair begins before its range (first slot) or in it (second)
+        float *slot = parts + (2ull * blockIdx.x + (cur.at == 0 ? 1 : 0)) * S::kPartFloats;
+        const float *parts_o[kWarps];
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) parts_o[w] = reinterpret_cast<float *>(smem + flags[kWarps * 4 + 1 + w]);
         for (uint32_t i = threadIdx.x; i < heads * (D / 2); i += kThreads) {
             const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
             float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) big = fmaxf(big, join[w * kPartFloats + S::kHeads * D + head]);
+            for (uint32_t w = 0; w < kWarps; ++w) big = fmaxf(big, sums[w * S::kHeads + head].x);
             const float ref = big == -INFINITY ? 0.0f : big;
 #pragma unroll
             for (uint32_t w = 0; w < kWarps; ++w) {
-                const float *p = join + w * kPartFloats;
-                const float f = ex2(p[S::kHeads * D + head] - ref);
-                sum = fmaf(f, p[S::kHeads * (D + 1) + head], sum);
-                x = fmaf(f, p[head * D + d], x);
-                y = fmaf(f, p[head * D + d + 1], y);
+                const float2 ml = sums[w * S::kHeads + head], v = *reinterpret_cast<const float2 *>(parts_o[w] + head * D + d);
+                const float f = ex2(ml.x - ref);
+                sum = fmaf(f, ml.y, sum);
+                x = fmaf(f, v.x, x);
+                y = fmaf(f, v.y, y);
             }
             if (whole) write_out(head, d, x, y, big, sum);
             else {
                 *reinterpret_cast<float2 *>(slot + head * D + d) = make_float2(x, y);
-                if (d == 0) {
-                    slot[S::kHeads * D + head] = big;
-                    slot[S::kHeads * (D + 1) + head] = sum;
-                }
+                if (d == 0) *reinterpret_cast<float2 *>(slot + S::kHeads * D + 2 * head) = make_float2(big, sum);
             }
         }
         if (!whole) {
@@ -691,13 +738,13 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
                     const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
                     float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
                     for (uint64_t c = c_first; c <= c_last; ++c) {
-                        const float *p = parts + (2 * c + (c == c_first ? 1 : 0)) * kPartFloats;
-                        const float pm = __ldcg(p + S::kHeads * D + head), pl = __ldcg(p + S::kHeads * (D + 1) + head);
+                        const float *p = parts + (2 * c + (c == c_first ? 1 : 0)) * S::kPartFloats;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + S::kHeads * D + 2 * head));
                         const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + head * D + d));
-                        const float now = fmaxf(big, pm), ref = now == -INFINITY ? 0.0f : now;
-                        const float f = ex2(big - ref), g = ex2(pm - ref);
+                        const float now = fmaxf(big, ml.x), ref = now == -INFINITY ? 0.0f : now;
+                        const float f = ex2(big - ref), g = ex2(ml.x - ref);
                         big = now;
-                        sum = sum * f + pl * g;
+                        sum = sum * f + ml.y * g;
                         x = x * f + v.x * g;
                         y = y * f + v.y * g;
                     }
@@ -705,7 +752,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const PagedAttendArgs 
                 }
             }
         }
-        if (!next_segment(cur, start)) break;
+        if (!next_item(cur)) break;
         __syncthreads();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
