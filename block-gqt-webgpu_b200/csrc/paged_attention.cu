@@ -164,40 +164,42 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
         return n < 0 ? 0 : (int32_t)min((uint32_t)n, a.width << shift);
     };
     // ---- the deal ----
-    auto block_sum = [&](uint64_t x) {
-        uint64_t *part = reinterpret_cast<uint64_t *>(sums), all = 0;
+    // (every warp for itself: lanes over the requests, sums by shuffles, no barrier)
+    auto warp_sum = [](uint64_t x) {
 #pragma unroll
         for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        if (lane == 0) part[warp] = x;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) all += part[w];
-        __syncthreads();
-        return all;
+        return x;
     };
-    uint64_t mine = 0;
-    for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
+    uint64_t all_units = 0;
+    bool past_table = false;
+#pragma unroll 4
+    for (uint32_t b = lane; b < a.batch; b += 32) {
         const int32_t n = length(b);
-        if (n != __ldg(a.lengths + b) && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
-        mine += (uint32_t)(n + T - 1) / T;
+        past_table |= n != __ldg(a.lengths + b);
+        all_units += (uint32_t)(n + T - 1) / T;
     }
-    const uint64_t all_units = block_sum(mine) * pairs;
-    // a request whose quad of pairs is within a CTA's share of the units goes by quads
-    const uint64_t share = all_units / gridDim.x;
+    if (past_table && blockIdx.x == 0 && warp == 0) atomicOr(a.status, kStatusBadExtent);
+    all_units = warp_sum(all_units) * pairs;
+    // A request goes by quads if a quad of its pairs is within a CTA's share of the units, or if
+    // it has two units or less, where a pair spread over four warps gains nothing.
+    const uint32_t quad_units = (uint32_t)max((uint64_t)2, min(all_units / gridDim.x / 4, (uint64_t)1 << 30));
     auto plan = [&](Cursor &c) {  // from c.b and c.len
         c.units = (uint32_t)(c.len + T - 1) / T;
-        c.quad = pairs > 1 && 4ull * c.units <= share;
+        c.quad = pairs > 1 && c.units <= quad_units;
         c.items = c.len == 0 ? 0 : c.quad ? (pairs + 3) / 4 : pairs;
         c.weight = (c.quad ? 4 * c.units : c.units) + kItemCost;
     };
-    mine = 0;
-    for (uint32_t b = threadIdx.x; b < a.batch; b += kThreads) {
+    uint64_t total = 0, all_items = 0;
+#pragma unroll 4
+    for (uint32_t b = lane; b < a.batch; b += 32) {
         Cursor c;
         c.len = length(b);
         plan(c);
-        mine += (uint64_t)c.items * c.weight;
+        all_items += c.items;
+        total += (uint64_t)c.items * c.weight;
     }
-    const uint64_t total = block_sum(mine);
+    total = warp_sum(total);
+    all_items = warp_sum(all_items);
     // a request without tokens: zeros
     for (uint32_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
         if (length(b) != 0) continue;
@@ -206,10 +208,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
         if (a.lse)
             for (uint32_t i = threadIdx.x; i < a.q_heads; i += kThreads) a.lse[(uint64_t)b * a.q_heads + i] = -INFINITY;
     }
-    const uint64_t most = (all_units + kWarps - 1) / kWarps;
-    const uint64_t ctas = most < gridDim.x ? most : gridDim.x;
+    // as many CTAs as there are items, or rounds of four units
+    const uint64_t most = max(all_items, all_units / kWarps);
+    const uint32_t ctas = (uint32_t)min(most, (uint64_t)gridDim.x);
     if (blockIdx.x >= ctas) return;
-    const uint64_t first = (uint64_t)blockIdx.x * total / ctas, last = (uint64_t)(blockIdx.x + 1) * total / ctas;
+    // equal ranges: the first `over` CTAs have one place more
+    const uint64_t each = total / ctas, over = total - each * ctas;
+    const uint64_t first = blockIdx.x * each + min((uint64_t)blockIdx.x, over);
+    const uint64_t last = first + each + (blockIdx.x < over ? 1 : 0);
+    auto owner = [&](uint64_t place) {
+        const uint64_t head = over * (each + 1);
+        return (uint32_t)(place < head ? place / (each + 1) : over + (place - head) / each);
+    };
     // this CTA's share of the item: a unit, or a quad, belongs to the CTA whose range holds its place
     auto take = [&](Cursor &c) {
         if (c.quad) {
@@ -281,7 +291,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
     auto settle = [&]() {  // moves `pre` to the warp's next unit, if there is one, and loads its page indices
         while (more && pre_unit >= pre.end) {
             more = next_item(pre);
-            if (more) pre_unit = unit0(pre);
+            if (!more) break;
+            pre_unit = unit0(pre);
+            // its queries, which are loaded when the ring gets there
+            const uint32_t p = pair_of(pre), h = p % blocks * S::kHeads + lane / 2;
+            if (p < pairs && lane / 2 < (uint32_t)S::kHeads && h < a.group) {
+                const uint16_t *at = static_cast<const uint16_t *>(a.q) + (int64_t)pre.b * a.q_batch +
+                                     (int64_t)(p / blocks * a.group + h) * a.q_head + (lane & 1u) * (D / 2);
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+            }
         }
         if (more) {
             const uint32_t t = pre_unit * T + (lane << shift);
@@ -354,22 +372,54 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                 const uint32_t h = n * 8 + row4;
                 const int64_t at = (int64_t)cur.b * a.q_batch + (int64_t)(head0 + h) * a.q_head;
                 big[n] = 0.0f;
+                uint16_t raw[KS][4];  // slot (s, e): in the order in which the key words hold the dimensions
+                if (h >= heads) {
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) raw[s][0] = raw[s][1] = raw[s][2] = raw[s][3] = 0;
+                } else if (a.q_even) {
+                    const uint16_t *src = static_cast<const uint16_t *>(a.q) + at;
+                    if constexpr (F >= F_INT8) {
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j) {  // eight dimensions a load
+                            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(
+                                src + (F == F_INT8 ? 64 * (j / 2) + 16 * col4 + 8 * (j % 2) : 32 * j + 8 * col4)));
+                            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const uint16_t v = (uint16_t)(w[k / 2] >> 16 * (k & 1));
+                                if constexpr (F == F_INT8) raw[2 * j + k / 4][k % 4] = v;
+                                else raw[2 * j + k % 4 / 2][k / 4 + 2 * (k & 1)] = v;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < KS; ++s)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t x = __ldg(reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * col4 + 8 * e));
+                                raw[s][2 * e] = (uint16_t)x;
+                                raw[s][2 * e + 1] = (uint16_t)(x >> 16);
+                            }
+                    }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            int d;
+                            if constexpr (F == F_INT8) d = 64 * (s / 4) + 16 * col4 + 4 * (s % 4) + e;
+                            else if constexpr (F == F_INT4)
+                                d = 32 * (s / 2) + 8 * col4 + 2 * (s % 2) + (e & 1) * 4 + (e >> 1);
+                            else d = 16 * s + 2 * col4 + (e & 1) + 8 * (e >> 1);
+                            raw[s][e] = static_cast<const uint16_t *>(a.q)[at + d];
+                        }
+                }
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        int d;  // the dimension in slot (s, e) of this thread, in the order of the key words
-                        if constexpr (F == F_INT8) d = 64 * (s / 4) + 16 * col4 + 4 * (s % 4) + e;
-                        else if constexpr (F == F_INT4)
-                            d = 32 * (s / 2) + 8 * col4 + 2 * (s % 2) + (e & 1) * 4 + (e >> 1);
-                        else d = 16 * s + 2 * col4 + (e & 1) + 8 * (e >> 1);
-                        float v = 0.0f;
-                        if (h < heads)
-                            v = a.dtype == BGTQ_F16
-                                    ? __half2float(static_cast<const __half *>(a.q)[at + d])
-                                    : __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[at + d]);
-                        x[n][s][e] = v;
-                        big[n] = fmaxf(big[n], fabsf(v));
+                        x[n][s][e] = a.dtype == BGTQ_F16 ? __half2float(__ushort_as_half(raw[s][e])) : from_bf16(raw[s][e]);
+                        big[n] = fmaxf(big[n], fabsf(x[n][s][e]));
                     }
             }
 #pragma unroll
@@ -694,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
         const bool whole = cur.at == 0 && cur.end == cur.units;
         // the CTAs that hold its first and its last unit
         const uint64_t from = cur.base + kItemCost;
-        const uint64_t c_first = ((from + 1) * ctas - 1) / total, c_last = ((from + cur.units) * ctas - 1) / total;
+        const uint32_t c_first = whole ? 0 : owner(from), c_last = whole ? 0 : owner(from + cur.units - 1);
         // at most one pair that is not whole begins in a CTA's range: its counter is that CTA's
         uint32_t *counter = static_cast<uint32_t *>(a.workspace) + c_first;
         float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters);
@@ -728,8 +778,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
             __syncthreads();
             if (threadIdx.x == 0) {
                 const uint32_t n = atomicAdd(counter, 1u);
-                flags[kWarps * 4] = n == (uint32_t)(c_last - c_first);
-                if (n == (uint32_t)(c_last - c_first)) *counter = 0;
+                flags[kWarps * 4] = n == c_last - c_first;
+                if (n == c_last - c_first) *counter = 0;
             }
             __syncthreads();
             if (flags[kWarps * 4]) {
@@ -737,8 +787,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                 for (uint32_t i = threadIdx.x; i < heads * (D / 2); i += kThreads) {
                     const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
                     float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
-                    for (uint64_t c = c_first; c <= c_last; ++c) {
-                        const float *p = parts + (2 * c + (c == c_first ? 1 : 0)) * S::kPartFloats;
+                    for (uint32_t c = c_first; c <= c_last; ++c) {
+                        const float *p = parts + (2ull * c + (c == c_first ? 1 : 0)) * S::kPartFloats;
                         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + S::kHeads * D + 2 * head));
                         const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + head * D + d));
                         const float now = fmaxf(big, ml.x), ref = now == -INFINITY ? 0.0f : now;
@@ -788,6 +838,7 @@ cudaError_t run(const PagedAttendArgs &a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     PagedAttendArgs b = a;
     b.counters = counter_bytes();
+    b.q_even = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_batch % 8 == 0 && a.q_head % 8 == 0;
     kernel<<<(uint32_t)(sms * resident[dev]), kThreads, S::kSmem, s>>>(b);
     return cudaGetLastError();
 }

@@ -56,7 +56,8 @@ struct PagedAttendArgs {
     float *lse;  // nullable
     void *workspace;
     uint32_t batch, q_heads, group, width;
-    uint32_t counters;  // bytes of the workspace's counters (the launcher's)
+    uint32_t counters;  // the launcher's: bytes of the workspace's counters
+    uint32_t q_even;    // the launcher's: query rows are 16-byte aligned
     float scale;  // of the logits, times log2(e)
     bgtq_dtype dtype;
     uint32_t *status;
