@@ -1,7 +1,28 @@
-// Attention of a packed batch of prompts of different lengths: row i of sequence s attends
-// keys j of the same sequence, with the causal mask j <= i + (keys - queries), softmax with a
-// running maximum and sum (FP32).  A row that sees no key gives zeros and a log sum of minus
-// infinity.
+// Attention of a packed batch of prompts of different lengths on the fifth-generation tensor
+// cores: row i of sequence s attends keys j of the same sequence, with the causal mask
+// j <= i + (keys - queries), softmax with a running maximum and sum (FP32).  A row that sees
+// no key gives zeros and a log sum of minus infinity.
+//
+// A work item is a block of consecutive positions of one sequence with all query heads of one
+// KV head: 128 rows a tile, floor(128 / group) positions x group heads, two tiles an item (one
+// where there are few items), which share every K and V tile of 128 keys.  A CTA takes items
+// until none is left.  Its twelve warps have roles:
+//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, a thread a row: logits out of tensor memory,
+//                   mask, running maximum, probabilities back into tensor memory (as 16-bit
+//                   pairs in the columns where the logits were), and the output at the end
+//   warp 8          TMA loads of Q, K and V (128-byte swizzle) into a ring of K / V tiles
+//   warp 9          the products, one thread: S = Q K^T (operands in shared memory) and
+//                   O += P V (P in tensor memory, V as it lies), FP32 accumulators in
+//                   tensor memory; while one tile's logits are in softmax, the other's products run
+//   warp 10         the deal: items in order of falling length, dealt back and forth over the CTAs
+//   warp 11         V tiles at a sequence's end or on the diagonal, before they are multiplied:
+//                   rows past the end (another sequence's, or nothing) are zeroed, and an
+//                   infinity or a NaN, which the zero probability of a row that does not see
+//                   it would turn into a NaN, is taken out and given to the rows that do see it
+// The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the
+// last time: until then probabilities are taken relative to the older maximum, so they stay
+// below 2^8, and P is FP16 or BF16 (the inputs' type) with the same relative error.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -11,71 +32,662 @@ namespace bgtq {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kThreads = 384, kRows = 128, kKeys = 128;
+constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
+constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
-__device__ __forceinline__ float as_float(const void *p, int64_t i, bgtq_dtype t) {
-    return t == BGTQ_F16 ? __half2float(static_cast<const __half *>(p)[i])
-                         : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+// ---- device helpers -----------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t n) {
+    asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+// Waits for the phase of `parity`, for a bounded number of polls.  False: it ran out, or another
+// role's did (`stop`).
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *stop) {
+    for (uint32_t i = 0; i < 1u << 22; ++i) {
+        if (bar_try(bar, parity)) return true;
+        if ((i & 63u) == 63u && *stop) return false;
+    }
+    *stop = 1;
+    return false;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *stop) {
+    if (bar_try(bar, parity)) return true;
+    return bar_wait_slow(bar, parity, stop);
+}
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+                 "[%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A shared-memory operand: 128-byte swizzle, 8-row groups 1024 bytes apart, `lbo` between
+// 64-element column blocks of an operand whose rows run along the contraction.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)((lbo >> 4) & 0x3fffu) << 16 | (uint64_t)(1024u >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16, FP32 accumulators, M = 128: the operands' type, whether B's rows run along the contraction, N.
+__host__ __device__ constexpr uint32_t product(bool bf16, uint32_t b_rows, uint32_t n) {
+    return (1u << 4) | (bf16 ? 1u << 7 | 1u << 10 : 0u) | b_rows << 16 | (n >> 3) << 17 | (kRows >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
+                 : "memory");
+}
+#define BGTQ_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define BGTQ_V8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 columns of this thread's lane of tensor memory.
+__device__ __forceinline__ void tm_load(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                 "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : BGTQ_R8(r, 0), BGTQ_R8(r, 8), BGTQ_R8(r, 16), BGTQ_R8(r, 24) : "r"(at));
+}
+__device__ __forceinline__ void tm_store(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+                 ::BGTQ_V8(r, 0), BGTQ_V8(r, 8), BGTQ_V8(r, 16), BGTQ_V8(r, 24), "r"(at) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
 }
 
-// One warp per (token, query head), its lanes over the head's dimensions.
+// ---- shared memory ---------------------------------------------------------------------------
+
 template <int D>
-__global__ void __launch_bounds__(128) prompt_kernel(const PromptArgs a) {
-    constexpr int N = D / 32;
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= a.q_tokens * a.q_heads) return;
-    const int64_t t = (int64_t)(row / a.q_heads);
-    const uint32_t h = (uint32_t)(row % a.q_heads), kh = h / a.group;
-    // the sequence that holds token t; one whose starts fall or pass the token counts holds none
-    int64_t q0 = 0, k0 = 0, nq = 0, nk = 0, seen = 0;
-    for (uint32_t i = 0; i < a.sequences; ++i) {
-        const int64_t q_at = a.starts[i], k_at = a.key_starts[i];
-        const int64_t n = (int64_t)a.starts[i + 1] - q_at, m = (int64_t)a.key_starts[i + 1] - k_at;
-        if (q_at < 0 || k_at < 0 || n < 0 || m < 0 || q_at + n > (int64_t)a.q_tokens || k_at + m > (int64_t)a.k_tokens) {
-            if (row == 0 && lane == 0) atomicOr(a.status, kStatusBadExtent);
-        } else if (t >= q_at && t < q_at + n) {
-            q0 = q_at, k0 = k_at, nq = n, nk = m, seen = m;
+struct Plan {
+    static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
+    static constexpr uint32_t kChunk = kRows * 128;                // bytes: 128 rows of 64 16-bit elements
+    static constexpr uint32_t kTile = kChunks * kChunk;
+    static constexpr uint32_t kSlots = D == 128 ? 4 : 8;           // K and V tiles in the ring
+    static constexpr uint32_t kQ = 0, kRing = 2 * kTile, kAfter = kRing + kSlots * kTile;
+    static constexpr uint32_t kBad = kAfter;                       // [2 items][3 kinds][D] first keys
+    static constexpr uint32_t kItems = kBad + 2 * 3 * D * 2;       // [2] Item
+    static constexpr uint32_t kBars = kItems + 2 * 32;
+    static constexpr uint32_t kBarCount = 3 * kSlots + 15;
+    static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
+    static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
+};
+
+struct Item {
+    int32_t token, count;  // first query row, positions (0: no more items)
+    int32_t pos, head;     // first position in the sequence, KV head
+    int32_t key, keys;     // first key row, the sequence's keys
+    int32_t shift;         // keys - queries
+    int32_t pad;
+};
+
+struct TileSpan {
+    int32_t count, tiles, first;  // positions, key tiles, keys that the first row sees
+};
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a,
+                                                             const __grid_constant__ CUtensorMap mq,
+                                                             const __grid_constant__ CUtensorMap mk,
+                                                             const __grid_constant__ CUtensorMap mv) {
+    using P = Plan<D>;
+    extern __shared__ unsigned char raw[];
+    unsigned char *sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_addr(sm), warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint16_t *bad = reinterpret_cast<uint16_t *>(sm + P::kBad);
+    volatile Item *items = reinterpret_cast<volatile Item *>(sm + P::kItems);
+    volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(sm + P::kWords);
+    volatile uint32_t *stop = words + 1, *bad_flag = words + 2;  // bad_flag[2]
+    const uint32_t bars = base + P::kBars;
+    auto bar = [&](uint32_t i) { return bars + 8u * i; };
+    constexpr uint32_t B_FULL = 0, B_FREE = P::kSlots, B_QFULL = 2 * P::kSlots, B_QFREE = B_QFULL + 2, B_S = B_QFREE + 2,
+                       B_P = B_S + 2, B_O = B_P + 2, B_RAW = B_O + 2, B_ITEM = B_RAW + P::kSlots, B_TAKEN = B_ITEM + 2, B_END = B_TAKEN + 2;
+    const uint32_t per = kRows / a.group;  // positions of a tile
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(base + P::kWords) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < P::kSlots; ++i) {
+            bar_init(bar(B_FULL + i), 1);
+            bar_init(bar(B_FREE + i), 1);
+            bar_init(bar(B_RAW + i), 1);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            bar_init(bar(B_QFULL + i), 1);
+            bar_init(bar(B_QFREE + i), 1);
+            bar_init(bar(B_S + i), 1);
+            bar_init(bar(B_P + i), 4);
+            bar_init(bar(B_O + i), 1);
+            bar_init(bar(B_ITEM + i), 1);
+            bar_init(bar(B_TAKEN + i), 11);
+        }
+        bar_init(bar(B_END), 1);
+        words[1] = words[2] = words[3] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async();
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = words[0];
+
+    // a whole warp's wait: all of its lanes see the same answer
+    auto all_wait = [&](uint32_t b, uint32_t parity) { return (bool)__all_sync(0xffffffffu, bar_wait(b, parity, stop)); };
+    // The item in slot n & 1 of the deal, when it is there; a role gives it back with `taken`.
+    auto next = [&](uint32_t n, Item &it) {
+        if (!all_wait(bar(B_ITEM + (n & 1)), (n >> 1) & 1)) return false;
+        const volatile Item &s = items[n & 1];
+        it.token = s.token, it.count = s.count, it.pos = s.pos, it.head = s.head;
+        it.key = s.key, it.keys = s.keys, it.shift = s.shift;
+        return it.count != 0;
+    };
+    auto taken = [&](uint32_t n) {
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(B_TAKEN + (n & 1)));
+    };
+    auto span = [&](const Item &it, int t) {
+        TileSpan s;
+        const int32_t at = t * (int32_t)per;
+        s.count = max(0, min((int32_t)per, it.count - at));
+        const int32_t from = it.pos + at + it.shift + 1;  // keys that the first row sees, if causal
+        const int32_t upto = a.causal ? max(0, min(it.keys, from + s.count - 1)) : it.keys;
+        s.tiles = s.count ? (upto + (int32_t)kKeys - 1) / (int32_t)kKeys : 0;
+        s.first = a.causal ? max(0, min(it.keys, from)) : it.keys;
+        return s;
+    };
+
+    if (warp < 8) {
+        // ---- softmax: thread = row of tile t ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int t = warp >> 2;
+        const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
+        const uint32_t lanes = (warp & 3u) * 32u << 16;
+        const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
+        uint32_t phase_s = 0, phase_o = 0;
+        Item it;
+        for (uint32_t n = 0; next(n, it); ++n) {
+            const TileSpan sp = span(it, t);
+            const bool live = p < (uint32_t)sp.count;
+            int32_t sees = it.keys;
+            if (a.causal) sees = max(0, min(it.keys, it.pos + t * (int32_t)per + (int32_t)p + it.shift + 1));
+            float ref = -INFINITY, sum = 0.0f;  // the maximum that probabilities are relative to (log2 units)
+            bool fine = true;
+            for (int32_t j = 0; j < sp.tiles; ++j) {
+                if (!(fine = all_wait(bar(B_S + t), phase_s))) break;
+                phase_s ^= 1;
+                tc_after();
+                uint32_t x[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tm_load(ts + 32 * c, x + 32 * c);
+                tc_wait_ld();
+                float *s = reinterpret_cast<float *>(x);
+                if ((j + 1) * (int32_t)kKeys > sp.first) {
+                    const int32_t left = sees - j * (int32_t)kKeys;
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i >= left) s[i] = -INFINITY;
+                }
+                float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+                for (int i = 4; i < 128; i += 4) {
+                    m0 = fmaxf(m0, s[i]);
+                    m1 = fmaxf(m1, s[i + 1]);
+                    m2 = fmaxf(m2, s[i + 2]);
+                    m3 = fmaxf(m3, s[i + 3]);
+                }
+                const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.scale;
+                if (j == 0) ref = top;
+                else if (__any_sync(0xffffffffu, top > ref + kLazy)) {
+                    const float now = fmaxf(ref, top), f = now == -INFINITY ? 1.0f : ex2(ref - now);
+                    ref = now;
+                    sum *= f;
+                    // the products of the last tile are done: S of this one was issued after them
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tm_load(to + 32 * c, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tm_store(to + 32 * c, o);
+                    }
+                }
+                const float from = ref == -INFINITY ? 0.0f : ref;
+                float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 128; i += 2) {
+                    const float e0 = ex2(fmaf(s[i], a.scale, -from)), e1 = ex2(fmaf(s[i + 1], a.scale, -from));
+                    l0 += e0;
+                    l1 += e1;
+                    x[i / 2] = pack<BF>(e0, e1);
+                }
+                sum += l0 + l1;
+                tm_store(ts, x);
+                tm_store(ts + 32, x + 32);
+                tc_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(bar(B_P + t));
+            }
+            if (fine && sp.count) {
+                if (sp.tiles) {
+                    if (!(fine = all_wait(bar(B_O + t), phase_o))) break;
+                    phase_o ^= 1;
+                    tc_after();
+                }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const uint32_t flagged = bad_flag[n & 1];
+                const uint64_t at = (uint64_t)(it.token + t * (int32_t)per + (int32_t)p) * a.q_heads + it.head * a.group + g;
+                uint16_t *out = static_cast<uint16_t *>(a.out) + at * D;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    if (sp.tiles) {
+                        tm_load(to + 32 * c, o);
+                        tc_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0;
+                    }
+                    if (sees == 0) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0;
+                    }
+                    if (flagged) {
+                        // infinities and NaN that this row sees: keys from `key0` on were looked through
+                        const int32_t key0 = max(0, (span(it, 0).first / (int32_t)kKeys)) * (int32_t)kKeys;
+                        const uint16_t *first = bad + (n & 1) * 3 * D + 32 * c;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
+                            if (key0 + first[2 * D + i] < sees || (up && down)) o[i] = 0x7fc00000u;
+                            else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
+                        }
+                    }
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 v;
+                            v.x = pack<BF>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                            v.y = pack<BF>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                            v.z = pack<BF>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                            v.w = pack<BF>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                            *reinterpret_cast<uint4 *>(out + 32 * c + i) = v;
+                        }
+                    }
+                }
+                if (live && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                tc_before();
+            }
+            if (!fine) break;
+            taken(n);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ---- loads ----
+            // A tile that warp 11 looks through lands on its slot's raw barrier, and warp 11 arrives on the
+            // full one when it is done with it.
+            uint32_t slot = 0, free_phase = 1, q_phase[2] = {1, 1}, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
+            Item it;
+            bool fine = true;
+            for (uint32_t n = 0; fine && next(n, it); ++n) {
+                const TileSpan s0 = span(it, 0), s1 = span(it, 1);
+                const int32_t tiles = max(s0.tiles, s1.tiles);
+                if (lane == 0) {
+                    auto load_q = [&](int t) {
+                        if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase[t], stop))) return;
+                        q_phase[t] ^= 1;
+                        bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+                            tma3(base + P::kQ + t * P::kTile + c * P::kChunk, &mq, bar(B_QFULL + t), 64 * c,
+                                 it.head * (int32_t)a.group, it.token + t * (int32_t)per);
+                    };
+                    auto load_kv = [&](const CUtensorMap *map, int32_t j, bool look) {
+                        if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
+                        const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
+                        bar_expect(on, P::kTile);
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+                            tma3(base + P::kRing + slot * P::kTile + c * P::kChunk, map, on, 64 * c, it.head,
+                                 it.key + j * (int32_t)kKeys);
+                        issued |= bit;
+                        raw = look ? raw | bit : raw & ~bit;
+                        full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
+                        raw_phase ^= look ? bit : 0;
+                        if (++slot == P::kSlots) slot = 0, free_phase ^= 1;
+                    };
+                    if (s0.tiles) load_q(0);
+                    if (tiles) load_kv(&mk, 0, false);
+                    if (s1.tiles) load_q(1);
+                    for (int32_t j = 0; j < tiles && fine; ++j) {
+                        load_kv(&mv, j, (j + 1) * (int32_t)kKeys > s0.first);
+                        if (j + 1 < tiles) load_kv(&mk, j + 1, false);
+                    }
+                }
+                fine = __shfl_sync(0xffffffffu, fine, 0);
+                taken(n);
+            }
+            // copies in flight land before the CTA ends (they have, unless a wait ran out)
+            if (lane == 0 && *stop) {
+                uint32_t none = 0;
+                for (uint32_t i = 0; i < P::kSlots; ++i)
+                    if (issued >> i & 1u)
+                        bar_wait(bar((raw >> i & 1u ? B_RAW : B_FULL) + i), raw >> i & 1u ? ~raw_phase >> i & 1u : full_phase >> i & 1u,
+                                 &none);
+                for (int t = 0; t < 2; ++t) bar_wait(bar(B_QFULL + t), q_phase[t] ^ 1u, &none);
+            }
+        } else if (warp == 9) {
+            // ---- products ----
+            uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;
+            constexpr uint32_t ID_S = product(BF, 0, kKeys), ID_O = product(BF, 1, D);
+            Item it;
+            bool fine = true;
+            for (uint32_t n = 0; fine && next(n, it); ++n) {
+                const TileSpan sp[2] = {span(it, 0), span(it, 1)};
+                const int32_t tiles = max(sp[0].tiles, sp[1].tiles);
+                if (lane == 0) {
+                    auto advance = [&]() {
+                        if (++slot == P::kSlots) slot = 0, full_phase ^= 1;
+                    };
+                    auto logits = [&](int t, uint32_t k, bool end) {
+                        const uint32_t q_at = base + P::kQ + t * P::kTile, k_at = base + P::kRing + k * P::kTile;
+#pragma unroll
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+#pragma unroll
+                            for (uint32_t s = 0; s < 4; ++s)
+                                mma_ss(tmem + t * 128, operand(q_at + c * P::kChunk + 32 * s, 0),
+                                       operand(k_at + c * P::kChunk + 32 * s, 0), ID_S, c | s);
+                        tc_commit(bar(B_S + t));
+                        if (end) tc_commit(bar(B_QFREE + t));
+                    };
+                    // the first logits of both tiles
+                    uint32_t k = slot;
+                    if (tiles) {
+                        for (int t = 0; t < 2 && fine; ++t) {
+                            if (!sp[t].tiles) continue;
+                            if (!(fine = bar_wait(bar(B_QFULL + t), q_phase >> t & 1u, stop))) break;
+                            q_phase ^= 1u << t;
+                            if (!(fine = bar_wait(bar(B_FULL + k), full_phase, stop))) break;
+                            tc_after();
+                            logits(t, k, sp[t].tiles == 1);
+                        }
+                        if (fine) tc_commit(bar(B_FREE + k));
+                        advance();
+                    }
+                    for (int32_t j = 0; j < tiles && fine; ++j) {
+                        const uint32_t v = slot;
+                        if (!(fine = bar_wait(bar(B_FULL + v), full_phase, stop))) break;
+                        advance();
+                        k = slot;
+                        const bool more = j + 1 < tiles;
+                        for (int t = 0; t < 2; ++t) {
+                            if (j >= sp[t].tiles) continue;
+                            if (!(fine = bar_wait(bar(B_P + t), p_phase >> t & 1u, stop))) break;
+                            p_phase ^= 1u << t;
+                            tc_after();
+#pragma unroll
+                            for (uint32_t s = 0; s < 8; ++s)
+                                mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * s,
+                                       operand(base + P::kRing + v * P::kTile + s * 2048u, P::kChunk), ID_O, j | (int32_t)s);
+                            if (j + 1 < sp[t].tiles) {
+                                if (!(fine = bar_wait(bar(B_FULL + k), full_phase, stop))) break;
+                                tc_after();
+                                logits(t, k, j + 2 == sp[t].tiles);
+                            } else tc_commit(bar(B_O + t));
+                        }
+                        if (!fine) break;
+                        tc_commit(bar(B_FREE + v));
+                        if (more) {
+                            tc_commit(bar(B_FREE + k));
+                            advance();
+                        }
+                    }
+                }
+                fine = __shfl_sync(0xffffffffu, fine, 0);
+                taken(n);
+            }
+            // products in flight end before the tensor memory is given back
+            if (lane == 0 && *stop) {
+                uint32_t none = 0;
+                tc_commit(bar(B_END));
+                bar_wait(bar(B_END), 0, &none);
+            }
+        } else if (warp == 10) {
+            // ---- the deal ----
+            // Sequence s has ceil(queries / (tiles per item)) blocks; block b of every sequence that
+            // has it is level b.  Items go by falling level (the last blocks see the most keys), a level's
+            // sequences in order, KV heads innermost; item r goes to CTA r of a round, rounds back and forth.
+            const int32_t block = (int32_t)(a.tiles * per);
+            auto blocks_of = [&](uint32_t s) -> int32_t {
+                if (s >= a.sequences) return 0;
+                const int32_t q0 = __ldg(a.starts + s), q1 = __ldg(a.starts + s + 1);
+                const int32_t k0 = __ldg(a.key_starts + s), k1 = __ldg(a.key_starts + s + 1);
+                if (q0 < 0 || k0 < 0 || q1 < q0 || k1 < k0 || (uint64_t)q1 > a.q_tokens || (uint64_t)k1 > a.k_tokens) {
+                    if (blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
+                    return 0;
+                }
+                return (q1 - q0 + block - 1) / block;
+            };
+            int32_t level = 0;
+            for (uint32_t s = lane; s < a.sequences; s += 32) level = max(level, blocks_of(s));
+            level = __reduce_max_sync(0xffffffffu, level);
+            uint64_t before = 0, upto = 0;  // items of levels above this one, and with it
+            uint64_t r = blockIdx.x;
+            for (uint32_t n = 0;; ++n) {
+                r = (uint64_t)n * gridDim.x + (n & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                while (upto <= r && level > 0) {
+                    --level;
+                    before = upto;
+                    uint32_t c = 0;
+                    for (uint32_t s = lane; s < a.sequences; s += 32) c += blocks_of(s) > level;
+                    upto += (uint64_t)__reduce_add_sync(0xffffffffu, c) * a.kv_heads;
+                }
+                Item it{};
+                if (r < upto) {
+                    uint32_t nth = (uint32_t)((r - before) / a.kv_heads);
+                    it.head = (int32_t)((r - before) % a.kv_heads);
+                    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 32) {
+                        const uint32_t has = __ballot_sync(0xffffffffu, blocks_of(s0 + lane) > level);
+                        const uint32_t c = __popc(has);
+                        if (nth >= c) {
+                            nth -= c;
+                            continue;
+                        }
+                        const uint32_t s = s0 + __fns(has, 0, nth + 1);
+                        const int32_t q0 = __ldg(a.starts + s), nq = __ldg(a.starts + s + 1) - q0;
+                        it.pos = level * block;
+                        it.token = q0 + it.pos;
+                        it.count = min(block, nq - it.pos);
+                        it.key = __ldg(a.key_starts + s);
+                        it.keys = __ldg(a.key_starts + s + 1) - it.key;
+                        it.shift = it.keys - nq;
+                        break;
+                    }
+                }
+                if (n >= 2 && !all_wait(bar(B_TAKEN + (n & 1)), ((n >> 1) & 1) ^ 1)) break;
+                if (lane == 0) {
+                    volatile Item &d = items[n & 1];
+                    d.token = it.token, d.count = it.count, d.pos = it.pos, d.head = it.head;
+                    d.key = it.key, d.keys = it.keys, d.shift = it.shift;
+                    bad_flag[n & 1] = 0;
+                    bar_arrive(bar(B_ITEM + (n & 1)));
+                }
+                __syncwarp();
+                if (it.count == 0) break;
+            }
+        } else {
+            // ---- V tiles that not every row sees ----
+            uint32_t slot = 0, raw_phase = 0;
+            Item it;
+            bool fine = true;
+            for (uint32_t n = 0; fine && next(n, it); ++n) {
+                const TileSpan s0 = span(it, 0), s1 = span(it, 1);
+                const int32_t tiles = max(s0.tiles, s1.tiles), begin = max(0, s0.first / (int32_t)kKeys);
+                uint16_t *first = bad + (n & 1) * 3 * D;
+                bool cleared = false;
+                for (int32_t j = 0; j < tiles; ++j) {
+                    const uint32_t v = slot + 1;  // K tiles in even slots, V tiles in odd ones
+                    slot = slot + 2 == P::kSlots ? 0 : slot + 2;
+                    if ((j + 1) * (int32_t)kKeys <= s0.first) continue;
+                    if (!(fine = all_wait(bar(B_RAW + v), raw_phase >> v & 1u))) break;
+                    raw_phase ^= 1u << v;
+                    unsigned char *tile = sm + P::kRing + v * P::kTile;
+                    const int32_t rows = min((int32_t)kKeys, it.keys - j * (int32_t)kKeys);
+                    uint32_t found = 0;
+                    for (uint32_t c = 0; c < P::kChunks; ++c)
+#pragma unroll 4
+                        for (uint32_t i = lane; i < kKeys * 8; i += 32) {
+                            uint4 *w = reinterpret_cast<uint4 *>(tile + c * P::kChunk + i * 16);
+                            if ((int32_t)(i >> 3) >= rows) *w = make_uint4(0, 0, 0, 0);
+                            else {
+                                const uint4 x = *w;
+                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                                    found |= (y[k] & E) == E || (y[k] >> 16 & E) == E;
+                                }
+                            }
+                        }
+                    if (__any_sync(0xffffffffu, found)) {
+                        if (!cleared) {
+                            for (uint32_t i = lane; i < 3 * D; i += 32) first[i] = 0xffff;
+                            cleared = true;
+                        }
+                        __syncwarp();
+                        for (uint32_t d = lane; d < (uint32_t)D; d += 32)
+                            for (int32_t k = 0; k < rows; ++k) {
+                                uint16_t *w = reinterpret_cast<uint16_t *>(tile + d / 64 * P::kChunk + k * 128 +
+                                                                           (((d % 64 / 8) ^ (k & 7)) << 4)) + d % 8;
+                                constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
+                                const uint32_t x = *w;
+                                if ((x & E) != E) continue;
+                                *w = 0;
+                                const uint32_t kind = (x & 0x7fffu) != E ? 2 : x >> 15;  // 0 inf, 1 -inf, 2 NaN
+                                const uint32_t at = (uint32_t)((j - begin) * (int32_t)kKeys + k);
+                                if (at < first[kind * D + d]) first[kind * D + d] = (uint16_t)at;
+                            }
+                        __syncwarp();
+                        if (lane == 0) bad_flag[n & 1] = 1;
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar(B_FULL + v));
+                }
+                taken(n);
+            }
         }
     }
-    if (nq == 0) return;
-    if (a.causal) seen = min(seen, max((int64_t)0, t - q0 + 1 + nk - nq));
-    float q[N], o[N] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) q[i] = as_float(a.q, t * a.q_token + (int64_t)h * a.q_head + 32 * i + lane, a.dtype);
-    for (int64_t j = k0; j < k0 + seen; ++j) {
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            s = fmaf(q[i], as_float(a.k, j * a.k_token + (int64_t)kh * a.k_head + 32 * i + lane, a.dtype), s);
-#pragma unroll
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.scale;
-        const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-        const float old = exp2f(m - ref), p = exp2f(s - ref);
-        m = mn;
-        l = fmaf(l, old, p);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            o[i] = fmaf(p, as_float(a.v, j * a.v_token + (int64_t)kh * a.v_head + 32 * i + lane, a.dtype), o[i] * old);
+    // every role has left its loop; on a timeout the waits above were cut short
+    __syncwarp();
+    tc_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *stop) atomicOr(a.status, kStatusTimeout);
+    if (warp == 8) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint64_t at = row * D + 32 * i + lane;
-        if (a.dtype == BGTQ_F16) static_cast<__half *>(a.out)[at] = __float2half_rn(o[i] * inv);
-        else static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(o[i] * inv);
+}
+
+// ---- launch ------------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+    static const EncodeTiled f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+
+// [tokens][heads][dim] as boxes of `rows` tokens x `heads_box` heads x 64 dimensions.
+bool make_map(CUtensorMap *m, bool bf16, const void *p, uint32_t dim, uint32_t heads, uint64_t tokens, int64_t head,
+              int64_t token, uint32_t heads_box, uint32_t rows) {
+    const cuuint64_t size[3] = {dim, heads, tokens};
+    const cuuint64_t stride[2] = {(cuuint64_t)head * 2, (cuuint64_t)token * 2};
+    const cuuint32_t box[3] = {64, heads_box, rows}, step[3] = {1, 1, 1};
+    return encoder()(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(p),
+                     size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF>
+cudaError_t run(const PromptArgs &args, cudaStream_t s) {
+    using P = Plan<D>;
+    if (!encoder()) return cudaErrorNotSupported;
+    auto kernel = prompt_kernel<D, BF>;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    static bool ready[64] = {};
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kTotal);
+        if (e != cudaSuccess) return e;
+        ready[dev] = true;
     }
-    if (a.lse && lane == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    PromptArgs a = args;
+    const uint32_t per = kRows / a.group;
+    CUtensorMap mq, mk, mv;
+    // without any key nothing is loaded; the maps only have to be valid
+    const bool keys = a.k_tokens != 0;
+    if (!make_map(&mq, BF, a.q, D, a.q_heads, a.q_tokens, a.q_head, a.q_token, a.group, per) ||
+        !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, kKeys) ||
+        !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, kKeys))
+        return cudaErrorInvalidValue;
+    // two tiles an item share K and V loads; where that leaves SMs without work, one
+    const uint64_t items2 = a.kv_heads * ((a.q_tokens + 2 * per - 1) / (2 * per));
+    a.tiles = items2 >= (uint64_t)sms ? 2 : 1;
+    const uint64_t most = a.kv_heads * ((a.q_tokens + a.tiles * per - 1) / (a.tiles * per) + a.sequences);
+    kernel<<<(uint32_t)(most < (uint64_t)sms ? most : sms), kThreads, P::kTotal, s>>>(a, mq, mk, mv);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s) {
-    const uint64_t blocks = (a.q_tokens * a.q_heads + 3) / 4;
-    if (blocks > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-    if (a.dim == 64) prompt_kernel<64><<<(uint32_t)blocks, 128, 0, s>>>(a);
-    else prompt_kernel<128><<<(uint32_t)blocks, 128, 0, s>>>(a);
-    return cudaGetLastError();
+    if (a.dtype == BGTQ_BF16) return a.dim == 64 ? run<64, true>(a, s) : run<128, true>(a, s);
+    return a.dim == 64 ? run<64, false>(a, s) : run<128, false>(a, s);
 }
 
 }  // namespace bgtq

@@ -71,6 +71,7 @@ struct PromptArgs {
     float *lse;                           // [q_tokens][q_heads], nullable
     uint64_t q_tokens, k_tokens;
     uint32_t sequences, q_heads, kv_heads, group, dim;
+    uint32_t tiles;  // the launcher's: row tiles of a work item
     float scale;  // of the logits, times log2(e)
     int causal;
     bgtq_dtype dtype;
