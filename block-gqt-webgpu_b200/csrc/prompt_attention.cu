@@ -32,7 +32,7 @@ namespace bgtq {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kThreads = 384, kRows = 128, kKeys = 128;
+constexpr uint32_t kThreads = 384, kRows = 128;
 constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
@@ -71,6 +71,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
                  "[%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -113,6 +119,10 @@ __device__ __forceinline__ void tm_store(uint32_t at, const uint32_t *r) {
                  "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
                  ::BGTQ_V8(r, 0), BGTQ_V8(r, 8), BGTQ_V8(r, 16), BGTQ_V8(r, 24), "r"(at) : "memory");
 }
+__device__ __forceinline__ void tm_store16(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15};" ::BGTQ_V8(r, 0), BGTQ_V8(r, 8), "r"(at) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -133,15 +143,19 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {
 
 template <int D>
 struct Plan {
+    // Keys of a tile: as many as leave room for two tiles of logits and the outputs of both row
+    // tiles in the 512 columns of tensor memory.
+    static constexpr uint32_t kKeys = D == 128 ? 64 : 96;
+    static constexpr uint32_t kColO = 4 * kKeys;                   // the first column of the outputs
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
-    static constexpr uint32_t kChunk = kRows * 128;                // bytes: 128 rows of 64 16-bit elements
-    static constexpr uint32_t kTile = kChunks * kChunk;
-    static constexpr uint32_t kSlots = D == 128 ? 4 : 8;           // K and V tiles in the ring
-    static constexpr uint32_t kQ = 0, kRing = 2 * kTile, kAfter = kRing + kSlots * kTile;
+    static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
+    static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
+    static constexpr uint32_t kSlots = D == 128 ? 8 : 10;          // K and V tiles in the ring
+    static constexpr uint32_t kQ = 0, kRing = 2 * kQTile, kAfter = kRing + kSlots * kTile;
     static constexpr uint32_t kBad = kAfter;                       // [2 items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + 2 * 3 * D * 2;       // [2] Item
     static constexpr uint32_t kBars = kItems + 2 * 32;
-    static constexpr uint32_t kBarCount = 3 * kSlots + 15;
+    static constexpr uint32_t kBarCount = 3 * kSlots + 21;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
     static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
 };
@@ -164,9 +178,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                                              const __grid_constant__ CUtensorMap mk,
                                                              const __grid_constant__ CUtensorMap mv) {
     using P = Plan<D>;
+    constexpr int32_t kKeys = (int32_t)P::kKeys;
     extern __shared__ unsigned char raw[];
     unsigned char *sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-    const uint32_t base = smem_addr(sm), warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t base = smem_addr(sm), warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const uint32_t lane = threadIdx.x & 31u;
     uint16_t *bad = reinterpret_cast<uint16_t *>(sm + P::kBad);
     volatile Item *items = reinterpret_cast<volatile Item *>(sm + P::kItems);
     volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(sm + P::kWords);
@@ -174,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const uint32_t bars = base + P::kBars;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     constexpr uint32_t B_FULL = 0, B_FREE = P::kSlots, B_QFULL = 2 * P::kSlots, B_QFREE = B_QFULL + 2, B_S = B_QFREE + 2,
-                       B_P = B_S + 2, B_O = B_P + 2, B_RAW = B_O + 2, B_ITEM = B_RAW + P::kSlots, B_TAKEN = B_ITEM + 2, B_END = B_TAKEN + 2;
+                       B_P = B_S + 4, B_O = B_P + 4, B_RAW = B_O + 4, B_ITEM = B_RAW + P::kSlots, B_TAKEN = B_ITEM + 2, B_END = B_TAKEN + 2;
     const uint32_t per = kRows / a.group;  // positions of a tile
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(base + P::kWords) : "memory");
@@ -189,9 +205,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (uint32_t i = 0; i < 2; ++i) {
             bar_init(bar(B_QFULL + i), 1);
             bar_init(bar(B_QFREE + i), 1);
-            bar_init(bar(B_S + i), 1);
-            bar_init(bar(B_P + i), 4);
-            bar_init(bar(B_O + i), 1);
+            bar_init(bar(B_S + 2 * i), 1);
+            bar_init(bar(B_S + 2 * i + 1), 1);
+            bar_init(bar(B_P + 2 * i), 4);
+            bar_init(bar(B_P + 2 * i + 1), 4);
+            bar_init(bar(B_O + 2 * i), 1);
+            bar_init(bar(B_O + 2 * i + 1), 1);
             bar_init(bar(B_ITEM + i), 1);
             bar_init(bar(B_TAKEN + i), 11);
         }
@@ -211,8 +230,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto next = [&](uint32_t n, Item &it) {
         if (!all_wait(bar(B_ITEM + (n & 1)), (n >> 1) & 1)) return false;
         const volatile Item &s = items[n & 1];
-        it.token = s.token, it.count = s.count, it.pos = s.pos, it.head = s.head;
-        it.key = s.key, it.keys = s.keys, it.shift = s.shift;
+        // from one lane: uniform over the warp, for the compiler too
+        it.token = __shfl_sync(0xffffffffu, s.token, 0), it.count = __shfl_sync(0xffffffffu, s.count, 0);
+        it.pos = __shfl_sync(0xffffffffu, s.pos, 0), it.head = __shfl_sync(0xffffffffu, s.head, 0);
+        it.key = __shfl_sync(0xffffffffu, s.key, 0), it.keys = __shfl_sync(0xffffffffu, s.keys, 0);
+        it.shift = __shfl_sync(0xffffffffu, s.shift, 0);
         return it.count != 0;
     };
     auto taken = [&](uint32_t n) {
@@ -225,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         s.count = max(0, min((int32_t)per, it.count - at));
         const int32_t from = it.pos + at + it.shift + 1;  // keys that the first row sees, if causal
         const int32_t upto = a.causal ? max(0, min(it.keys, from + s.count - 1)) : it.keys;
-        s.tiles = s.count ? (upto + (int32_t)kKeys - 1) / (int32_t)kKeys : 0;
+        s.tiles = s.count ? (upto + kKeys - 1) / kKeys : 0;
         s.first = a.causal ? max(0, min(it.keys, from)) : it.keys;
         return s;
     };
@@ -236,8 +258,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int t = warp >> 2;
         const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
         const uint32_t lanes = (warp & 3u) * 32u << 16;
-        const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * D;
-        uint32_t phase_s = 0, phase_o = 0;
+        const uint32_t to = tmem + lanes + P::kColO + t * D;
+        // A bit for each of the two buffers of logits: the phase that its logits come in, and that of
+        // the last product O += P V asked for from it.
+        uint32_t phase_s = 0, phase_o = 3;
         Item it;
         for (uint32_t n = 0; next(n, it); ++n) {
             const TileSpan sp = span(it, t);
@@ -247,23 +271,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             float ref = -INFINITY, sum = 0.0f;  // the maximum that probabilities are relative to (log2 units)
             bool fine = true;
             for (int32_t j = 0; j < sp.tiles; ++j) {
-                if (!(fine = all_wait(bar(B_S + t), phase_s))) break;
-                phase_s ^= 1;
+                const uint32_t buf = j & 1, ts = tmem + lanes + (2 * t + buf) * kKeys;
+                if (!(fine = all_wait(bar(B_S + 2 * t + buf), phase_s >> buf & 1u))) break;
+                phase_s ^= 1u << buf;
                 tc_after();
-                uint32_t x[128];
+                uint32_t x[kKeys];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tm_load(ts + 32 * c, x + 32 * c);
+                for (int c = 0; c < kKeys / 32; ++c) tm_load(ts + 32 * c, x + 32 * c);
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
-                if ((j + 1) * (int32_t)kKeys > sp.first) {
-                    const int32_t left = sees - j * (int32_t)kKeys;
+                if ((j + 1) * kKeys > sp.first) {
+                    const int32_t left = sees - j * kKeys;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
+                    for (int i = 0; i < kKeys; ++i)
                         if (i >= left) s[i] = -INFINITY;
                 }
                 float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-                for (int i = 4; i < 128; i += 4) {
+                for (int i = 4; i < kKeys; i += 4) {
                     m0 = fmaxf(m0, s[i]);
                     m1 = fmaxf(m1, s[i + 1]);
                     m2 = fmaxf(m2, s[i + 2]);
@@ -272,10 +297,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.scale;
                 if (j == 0) ref = top;
                 else if (__any_sync(0xffffffffu, top > ref + kLazy)) {
+                    // not under a product that is still adding to the outputs
+                    if (!(fine = all_wait(bar(B_O + 2 * t + (buf ^ 1u)), phase_o >> (buf ^ 1u) & 1u))) break;
+                    tc_after();
                     const float now = fmaxf(ref, top), f = now == -INFINITY ? 1.0f : ex2(ref - now);
                     ref = now;
                     sum *= f;
-                    // the products of the last tile are done: S of this one was issued after them
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t o[32];
@@ -289,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const float from = ref == -INFINITY ? 0.0f : ref;
                 float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 128; i += 2) {
+                for (int i = 0; i < kKeys; i += 2) {
                     const float e0 = ex2(fmaf(s[i], a.scale, -from)), e1 = ex2(fmaf(s[i + 1], a.scale, -from));
                     l0 += e0;
                     l1 += e1;
@@ -297,16 +324,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 sum += l0 + l1;
                 tm_store(ts, x);
-                tm_store(ts + 32, x + 32);
+                if constexpr (kKeys == 96) tm_store16(ts + 32, x + 32);
                 tc_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(bar(B_P + t));
+                if (lane == 0) bar_arrive(bar(B_P + 2 * t + buf));
+                phase_o ^= 1u << buf;
             }
             if (fine && sp.count) {
                 if (sp.tiles) {
-                    if (!(fine = all_wait(bar(B_O + t), phase_o))) break;
-                    phase_o ^= 1;
+                    const uint32_t buf = (sp.tiles - 1) & 1;
+                    if (!(fine = all_wait(bar(B_O + 2 * t + buf), phase_o >> buf & 1u))) break;
                     tc_after();
                 }
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -329,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                     if (flagged) {
                         // infinities and NaN that this row sees: keys from `key0` on were looked through
-                        const int32_t key0 = max(0, (span(it, 0).first / (int32_t)kKeys)) * (int32_t)kKeys;
+                        const int32_t key0 = max(0, (span(it, 0).first / kKeys)) * kKeys;
                         const uint16_t *first = bad + (n & 1) * 3 * D + 32 * c;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
@@ -374,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         q_phase[t] ^= 1;
                         bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
                         for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(base + P::kQ + t * P::kTile + c * P::kChunk, &mq, bar(B_QFULL + t), 64 * c,
+                            tma3(base + P::kQ + t * P::kQTile + c * P::kQChunk, &mq, bar(B_QFULL + t), 64 * c,
                                  it.head * (int32_t)a.group, it.token + t * (int32_t)per);
                     };
                     auto load_kv = [&](const CUtensorMap *map, int32_t j, bool look) {
@@ -383,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         bar_expect(on, P::kTile);
                         for (uint32_t c = 0; c < P::kChunks; ++c)
                             tma3(base + P::kRing + slot * P::kTile + c * P::kChunk, map, on, 64 * c, it.head,
-                                 it.key + j * (int32_t)kKeys);
+                                 it.key + j * kKeys);
                         issued |= bit;
                         raw = look ? raw | bit : raw & ~bit;
                         full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
@@ -393,9 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     if (s0.tiles) load_q(0);
                     if (tiles) load_kv(&mk, 0, false);
                     if (s1.tiles) load_q(1);
+                    if (tiles > 1) load_kv(&mk, 1, false);
                     for (int32_t j = 0; j < tiles && fine; ++j) {
-                        load_kv(&mv, j, (j + 1) * (int32_t)kKeys > s0.first);
-                        if (j + 1 < tiles) load_kv(&mk, j + 1, false);
+                        load_kv(&mv, j, (j + 1) * kKeys > s0.first);
+                        if (j + 2 < tiles) load_kv(&mk, j + 2, false);
                     }
                 }
                 fine = __shfl_sync(0xffffffffu, fine, 0);
@@ -413,71 +442,81 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         } else if (warp == 9) {
             // ---- products ----
             uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;
-            constexpr uint32_t ID_S = product(BF, 0, kKeys), ID_O = product(BF, 1, D);
+            constexpr uint32_t ID_S = product(BF, 0, P::kKeys), ID_O = product(BF, 1, D);
             Item it;
             bool fine = true;
             for (uint32_t n = 0; fine && next(n, it); ++n) {
                 const TileSpan sp[2] = {span(it, 0), span(it, 1)};
                 const int32_t tiles = max(sp[0].tiles, sp[1].tiles);
-                if (lane == 0) {
+                {
                     auto advance = [&]() {
                         if (++slot == P::kSlots) slot = 0, full_phase ^= 1;
                     };
-                    auto logits = [&](int t, uint32_t k, bool end) {
-                        const uint32_t q_at = base + P::kQ + t * P::kTile, k_at = base + P::kRing + k * P::kTile;
+                    auto logits = [&](int t, uint32_t k, int32_t j) {
+                        const uint32_t q_at = base + P::kQ + t * P::kQTile, k_at = base + P::kRing + k * P::kTile;
+                        const uint32_t buf = 2 * t + (j & 1);
+                        if (!elect()) return;
 #pragma unroll
                         for (uint32_t c = 0; c < P::kChunks; ++c)
 #pragma unroll
                             for (uint32_t s = 0; s < 4; ++s)
-                                mma_ss(tmem + t * 128, operand(q_at + c * P::kChunk + 32 * s, 0),
+                                mma_ss(tmem + buf * kKeys, operand(q_at + c * P::kQChunk + 32 * s, 0),
                                        operand(k_at + c * P::kChunk + 32 * s, 0), ID_S, c | s);
-                        tc_commit(bar(B_S + t));
-                        if (end) tc_commit(bar(B_QFREE + t));
+                        tc_commit(bar(B_S + buf));
+                        if (j + 1 == sp[t].tiles) tc_commit(bar(B_QFREE + t));
                     };
-                    // the first logits of both tiles
-                    uint32_t k = slot;
-                    if (tiles) {
-                        for (int t = 0; t < 2 && fine; ++t) {
-                            if (!sp[t].tiles) continue;
-                            if (!(fine = bar_wait(bar(B_QFULL + t), q_phase >> t & 1u, stop))) break;
-                            q_phase ^= 1u << t;
-                            if (!(fine = bar_wait(bar(B_FULL + k), full_phase, stop))) break;
-                            tc_after();
-                            logits(t, k, sp[t].tiles == 1);
-                        }
-                        if (fine) tc_commit(bar(B_FREE + k));
+                    // the logits run two tiles ahead of the outputs
+                    for (int32_t j = 0; j < 2 && j < tiles && fine; ++j) {
+                        const uint32_t k = slot;
+                        if (!(fine = all_wait(bar(B_FULL + k), full_phase))) break;
                         advance();
-                    }
-                    for (int32_t j = 0; j < tiles && fine; ++j) {
-                        const uint32_t v = slot;
-                        if (!(fine = bar_wait(bar(B_FULL + v), full_phase, stop))) break;
-                        advance();
-                        k = slot;
-                        const bool more = j + 1 < tiles;
                         for (int t = 0; t < 2; ++t) {
                             if (j >= sp[t].tiles) continue;
-                            if (!(fine = bar_wait(bar(B_P + t), p_phase >> t & 1u, stop))) break;
-                            p_phase ^= 1u << t;
+                            if (j == 0) {
+                                if (!(fine = all_wait(bar(B_QFULL + t), q_phase >> t & 1u))) break;
+                                q_phase ^= 1u << t;
+                            }
                             tc_after();
+                            logits(t, k, j);
+                        }
+                        __syncwarp();
+                        if (fine && elect()) tc_commit(bar(B_FREE + k));
+                    }
+                    for (int32_t j = 0; j < tiles && fine; ++j) {
+                        const uint32_t v = slot, buf = j & 1;
+                        if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
+                        advance();
+                        const uint32_t k = slot;
+                        for (int t = 0; t < 2; ++t) {
+                            if (j >= sp[t].tiles) continue;
+                            const uint32_t tb = 2 * t + buf;
+                            if (!(fine = all_wait(bar(B_P + tb), p_phase >> tb & 1u))) break;
+                            p_phase ^= 1u << tb;
+                            tc_after();
+                            if (elect()) {
 #pragma unroll
-                            for (uint32_t s = 0; s < 8; ++s)
-                                mma_ts(tmem + 256 + t * D, tmem + t * 128 + 8 * s,
+                            for (uint32_t s = 0; s < P::kKeys / 16; ++s)
+                                mma_ts(tmem + P::kColO + t * D, tmem + tb * kKeys + 8 * s,
                                        operand(base + P::kRing + v * P::kTile + s * 2048u, P::kChunk), ID_O, j | (int32_t)s);
-                            if (j + 1 < sp[t].tiles) {
-                                if (!(fine = bar_wait(bar(B_FULL + k), full_phase, stop))) break;
+                            tc_commit(bar(B_O + tb));
+                            }
+                            __syncwarp();
+                            if (j + 2 < sp[t].tiles) {
+                                if (!(fine = all_wait(bar(B_FULL + k), full_phase))) break;
                                 tc_after();
-                                logits(t, k, j + 2 == sp[t].tiles);
-                            } else tc_commit(bar(B_O + t));
+                                logits(t, k, j + 2);
+                            }
                         }
                         if (!fine) break;
-                        tc_commit(bar(B_FREE + v));
-                        if (more) {
-                            tc_commit(bar(B_FREE + k));
-                            advance();
+                        __syncwarp();
+                        if (elect()) {
+                            tc_commit(bar(B_FREE + v));
+                            if (j + 2 < tiles) tc_commit(bar(B_FREE + k));
                         }
+                        __syncwarp();
+                        if (j + 2 < tiles) advance();
                     }
                 }
-                fine = __shfl_sync(0xffffffffu, fine, 0);
                 taken(n);
             }
             // products in flight end before the tensor memory is given back
@@ -556,21 +595,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             bool fine = true;
             for (uint32_t n = 0; fine && next(n, it); ++n) {
                 const TileSpan s0 = span(it, 0), s1 = span(it, 1);
-                const int32_t tiles = max(s0.tiles, s1.tiles), begin = max(0, s0.first / (int32_t)kKeys);
+                const int32_t tiles = max(s0.tiles, s1.tiles), begin = max(0, s0.first / kKeys);
                 uint16_t *first = bad + (n & 1) * 3 * D;
                 bool cleared = false;
                 for (int32_t j = 0; j < tiles; ++j) {
-                    const uint32_t v = slot + 1;  // K tiles in even slots, V tiles in odd ones
-                    slot = slot + 2 == P::kSlots ? 0 : slot + 2;
-                    if ((j + 1) * (int32_t)kKeys <= s0.first) continue;
+                    if ((j + 1) * kKeys <= s0.first) continue;
+                    // in the order K 0, K 1, V 0, K 2, V 1, .. of the item's loads
+                    const uint32_t v = (slot + (uint32_t)min(2 * j + 2, 2 * tiles - 1)) % P::kSlots;
                     if (!(fine = all_wait(bar(B_RAW + v), raw_phase >> v & 1u))) break;
                     raw_phase ^= 1u << v;
                     unsigned char *tile = sm + P::kRing + v * P::kTile;
-                    const int32_t rows = min((int32_t)kKeys, it.keys - j * (int32_t)kKeys);
+                    const int32_t rows = min(kKeys, it.keys - j * kKeys);
                     uint32_t found = 0;
                     for (uint32_t c = 0; c < P::kChunks; ++c)
 #pragma unroll 4
-                        for (uint32_t i = lane; i < kKeys * 8; i += 32) {
+                        for (uint32_t i = lane; i < P::kKeys * 8; i += 32) {
                             uint4 *w = reinterpret_cast<uint4 *>(tile + c * P::kChunk + i * 16);
                             if ((int32_t)(i >> 3) >= rows) *w = make_uint4(0, 0, 0, 0);
                             else {
@@ -598,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                 if ((x & E) != E) continue;
                                 *w = 0;
                                 const uint32_t kind = (x & 0x7fffu) != E ? 2 : x >> 15;  // 0 inf, 1 -inf, 2 NaN
-                                const uint32_t at = (uint32_t)((j - begin) * (int32_t)kKeys + k);
+                                const uint32_t at = (uint32_t)((j - begin) * kKeys + k);
                                 if (at < first[kind * D + d]) first[kind * D + d] = (uint16_t)at;
                             }
                         __syncwarp();
@@ -608,6 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     __syncwarp();
                     if (lane == 0) bar_arrive(bar(B_FULL + v));
                 }
+                slot = (slot + 2 * (uint32_t)tiles) % P::kSlots;
                 taken(n);
             }
         }
@@ -672,8 +712,8 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
     // without any key nothing is loaded; the maps only have to be valid
     const bool keys = a.k_tokens != 0;
     if (!make_map(&mq, BF, a.q, D, a.q_heads, a.q_tokens, a.q_head, a.q_token, a.group, per) ||
-        !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, kKeys) ||
-        !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, kKeys))
+        !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, P::kKeys) ||
+        !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, P::kKeys))
         return cudaErrorInvalidValue;
     // two tiles an item share K and V loads; where that leaves SMs without work, one
     const uint64_t items2 = a.kv_heads * ((a.q_tokens + 2 * per - 1) / (2 * per));
