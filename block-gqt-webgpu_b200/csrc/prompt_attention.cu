@@ -5,17 +5,18 @@
 //
 // A work item is a block of consecutive positions of one sequence with all query heads of one
 // KV head: 128 rows a tile, floor(128 / group) positions x group heads, two tiles an item (one
-// where there are few items), which share every K and V tile of 128 keys.  A CTA takes items
-// until none is left.  Its twelve warps have roles:
+// where there are few items), which share every K and V tile.  A CTA takes items until none is
+// left.  Its sixteen warps have roles:
 //   warps 0-3, 4-7  softmax of tile 0 and of tile 1, a thread a row: logits out of tensor memory,
 //                   mask, running maximum, probabilities back into tensor memory (as 16-bit
 //                   pairs in the columns where the logits were), and the output at the end
 //   warp 8          TMA loads of Q, K and V (128-byte swizzle) into a ring of K / V tiles
-//   warp 9          the products, one thread: S = Q K^T (operands in shared memory) and
-//                   O += P V (P in tensor memory, V as it lies), FP32 accumulators in
-//                   tensor memory; while one tile's logits are in softmax, the other's products run
-//   warp 10         the deal: items in order of falling length, dealt back and forth over the CTAs
-//   warp 11         V tiles at a sequence's end or on the diagonal, before they are multiplied:
+//   warps 9, 10     the products of tile 0 and of tile 1: S = Q K^T (operands in shared memory), two
+//                   K tiles ahead of softmax, and O += P V (P in tensor memory, V as it lies), FP32
+//                   accumulators in tensor memory.  A warp of its own for each row tile keeps the waits
+//                   of one chain under the products of the other
+//   warp 11         the deal: items in order of falling length, dealt back and forth over the CTAs
+//   warps 12-15     V tiles at a sequence's end or on the diagonal, before they are multiplied:
 //                   rows past the end (another sequence's, or nothing) are zeroed, and an
 //                   infinity or a NaN, which the zero probability of a row that does not see
 //                   it would turn into a NaN, is taken out and given to the rows that do see it
@@ -32,7 +33,7 @@ namespace bgtq {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kThreads = 384, kRows = 128;
+constexpr uint32_t kThreads = 512, kRows = 128;
 constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
@@ -86,25 +87,23 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// A shared-memory operand: 128-byte swizzle, 8-row groups 1024 bytes apart, `lbo` between
-// 64-element column blocks of an operand whose rows run along the contraction.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)((lbo >> 4) & 0x3fffu) << 16 | (uint64_t)(1024u >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// A shared-memory operand, low word: address, and the distance between 64-element column blocks of an
+// operand whose rows run along the contraction.  High word: 8-row groups 1024 bytes apart, 128-byte swizzle.
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t lbo) { return addr >> 4 | (lbo >> 4) << 16; }
+constexpr uint32_t kOperandHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
 // kind::f16, FP32 accumulators, M = 128: the operands' type, whether B's rows run along the contraction, N.
 __host__ __device__ constexpr uint32_t product(bool bf16, uint32_t b_rows, uint32_t n) {
     return (1u << 4) | (bf16 ? 1u << 7 | 1u << 10 : 0u) | b_rows << 16 | (n >> 3) << 17 | (kRows >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
-                 : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\t"
+                 "mov.b64 y, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "r"(b), "r"(id), "r"(acc), "n"(kOperandHigh) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id),
+                 "r"(acc), "n"(kOperandHigh) : "memory");
 }
 #define BGTQ_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define BGTQ_V8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
@@ -155,7 +154,7 @@ struct Plan {
     static constexpr uint32_t kBad = kAfter;                       // [2 items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + 2 * 3 * D * 2;       // [2] Item
     static constexpr uint32_t kBars = kItems + 2 * 32;
-    static constexpr uint32_t kBarCount = 3 * kSlots + 21;
+    static constexpr uint32_t kBarCount = 3 * kSlots + 22;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
     static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
 };
@@ -198,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < P::kSlots; ++i) {
-            bar_init(bar(B_FULL + i), 1);
-            bar_init(bar(B_FREE + i), 1);
+            bar_init(bar(B_FULL + i), 4);
+            bar_init(bar(B_FREE + i), 2);
             bar_init(bar(B_RAW + i), 1);
         }
         for (uint32_t i = 0; i < 2; ++i) {
@@ -212,9 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             bar_init(bar(B_O + 2 * i), 1);
             bar_init(bar(B_O + 2 * i + 1), 1);
             bar_init(bar(B_ITEM + i), 1);
-            bar_init(bar(B_TAKEN + i), 11);
+            bar_init(bar(B_TAKEN + i), 15);
         }
         bar_init(bar(B_END), 1);
+        bar_init(bar(B_END + 1), 1);
         words[1] = words[2] = words[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (warp < 8) {
         // ---- softmax: thread = row of tile t ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int t = warp >> 2;
         const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
         const uint32_t lanes = (warp & 3u) * 32u << 16;
@@ -388,8 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
             // ---- loads ----
-            // A tile that warp 11 looks through lands on its slot's raw barrier, and warp 11 arrives on the
-            // full one when it is done with it.
+            // A tile that warps 12-15 look through lands on its slot's raw barrier, and they arrive on the
+            // full one when they are done with it.
             uint32_t slot = 0, free_phase = 1, q_phase[2] = {1, 1}, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
             Item it;
             bool fine = true;
@@ -409,6 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
                         const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
                         bar_expect(on, P::kTile);
+                        if (!look)
+                            for (int i = 0; i < 3; ++i) bar_arrive(on);
                         for (uint32_t c = 0; c < P::kChunks; ++c)
                             tma3(base + P::kRing + slot * P::kTile + c * P::kChunk, map, on, 64 * c, it.head,
                                  it.key + j * kKeys);
@@ -439,93 +441,89 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                  &none);
                 for (int t = 0; t < 2; ++t) bar_wait(bar(B_QFULL + t), q_phase[t] ^ 1u, &none);
             }
-        } else if (warp == 9) {
-            // ---- products ----
+        } else if (warp <= 10) {
+            // ---- products of tile t: the warp stays together, one lane issues ----
+            const int t = (int)warp - 9;
             uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;
             constexpr uint32_t ID_S = product(BF, 0, P::kKeys), ID_O = product(BF, 1, D);
+            const uint32_t q_at = base + P::kQ + t * P::kQTile, s_at = tmem + 2 * t * kKeys, o_at = tmem + P::kColO + t * D;
             Item it;
             bool fine = true;
             for (uint32_t n = 0; fine && next(n, it); ++n) {
-                const TileSpan sp[2] = {span(it, 0), span(it, 1)};
-                const int32_t tiles = max(sp[0].tiles, sp[1].tiles);
-                {
-                    auto advance = [&]() {
-                        if (++slot == P::kSlots) slot = 0, full_phase ^= 1;
-                    };
-                    auto logits = [&](int t, uint32_t k, int32_t j) {
-                        const uint32_t q_at = base + P::kQ + t * P::kQTile, k_at = base + P::kRing + k * P::kTile;
-                        const uint32_t buf = 2 * t + (j & 1);
-                        if (!elect()) return;
+                const TileSpan sp = span(it, t), other = span(it, t ^ 1);
+                const int32_t tiles = max(sp.tiles, other.tiles);
+                auto advance = [&]() {
+                    if (++slot == P::kSlots) slot = 0, full_phase ^= 1;
+                };
+                // the logits of K tile j (in slot k), and the slot's release
+                auto logits = [&](uint32_t k, int32_t j) {
+                    if (!elect()) return;
+                    if (j >= sp.tiles) {
+                        bar_arrive(bar(B_FREE + k));
+                        return;
+                    }
+                    const uint32_t q = operand(q_at, 0), key = operand(base + P::kRing + k * P::kTile, 0), d = s_at + (j & 1) * kKeys;
 #pragma unroll
-                        for (uint32_t c = 0; c < P::kChunks; ++c)
+                    for (uint32_t c = 0; c < P::kChunks; ++c)
 #pragma unroll
-                            for (uint32_t s = 0; s < 4; ++s)
-                                mma_ss(tmem + buf * kKeys, operand(q_at + c * P::kQChunk + 32 * s, 0),
-                                       operand(k_at + c * P::kChunk + 32 * s, 0), ID_S, c | s);
-                        tc_commit(bar(B_S + buf));
-                        if (j + 1 == sp[t].tiles) tc_commit(bar(B_QFREE + t));
-                    };
-                    // the logits run two tiles ahead of the outputs
-                    for (int32_t j = 0; j < 2 && j < tiles && fine; ++j) {
-                        const uint32_t k = slot;
+                        for (uint32_t s = 0; s < 4; ++s)
+                            mma_ss(d, q + (c * P::kQChunk + 32 * s) / 16, key + (c * P::kChunk + 32 * s) / 16, ID_S, c | s);
+                    tc_commit(bar(B_S + 2 * t + (j & 1)));
+                    tc_commit(bar(B_FREE + k));
+                    if (j + 1 == sp.tiles) tc_commit(bar(B_QFREE + t));
+                };
+                if (sp.tiles) {
+                    if (!(fine = all_wait(bar(B_QFULL + t), q_phase))) break;
+                    q_phase ^= 1;
+                }
+                // the logits run two tiles ahead of the outputs
+                for (int32_t j = 0; j < 2 && j < tiles; ++j) {
+                    if (!(fine = all_wait(bar(B_FULL + slot), full_phase))) break;
+                    tc_after();
+                    logits(slot, j);
+                    __syncwarp();
+                    advance();
+                }
+                for (int32_t j = 0; j < tiles && fine; ++j) {
+                    const uint32_t v = slot;
+                    if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
+                    advance();
+                    const uint32_t k = slot;
+                    const bool more = j + 2 < tiles;
+                    if (more) {
                         if (!(fine = all_wait(bar(B_FULL + k), full_phase))) break;
                         advance();
-                        for (int t = 0; t < 2; ++t) {
-                            if (j >= sp[t].tiles) continue;
-                            if (j == 0) {
-                                if (!(fine = all_wait(bar(B_QFULL + t), q_phase >> t & 1u))) break;
-                                q_phase ^= 1u << t;
-                            }
-                            tc_after();
-                            logits(t, k, j);
-                        }
-                        __syncwarp();
-                        if (fine && elect()) tc_commit(bar(B_FREE + k));
                     }
-                    for (int32_t j = 0; j < tiles && fine; ++j) {
-                        const uint32_t v = slot, buf = j & 1;
-                        if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
-                        advance();
-                        const uint32_t k = slot;
-                        for (int t = 0; t < 2; ++t) {
-                            if (j >= sp[t].tiles) continue;
-                            const uint32_t tb = 2 * t + buf;
-                            if (!(fine = all_wait(bar(B_P + tb), p_phase >> tb & 1u))) break;
-                            p_phase ^= 1u << tb;
-                            tc_after();
-                            if (elect()) {
+                    const uint32_t buf = j & 1;
+                    if (j < sp.tiles) {
+                        if (!(fine = all_wait(bar(B_P + 2 * t + buf), p_phase >> buf & 1u))) break;
+                        p_phase ^= 1u << buf;
+                    }
+                    tc_after();
+                    if (elect()) {
+                        if (j < sp.tiles) {
+                            const uint32_t val = operand(base + P::kRing + v * P::kTile, P::kChunk), pr = s_at + buf * kKeys;
 #pragma unroll
                             for (uint32_t s = 0; s < P::kKeys / 16; ++s)
-                                mma_ts(tmem + P::kColO + t * D, tmem + tb * kKeys + 8 * s,
-                                       operand(base + P::kRing + v * P::kTile + s * 2048u, P::kChunk), ID_O, j | (int32_t)s);
-                            tc_commit(bar(B_O + tb));
-                            }
-                            __syncwarp();
-                            if (j + 2 < sp[t].tiles) {
-                                if (!(fine = all_wait(bar(B_FULL + k), full_phase))) break;
-                                tc_after();
-                                logits(t, k, j + 2);
-                            }
-                        }
-                        if (!fine) break;
-                        __syncwarp();
-                        if (elect()) {
+                                mma_ts(o_at, pr + 8 * s, val + s * 128, ID_O, j | (int32_t)s);
+                            tc_commit(bar(B_O + 2 * t + buf));
                             tc_commit(bar(B_FREE + v));
-                            if (j + 2 < tiles) tc_commit(bar(B_FREE + k));
-                        }
-                        __syncwarp();
-                        if (j + 2 < tiles) advance();
+                        } else bar_arrive(bar(B_FREE + v));
                     }
+                    __syncwarp();
+                    if (more) logits(k, j + 2);
+                    __syncwarp();
                 }
-                taken(n);
+                if (fine) taken(n);
             }
             // products in flight end before the tensor memory is given back
-            if (lane == 0 && *stop) {
+            __syncwarp();
+            if (*stop && elect()) {
                 uint32_t none = 0;
-                tc_commit(bar(B_END));
-                bar_wait(bar(B_END), 0, &none);
+                tc_commit(bar(B_END + t));
+                bar_wait(bar(B_END + t), 0, &none);
             }
-        } else if (warp == 10) {
+        } else if (warp == 11) {
             // ---- the deal ----
             // Sequence s has ceil(queries / (tiles per item)) blocks; block b of every sequence that
             // has it is level b.  Items go by falling level (the last blocks see the most keys), a level's
@@ -589,7 +587,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (it.count == 0) break;
             }
         } else {
-            // ---- V tiles that not every row sees ----
+            // ---- V tiles that not every row sees: each of four warps its share of the dimensions ----
+            constexpr uint32_t kUnits = D / 8 / 4;  // 16-byte units of a row in a warp's share
+            const uint32_t share = warp - 12;
             uint32_t slot = 0, raw_phase = 0;
             Item it;
             bool fine = true;
@@ -597,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const TileSpan s0 = span(it, 0), s1 = span(it, 1);
                 const int32_t tiles = max(s0.tiles, s1.tiles), begin = max(0, s0.first / kKeys);
                 uint16_t *first = bad + (n & 1) * 3 * D;
-                bool cleared = false;
-                for (int32_t j = 0; j < tiles; ++j) {
+                for (uint32_t i = lane; i < 3 * D / 4; i += 32) first[i / (D / 4) * D + share * (D / 4) + i % (D / 4)] = 0xffff;
+                for (int32_t j = begin; j < tiles; ++j) {
                     if ((j + 1) * kKeys <= s0.first) continue;
                     // in the order K 0, K 1, V 0, K 2, V 1, .. of the item's loads
                     const uint32_t v = (slot + (uint32_t)min(2 * j + 2, 2 * tiles - 1)) % P::kSlots;
@@ -607,32 +607,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     unsigned char *tile = sm + P::kRing + v * P::kTile;
                     const int32_t rows = min(kKeys, it.keys - j * kKeys);
                     uint32_t found = 0;
-                    for (uint32_t c = 0; c < P::kChunks; ++c)
+                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
 #pragma unroll 4
-                        for (uint32_t i = lane; i < P::kKeys * 8; i += 32) {
-                            uint4 *w = reinterpret_cast<uint4 *>(tile + c * P::kChunk + i * 16);
-                            if ((int32_t)(i >> 3) >= rows) *w = make_uint4(0, 0, 0, 0);
-                            else {
-                                const uint4 x = *w;
-                                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+                    for (uint32_t i = lane; i < P::kKeys * kUnits; i += 32) {
+                        const uint32_t r = i / kUnits, u = share * kUnits + i % kUnits;
+                        uint4 *w = reinterpret_cast<uint4 *>(tile + u / 8 * P::kChunk + r * 128 + ((u % 8 ^ (r & 7)) << 4));
+                        if ((int32_t)r >= rows) *w = make_uint4(0, 0, 0, 0);
+                        else {
+                            const uint4 x = *w;
+                            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
-                                    found |= (y[k] & E) == E || (y[k] >> 16 & E) == E;
-                                }
-                            }
+                            for (int k = 0; k < 4; ++k) found |= (y[k] & E) == E || (y[k] >> 16 & E) == E;
                         }
+                    }
                     if (__any_sync(0xffffffffu, found)) {
-                        if (!cleared) {
-                            for (uint32_t i = lane; i < 3 * D; i += 32) first[i] = 0xffff;
-                            cleared = true;
-                        }
                         __syncwarp();
-                        for (uint32_t d = lane; d < (uint32_t)D; d += 32)
+                        for (uint32_t i = lane; i < (uint32_t)D / 4; i += 32) {
+                            const uint32_t d = share * (D / 4) + i;
                             for (int32_t k = 0; k < rows; ++k) {
                                 uint16_t *w = reinterpret_cast<uint16_t *>(tile + d / 64 * P::kChunk + k * 128 +
                                                                            (((d % 64 / 8) ^ (k & 7)) << 4)) + d % 8;
-                                constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
                                 const uint32_t x = *w;
                                 if ((x & E) != E) continue;
                                 *w = 0;
@@ -640,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                 const uint32_t at = (uint32_t)((j - begin) * kKeys + k);
                                 if (at < first[kind * D + d]) first[kind * D + d] = (uint16_t)at;
                             }
-                        __syncwarp();
+                        }
                         if (lane == 0) bad_flag[n & 1] = 1;
                     }
                     fence_async();
@@ -648,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     if (lane == 0) bar_arrive(bar(B_FULL + v));
                 }
                 slot = (slot + 2 * (uint32_t)tiles) % P::kSlots;
-                taken(n);
+                if (fine) taken(n);
             }
         }
     }
