@@ -127,6 +127,32 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {  // NaN if one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+// 2^(x c - from) of two values on the FMA pipe, for a whole `from` (below 2^20 in magnitude) and x c - from >= -126:
+// adding 1.5 * 2^23 - from rounds x c to a whole number n in the low mantissa bits, and 2^f of the
+// rest, -1/2 <= f <= 1/2, is the polynomial of degree 4 with the least largest relative error on
+// that interval (Remez exchange): 2.7e-6 in FP32, 4e-8 on average.  n goes into the exponent.
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ float2 ex2_fma(float2 x, float2 c, float2 shift) {
+    const float2 t = __ffma2_rn(x, c, shift);                                   // shift = kRound - from
+    const float2 f = __ffma2_rn(x, c, __fadd2_rn(shift, make_float2(-t.x, -t.y)));
+    float2 p = __ffma2_rn(f, make_float2(0.0095701022f, 0.0095701022f), make_float2(0.055917859f, 0.055917859f));
+    p = __ffma2_rn(p, f, make_float2(0.24024744f, 0.24024744f));
+    p = __ffma2_rn(p, f, make_float2(0.69312179f, 0.69312179f));
+    p = __ffma2_rn(p, f, make_float2(0.99999928f, 0.99999928f));
+    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+    return p;
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack(float x, float y) {
     if constexpr (BF) {
@@ -150,6 +176,7 @@ struct Plan {
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
     static constexpr uint32_t kSlots = D == 128 ? 8 : 10;          // K and V tiles in the ring
+    static constexpr int kFma = 6;                                 // exponentials of 16 on the FMA pipe
     static constexpr uint32_t kQ = 0, kRing = 2 * kQTile, kAfter = kRing + kSlots * kTile;
     static constexpr uint32_t kBad = kAfter;                       // [2 items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + 2 * 3 * D * 2;       // [2] Item
@@ -262,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         // A bit for each of the two buffers of logits: the phase that its logits come in, and that of
         // the last product O += P V asked for from it.
         uint32_t phase_s = 0, phase_o = 3;
+        const float inv_scale = 1.0f / a.scale;
         Item it;
         for (uint32_t n = 0; next(n, it); ++n) {
             const TileSpan sp = span(it, t);
@@ -280,7 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int c = 0; c < kKeys / 32; ++c) tm_load(ts + 32 * c, x + 32 * c);
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
-                if ((j + 1) * kKeys > sp.first) {
+                const bool masked = (j + 1) * kKeys > sp.first;
+                if (masked) {
                     const int32_t left = sees - j * kKeys;
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i)
@@ -288,20 +317,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-                for (int i = 4; i < kKeys; i += 4) {
-                    m0 = fmaxf(m0, s[i]);
-                    m1 = fmaxf(m1, s[i + 1]);
-                    m2 = fmaxf(m2, s[i + 2]);
-                    m3 = fmaxf(m3, s[i + 3]);
+                for (int i = 4; i + 7 < kKeys; i += 8) {
+                    m0 = max3_nan(m0, s[i], s[i + 1]);
+                    m1 = max3_nan(m1, s[i + 2], s[i + 3]);
+                    m2 = max3_nan(m2, s[i + 4], s[i + 5]);
+                    m3 = max3_nan(m3, s[i + 6], s[i + 7]);
                 }
-                const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.scale;
+                m0 = max3_nan(m0, s[kKeys - 4], s[kKeys - 3]);
+                m1 = max3_nan(m1, s[kKeys - 2], s[kKeys - 1]);
+                // whole numbers (ex2_fma); a row that is no query stands at 0 and asks for nothing
+                const float top = live ? ceilf(max_nan(max3_nan(m0, m1, m2), m3) * a.scale) : 0.0f;
+                const bool grown = !(top <= ref + kLazy);  // each row for itself: no result depends on a neighbour
                 if (j == 0) ref = top;
-                else if (__any_sync(0xffffffffu, top > ref + kLazy)) {
+                else if (__any_sync(0xffffffffu, grown)) {
                     // not under a product that is still adding to the outputs
                     if (!(fine = all_wait(bar(B_O + 2 * t + (buf ^ 1u)), phase_o >> (buf ^ 1u) & 1u))) break;
                     tc_after();
-                    const float now = fmaxf(ref, top), f = now == -INFINITY ? 1.0f : ex2(ref - now);
-                    ref = now;
+                    const float f = grown ? ex2(ref - max_nan(ref, top)) : 1.0f;
+                    if (grown) ref = max_nan(ref, top);
                     sum *= f;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
@@ -314,15 +347,35 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                 }
                 const float from = ref == -INFINITY ? 0.0f : ref;
-                float l0 = 0.0f, l1 = 0.0f;
+                const float2 scale2 = make_float2(a.scale, a.scale), from2 = make_float2(-from, -from);
+                float2 total = make_float2(0.0f, 0.0f);
+                // Of 16 logits kFma take the FMA pipe: ex2 alone has 16 lanes an SM and clock.  Tiles with a
+                // mask, and rows with an infinity, a NaN or a maximum past 2^20 in them, do without.
+                const bool careful = masked || !(fabsf(from) <= 1048576.0f);
+                if (careful) {
 #pragma unroll
-                for (int i = 0; i < kKeys; i += 2) {
-                    const float e0 = ex2(fmaf(s[i], a.scale, -from)), e1 = ex2(fmaf(s[i + 1], a.scale, -from));
-                    l0 += e0;
-                    l1 += e1;
-                    x[i / 2] = pack<BF>(e0, e1);
+                    for (int i = 0; i < kKeys; i += 2) {
+                        const float2 y = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        total = __fadd2_rn(total, e);
+                        x[i / 2] = pack<BF>(e.x, e.y);
+                    }
+                } else {
+                    const float least = (from - 126.0f) * inv_scale;
+                    const float2 shift = make_float2(kRound - from, kRound - from);
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 2) {
+                        float2 e;
+                        if (i % 16 < P::kFma) e = ex2_fma(make_float2(fmaxf(s[i], least), fmaxf(s[i + 1], least)), scale2, shift);
+                        else {
+                            const float2 y = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
+                            e = make_float2(ex2(y.x), ex2(y.y));
+                        }
+                        total = __fadd2_rn(total, e);
+                        x[i / 2] = pack<BF>(e.x, e.y);
+                    }
                 }
-                sum += l0 + l1;
+                sum += total.x + total.y;
                 tm_store(ts, x);
                 if constexpr (kKeys == 96) tm_store16(ts + 32, x + 32);
                 tc_wait_st();
@@ -337,7 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     if (!(fine = all_wait(bar(B_O + 2 * t + buf), phase_o >> buf & 1u))) break;
                     tc_after();
                 }
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const bool none = sees == 0 || sum == 0.0f;
+                const float inv = none ? 0.0f : 1.0f / sum;
                 const uint32_t flagged = bad_flag[n & 1];
                 const uint64_t at = (uint64_t)(it.token + t * (int32_t)per + (int32_t)p) * a.q_heads + it.head * a.group + g;
                 uint16_t *out = static_cast<uint16_t *>(a.out) + at * D;
@@ -378,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         }
                     }
                 }
-                if (live && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                if (live && a.lse) a.lse[at] = none ? -INFINITY : (ref + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;
