@@ -4,22 +4,25 @@
 // no key gives zeros and a log sum of minus infinity.
 //
 // A work item is a block of consecutive positions of one sequence with all query heads of one
-// KV head: 128 rows a tile, floor(128 / group) positions x group heads, two tiles an item (one
-// where there are few items), which share every K and V tile.  A CTA takes items until none is
-// left.  Its sixteen warps have roles:
-//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, a thread a row: logits out of tensor memory,
-//                   mask, running maximum, probabilities back into tensor memory (as 16-bit
-//                   pairs in the columns where the logits were), and the output at the end
-//   warp 8          TMA loads of Q, K and V (128-byte swizzle) into a ring of K / V tiles
-//   warps 9, 10     the products of tile 0 and of tile 1: S = Q K^T (operands in shared memory), two
-//                   K tiles ahead of softmax, and O += P V (P in tensor memory, V as it lies), FP32
-//                   accumulators in tensor memory.  A warp of its own for each row tile keeps the waits
-//                   of one chain under the products of the other
-//   warp 11         the deal: items in order of falling length, dealt back and forth over the CTAs
-//   warps 12-15     V tiles at a sequence's end or on the diagonal, before they are multiplied:
-//                   rows past the end (another sequence's, or nothing) are zeroed, and an
-//                   infinity or a NaN, which the zero probability of a row that does not see
-//                   it would turn into a NaN, is taken out and given to the rows that do see it
+// KV head: 128 rows a tile, floor(128 / group) positions x group heads, up to four tiles (head
+// dim 64) or two (128), which share every K and V tile of 64 keys.  Tensor memory sets these
+// numbers: logits and outputs of all row tiles fill its 512 columns, 4 x (64 + 64) at head dim 64,
+// 2 x (2 x 64 + 128) at 128, where the logits are double-buffered instead.  A CTA takes items
+// until none is left.  Its warps have roles:
+//   softmax     four warps a row tile, a thread a row: logits out of tensor memory, mask, running
+//               maximum, probabilities back into tensor memory (as 16-bit pairs in the columns
+//               where the logits were), and the outputs at the end
+//   deal, loads one warp: the items in order of falling length, dealt back and forth over the
+//               CTAs, and the TMA loads of Q, K and V (128-byte swizzle) into a ring of stages
+//   products    two warps, each for half of the row tiles: S = Q K^T (operands in shared memory)
+//               ahead of softmax and O += P V (P in tensor memory, V as it lies), FP32
+//               accumulators in tensor memory.  The warp stays together and one lane issues, so
+//               that the operands sit in uniform registers; a stage holds V j and the next K
+//               tile to come, so that a step has two waits and two commits
+//   ends        one warp: V tiles at a sequence's end or on the diagonal, before they are
+//               multiplied: rows past the end (another sequence's, or nothing) are zeroed, and an
+//               infinity or a NaN, which the zero probability of a row that does not see it would
+//               turn into a NaN, is taken out and given to the rows that do see it
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time: until then probabilities are taken relative to the older maximum, so they stay
 // below 2^8, and P is FP16 or BF16 (the inputs' type) with the same relative error.
@@ -33,8 +36,9 @@ namespace bgtq {
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kThreads = 512, kRows = 128;
+constexpr uint32_t kRows = 128;
 constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
+constexpr uint32_t kDeal = 4;            // items dealt ahead
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
 // ---- device helpers -----------------------------------------------------------------------
@@ -118,6 +122,10 @@ __device__ __forceinline__ void tm_store(uint32_t at, const uint32_t *r) {
                  "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
                  ::BGTQ_V8(r, 0), BGTQ_V8(r, 8), BGTQ_V8(r, 16), BGTQ_V8(r, 24), "r"(at) : "memory");
 }
+__device__ __forceinline__ void tm_load16(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                 "%15}, [%16];" : BGTQ_R8(r, 0), BGTQ_R8(r, 8) : "r"(at));
+}
 __device__ __forceinline__ void tm_store16(uint32_t at, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
                  "%13, %14, %15};" ::BGTQ_V8(r, 0), BGTQ_V8(r, 8), "r"(at) : "memory");
@@ -127,31 +135,31 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3_nan(float x, float y, float z) {  // NaN if one of them is
+__device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
-__device__ __forceinline__ float max_nan(float x, float y) {
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one of them is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
     return r;
 }
-// 2^(x c - from) of two values on the FMA pipe, for a whole `from` (below 2^20 in magnitude) and x c - from >= -126:
-// adding 1.5 * 2^23 - from rounds x c to a whole number n in the low mantissa bits, and 2^f of the
-// rest, -1/2 <= f <= 1/2, is the polynomial of degree 4 with the least largest relative error on
-// that interval (Remez exchange): 2.7e-6 in FP32, 4e-8 on average.  n goes into the exponent.
-constexpr float kRound = 12582912.0f;
-__device__ __forceinline__ float2 ex2_fma(float2 x, float2 c, float2 shift) {
-    const float2 t = __ffma2_rn(x, c, shift);                                   // shift = kRound - from
-    const float2 f = __ffma2_rn(x, c, __fadd2_rn(shift, make_float2(-t.x, -t.y)));
+// 2^y of two values on the FMA pipe, y below 2^20 (from -126 down: about 2^-126, NaN: NaN): adding 1.5 * 2^23
+// rounds y to a whole number n in the low mantissa bits, and 2^f of the rest, -1/2 <= f <= 1/2, is
+// the polynomial of degree 4 with the least largest relative error on that interval (Remez
+// exchange): 2.7e-6 in FP32, 4e-8 on average.
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+    constexpr float kRound = 12582912.0f;
+    y = make_float2(max_nan(y.x, -126.0f), max_nan(y.y, -126.0f));
+    const float2 t = __fadd2_rn(y, make_float2(kRound, kRound));
+    const float2 f = __ffma2_rn(__fadd2_rn(t, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), y);
     float2 p = __ffma2_rn(f, make_float2(0.0095701022f, 0.0095701022f), make_float2(0.055917859f, 0.055917859f));
     p = __ffma2_rn(p, f, make_float2(0.24024744f, 0.24024744f));
     p = __ffma2_rn(p, f, make_float2(0.69312179f, 0.69312179f));
     p = __ffma2_rn(p, f, make_float2(0.99999928f, 0.99999928f));
-    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-    return p;
+    return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                     __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -168,20 +176,24 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {
 
 template <int D>
 struct Plan {
-    // Keys of a tile: as many as leave room for two tiles of logits and the outputs of both row
-    // tiles in the 512 columns of tensor memory.
-    static constexpr uint32_t kKeys = D == 128 ? 64 : 96;
-    static constexpr uint32_t kColO = 4 * kKeys;                   // the first column of the outputs
+    static constexpr uint32_t kTiles = D == 64 ? 4 : 2;            // row tiles of an item, at most
+    static constexpr uint32_t kBufs = D == 64 ? 1 : 2;             // of logits, for each row tile
+    static constexpr uint32_t kKeys = 64;                          // of a K or V tile
+    static constexpr uint32_t kColO = kTiles * kBufs * kKeys;      // the first column of the outputs
+    static constexpr uint32_t kThreads = 128 * kTiles + 128;
+    // Registers: kThreads x kAll at launch, 128 kTiles x kSoft + 128 x kRest afterwards, 61440 or 64512 in all.
+    static constexpr uint32_t kSoft = D == 64 ? 104 : 216, kRest = D == 64 ? 64 : 72;
+    static constexpr int kFma = D == 64 ? 2 : 6;                   // exponentials of 16 on the FMA pipe
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
-    static constexpr uint32_t kSlots = D == 128 ? 8 : 10;          // K and V tiles in the ring
-    static constexpr int kFma = 6;                                 // exponentials of 16 on the FMA pipe
-    static constexpr uint32_t kQ = 0, kRing = 2 * kQTile, kAfter = kRing + kSlots * kTile;
-    static constexpr uint32_t kBad = kAfter;                       // [2 items][3 kinds][D] first keys
-    static constexpr uint32_t kItems = kBad + 2 * 3 * D * 2;       // [2] Item
-    static constexpr uint32_t kBars = kItems + 2 * 32;
-    static constexpr uint32_t kBarCount = 3 * kSlots + 22;
+    static constexpr uint32_t kStages = D == 128 ? 4 : 7;          // of two K or V tiles in the ring
+    static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kAfter = kRing + kStages * 2 * kTile;
+    static constexpr uint32_t kOut = kAfter;                       // [softmax warps][32 rows][64 bytes] of outputs
+    static constexpr uint32_t kBad = kOut + 4 * kTiles * 2048;                         // [kDeal items][3 kinds][D] first keys
+    static constexpr uint32_t kItems = kBad + kDeal * 3 * D * 2;   // [kDeal] Item
+    static constexpr uint32_t kBars = kItems + kDeal * 32;
+    static constexpr uint32_t kBarCount = 3 * kStages + 2 * kTiles + 2 * kTiles * kBufs + 2 * kDeal + 2;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
     static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
 };
@@ -199,12 +211,13 @@ struct TileSpan {
 };
 
 template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a,
+__global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a,
                                                              const __grid_constant__ CUtensorMap mq,
                                                              const __grid_constant__ CUtensorMap mk,
                                                              const __grid_constant__ CUtensorMap mv) {
     using P = Plan<D>;
     constexpr int32_t kKeys = (int32_t)P::kKeys;
+    constexpr uint32_t NT = P::kTiles, NB = P::kBufs;
     extern __shared__ unsigned char raw[];
     unsigned char *sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
     const uint32_t base = smem_addr(sm), warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -212,37 +225,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     uint16_t *bad = reinterpret_cast<uint16_t *>(sm + P::kBad);
     volatile Item *items = reinterpret_cast<volatile Item *>(sm + P::kItems);
     volatile uint32_t *words = reinterpret_cast<volatile uint32_t *>(sm + P::kWords);
-    volatile uint32_t *stop = words + 1, *bad_flag = words + 2;  // bad_flag[2]
+    volatile uint32_t *stop = words + 1, *bad_flag = words + 2;  // bad_flag[kDeal]
     const uint32_t bars = base + P::kBars;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
-    constexpr uint32_t B_FULL = 0, B_FREE = P::kSlots, B_QFULL = 2 * P::kSlots, B_QFREE = B_QFULL + 2, B_S = B_QFREE + 2,
-                       B_P = B_S + 4, B_O = B_P + 4, B_RAW = B_O + 4, B_ITEM = B_RAW + P::kSlots, B_TAKEN = B_ITEM + 2, B_END = B_TAKEN + 2;
+    // a stage is full, free, or (raw) to be looked through first; of each row tile: its queries are there, its
+    // queries are read; of each buffer of logits: they are there, and what was asked of the tensor cores
+    // before them is done; the probabilities are; of each item: it is dealt, it is given back
+    constexpr uint32_t B_FULL = 0, B_FREE = P::kStages, B_RAW = 2 * P::kStages, B_QFULL = 3 * P::kStages,
+                       B_QFREE = B_QFULL + NT, B_S = B_QFREE + NT, B_P = B_S + NT * NB, B_ITEM = B_P + NT * NB,
+                       B_TAKEN = B_ITEM + kDeal, B_END = B_TAKEN + kDeal;
+    constexpr uint32_t W_LOAD = 4 * NT, W_MMA = W_LOAD + 1, W_ENDS = W_LOAD + 3;  // the warps past softmax
     const uint32_t per = kRows / a.group;  // positions of a tile
-    if (warp == 8) {
+    if (warp == W_LOAD) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(base + P::kWords) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < P::kSlots; ++i) {
-            bar_init(bar(B_FULL + i), 4);
+        for (uint32_t i = 0; i < P::kStages; ++i) {
+            bar_init(bar(B_FULL + i), 1);
             bar_init(bar(B_FREE + i), 2);
             bar_init(bar(B_RAW + i), 1);
         }
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < NT; ++i) {
             bar_init(bar(B_QFULL + i), 1);
             bar_init(bar(B_QFREE + i), 1);
-            bar_init(bar(B_S + 2 * i), 1);
-            bar_init(bar(B_S + 2 * i + 1), 1);
-            bar_init(bar(B_P + 2 * i), 4);
-            bar_init(bar(B_P + 2 * i + 1), 4);
-            bar_init(bar(B_O + 2 * i), 1);
-            bar_init(bar(B_O + 2 * i + 1), 1);
+        }
+        for (uint32_t i = 0; i < NT * NB; ++i) {
+            bar_init(bar(B_S + i), 1);
+            bar_init(bar(B_P + i), 4);
+        }
+        for (uint32_t i = 0; i < kDeal; ++i) {
             bar_init(bar(B_ITEM + i), 1);
-            bar_init(bar(B_TAKEN + i), 15);
+            bar_init(bar(B_TAKEN + i), 4 * NT + 3);  // all warps but the dealer
         }
         bar_init(bar(B_END), 1);
         bar_init(bar(B_END + 1), 1);
-        words[1] = words[2] = words[3] = 0;
+        for (uint32_t i = 1; i < 2 + kDeal; ++i) words[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
@@ -252,11 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const uint32_t tmem = words[0];
 
     // a whole warp's wait: all of its lanes see the same answer
-    auto all_wait = [&](uint32_t b, uint32_t parity) { return (bool)__all_sync(0xffffffffu, bar_wait(b, parity, stop)); };
-    // The item in slot n & 1 of the deal, when it is there; a role gives it back with `taken`.
+    auto all_wait = [&](uint32_t b, uint32_t parity) {
+        if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
+        return (bool)__all_sync(0xffffffffu, bar_wait_slow(b, parity, stop));
+    };
+    // Item n of the deal, when it is there; a role gives its slot back with `taken`.
     auto next = [&](uint32_t n, Item &it) {
-        if (!all_wait(bar(B_ITEM + (n & 1)), (n >> 1) & 1)) return false;
-        const volatile Item &s = items[n & 1];
+        if (!all_wait(bar(B_ITEM + n % kDeal), n / kDeal & 1)) return false;
+        const volatile Item &s = items[n % kDeal];
         // from one lane: uniform over the warp, for the compiler too
         it.token = __shfl_sync(0xffffffffu, s.token, 0), it.count = __shfl_sync(0xffffffffu, s.count, 0);
         it.pos = __shfl_sync(0xffffffffu, s.pos, 0), it.head = __shfl_sync(0xffffffffu, s.head, 0);
@@ -266,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     };
     auto taken = [&](uint32_t n) {
         __syncwarp();
-        if (lane == 0) bar_arrive(bar(B_TAKEN + (n & 1)));
+        if (lane == 0) bar_arrive(bar(B_TAKEN + n % kDeal));
     };
     auto span = [&](const Item &it, int t) {
         TileSpan s;
@@ -278,18 +299,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         s.first = a.causal ? max(0, min(it.keys, from)) : it.keys;
         return s;
     };
+    auto tiles_of = [&](const Item &it) {  // K tiles that any of its row tiles takes
+        int32_t n = 0;
+        for (uint32_t t = 0; t < NT; ++t) n = max(n, span(it, (int)t).tiles);
+        return n;
+    };
 
-    if (warp < 8) {
+    if (warp < 4 * NT) {
         // ---- softmax: thread = row of tile t ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        const int t = warp >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kSoft));
+        const int t = (int)warp >> 2;
         const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
         const uint32_t lanes = (warp & 3u) * 32u << 16;
         const uint32_t to = tmem + lanes + P::kColO + t * D;
-        // A bit for each of the two buffers of logits: the phase that its logits come in, and that of
-        // the last product O += P V asked for from it.
-        uint32_t phase_s = 0, phase_o = 3;
-        const float inv_scale = 1.0f / a.scale;
+        uint32_t phase = 0;  // a bit for each buffer of logits
         Item it;
         for (uint32_t n = 0; next(n, it); ++n) {
             const TileSpan sp = span(it, t);
@@ -299,120 +322,107 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             float ref = -INFINITY, sum = 0.0f;  // the maximum that probabilities are relative to (log2 units)
             bool fine = true;
             for (int32_t j = 0; j < sp.tiles; ++j) {
-                const uint32_t buf = j & 1, ts = tmem + lanes + (2 * t + buf) * kKeys;
-                if (!(fine = all_wait(bar(B_S + 2 * t + buf), phase_s >> buf & 1u))) break;
-                phase_s ^= 1u << buf;
+                const uint32_t buf = j % NB, ts = tmem + lanes + (NB * t + buf) * kKeys;
+                if (!(fine = all_wait(bar(B_S + NB * t + buf), phase >> buf & 1u))) break;
+                phase ^= 1u << buf;
                 tc_after();
                 uint32_t x[kKeys];
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) tm_load(ts + 32 * c, x + 32 * c);
+                tm_load(ts, x);
+                tm_load(ts + 32, x + 32);
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
-                const bool masked = (j + 1) * kKeys > sp.first;
-                if (masked) {
+                if ((j + 1) * kKeys > sp.first) {
                     const int32_t left = sees - j * kKeys;
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i)
                         if (i >= left) s[i] = -INFINITY;
                 }
-                float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+                float m0 = max3(s[0], s[1], s[2]), m1 = max3(s[3], s[4], s[5]), m2 = max3(s[6], s[7], s[8]);
+                float m3 = max3(s[9], s[10], s[11]);
 #pragma unroll
-                for (int i = 4; i + 7 < kKeys; i += 8) {
-                    m0 = max3_nan(m0, s[i], s[i + 1]);
-                    m1 = max3_nan(m1, s[i + 2], s[i + 3]);
-                    m2 = max3_nan(m2, s[i + 4], s[i + 5]);
-                    m3 = max3_nan(m3, s[i + 6], s[i + 7]);
+                for (int i = 12; i + 7 < kKeys; i += 8) {
+                    m0 = max3(m0, s[i], s[i + 1]);
+                    m1 = max3(m1, s[i + 2], s[i + 3]);
+                    m2 = max3(m2, s[i + 4], s[i + 5]);
+                    m3 = max3(m3, s[i + 6], s[i + 7]);
                 }
-                m0 = max3_nan(m0, s[kKeys - 4], s[kKeys - 3]);
-                m1 = max3_nan(m1, s[kKeys - 2], s[kKeys - 1]);
-                // whole numbers (ex2_fma); a row that is no query stands at 0 and asks for nothing
-                const float top = live ? ceilf(max_nan(max3_nan(m0, m1, m2), m3) * a.scale) : 0.0f;
-                const bool grown = !(top <= ref + kLazy);  // each row for itself: no result depends on a neighbour
+                m0 = max3(m0, s[kKeys - 4], s[kKeys - 3]);
+                m1 = max3(m1, s[kKeys - 2], s[kKeys - 1]);
+                const float top = fmaxf(max3(m0, m1, m2), m3) * a.scale;
+                const bool grown = top > ref + kLazy;  // each row for itself: no result depends on a neighbour
                 if (j == 0) ref = top;
                 else if (__any_sync(0xffffffffu, grown)) {
-                    // not under a product that is still adding to the outputs
-                    if (!(fine = all_wait(bar(B_O + 2 * t + (buf ^ 1u)), phase_o >> (buf ^ 1u) & 1u))) break;
-                    tc_after();
-                    const float f = grown ? ex2(ref - max_nan(ref, top)) : 1.0f;
-                    if (grown) ref = max_nan(ref, top);
+                    // not under a product that is still adding to the outputs: the other buffer's next logits
+                    // come after it (with one buffer, these did)
+                    if (NB == 2) {
+                        if (!(fine = all_wait(bar(B_S + NB * t + (buf ^ 1u)), phase >> (buf ^ 1u) & 1u))) break;
+                        tc_after();
+                    }
+                    const float f = grown ? ex2(ref - top) : 1.0f;
+                    if (grown) ref = top;
                     sum *= f;
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tm_load(to + 32 * c, o);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tm_load16(to + 16 * c, o);
                         tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tm_store(to + 32 * c, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tm_store16(to + 16 * c, o);
                     }
                 }
                 const float from = ref == -INFINITY ? 0.0f : ref;
                 const float2 scale2 = make_float2(a.scale, a.scale), from2 = make_float2(-from, -from);
                 float2 total = make_float2(0.0f, 0.0f);
-                // Of 16 logits kFma take the FMA pipe: ex2 alone has 16 lanes an SM and clock.  Tiles with a
-                // mask, and rows with an infinity, a NaN or a maximum past 2^20 in them, do without.
-                const bool careful = masked || !(fabsf(from) <= 1048576.0f);
-                if (careful) {
 #pragma unroll
-                    for (int i = 0; i < kKeys; i += 2) {
-                        const float2 y = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
-                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                        total = __fadd2_rn(total, e);
-                        x[i / 2] = pack<BF>(e.x, e.y);
-                    }
-                } else {
-                    const float least = (from - 126.0f) * inv_scale;
-                    const float2 shift = make_float2(kRound - from, kRound - from);
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 2) {
-                        float2 e;
-                        if (i % 16 < P::kFma) e = ex2_fma(make_float2(fmaxf(s[i], least), fmaxf(s[i + 1], least)), scale2, shift);
-                        else {
-                            const float2 y = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
-                            e = make_float2(ex2(y.x), ex2(y.y));
-                        }
-                        total = __fadd2_rn(total, e);
-                        x[i / 2] = pack<BF>(e.x, e.y);
-                    }
+                for (int i = 0; i < kKeys; i += 2) {
+                    const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
+                    const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
+                    total = __fadd2_rn(total, e);
+                    x[i / 2] = pack<BF>(e.x, e.y);
                 }
                 sum += total.x + total.y;
                 tm_store(ts, x);
-                if constexpr (kKeys == 96) tm_store16(ts + 32, x + 32);
                 tc_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(bar(B_P + 2 * t + buf));
-                phase_o ^= 1u << buf;
+                if (lane == 0) bar_arrive(bar(B_P + NB * t + buf));
             }
             if (fine && sp.count) {
-                if (sp.tiles) {
-                    const uint32_t buf = (sp.tiles - 1) & 1;
-                    if (!(fine = all_wait(bar(B_O + 2 * t + buf), phase_o >> buf & 1u))) break;
-                    tc_after();
+                // the last products of every buffer
+                for (uint32_t buf = 0; buf < NB && (int32_t)buf < sp.tiles && fine; ++buf) {
+                    fine = all_wait(bar(B_S + NB * t + buf), phase >> buf & 1u);
+                    phase ^= 1u << buf;
                 }
-                const bool none = sees == 0 || sum == 0.0f;
+                if (!fine) break;
+                tc_after();
+                const bool none = sees == 0;
                 const float inv = none ? 0.0f : 1.0f / sum;
-                const uint32_t flagged = bad_flag[n & 1];
-                const uint64_t at = (uint64_t)(it.token + t * (int32_t)per + (int32_t)p) * a.q_heads + it.head * a.group + g;
-                uint16_t *out = static_cast<uint16_t *>(a.out) + at * D;
+                const uint32_t flagged = bad_flag[n % kDeal];
+                // 32 dimensions at a time, turned through shared memory so that four lanes write 64 bytes of a row
+                unsigned char *turn = sm + P::kOut + warp * 2048;
+                const int64_t first_row = (int64_t)(it.token + t * (int32_t)per) * a.q_heads + it.head * a.group;
+                int64_t to_row[4];  // of the rows that this lane writes for: 8 i + lane / 4 of the warp's, -1 for none
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t r = (warp & 3u) * 32 + 8 * i + lane / 4, rp = r / a.group;
+                    to_row[i] = rp < (uint32_t)sp.count ? first_row + (int64_t)rp * a.q_heads + r % a.group : -1;
+                }
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
                     if (sp.tiles) {
                         tm_load(to + 32 * c, o);
                         tc_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0;
                     }
-                    if (sees == 0) {
+                    if (none) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = 0;
                     }
                     if (flagged) {
                         // infinities and NaN that this row sees: keys from `key0` on were looked through
-                        const int32_t key0 = max(0, (span(it, 0).first / kKeys)) * kKeys;
-                        const uint16_t *first = bad + (n & 1) * 3 * D + 32 * c;
+                        const int32_t key0 = max(0, span(it, 0).first / kKeys) * kKeys;
+                        const uint16_t *first = bad + n % kDeal * 3 * D + 32 * c;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
@@ -420,164 +430,34 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
                         }
                     }
-                    if (live) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint4 v;
-                            v.x = pack<BF>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                            v.y = pack<BF>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                            v.z = pack<BF>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                            v.w = pack<BF>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(out + 32 * c + i) = v;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 v;
+                        v.x = pack<BF>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+                        v.y = pack<BF>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+                        v.z = pack<BF>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+                        v.w = pack<BF>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+                        *reinterpret_cast<uint4 *>(turn + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = v;
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t r = 8 * i + lane / 4;
+                        const uint4 v = *reinterpret_cast<uint4 *>(turn + r * 64 + (((lane & 3u) ^ (r >> 1 & 3u)) << 4));
+                        if (to_row[i] >= 0)
+                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to_row[i] * D + 32 * c + 8 * (lane & 3u)) = v;
+                    }
+                    __syncwarp();
                 }
-                if (live && a.lse) a.lse[at] = none ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                if (live && a.lse) a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;
             taken(n);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 8) {
-            // ---- loads ----
-            // A tile that warps 12-15 look through lands on its slot's raw barrier, and they arrive on the
-            // full one when they are done with it.
-            uint32_t slot = 0, free_phase = 1, q_phase[2] = {1, 1}, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
-            Item it;
-            bool fine = true;
-            for (uint32_t n = 0; fine && next(n, it); ++n) {
-                const TileSpan s0 = span(it, 0), s1 = span(it, 1);
-                const int32_t tiles = max(s0.tiles, s1.tiles);
-                if (lane == 0) {
-                    auto load_q = [&](int t) {
-                        if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase[t], stop))) return;
-                        q_phase[t] ^= 1;
-                        bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
-                        for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(base + P::kQ + t * P::kQTile + c * P::kQChunk, &mq, bar(B_QFULL + t), 64 * c,
-                                 it.head * (int32_t)a.group, it.token + t * (int32_t)per);
-                    };
-                    auto load_kv = [&](const CUtensorMap *map, int32_t j, bool look) {
-                        if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
-                        const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
-                        bar_expect(on, P::kTile);
-                        if (!look)
-                            for (int i = 0; i < 3; ++i) bar_arrive(on);
-                        for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(base + P::kRing + slot * P::kTile + c * P::kChunk, map, on, 64 * c, it.head,
-                                 it.key + j * kKeys);
-                        issued |= bit;
-                        raw = look ? raw | bit : raw & ~bit;
-                        full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
-                        raw_phase ^= look ? bit : 0;
-                        if (++slot == P::kSlots) slot = 0, free_phase ^= 1;
-                    };
-                    if (s0.tiles) load_q(0);
-                    if (tiles) load_kv(&mk, 0, false);
-                    if (s1.tiles) load_q(1);
-                    if (tiles > 1) load_kv(&mk, 1, false);
-                    for (int32_t j = 0; j < tiles && fine; ++j) {
-                        load_kv(&mv, j, (j + 1) * kKeys > s0.first);
-                        if (j + 2 < tiles) load_kv(&mk, j + 2, false);
-                    }
-                }
-                fine = __shfl_sync(0xffffffffu, fine, 0);
-                taken(n);
-            }
-            // copies in flight land before the CTA ends (they have, unless a wait ran out)
-            if (lane == 0 && *stop) {
-                uint32_t none = 0;
-                for (uint32_t i = 0; i < P::kSlots; ++i)
-                    if (issued >> i & 1u)
-                        bar_wait(bar((raw >> i & 1u ? B_RAW : B_FULL) + i), raw >> i & 1u ? ~raw_phase >> i & 1u : full_phase >> i & 1u,
-                                 &none);
-                for (int t = 0; t < 2; ++t) bar_wait(bar(B_QFULL + t), q_phase[t] ^ 1u, &none);
-            }
-        } else if (warp <= 10) {
-            // ---- products of tile t: the warp stays together, one lane issues ----
-            const int t = (int)warp - 9;
-            uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;
-            constexpr uint32_t ID_S = product(BF, 0, P::kKeys), ID_O = product(BF, 1, D);
-            const uint32_t q_at = base + P::kQ + t * P::kQTile, s_at = tmem + 2 * t * kKeys, o_at = tmem + P::kColO + t * D;
-            Item it;
-            bool fine = true;
-            for (uint32_t n = 0; fine && next(n, it); ++n) {
-                const TileSpan sp = span(it, t), other = span(it, t ^ 1);
-                const int32_t tiles = max(sp.tiles, other.tiles);
-                auto advance = [&]() {
-                    if (++slot == P::kSlots) slot = 0, full_phase ^= 1;
-                };
-                // the logits of K tile j (in slot k), and the slot's release
-                auto logits = [&](uint32_t k, int32_t j) {
-                    if (!elect()) return;
-                    if (j >= sp.tiles) {
-                        bar_arrive(bar(B_FREE + k));
-                        return;
-                    }
-                    const uint32_t q = operand(q_at, 0), key = operand(base + P::kRing + k * P::kTile, 0), d = s_at + (j & 1) * kKeys;
-#pragma unroll
-                    for (uint32_t c = 0; c < P::kChunks; ++c)
-#pragma unroll
-                        for (uint32_t s = 0; s < 4; ++s)
-                            mma_ss(d, q + (c * P::kQChunk + 32 * s) / 16, key + (c * P::kChunk + 32 * s) / 16, ID_S, c | s);
-                    tc_commit(bar(B_S + 2 * t + (j & 1)));
-                    tc_commit(bar(B_FREE + k));
-                    if (j + 1 == sp.tiles) tc_commit(bar(B_QFREE + t));
-                };
-                if (sp.tiles) {
-                    if (!(fine = all_wait(bar(B_QFULL + t), q_phase))) break;
-                    q_phase ^= 1;
-                }
-                // the logits run two tiles ahead of the outputs
-                for (int32_t j = 0; j < 2 && j < tiles; ++j) {
-                    if (!(fine = all_wait(bar(B_FULL + slot), full_phase))) break;
-                    tc_after();
-                    logits(slot, j);
-                    __syncwarp();
-                    advance();
-                }
-                for (int32_t j = 0; j < tiles && fine; ++j) {
-                    const uint32_t v = slot;
-                    if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
-                    advance();
-                    const uint32_t k = slot;
-                    const bool more = j + 2 < tiles;
-                    if (more) {
-                        if (!(fine = all_wait(bar(B_FULL + k), full_phase))) break;
-                        advance();
-                    }
-                    const uint32_t buf = j & 1;
-                    if (j < sp.tiles) {
-                        if (!(fine = all_wait(bar(B_P + 2 * t + buf), p_phase >> buf & 1u))) break;
-                        p_phase ^= 1u << buf;
-                    }
-                    tc_after();
-                    if (elect()) {
-                        if (j < sp.tiles) {
-                            const uint32_t val = operand(base + P::kRing + v * P::kTile, P::kChunk), pr = s_at + buf * kKeys;
-#pragma unroll
-                            for (uint32_t s = 0; s < P::kKeys / 16; ++s)
-                                mma_ts(o_at, pr + 8 * s, val + s * 128, ID_O, j | (int32_t)s);
-                            tc_commit(bar(B_O + 2 * t + buf));
-                            tc_commit(bar(B_FREE + v));
-                        } else bar_arrive(bar(B_FREE + v));
-                    }
-                    __syncwarp();
-                    if (more) logits(k, j + 2);
-                    __syncwarp();
-                }
-                if (fine) taken(n);
-            }
-            // products in flight end before the tensor memory is given back
-            __syncwarp();
-            if (*stop && elect()) {
-                uint32_t none = 0;
-                tc_commit(bar(B_END + t));
-                bar_wait(bar(B_END + t), 0, &none);
-            }
-        } else if (warp == 11) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kRest));
+        if (warp == W_LOAD) {
             // ---- the deal ----
             // Sequence s has ceil(queries / (tiles per item)) blocks; block b of every sequence that
             // has it is level b.  Items go by falling level (the last blocks see the most keys), a level's
@@ -593,26 +473,36 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 return (q1 - q0 + block - 1) / block;
             };
-            int32_t level = 0;
-            for (uint32_t s = lane; s < a.sequences; s += 32) level = max(level, blocks_of(s));
-            level = __reduce_max_sync(0xffffffffu, level);
-            uint64_t before = 0, upto = 0;  // items of levels above this one, and with it
-            uint64_t r = blockIdx.x;
-            for (uint32_t n = 0;; ++n) {
-                r = (uint64_t)n * gridDim.x + (n & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                while (upto <= r && level > 0) {
-                    --level;
-                    before = upto;
-                    uint32_t c = 0;
-                    for (uint32_t s = lane; s < a.sequences; s += 32) c += blocks_of(s) > level;
-                    upto += (uint64_t)__reduce_add_sync(0xffffffffu, c) * a.kv_heads;
-                }
+            // (the blocks of the first 32 sequences stay in the lanes)
+            const int32_t mine = blocks_of(lane);
+            auto blocks_at = [&](uint32_t s) { return s < 32 ? mine : blocks_of(s); };
+            // blocks at or above a level, over all sequences
+            auto above = [&](int32_t level) {
+                uint32_t c = 0;
+                for (uint32_t s = lane; s < a.sequences; s += 32) c += (uint32_t)max(0, blocks_at(s) - level);
+                return __reduce_add_sync(0xffffffffu, c);
+            };
+            int32_t high = 0;  // the blocks of the longest sequence
+            for (uint32_t s = lane; s < a.sequences; s += 32) high = max(high, blocks_at(s));
+            high = __reduce_max_sync(0xffffffffu, high);
+            const uint64_t upto = (uint64_t)above(0) * a.kv_heads;
+            auto deal = [&](uint32_t n) {
+                const uint64_t r = (uint64_t)n * gridDim.x + (n & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 Item it{};
                 if (r < upto) {
-                    uint32_t nth = (uint32_t)((r - before) / a.kv_heads);
-                    it.head = (int32_t)((r - before) % a.kv_heads);
+                    // the highest level with more than r / heads blocks at or above it; levels only fall from item to item
+                    const uint32_t rank = (uint32_t)(r / a.kv_heads);
+                    it.head = (int32_t)(r % a.kv_heads);
+                    int32_t level = 0;
+                    for (int32_t top = high; top - level > 1;) {
+                        const int32_t mid = (level + top) / 2;
+                        if (above(mid) > rank) level = mid;
+                        else top = mid;
+                    }
+                    high = level + 1;
+                    uint32_t nth = rank - above(level + 1);
                     for (uint32_t s0 = 0; s0 < a.sequences; s0 += 32) {
-                        const uint32_t has = __ballot_sync(0xffffffffu, blocks_of(s0 + lane) > level);
+                        const uint32_t has = __ballot_sync(0xffffffffu, (s0 ? blocks_of(s0 + lane) : mine) > level);
                         const uint32_t c = __popc(has);
                         if (nth >= c) {
                             nth -= c;
@@ -629,42 +519,184 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         break;
                     }
                 }
-                if (n >= 2 && !all_wait(bar(B_TAKEN + (n & 1)), ((n >> 1) & 1) ^ 1)) break;
+                if (n >= kDeal && !all_wait(bar(B_TAKEN + n % kDeal), (n / kDeal & 1) ^ 1)) return;
                 if (lane == 0) {
-                    volatile Item &d = items[n & 1];
+                    volatile Item &d = items[n % kDeal];
                     d.token = it.token, d.count = it.count, d.pos = it.pos, d.head = it.head;
                     d.key = it.key, d.keys = it.keys, d.shift = it.shift;
-                    bad_flag[n & 1] = 0;
-                    bar_arrive(bar(B_ITEM + (n & 1)));
+                    bad_flag[n % kDeal] = 0;
+                    bar_arrive(bar(B_ITEM + n % kDeal));
                 }
                 __syncwarp();
-                if (it.count == 0) break;
+            };
+            // ---- loads ----
+            // A stage that the last warp looks through lands on its raw barrier, and that warp arrives on the full
+            // one when it is done with it.
+            uint32_t slot = 0, free_phase = 1, q_phase = (1u << NT) - 1, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
+            uint32_t q_issued = 0;
+            Item it;
+            bool fine = true;
+            deal(0);
+            for (uint32_t n = 0; fine && next(n, it); ++n) {
+                deal(n + 1);
+                const int32_t tiles = tiles_of(it), first = span(it, 0).first;
+                if (lane == 0) {
+                    auto load_q = [&](int t) {
+                        if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase >> t & 1u, stop))) return;
+                        q_phase ^= 1u << t;
+                        q_issued |= 1u << t;
+                        bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+                            tma3(base + P::kQ + t * P::kQTile + c * P::kQChunk, &mq, bar(B_QFULL + t), 64 * c,
+                                 it.head * (int32_t)a.group, it.token + t * (int32_t)per);
+                    };
+                    // first the K tiles that logits run ahead by, then V j and K j + NB: rows of tiles, -1 for none
+                    auto load = [&](const CUtensorMap *map, int32_t one, int32_t two, bool look) {
+                        if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
+                        const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
+                        bar_expect(on, P::kTile * (two < 0 ? 1u : 2u));
+                        const uint32_t dst = base + P::kRing + slot * 2 * P::kTile;
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+                            tma3(dst + c * P::kChunk, map, on, 64 * c, it.head, it.key + one * kKeys);
+                        if (two >= 0)
+                            for (uint32_t c = 0; c < P::kChunks; ++c)
+                                tma3(dst + P::kTile + c * P::kChunk, &mk, on, 64 * c, it.head, it.key + two * kKeys);
+                        issued |= bit;
+                        raw = look ? raw | bit : raw & ~bit;
+                        full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
+                        raw_phase ^= look ? bit : 0;
+                        if (++slot == P::kStages) slot = 0, free_phase ^= 1;
+                    };
+                    if (span(it, 0).tiles) load_q(0);
+                    if (tiles) load(&mk, 0, NB == 2 && tiles > 1 ? 1 : -1, false);
+                    for (uint32_t t = 1; t < NT; ++t)
+                        if (span(it, (int)t).tiles) load_q((int)t);
+                    for (int32_t j = 0; j < tiles && fine; ++j)
+                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (j + 1) * kKeys > first);
+                }
+                fine = __shfl_sync(0xffffffffu, fine, 0);
+            }
+            // copies in flight land before the CTA ends (they have, unless a wait ran out)
+            if (lane == 0 && *stop) {
+                uint32_t none = 0;
+                for (uint32_t i = 0; i < P::kStages; ++i)
+                    if (issued >> i & 1u)
+                        bar_wait(bar((raw >> i & 1u ? B_RAW : B_FULL) + i), raw >> i & 1u ? ~raw_phase >> i & 1u : full_phase >> i & 1u,
+                                 &none);
+                for (uint32_t t = 0; t < NT; ++t)
+                    if (q_issued >> t & 1u) bar_wait(bar(B_QFULL + t), q_phase >> t & 1u, &none);
+            }
+        } else if (warp < W_ENDS) {
+            // ---- products of every second row tile: the warp stays together, one lane issues ----
+            const uint32_t half = warp - W_MMA;
+            uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;  // p_phase: a bit for each buffer of every tile
+            constexpr uint32_t ID_S = product(BF, 0, P::kKeys), ID_O = product(BF, 1, D), MINE = NT / 2;
+            Item it;
+            bool fine = true;
+            for (uint32_t n = 0; fine && next(n, it); ++n) {
+                const int32_t tiles = tiles_of(it);
+                if (!tiles) {
+                    taken(n);
+                    continue;
+                }
+                int32_t mine[MINE];
+#pragma unroll
+                for (uint32_t i = 0; i < MINE; ++i) mine[i] = span(it, (int)(half + 2 * i)).tiles;
+                auto advance = [&]() {
+                    if (++slot == P::kStages) slot = 0, full_phase ^= 1;
+                };
+                // the logits of row tile t and K tile j, which lies at `k_at`
+                auto logits = [&](uint32_t t, uint32_t k_at, int32_t j) {
+                    const uint32_t q = operand(base + P::kQ + t * P::kQTile, 0), key = operand(k_at, 0);
+                    const uint32_t d = tmem + (NB * t + j % NB) * kKeys;
+#pragma unroll
+                    for (uint32_t c = 0; c < P::kChunks; ++c)
+#pragma unroll
+                        for (uint32_t s = 0; s < 4; ++s)
+                            mma_ss(d, q + (c * P::kQChunk + 32 * s) / 16, key + (c * P::kChunk + 32 * s) / 16, ID_S, c | s);
+                };
+                // logits run NB tiles ahead of the outputs
+                if (!(fine = all_wait(bar(B_FULL + slot), full_phase))) break;
+#pragma unroll
+                for (uint32_t i = 0; i < MINE; ++i) {
+                    if (!mine[i]) continue;
+                    const uint32_t t = half + 2 * i;
+                    if (!(fine = all_wait(bar(B_QFULL + t), q_phase >> t & 1u))) break;
+                    q_phase ^= 1u << t;
+                    tc_after();
+                    if (elect()) {
+                        const uint32_t at = base + P::kRing + slot * 2 * P::kTile;
+                        logits(t, at, 0);
+                        tc_commit(bar(B_S + NB * t));
+                        if (NB == 2 && mine[i] > 1) {
+                            logits(t, at + P::kTile, 1);
+                            tc_commit(bar(B_S + NB * t + 1));
+                        }
+                        if (mine[i] <= (int32_t)NB) tc_commit(bar(B_QFREE + t));
+                    }
+                    __syncwarp();
+                }
+                if (!fine) break;
+                if (elect()) tc_commit(bar(B_FREE + slot));
+                __syncwarp();
+                advance();
+                for (int32_t j = 0; j < tiles; ++j) {
+                    const uint32_t v = slot, at = base + P::kRing + v * 2 * P::kTile;
+                    if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
+                    advance();
+#pragma unroll
+                    for (uint32_t i = 0; i < MINE; ++i) {
+                        if (j >= mine[i]) continue;
+                        const uint32_t t = half + 2 * i, tb = NB * t + j % NB;
+                        if (!(fine = all_wait(bar(B_P + tb), p_phase >> tb & 1u))) break;
+                        p_phase ^= 1u << tb;
+                        tc_after();
+                        if (elect()) {
+                            const uint32_t val = operand(at, P::kChunk), pr = tmem + tb * kKeys, o = tmem + P::kColO + t * D;
+#pragma unroll
+                            for (uint32_t s = 0; s < P::kKeys / 16; ++s) mma_ts(o, pr + 8 * s, val + s * 128, ID_O, j | (int32_t)s);
+                            if (j + (int32_t)NB < mine[i]) logits(t, at + P::kTile, j + (int32_t)NB);
+                            tc_commit(bar(B_S + tb));  // at the end with nothing but the outputs before it
+                            if (j + (int32_t)NB + 1 == mine[i]) tc_commit(bar(B_QFREE + t));
+                        }
+                        __syncwarp();
+                    }
+                    if (!fine) break;
+                    if (elect()) tc_commit(bar(B_FREE + v));
+                    __syncwarp();
+                }
+                if (fine) taken(n);
+            }
+            // products in flight end before the tensor memory is given back
+            __syncwarp();
+            if (*stop && elect()) {
+                uint32_t none = 0;
+                tc_commit(bar(B_END + half));
+                bar_wait(bar(B_END + half), 0, &none);
             }
         } else {
-            // ---- V tiles that not every row sees: each of four warps its share of the dimensions ----
-            constexpr uint32_t kUnits = D / 8 / 4;  // 16-byte units of a row in a warp's share
-            const uint32_t share = warp - 12;
+            // ---- V tiles that not every row sees ----
             uint32_t slot = 0, raw_phase = 0;
             Item it;
             bool fine = true;
             for (uint32_t n = 0; fine && next(n, it); ++n) {
-                const TileSpan s0 = span(it, 0), s1 = span(it, 1);
-                const int32_t tiles = max(s0.tiles, s1.tiles), begin = max(0, s0.first / kKeys);
-                uint16_t *first = bad + (n & 1) * 3 * D;
-                for (uint32_t i = lane; i < 3 * D / 4; i += 32) first[i / (D / 4) * D + share * (D / 4) + i % (D / 4)] = 0xffff;
+                const TileSpan s0 = span(it, 0);
+                const int32_t tiles = tiles_of(it), begin = max(0, s0.first / kKeys);
+                uint16_t *first = bad + n % kDeal * 3 * D;
+                if (begin < tiles)
+                    for (uint32_t i = lane; i < 3 * D; i += 32) first[i] = 0xffff;
                 for (int32_t j = begin; j < tiles; ++j) {
                     if ((j + 1) * kKeys <= s0.first) continue;
-                    // in the order K 0, K 1, V 0, K 2, V 1, .. of the item's loads
-                    const uint32_t v = (slot + (uint32_t)min(2 * j + 2, 2 * tiles - 1)) % P::kSlots;
+                    const uint32_t v = (slot + 1 + (uint32_t)j) % P::kStages;  // past the stage of the first K tiles
                     if (!(fine = all_wait(bar(B_RAW + v), raw_phase >> v & 1u))) break;
                     raw_phase ^= 1u << v;
-                    unsigned char *tile = sm + P::kRing + v * P::kTile;
+                    unsigned char *tile = sm + P::kRing + v * 2 * P::kTile;
                     const int32_t rows = min(kKeys, it.keys - j * kKeys);
                     uint32_t found = 0;
                     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
 #pragma unroll 4
-                    for (uint32_t i = lane; i < P::kKeys * kUnits; i += 32) {
-                        const uint32_t r = i / kUnits, u = share * kUnits + i % kUnits;
+                    for (uint32_t i = lane; i < P::kKeys * D / 8; i += 32) {
+                        const uint32_t r = i / (D / 8), u = i % (D / 8);
                         uint4 *w = reinterpret_cast<uint4 *>(tile + u / 8 * P::kChunk + r * 128 + ((u % 8 ^ (r & 7)) << 4));
                         if ((int32_t)r >= rows) *w = make_uint4(0, 0, 0, 0);
                         else {
@@ -676,8 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                     if (__any_sync(0xffffffffu, found)) {
                         __syncwarp();
-                        for (uint32_t i = lane; i < (uint32_t)D / 4; i += 32) {
-                            const uint32_t d = share * (D / 4) + i;
+                        for (uint32_t d = lane; d < (uint32_t)D; d += 32) {
                             for (int32_t k = 0; k < rows; ++k) {
                                 uint16_t *w = reinterpret_cast<uint16_t *>(tile + d / 64 * P::kChunk + k * 128 +
                                                                            (((d % 64 / 8) ^ (k & 7)) << 4)) + d % 8;
@@ -689,13 +720,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                 if (at < first[kind * D + d]) first[kind * D + d] = (uint16_t)at;
                             }
                         }
-                        if (lane == 0) bad_flag[n & 1] = 1;
+                        if (lane == 0) bad_flag[n % kDeal] = 1;
                     }
                     fence_async();
                     __syncwarp();
                     if (lane == 0) bar_arrive(bar(B_FULL + v));
                 }
-                slot = (slot + 2 * (uint32_t)tiles) % P::kSlots;
+                slot = (slot + (uint32_t)(tiles ? tiles + 1 : 0)) % P::kStages;
                 if (fine) taken(n);
             }
         }
@@ -705,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     tc_before();
     __syncthreads();
     if (threadIdx.x == 0 && *stop) atomicOr(a.status, kStatusTimeout);
-    if (warp == 8) {
+    if (warp == W_LOAD) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
@@ -763,11 +794,12 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
         !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, P::kKeys) ||
         !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, P::kKeys))
         return cudaErrorInvalidValue;
-    // two tiles an item share K and V loads; where that leaves SMs without work, one
-    const uint64_t items2 = a.kv_heads * ((a.q_tokens + 2 * per - 1) / (2 * per));
-    a.tiles = items2 >= (uint64_t)sms ? 2 : 1;
-    const uint64_t most = a.kv_heads * ((a.q_tokens + a.tiles * per - 1) / (a.tiles * per) + a.sequences);
-    kernel<<<(uint32_t)(most < (uint64_t)sms ? most : sms), kThreads, P::kTotal, s>>>(a, mq, mk, mv);
+    // The row tiles of an item share its K and V loads: as many as still leave every SM an item.
+    auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per)); };
+    a.tiles = P::kTiles;
+    while (a.tiles > 1 && items(a.tiles) < (uint64_t)sms) a.tiles /= 2;
+    const uint64_t most = items(a.tiles) + (uint64_t)a.kv_heads * a.sequences;
+    kernel<<<(uint32_t)(most < (uint64_t)sms ? most : sms), P::kThreads, P::kTotal, s>>>(a, mq, mk, mv);
     return cudaGetLastError();
 }
 
