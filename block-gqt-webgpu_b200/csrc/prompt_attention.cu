@@ -189,8 +189,9 @@ struct Plan {
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
     static constexpr uint32_t kStages = D == 128 ? 4 : 7;          // of two K or V tiles in the ring
     static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kAfter = kRing + kStages * 2 * kTile;
-    static constexpr uint32_t kOut = kAfter;                       // [softmax warps][32 rows][64 bytes] of outputs
-    static constexpr uint32_t kBad = kOut + 4 * kTiles * 2048;                         // [kDeal items][3 kinds][D] first keys
+    static constexpr int kTurn = D == 64 ? 16 : 32;                // dimensions of an output row stored at a time (registers)
+    static constexpr uint32_t kOut = kAfter;                       // [softmax warps][32 rows][kTurn] outputs
+    static constexpr uint32_t kBad = kOut + 4 * kTiles * 64 * kTurn;                    // [kDeal items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + kDeal * 3 * D * 2;   // [kDeal] Item
     static constexpr uint32_t kBars = kItems + kDeal * 32;
     static constexpr uint32_t kBarCount = 3 * kStages + 2 * kTiles + 2 * kTiles * kBufs + 2 * kDeal + 2;
@@ -399,53 +400,53 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 const bool none = sees == 0;
                 const float inv = none ? 0.0f : 1.0f / sum;
                 const uint32_t flagged = bad_flag[n % kDeal];
-                // 32 dimensions at a time, turned through shared memory so that four lanes write 64 bytes of a row
-                unsigned char *turn = sm + P::kOut + warp * 2048;
+                // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
+                constexpr int kW = P::kTurn, kL = kW / 8;
+                unsigned char *turn = sm + P::kOut + warp * 64 * kW;
                 const int64_t first_row = (int64_t)(it.token + t * (int32_t)per) * a.q_heads + it.head * a.group;
-                int64_t to_row[4];  // of the rows that this lane writes for: 8 i + lane / 4 of the warp's, -1 for none
+                // 16-byte chunk c of row r: a phase of eight lanes meets 128 different bytes, writing and reading
+                auto chunk = [&](uint32_t r, uint32_t c) { return turn + r * 2 * kW + ((c ^ r / (8 / kL) % kL) << 4); };
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t r = (warp & 3u) * 32 + 8 * i + lane / 4, rp = r / a.group;
-                    to_row[i] = rp < (uint32_t)sp.count ? first_row + (int64_t)rp * a.q_heads + r % a.group : -1;
-                }
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
+                for (int c = 0; c < D / kW; ++c) {
+                    uint32_t o[kW];
                     if (sp.tiles) {
-                        tm_load(to + 32 * c, o);
+                        if constexpr (kW == 32) tm_load(to + kW * c, o);
+                        else tm_load16(to + kW * c, o);
                         tc_wait_ld();
                     }
                     if (none) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0;
+                        for (int i = 0; i < kW; ++i) o[i] = 0;
                     }
                     if (flagged) {
                         // infinities and NaN that this row sees: keys from `key0` on were looked through
                         const int32_t key0 = max(0, span(it, 0).first / kKeys) * kKeys;
-                        const uint16_t *first = bad + n % kDeal * 3 * D + 32 * c;
+                        const uint16_t *first = bad + n % kDeal * 3 * D + kW * c;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
+                        for (int i = 0; i < kW; ++i) {
                             const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
                             if (key0 + first[2 * D + i] < sees || (up && down)) o[i] = 0x7fc00000u;
                             else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < kL; ++i) {
                         uint4 v;
                         v.x = pack<BF>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
                         v.y = pack<BF>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
                         v.z = pack<BF>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
                         v.w = pack<BF>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-                        *reinterpret_cast<uint4 *>(turn + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = v;
+                        *reinterpret_cast<uint4 *>(chunk(lane, i)) = v;
                     }
                     __syncwarp();
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t r = 8 * i + lane / 4;
-                        const uint4 v = *reinterpret_cast<uint4 *>(turn + r * 64 + (((lane & 3u) ^ (r >> 1 & 3u)) << 4));
-                        if (to_row[i] >= 0)
-                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to_row[i] * D + 32 * c + 8 * (lane & 3u)) = v;
+                    for (int i = 0; i < kL; ++i) {
+                        const uint32_t r = (32 / kL) * i + lane / kL, tr = (warp & 3u) * 32 + r, rp = tr / a.group;
+                        const uint4 v = *reinterpret_cast<uint4 *>(chunk(r, lane % kL));
+                        if (rp < (uint32_t)sp.count) {
+                            const int64_t at = first_row + (int64_t)rp * a.q_heads + tr % a.group;
+                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at * D + kW * c + 8 * (lane % kL)) = v;
+                        }
                     }
                     __syncwarp();
                 }
