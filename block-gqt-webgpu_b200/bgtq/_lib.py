@@ -79,7 +79,7 @@ class PromptDesc(C.Structure):
         (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
                                  "v_token_stride", "v_head_stride")] + [
         ("starts", C.c_void_p), ("key_starts", C.c_void_p), ("causal", C.c_int), ("scale", C.c_float),
-        ("out", C.c_void_p), ("lse", C.c_void_p)]
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 # (name, restype, argtypes) for every exported symbol declared in include/bgtq.h
@@ -153,6 +153,7 @@ SIGNATURES = {
     "bgtq_paged_read": (I32, [P, P, U64, P, P, I32, P]),
     "bgtq_paged_attend_workspace": (I32, [P, U32, P]),
     "bgtq_paged_attend": (I32, [P, P, I32, U32, U32, I64, I64, P, I64, U32, P, C.c_float, P, P, P, SZ, P]),
+    "bgtq_prompt_workspace": (I32, [C.c_int, U32, P]),
     "bgtq_prompt_attend": (I32, [P, P]),
 }
 

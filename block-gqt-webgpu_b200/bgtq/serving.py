@@ -163,6 +163,20 @@ class PagedCache:
         return have
 
 
+_prompt_work = {}
+
+
+def _prompt_workspace(device: int, dim: int, stream: int):
+    """The stream's own workspace (calls on different streams may overlap)."""
+    have = _prompt_work.get((device, dim, stream))
+    if have is None:
+        need = C.c_size_t()
+        _lib.call("bgtq_prompt_workspace", device, dim, C.byref(need))
+        have = torch.zeros(need.value, dtype=torch.uint8, device=torch.device("cuda", device))
+        _prompt_work[device, dim, stream] = have
+    return have
+
+
 def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scale: float | None = None, out=None,
                      lse: bool = False):
     """Attention of a packed batch of prompts: q [tokens, q_heads, dim], k and v [key tokens,
@@ -205,9 +219,12 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
 
     (q, *sq), (k, *sk), (v, *sv) = even(q), even(k), even(v)
     dev = q.device.index
+    st = _stream(dev)
+    work = _prompt_workspace(dev, q.shape[2], st)
     p = _lib.PromptDesc(dev, _DTYPE[q.dtype], starts.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], q.shape[0],
                         k.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), *sq, *sk, *sv, starts.data_ptr(),
                         None if key_starts is None else key_starts.data_ptr(), int(bool(causal)),
-                        0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr())
-    _lib.call("bgtq_prompt_attend", C.byref(p), _stream(dev))
+                        0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr(),
+                        work.data_ptr(), work.numel())
+    _lib.call("bgtq_prompt_attend", C.byref(p), st)
     return (out, sums) if lse else out

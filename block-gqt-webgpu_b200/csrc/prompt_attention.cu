@@ -12,8 +12,7 @@
 //   softmax     four warps a row tile, a thread a row: logits out of tensor memory, mask, running
 //               maximum, probabilities back into tensor memory (as 16-bit pairs in the columns
 //               where the logits were), and the outputs at the end
-//   deal, loads one warp: the items in order of falling length, dealt back and forth over the
-//               CTAs, and the TMA loads of Q, K and V (128-byte swizzle) into a ring of stages
+//   deal, loads one warp: this CTA's share of the items, and the TMA loads of Q, K and V (128-byte swizzle) into a ring of stages
 //   products    two warps, each for half of the row tiles: S = Q K^T (operands in shared memory)
 //               ahead of softmax and O += P V (P in tensor memory, V as it lies), FP32
 //               accumulators in tensor memory.  The warp stays together and one lane issues, so
@@ -30,6 +29,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "serving.h"
 
 namespace bgtq {
@@ -39,6 +40,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kRows = 128;
 constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
 constexpr uint32_t kDeal = 4;            // items dealt ahead
+constexpr int64_t kItemCost = 384;       // what an item costs beside its keys, in keys: queries, outputs, joining
+constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while where items are few
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
 // ---- device helpers -----------------------------------------------------------------------
@@ -193,22 +196,25 @@ struct Plan {
     static constexpr uint32_t kOut = kAfter;                       // [softmax warps][32 rows][kTurn] outputs
     static constexpr uint32_t kBad = kOut + 4 * kTiles * 64 * kTurn;                    // [kDeal items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + kDeal * 3 * D * 2;   // [kDeal] Item
-    static constexpr uint32_t kBars = kItems + kDeal * 32;
-    static constexpr uint32_t kBarCount = 3 * kStages + 2 * kTiles + 2 * kTiles * kBufs + 2 * kDeal + 2;
+    static constexpr uint32_t kBars = kItems + kDeal * 48;
+    static constexpr uint32_t kBarCount = 3 * kStages + 2 * kTiles + 3 * kTiles * kBufs + 2 * kDeal + 2;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
     static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
 };
 
+// A work item, or the K tiles [from, upto) of one.
 struct Item {
     int32_t token, count;  // first query row, positions (0: no more items)
     int32_t pos, head;     // first position in the sequence, KV head
     int32_t key, keys;     // first key row, the sequence's keys
     int32_t shift;         // keys - queries
+    int32_t from, upto;
+    int32_t part, parts;   // the CTA that has the item's first K tile, how many CTAs have one (1: this is all of it)
     int32_t pad;
 };
 
 struct TileSpan {
-    int32_t count, tiles, first;  // positions, key tiles, keys that the first row sees
+    int32_t count, tiles, first;  // positions, K tiles of this piece, keys that the first row sees
 };
 
 template <int D, bool BF>
@@ -230,10 +236,11 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
     const uint32_t bars = base + P::kBars;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     // a stage is full, free, or (raw) to be looked through first; of each row tile: its queries are there, its
-    // queries are read; of each buffer of logits: they are there, and what was asked of the tensor cores
-    // before them is done; the probabilities are; of each item: it is dealt, it is given back
+    // queries are read; of each buffer of logits: they are there (and what was asked of the tensor cores before
+    // them is done), the probabilities are, the last product from it is done (a barrier of its own: the next
+    // item's logits may come before softmax has looked); of each item: it is dealt, it is given back
     constexpr uint32_t B_FULL = 0, B_FREE = P::kStages, B_RAW = 2 * P::kStages, B_QFULL = 3 * P::kStages,
-                       B_QFREE = B_QFULL + NT, B_S = B_QFREE + NT, B_P = B_S + NT * NB, B_ITEM = B_P + NT * NB,
+                       B_QFREE = B_QFULL + NT, B_S = B_QFREE + NT, B_P = B_S + NT * NB, B_O = B_P + NT * NB, B_ITEM = B_O + NT * NB,
                        B_TAKEN = B_ITEM + kDeal, B_END = B_TAKEN + kDeal;
     constexpr uint32_t W_LOAD = 4 * NT, W_MMA = W_LOAD + 1, W_ENDS = W_LOAD + 3;  // the warps past softmax
     const uint32_t per = kRows / a.group;  // positions of a tile
@@ -254,6 +261,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
         for (uint32_t i = 0; i < NT * NB; ++i) {
             bar_init(bar(B_S + i), 1);
             bar_init(bar(B_P + i), 4);
+            bar_init(bar(B_O + i), 1);
         }
         for (uint32_t i = 0; i < kDeal; ++i) {
             bar_init(bar(B_ITEM + i), 1);
@@ -275,15 +283,20 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
         if (__all_sync(0xffffffffu, bar_try(b, parity))) return true;
         return (bool)__all_sync(0xffffffffu, bar_wait_slow(b, parity, stop));
     };
-    // Item n of the deal, when it is there; a role gives its slot back with `taken`.
-    auto next = [&](uint32_t n, Item &it) {
-        if (!all_wait(bar(B_ITEM + n % kDeal), n / kDeal & 1)) return false;
+    auto read = [&](uint32_t n, Item &it) {
         const volatile Item &s = items[n % kDeal];
         // from one lane: uniform over the warp, for the compiler too
         it.token = __shfl_sync(0xffffffffu, s.token, 0), it.count = __shfl_sync(0xffffffffu, s.count, 0);
         it.pos = __shfl_sync(0xffffffffu, s.pos, 0), it.head = __shfl_sync(0xffffffffu, s.head, 0);
         it.key = __shfl_sync(0xffffffffu, s.key, 0), it.keys = __shfl_sync(0xffffffffu, s.keys, 0);
-        it.shift = __shfl_sync(0xffffffffu, s.shift, 0);
+        it.shift = __shfl_sync(0xffffffffu, s.shift, 0), it.from = __shfl_sync(0xffffffffu, s.from, 0);
+        it.upto = __shfl_sync(0xffffffffu, s.upto, 0), it.part = __shfl_sync(0xffffffffu, s.part, 0);
+        it.parts = __shfl_sync(0xffffffffu, s.parts, 0);
+    };
+    // Item n of the deal, when it is there; a role gives its slot back with `taken`.
+    auto next = [&](uint32_t n, Item &it) {
+        if (!all_wait(bar(B_ITEM + n % kDeal), n / kDeal & 1)) return false;
+        read(n, it);
         return it.count != 0;
     };
     auto taken = [&](uint32_t n) {
@@ -296,7 +309,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
         s.count = max(0, min((int32_t)per, it.count - at));
         const int32_t from = it.pos + at + it.shift + 1;  // keys that the first row sees, if causal
         const int32_t upto = a.causal ? max(0, min(it.keys, from + s.count - 1)) : it.keys;
-        s.tiles = s.count ? (upto + kKeys - 1) / kKeys : 0;
+        s.tiles = s.count ? max(0, min(it.upto, (upto + kKeys - 1) / kKeys) - it.from) : 0;
         s.first = a.causal ? max(0, min(it.keys, from)) : it.keys;
         return s;
     };
@@ -313,16 +326,25 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
         const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
         const uint32_t lanes = (warp & 3u) * 32u << 16;
         const uint32_t to = tmem + lanes + P::kColO + t * D;
-        uint32_t phase = 0;  // a bit for each buffer of logits
-        Item it;
-        for (uint32_t n = 0; next(n, it); ++n) {
-            const TileSpan sp = span(it, t);
-            const bool live = p < (uint32_t)sp.count;
-            int32_t sees = it.keys;
-            if (a.causal) sees = max(0, min(it.keys, it.pos + t * (int32_t)per + (int32_t)p + it.shift + 1));
+        uint32_t phase = 0, phase_o = 0;  // a bit for each buffer of logits
+        // keys that this thread's row sees
+        auto sees_of = [&](const Item &it) {
+            return a.causal ? max(0, min(it.keys, it.pos + t * (int32_t)per + (int32_t)p + it.shift + 1)) : it.keys;
+        };
+        // (of an item only what the loop needs stays in registers; the rest is read again at its end)
+        for (uint32_t n = 0;; ++n) {
+            int32_t tiles, unmasked, left;  // K tiles; keys that all rows see and that this row sees, from this piece's first on
+            {
+                Item it;
+                if (!next(n, it)) break;
+                const TileSpan sp = span(it, t);
+                tiles = sp.tiles;
+                unmasked = sp.first - it.from * kKeys;
+                left = sees_of(it) - it.from * kKeys;
+            }
             float ref = -INFINITY, sum = 0.0f;  // the maximum that probabilities are relative to (log2 units)
             bool fine = true;
-            for (int32_t j = 0; j < sp.tiles; ++j) {
+            for (int32_t j = 0; j < tiles; ++j) {
                 const uint32_t buf = j % NB, ts = tmem + lanes + (NB * t + buf) * kKeys;
                 if (!(fine = all_wait(bar(B_S + NB * t + buf), phase >> buf & 1u))) break;
                 phase ^= 1u << buf;
@@ -332,11 +354,10 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 tm_load(ts + 32, x + 32);
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
-                if ((j + 1) * kKeys > sp.first) {
-                    const int32_t left = sees - j * kKeys;
+                if ((j + 1) * kKeys > unmasked) {
 #pragma unroll
                     for (int i = 0; i < kKeys; ++i)
-                        if (i >= left) s[i] = -INFINITY;
+                        if (i >= left - j * kKeys) s[i] = -INFINITY;
                 }
                 float m0 = max3(s[0], s[1], s[2]), m1 = max3(s[3], s[4], s[5]), m2 = max3(s[6], s[7], s[8]);
                 float m3 = max3(s[9], s[10], s[11]);
@@ -354,9 +375,11 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 if (j == 0) ref = top;
                 else if (__any_sync(0xffffffffu, grown)) {
                     // not under a product that is still adding to the outputs: the other buffer's next logits
-                    // come after it (with one buffer, these did)
+                    // come after it, or nothing does (with one buffer, these logits did)
                     if (NB == 2) {
-                        if (!(fine = all_wait(bar(B_S + NB * t + (buf ^ 1u)), phase >> (buf ^ 1u) & 1u))) break;
+                        const uint32_t other = buf ^ 1u, on = NB * t + other;
+                        fine = j + 1 < tiles ? all_wait(bar(B_S + on), phase >> other & 1u) : all_wait(bar(B_O + on), phase_o >> other & 1u);
+                        if (!fine) break;
                         tc_after();
                     }
                     const float f = grown ? ex2(ref - top) : 1.0f;
@@ -389,17 +412,76 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) bar_arrive(bar(B_P + NB * t + buf));
             }
+            Item it;
+            read(n, it);
+            const TileSpan sp = span(it, t);
             if (fine && sp.count) {
+                const bool live = p < (uint32_t)sp.count;
+                const int32_t sees = sees_of(it);
                 // the last products of every buffer
                 for (uint32_t buf = 0; buf < NB && (int32_t)buf < sp.tiles && fine; ++buf) {
-                    fine = all_wait(bar(B_S + NB * t + buf), phase >> buf & 1u);
-                    phase ^= 1u << buf;
+                    fine = all_wait(bar(B_O + NB * t + buf), phase_o >> buf & 1u);
+                    phase_o ^= 1u << buf;
                 }
                 if (!fine) break;
                 tc_after();
+                const uint32_t flagged = bad_flag[n % kDeal];
+                // infinities and NaN among the values of the kW dimensions from d0 on that this row sees
+                auto overlay = [&](uint32_t *o, int d0, auto width) {
+                    // keys from `key0` on were looked through
+                    const int32_t key0 = max(0, span(it, 0).first / kKeys) * kKeys;
+                    const uint16_t *first = bad + n % kDeal * 3 * D + d0;
+#pragma unroll
+                    for (int i = 0; i < decltype(width)::value; ++i) {
+                        const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
+                        if (key0 + first[2 * D + i] < sees || (up && down)) o[i] = 0x7fc00000u;
+                        else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
+                    }
+                };
+                // Parts of an item go to the workspace, [warp][dimension, maximum, sum][lane], and the warp that
+                // is the last of its kind to finish joins them, in the order of the CTAs.
+                const bool whole = it.parts == 1;
+                float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters) +
+                               (uint64_t)warp * (D + 2) * 32 + lane;
+                constexpr uint64_t kSlot = (uint64_t)4 * NT * (D + 2) * 32;
+                auto part_of = [&](int32_t c) { return parts + (2ull * c + (c == it.part ? 1 : 0)) * kSlot; };
+                if (!whole) {
+                    float *mine = part_of((int32_t)blockIdx.x);
+                    __stcg(mine + D * 32, sp.tiles ? ref : -INFINITY);
+                    __stcg(mine + (D + 1) * 32, sp.tiles ? sum : 0.0f);
+                    if (sp.tiles) {
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tm_load16(to + 16 * c, o);
+                            tc_wait_ld();
+                            if (flagged) overlay(o, 16 * c, std::integral_constant<int, 16>());
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]));
+                        }
+                    }
+                    tc_before();
+                    __threadfence();
+                    __syncwarp();
+                    uint32_t *counter = static_cast<uint32_t *>(a.workspace) + (uint64_t)it.part * 4 * NT + warp;
+                    uint32_t before = 0;
+                    if (lane == 0) {
+                        before = atomicAdd(counter, 1u);
+                        if (before + 1 == (uint32_t)it.parts) *counter = 0;
+                    }
+                    if (__shfl_sync(0xffffffffu, before, 0) + 1 != (uint32_t)it.parts) {
+                        taken(n);
+                        continue;
+                    }
+                    __threadfence();
+                    ref = -INFINITY, sum = 0.0f;
+                    for (int32_t c = it.part; c < it.part + it.parts; ++c) ref = max_nan(ref, __ldcg(part_of(c) + D * 32));
+                    const float base_ref = ref == -INFINITY ? 0.0f : ref;
+                    for (int32_t c = it.part; c < it.part + it.parts; ++c)
+                        sum = fmaf(ex2(__ldcg(part_of(c) + D * 32) - base_ref), __ldcg(part_of(c) + (D + 1) * 32), sum);
+                }
                 const bool none = sees == 0;
                 const float inv = none ? 0.0f : 1.0f / sum;
-                const uint32_t flagged = bad_flag[n % kDeal];
                 // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
                 constexpr int kW = P::kTurn, kL = kW / 8;
                 unsigned char *turn = sm + P::kOut + warp * 64 * kW;
@@ -409,7 +491,19 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
 #pragma unroll
                 for (int c = 0; c < D / kW; ++c) {
                     uint32_t o[kW];
-                    if (sp.tiles) {
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < kW; ++i) o[i] = 0;
+                        for (int32_t q = it.part; q < it.part + it.parts; ++q) {
+                            const float *from = part_of(q);
+                            const float m = __ldcg(from + D * 32);
+                            if (m == -INFINITY) continue;  // no K tile of this row tile
+                            const float f = ex2(m - ref);
+#pragma unroll
+                            for (int i = 0; i < kW; ++i)
+                                o[i] = __float_as_uint(fmaf(f, __ldcg(from + (kW * c + i) * 32), __uint_as_float(o[i])));
+                        }
+                    } else if (sp.tiles) {
                         if constexpr (kW == 32) tm_load(to + kW * c, o);
                         else tm_load16(to + kW * c, o);
                         tc_wait_ld();
@@ -418,17 +512,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
 #pragma unroll
                         for (int i = 0; i < kW; ++i) o[i] = 0;
                     }
-                    if (flagged) {
-                        // infinities and NaN that this row sees: keys from `key0` on were looked through
-                        const int32_t key0 = max(0, span(it, 0).first / kKeys) * kKeys;
-                        const uint16_t *first = bad + n % kDeal * 3 * D + kW * c;
-#pragma unroll
-                        for (int i = 0; i < kW; ++i) {
-                            const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
-                            if (key0 + first[2 * D + i] < sees || (up && down)) o[i] = 0x7fc00000u;
-                            else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
-                        }
-                    }
+                    if (whole && flagged) overlay(o, kW * c, std::integral_constant<int, kW>());
 #pragma unroll
                     for (int i = 0; i < kL; ++i) {
                         uint4 v;
@@ -460,71 +544,149 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kRest));
         if (warp == W_LOAD) {
             // ---- the deal ----
-            // Sequence s has ceil(queries / (tiles per item)) blocks; block b of every sequence that
-            // has it is level b.  Items go by falling level (the last blocks see the most keys), a level's
-            // sequences in order, KV heads innermost; item r goes to CTA r of a round, rounds back and forth.
-            const int32_t block = (int32_t)(a.tiles * per);
-            auto blocks_of = [&](uint32_t s) -> int32_t {
-                if (s >= a.sequences) return 0;
+            // An item's price is its keys, as its last row sees them, and kItemCost.  Items stand in order - sequences,
+            // KV heads, blocks - on a line as long as their prices, K tile j of one at kItemCost + 64 j of its stretch,
+            // and the line is cut into equal ranges, one a CTA, none shorter than a tile: whatever the
+            // lengths are, all CTAs end together, and where items are few, their keys are split.
+            const int64_t block = (int64_t)a.tiles * per;
+            struct Seq {
+                int32_t q0, k0;
+                int64_t nq, nk, blocks, shift;
+            } sq;
+            auto load_seq = [&](uint32_t s) {
+                Seq q{};
+                if (s >= a.sequences) return q;
                 const int32_t q0 = __ldg(a.starts + s), q1 = __ldg(a.starts + s + 1);
                 const int32_t k0 = __ldg(a.key_starts + s), k1 = __ldg(a.key_starts + s + 1);
                 if (q0 < 0 || k0 < 0 || q1 < q0 || k1 < k0 || (uint64_t)q1 > a.q_tokens || (uint64_t)k1 > a.k_tokens) {
                     if (blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
-                    return 0;
+                    return q;
                 }
-                return (q1 - q0 + block - 1) / block;
+                q.q0 = q0, q.k0 = k0, q.nq = q1 - q0, q.nk = k1 - k0, q.shift = q.nk - q.nq;
+                q.blocks = (q.nq + block - 1) / block;
+                return q;
             };
-            // (the blocks of the first 32 sequences stay in the lanes)
-            const int32_t mine = blocks_of(lane);
-            auto blocks_at = [&](uint32_t s) { return s < 32 ? mine : blocks_of(s); };
-            // blocks at or above a level, over all sequences
-            auto above = [&](int32_t level) {
-                uint32_t c = 0;
-                for (uint32_t s = lane; s < a.sequences; s += 32) c += (uint32_t)max(0, blocks_at(s) - level);
-                return __reduce_add_sync(0xffffffffu, c);
+            // keys of block b, one at least
+            auto keys_of = [&](const Seq &q, int64_t b) {
+                if (!a.causal || b + 1 >= q.blocks) return max((int64_t)1, q.nk);
+                return max((int64_t)1, (b + 1) * block + q.shift);
             };
-            int32_t high = 0;  // the blocks of the longest sequence
-            for (uint32_t s = lane; s < a.sequences; s += 32) high = max(high, blocks_at(s));
-            high = __reduce_max_sync(0xffffffffu, high);
-            const uint64_t upto = (uint64_t)above(0) * a.kv_heads;
-            auto deal = [&](uint32_t n) {
-                const uint64_t r = (uint64_t)n * gridDim.x + (n & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                Item it{};
-                if (r < upto) {
-                    // the highest level with more than r / heads blocks at or above it; levels only fall from item to item
-                    const uint32_t rank = (uint32_t)(r / a.kv_heads);
-                    it.head = (int32_t)(r % a.kv_heads);
-                    int32_t level = 0;
-                    for (int32_t top = high; top - level > 1;) {
-                        const int32_t mid = (level + top) / 2;
-                        if (above(mid) > rank) level = mid;
+            // price of the blocks before b of one head
+            auto price = [&](const Seq &q, int64_t b) -> int64_t {
+                if (b == 0) return 0;
+                int64_t n = b * kItemCost;
+                if (!a.causal) return n + b * max((int64_t)1, q.nk);
+                const int64_t m = min(b, q.blocks - 1);  // all but the last block: (b + 1) block + shift keys, or 1
+                const int64_t z = min(m, max((int64_t)0, 1 - q.shift) / block);
+                n += z + block * (m * (m + 1) - z * (z + 1)) / 2 + q.shift * (m - z);
+                return b == q.blocks ? n + max((int64_t)1, q.nk) : n;
+            };
+            auto warp_sum = [](int64_t x) {
+#pragma unroll
+                for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+                return x;
+            };
+            int64_t total = 0, all = 0;
+            for (uint32_t s = lane; s < a.sequences; s += 32) {
+                const Seq q = load_seq(s);
+                total += a.kv_heads * price(q, q.blocks);
+                all += a.kv_heads * q.blocks;
+            }
+            total = warp_sum(total);
+            all = warp_sum(all);
+            const int64_t ctas = min(min((int64_t)gridDim.x, max((int64_t)1, total / kKeys)), max(all, total / kPiece));
+            bool some = ctas > 0 && (int64_t)blockIdx.x < ctas;
+            const int64_t each = some ? total / ctas : 1, over = some ? total - each * ctas : 0;
+            const int64_t start = blockIdx.x * each + min((int64_t)blockIdx.x, over);
+            const int64_t end = start + each + ((int64_t)blockIdx.x < over ? 1 : 0);
+            auto owner = [&](int64_t place) {
+                const int64_t head = over * (each + 1);
+                return (int32_t)(place < head ? place / (each + 1) : over + (place - head) / each);
+            };
+            uint32_t seq = 0;
+            int64_t head = 0, blk = 0, at = 0;  // the item at hand, and where it begins on the line
+            if (some) {
+                for (uint32_t s0 = 0;; s0 += 32) {  // ends: start < total
+                    const Seq q = load_seq(s0 + lane);
+                    const int64_t own = a.kv_heads * price(q, q.blocks);
+                    int64_t sum = own;
+#pragma unroll
+                    for (int w = 1; w < 32; w <<= 1) {
+                        const int64_t o = __shfl_up_sync(0xffffffffu, sum, w);
+                        if (lane >= (uint32_t)w) sum += o;
+                    }
+                    const uint32_t past = __ballot_sync(0xffffffffu, at + sum > start);
+                    if (past) {
+                        const uint32_t l = __ffs(past) - 1;
+                        at += __shfl_sync(0xffffffffu, sum - own, l);
+                        seq = s0 + l;
+                        break;
+                    }
+                    if (s0 + 32 >= a.sequences) {
+                        some = false;
+                        break;
+                    }
+                    at += __shfl_sync(0xffffffffu, sum, 31);
+                }
+                sq = load_seq(seq);
+                if (some) {
+                    const int64_t of_head = price(sq, sq.blocks);
+                    head = (start - at) / of_head;
+                    at += head * of_head;
+                    int64_t top = sq.blocks;  // the last block that begins at or before the start
+                    while (top - blk > 1) {
+                        const int64_t mid = (blk + top) / 2;
+                        if (at + price(sq, mid) <= start) blk = mid;
                         else top = mid;
                     }
-                    high = level + 1;
-                    uint32_t nth = rank - above(level + 1);
-                    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 32) {
-                        const uint32_t has = __ballot_sync(0xffffffffu, (s0 ? blocks_of(s0 + lane) : mine) > level);
-                        const uint32_t c = __popc(has);
-                        if (nth >= c) {
-                            nth -= c;
-                            continue;
+                    at += price(sq, blk);
+                }
+            }
+            auto deal = [&](uint32_t n) {
+                Item it{};
+                while (some && it.count == 0) {
+                    const int64_t keys = keys_of(sq, blk), from = at + kItemCost;
+                    const int64_t units = (keys + kKeys - 1) / kKeys;
+                    const int64_t one = start <= from ? 0 : min(units, (start - from + kKeys - 1) / kKeys);
+                    const int64_t two = end <= from ? 0 : min(units, (end - from + kKeys - 1) / kKeys);
+                    if (one < two) {
+                        it.pos = (int32_t)(blk * block);
+                        it.token = sq.q0 + it.pos;
+                        it.count = (int32_t)min(block, sq.nq - blk * block);
+                        it.head = (int32_t)head;
+                        it.key = sq.k0;
+                        it.keys = (int32_t)sq.nk;
+                        it.shift = (int32_t)sq.shift;
+                        it.from = (int32_t)one;
+                        it.upto = (int32_t)two;
+                        it.parts = 1;
+                        if (one > 0 || two < units) {
+                            it.part = owner(from);
+                            it.parts = owner(from + (units - 1) * kKeys) - it.part + 1;
                         }
-                        const uint32_t s = s0 + __fns(has, 0, nth + 1);
-                        const int32_t q0 = __ldg(a.starts + s), nq = __ldg(a.starts + s + 1) - q0;
-                        it.pos = level * block;
-                        it.token = q0 + it.pos;
-                        it.count = min(block, nq - it.pos);
-                        it.key = __ldg(a.key_starts + s);
-                        it.keys = __ldg(a.key_starts + s + 1) - it.key;
-                        it.shift = it.keys - nq;
-                        break;
+                    }
+                    at += kItemCost + keys;
+                    some = at < end;
+                    if (some && ++blk == sq.blocks) {
+                        blk = 0;
+                        if (++head == a.kv_heads) {
+                            head = 0;
+                            do {
+                                if (++seq >= a.sequences) {
+                                    some = false;
+                                    break;
+                                }
+                                sq = load_seq(seq);
+                            } while (sq.blocks == 0);
+                        }
                     }
                 }
                 if (n >= kDeal && !all_wait(bar(B_TAKEN + n % kDeal), (n / kDeal & 1) ^ 1)) return;
                 if (lane == 0) {
                     volatile Item &d = items[n % kDeal];
                     d.token = it.token, d.count = it.count, d.pos = it.pos, d.head = it.head;
-                    d.key = it.key, d.keys = it.keys, d.shift = it.shift;
+                    d.key = it.key, d.keys = it.keys, d.shift = it.shift, d.from = it.from, d.upto = it.upto;
+                    d.part = it.part, d.parts = it.parts;
                     bad_flag[n % kDeal] = 0;
                     bar_arrive(bar(B_ITEM + n % kDeal));
                 }
@@ -558,10 +720,11 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                         bar_expect(on, P::kTile * (two < 0 ? 1u : 2u));
                         const uint32_t dst = base + P::kRing + slot * 2 * P::kTile;
                         for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(dst + c * P::kChunk, map, on, 64 * c, it.head, it.key + one * kKeys);
+                            tma3(dst + c * P::kChunk, map, on, 64 * c, it.head, it.key + (it.from + one) * kKeys);
                         if (two >= 0)
                             for (uint32_t c = 0; c < P::kChunks; ++c)
-                                tma3(dst + P::kTile + c * P::kChunk, &mk, on, 64 * c, it.head, it.key + two * kKeys);
+                                tma3(dst + P::kTile + c * P::kChunk, &mk, on, 64 * c, it.head,
+                                     it.key + (it.from + two) * kKeys);
                         issued |= bit;
                         raw = look ? raw | bit : raw & ~bit;
                         full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
@@ -573,7 +736,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     for (uint32_t t = 1; t < NT; ++t)
                         if (span(it, (int)t).tiles) load_q((int)t);
                     for (int32_t j = 0; j < tiles && fine; ++j)
-                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (j + 1) * kKeys > first);
+                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (it.from + j + 1) * kKeys > first);
                 }
                 fine = __shfl_sync(0xffffffffu, fine, 0);
             }
@@ -656,8 +819,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                             const uint32_t val = operand(at, P::kChunk), pr = tmem + tb * kKeys, o = tmem + P::kColO + t * D;
 #pragma unroll
                             for (uint32_t s = 0; s < P::kKeys / 16; ++s) mma_ts(o, pr + 8 * s, val + s * 128, ID_O, j | (int32_t)s);
-                            if (j + (int32_t)NB < mine[i]) logits(t, at + P::kTile, j + (int32_t)NB);
-                            tc_commit(bar(B_S + tb));  // at the end with nothing but the outputs before it
+                            const bool more = j + (int32_t)NB < mine[i];
+                            if (more) logits(t, at + P::kTile, j + (int32_t)NB);
+                            tc_commit(bar((more ? B_S : B_O) + tb));
                             if (j + (int32_t)NB + 1 == mine[i]) tc_commit(bar(B_QFREE + t));
                         }
                         __syncwarp();
@@ -684,15 +848,15 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 const TileSpan s0 = span(it, 0);
                 const int32_t tiles = tiles_of(it), begin = max(0, s0.first / kKeys);
                 uint16_t *first = bad + n % kDeal * 3 * D;
-                if (begin < tiles)
+                if (begin < it.from + tiles)
                     for (uint32_t i = lane; i < 3 * D; i += 32) first[i] = 0xffff;
-                for (int32_t j = begin; j < tiles; ++j) {
-                    if ((j + 1) * kKeys <= s0.first) continue;
+                for (int32_t j = max(0, begin - it.from); j < tiles; ++j) {
+                    if ((it.from + j + 1) * kKeys <= s0.first) continue;
                     const uint32_t v = (slot + 1 + (uint32_t)j) % P::kStages;  // past the stage of the first K tiles
                     if (!(fine = all_wait(bar(B_RAW + v), raw_phase >> v & 1u))) break;
                     raw_phase ^= 1u << v;
                     unsigned char *tile = sm + P::kRing + v * 2 * P::kTile;
-                    const int32_t rows = min(kKeys, it.keys - j * kKeys);
+                    const int32_t rows = min(kKeys, it.keys - (it.from + j) * kKeys);
                     uint32_t found = 0;
                     constexpr uint32_t E = BF ? 0x7f80u : 0x7c00u;
 #pragma unroll 4
@@ -717,7 +881,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                                 if ((x & E) != E) continue;
                                 *w = 0;
                                 const uint32_t kind = (x & 0x7fffu) != E ? 2 : x >> 15;  // 0 inf, 1 -inf, 2 NaN
-                                const uint32_t at = (uint32_t)((j - begin) * kKeys + k);
+                                const uint32_t at = (uint32_t)((it.from + j - begin) * kKeys + k);
                                 if (at < first[kind * D + d]) first[kind * D + d] = (uint16_t)at;
                             }
                         }
@@ -771,6 +935,9 @@ bool make_map(CUtensorMap *m, bool bf16, const void *p, uint32_t dim, uint32_t h
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Bytes of the workspace's counters: one for every softmax warp of every CTA.
+uint32_t prompt_counters(int sms, uint32_t tiles) { return ((uint32_t)sms * tiles * 16 + 127) / 128 * 128; }
+
 template <int D, bool BF>
 cudaError_t run(const PromptArgs &args, cudaStream_t s) {
     using P = Plan<D>;
@@ -795,16 +962,29 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
         !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, P::kKeys) ||
         !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, P::kKeys))
         return cudaErrorInvalidValue;
-    // The row tiles of an item share its K and V loads: as many as still leave every SM an item.
-    auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per)); };
+    // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as still leave
+    // every SM kSteps K tiles or so.
+    constexpr uint64_t kSteps = 8;
+    auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.sequences); };
+    const uint64_t mean = a.k_tokens / a.sequences + 1;
     a.tiles = P::kTiles;
-    while (a.tiles > 1 && items(a.tiles) < (uint64_t)sms) a.tiles /= 2;
-    const uint64_t most = items(a.tiles) + (uint64_t)a.kv_heads * a.sequences;
-    kernel<<<(uint32_t)(most < (uint64_t)sms ? most : sms), P::kThreads, P::kTotal, s>>>(a, mq, mk, mv);
+    while (a.tiles > 1 && items(a.tiles) * mean < (uint64_t)sms * kSteps * P::kKeys) a.tiles /= 2;
+    const uint64_t most = items(a.tiles), pieces = most * (a.k_tokens + kItemCost) / kPiece + 1;
+    const uint64_t ctas = most > pieces ? most : pieces;
+    a.counters = prompt_counters(sms, P::kTiles);
+    kernel<<<(uint32_t)(ctas < (uint64_t)sms ? ctas : sms), P::kThreads, P::kTotal, s>>>(a, mq, mk, mv);
     return cudaGetLastError();
 }
 
 }  // namespace
+
+size_t prompt_workspace(uint32_t dim) {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    const uint32_t tiles = dim == 64 ? Plan<64>::kTiles : Plan<128>::kTiles;
+    return prompt_counters(sms, tiles) + 2ull * sms * tiles * kRows * (dim + 2) * 4;
+}
 
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s) {
     if (a.dtype == BGTQ_BF16) return a.dim == 64 ? run<64, true>(a, s) : run<128, true>(a, s);

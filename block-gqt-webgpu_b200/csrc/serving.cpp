@@ -176,6 +176,16 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
     return launched(launch_paged_attend(a, static_cast<cudaStream_t>(stream)), "Paged attention");
 }
 
+bgtq_status bgtq_prompt_workspace(int device, uint32_t dim, size_t *bytes) {
+    if (dim != 64 && dim != 128) return refuse("Prompt attention: head dim must be 64 or 128");
+    if (!bytes) return refuse("Prompt attention: null argument");
+    OnDevice on(device);
+    const size_t need = on.ok ? prompt_workspace(dim) : 0;
+    if (!need) return launched(cudaErrorInvalidDevice, "Prompt attention");
+    *bytes = need;
+    return BGTQ_OK;
+}
+
 bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream) {
     if (!p) return refuse("Prompt attention: null");
     PromptArgs a{};
@@ -200,6 +210,11 @@ bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream) {
     OnDevice on(p->device);
     a.status = on.ok ? device_status_word(p->device) : nullptr;
     if (!a.status) return launched(cudaErrorInvalidDevice, "Prompt attention");
+    const size_t need = prompt_workspace(p->dim);
+    if (!need) return launched(cudaErrorInvalidDevice, "Prompt attention");
+    if (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 128))
+        return refuse("Prompt attention: the workspace is too small or misaligned");
+    a.workspace = p->workspace;
     a.q = p->q;
     a.k = p->k;
     a.v = p->v;

@@ -71,7 +71,9 @@ struct PromptArgs {
     float *lse;                           // [q_tokens][q_heads], nullable
     uint64_t q_tokens, k_tokens;
     uint32_t sequences, q_heads, kv_heads, group, dim;
-    uint32_t tiles;  // the launcher's: row tiles of a work item
+    void *workspace;
+    uint32_t tiles;     // the launcher's: row tiles of a work item
+    uint32_t counters;  // the launcher's: bytes of the workspace's counters
     float scale;  // of the logits, times log2(e)
     int causal;
     bgtq_dtype dtype;
@@ -83,6 +85,8 @@ cudaError_t launch_paged_read(const PagedReadArgs &a, cudaStream_t s);
 // Bytes of the workspace that launch_paged_attend needs (counters first, zero between calls).
 size_t paged_attend_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t dim);
 cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t s);
+// Bytes of the workspace that launch_prompt needs (counters first, zero between calls).
+size_t prompt_workspace(uint32_t dim);
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s);
 
 }  // namespace bgtq

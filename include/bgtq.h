@@ -533,7 +533,12 @@ typedef struct bgtq_prompt {
     float scale;  /* of the logits, positive (0: 1 / sqrt(dim)) */
     void *out;    /* dense [q_tokens][q_heads][dim] of dtype */
     float *lse;   /* [q_tokens][q_heads] FP32, or null */
+    void *workspace; /* 128-byte aligned, zero-filled before its first use; every call leaves it
+                        ready for the next.  Calls that may overlap need their own. */
+    size_t workspace_bytes;
 } bgtq_prompt;
+/* Bytes of workspace that bgtq_prompt_attend needs for a head dim, whatever the batch. */
+bgtq_status bgtq_prompt_workspace(int device, uint32_t dim, size_t *bytes);
 bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream);
 
 /* Device status word written by kernels (0 = fine); reading it synchronises. */
