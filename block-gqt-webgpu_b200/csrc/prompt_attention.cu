@@ -42,6 +42,7 @@ constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_interna
 constexpr uint32_t kDeal = 4;            // items dealt ahead
 constexpr int64_t kItemCost = 384;       // what an item costs beside its keys, in keys: queries, outputs, joining
 constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while where items are few
+constexpr int32_t kWhole = 512;          // an item of no more keys than that is not split: joining costs as much
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
 // ---- device helpers -----------------------------------------------------------------------
@@ -212,6 +213,11 @@ struct Item {
     int32_t part, parts;   // the CTA that has the item's first K tile, how many CTAs have one (1: this is all of it)
     int32_t pad;
 };
+
+// Quotients of nonnegative numbers: 32-bit division where it will do, which is nearly always.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 
 struct TileSpan {
     int32_t count, tiles, first;  // positions, K tiles of this piece, keys that the first row sees
@@ -548,10 +554,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             // KV heads, blocks - on a line as long as their prices, K tile j of one at kItemCost + 64 j of its stretch,
             // and the line is cut into equal ranges, one a CTA, none shorter than a tile: whatever the
             // lengths are, all CTAs end together, and where items are few, their keys are split.
-            const int64_t block = (int64_t)a.tiles * per;
+            const int32_t block = (int32_t)(a.tiles * per);
             struct Seq {
-                int32_t q0, k0;
-                int64_t nq, nk, blocks, shift;
+                int32_t q0, k0, nq, nk, blocks, shift;
             } sq;
             auto load_seq = [&](uint32_t s) {
                 Seq q{};
@@ -563,23 +568,23 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     return q;
                 }
                 q.q0 = q0, q.k0 = k0, q.nq = q1 - q0, q.nk = k1 - k0, q.shift = q.nk - q.nq;
-                q.blocks = (q.nq + block - 1) / block;
+                q.blocks = (int32_t)(((uint32_t)q.nq + block - 1) / (uint32_t)block);
                 return q;
             };
             // keys of block b, one at least
-            auto keys_of = [&](const Seq &q, int64_t b) {
-                if (!a.causal || b + 1 >= q.blocks) return max((int64_t)1, q.nk);
-                return max((int64_t)1, (b + 1) * block + q.shift);
+            auto keys_of = [&](const Seq &q, int32_t b) {
+                if (!a.causal || b + 1 >= q.blocks) return max(1, q.nk);
+                return max(1, (b + 1) * block + q.shift);
             };
             // price of the blocks before b of one head
-            auto price = [&](const Seq &q, int64_t b) -> int64_t {
+            auto price = [&](const Seq &q, int32_t b) -> int64_t {
                 if (b == 0) return 0;
                 int64_t n = b * kItemCost;
-                if (!a.causal) return n + b * max((int64_t)1, q.nk);
-                const int64_t m = min(b, q.blocks - 1);  // all but the last block: (b + 1) block + shift keys, or 1
-                const int64_t z = min(m, max((int64_t)0, 1 - q.shift) / block);
-                n += z + block * (m * (m + 1) - z * (z + 1)) / 2 + q.shift * (m - z);
-                return b == q.blocks ? n + max((int64_t)1, q.nk) : n;
+                if (!a.causal) return n + (int64_t)b * max(1, q.nk);
+                const int32_t m = min(b, q.blocks - 1);  // all but the last block: (b + 1) block + shift keys, or 1
+                const int32_t z = q.shift < 0 ? min(m, (int32_t)((uint32_t)(1 - q.shift) / (uint32_t)block)) : 0;
+                n += z + (int64_t)block * (((int64_t)m * (m + 1) - (int64_t)z * (z + 1)) / 2) + (int64_t)q.shift * (m - z);
+                return b == q.blocks ? n + max(1, q.nk) : n;
             };
             auto warp_sum = [](int64_t x) {
 #pragma unroll
@@ -596,15 +601,16 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             all = warp_sum(all);
             const int64_t ctas = min(min((int64_t)gridDim.x, max((int64_t)1, total / kKeys)), max(all, total / kPiece));
             bool some = ctas > 0 && (int64_t)blockIdx.x < ctas;
-            const int64_t each = some ? total / ctas : 1, over = some ? total - each * ctas : 0;
+            const int64_t each = some ? quotient(total, ctas) : 1, over = some ? total - each * ctas : 0;
             const int64_t start = blockIdx.x * each + min((int64_t)blockIdx.x, over);
             const int64_t end = start + each + ((int64_t)blockIdx.x < over ? 1 : 0);
             auto owner = [&](int64_t place) {
                 const int64_t head = over * (each + 1);
-                return (int32_t)(place < head ? place / (each + 1) : over + (place - head) / each);
+                return (int32_t)(place < head ? quotient(place, each + 1) : over + quotient(place - head, each));
             };
             uint32_t seq = 0;
-            int64_t head = 0, blk = 0, at = 0;  // the item at hand, and where it begins on the line
+            int32_t head = 0, blk = 0;
+            int64_t at = 0;  // the item at hand begins there on the line
             if (some) {
                 for (uint32_t s0 = 0;; s0 += 32) {  // ends: start < total
                     const Seq q = load_seq(s0 + lane);
@@ -631,11 +637,11 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 sq = load_seq(seq);
                 if (some) {
                     const int64_t of_head = price(sq, sq.blocks);
-                    head = (start - at) / of_head;
+                    head = (int32_t)quotient(start - at, of_head);
                     at += head * of_head;
-                    int64_t top = sq.blocks;  // the last block that begins at or before the start
+                    int32_t top = sq.blocks;  // the last block that begins at or before the start
                     while (top - blk > 1) {
-                        const int64_t mid = (blk + top) / 2;
+                        const int32_t mid = (blk + top) / 2;
                         if (at + price(sq, mid) <= start) blk = mid;
                         else top = mid;
                     }
@@ -645,31 +651,37 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             auto deal = [&](uint32_t n) {
                 Item it{};
                 while (some && it.count == 0) {
-                    const int64_t keys = keys_of(sq, blk), from = at + kItemCost;
-                    const int64_t units = (keys + kKeys - 1) / kKeys;
-                    const int64_t one = start <= from ? 0 : min(units, (start - from + kKeys - 1) / kKeys);
-                    const int64_t two = end <= from ? 0 : min(units, (end - from + kKeys - 1) / kKeys);
+                    const int32_t keys = keys_of(sq, blk), units = (keys + kKeys - 1) / kKeys;
+                    const int64_t from = at + kItemCost;
+                    int32_t one, two;
+                    if (keys <= kWhole) {  // where it begins
+                        one = 0;
+                        two = at >= start ? units : 0;
+                    } else {
+                        one = start <= from ? 0 : (int32_t)min((int64_t)units, (start - from + kKeys - 1) / kKeys);
+                        two = end <= from ? 0 : (int32_t)min((int64_t)units, (end - from + kKeys - 1) / kKeys);
+                    }
                     if (one < two) {
-                        it.pos = (int32_t)(blk * block);
+                        it.pos = blk * block;
                         it.token = sq.q0 + it.pos;
-                        it.count = (int32_t)min(block, sq.nq - blk * block);
-                        it.head = (int32_t)head;
+                        it.count = min(block, sq.nq - blk * block);
+                        it.head = head;
                         it.key = sq.k0;
-                        it.keys = (int32_t)sq.nk;
-                        it.shift = (int32_t)sq.shift;
-                        it.from = (int32_t)one;
-                        it.upto = (int32_t)two;
+                        it.keys = sq.nk;
+                        it.shift = sq.shift;
+                        it.from = one;
+                        it.upto = two;
                         it.parts = 1;
                         if (one > 0 || two < units) {
                             it.part = owner(from);
-                            it.parts = owner(from + (units - 1) * kKeys) - it.part + 1;
+                            it.parts = owner(from + (int64_t)(units - 1) * kKeys) - it.part + 1;
                         }
                     }
                     at += kItemCost + keys;
                     some = at < end;
                     if (some && ++blk == sq.blocks) {
                         blk = 0;
-                        if (++head == a.kv_heads) {
+                        if (++head == (int32_t)a.kv_heads) {
                             head = 0;
                             do {
                                 if (++seq >= a.sequences) {
@@ -962,13 +974,11 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
         !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, P::kKeys) ||
         !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, P::kKeys))
         return cudaErrorInvalidValue;
-    // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as still leave
-    // every SM kSteps K tiles or so.
-    constexpr uint64_t kSteps = 8;
-    auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.sequences); };
-    const uint64_t mean = a.k_tokens / a.sequences + 1;
+    // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as possible,
+    // while that makes half as many items as there are SMs.
+    auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.sequences - 1); };
     a.tiles = P::kTiles;
-    while (a.tiles > 1 && items(a.tiles) * mean < (uint64_t)sms * kSteps * P::kKeys) a.tiles /= 2;
+    while (a.tiles > 1 && 2 * items(a.tiles) <= (uint64_t)sms) a.tiles /= 2;
     const uint64_t most = items(a.tiles), pieces = most * (a.k_tokens + kItemCost) / kPiece + 1;
     const uint64_t ctas = most > pieces ? most : pieces;
     a.counters = prompt_counters(sms, P::kTiles);
