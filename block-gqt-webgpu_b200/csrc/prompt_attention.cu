@@ -492,6 +492,12 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 constexpr int kW = P::kTurn, kL = kW / 8;
                 unsigned char *turn = sm + P::kOut + warp * 64 * kW;
                 const int64_t first_row = (int64_t)(it.token + t * (int32_t)per) * a.q_heads + it.head * a.group;
+                int32_t to_row[kL];  // of the rows that this lane writes for, from first_row on; -1 for none
+#pragma unroll
+                for (int i = 0; i < kL; ++i) {
+                    const uint32_t tr = (warp & 3u) * 32 + (32 / kL) * i + lane / kL, rp = tr / a.group;
+                    to_row[i] = rp < (uint32_t)sp.count ? (int32_t)(rp * a.q_heads + tr % a.group) : -1;
+                }
                 // 16-byte chunk c of row r: a phase of eight lanes meets 128 different bytes, writing and reading
                 auto chunk = [&](uint32_t r, uint32_t c) { return turn + r * 2 * kW + ((c ^ r / (8 / kL) % kL) << 4); };
 #pragma unroll
@@ -531,12 +537,10 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < kL; ++i) {
-                        const uint32_t r = (32 / kL) * i + lane / kL, tr = (warp & 3u) * 32 + r, rp = tr / a.group;
-                        const uint4 v = *reinterpret_cast<uint4 *>(chunk(r, lane % kL));
-                        if (rp < (uint32_t)sp.count) {
-                            const int64_t at = first_row + (int64_t)rp * a.q_heads + tr % a.group;
-                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at * D + kW * c + 8 * (lane % kL)) = v;
-                        }
+                        const uint4 v = *reinterpret_cast<uint4 *>(chunk((32 / kL) * i + lane / kL, lane % kL));
+                        if (to_row[i] >= 0)
+                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (first_row + to_row[i]) * D + kW * c +
+                                                       8 * (lane % kL)) = v;
                     }
                     __syncwarp();
                 }
@@ -586,19 +590,38 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 n += z + (int64_t)block * (((int64_t)m * (m + 1) - (int64_t)z * (z + 1)) / 2) + (int64_t)q.shift * (m - z);
                 return b == q.blocks ? n + max(1, q.nk) : n;
             };
-            auto warp_sum = [](int64_t x) {
+            // the first 32 sequences stay in the lanes, with the price of all before each of them and its own
+            const Seq mine = load_seq(lane);
+            const int64_t own = a.kv_heads * price(mine, mine.blocks);
+            auto scan = [&](int64_t x) {
 #pragma unroll
-                for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+                for (int w = 1; w < 32; w <<= 1) {
+                    const int64_t o = __shfl_up_sync(0xffffffffu, x, w);
+                    if (lane >= (uint32_t)w) x += o;
+                }
                 return x;
             };
-            int64_t total = 0, all = 0;
-            for (uint32_t s = lane; s < a.sequences; s += 32) {
-                const Seq q = load_seq(s);
-                total += a.kv_heads * price(q, q.blocks);
-                all += a.kv_heads * q.blocks;
+            const int64_t own_upto = scan(own);
+            auto get_seq = [&](uint32_t s) {
+                if (s >= 32) return load_seq(s);
+                Seq q;
+                q.q0 = __shfl_sync(0xffffffffu, mine.q0, s), q.k0 = __shfl_sync(0xffffffffu, mine.k0, s);
+                q.nq = __shfl_sync(0xffffffffu, mine.nq, s), q.nk = __shfl_sync(0xffffffffu, mine.nk, s);
+                q.blocks = __shfl_sync(0xffffffffu, mine.blocks, s), q.shift = q.nk - q.nq;
+                return q;
+            };
+            int64_t total = __shfl_sync(0xffffffffu, own_upto, 31);
+            uint32_t blocks = (uint32_t)mine.blocks;
+            if (a.sequences > 32) {
+                int64_t rest = 0;
+                for (uint32_t s = lane + 32; s < a.sequences; s += 32) {
+                    const Seq q = load_seq(s);
+                    rest += a.kv_heads * price(q, q.blocks);
+                    blocks += (uint32_t)q.blocks;
+                }
+                total += __shfl_sync(0xffffffffu, scan(rest), 31);
             }
-            total = warp_sum(total);
-            all = warp_sum(all);
+            const int64_t all = (int64_t)__reduce_add_sync(0xffffffffu, blocks) * a.kv_heads;
             const int64_t ctas = min(min((int64_t)gridDim.x, max((int64_t)1, total / kKeys)), max(all, total / kPiece));
             bool some = ctas > 0 && (int64_t)blockIdx.x < ctas;
             const int64_t each = some ? quotient(total, ctas) : 1, over = some ? total - each * ctas : 0;
@@ -613,18 +636,16 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             int64_t at = 0;  // the item at hand begins there on the line
             if (some) {
                 for (uint32_t s0 = 0;; s0 += 32) {  // ends: start < total
-                    const Seq q = load_seq(s0 + lane);
-                    const int64_t own = a.kv_heads * price(q, q.blocks);
-                    int64_t sum = own;
-#pragma unroll
-                    for (int w = 1; w < 32; w <<= 1) {
-                        const int64_t o = __shfl_up_sync(0xffffffffu, sum, w);
-                        if (lane >= (uint32_t)w) sum += o;
+                    int64_t price_of = own, upto = own_upto;
+                    if (s0) {
+                        const Seq q = load_seq(s0 + lane);
+                        price_of = a.kv_heads * price(q, q.blocks);
+                        upto = scan(price_of);
                     }
-                    const uint32_t past = __ballot_sync(0xffffffffu, at + sum > start);
+                    const uint32_t past = __ballot_sync(0xffffffffu, at + upto > start);
                     if (past) {
                         const uint32_t l = __ffs(past) - 1;
-                        at += __shfl_sync(0xffffffffu, sum - own, l);
+                        at += __shfl_sync(0xffffffffu, upto - price_of, l);
                         seq = s0 + l;
                         break;
                     }
@@ -632,10 +653,10 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                         some = false;
                         break;
                     }
-                    at += __shfl_sync(0xffffffffu, sum, 31);
+                    at += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                sq = load_seq(seq);
                 if (some) {
+                    sq = get_seq(seq);
                     const int64_t of_head = price(sq, sq.blocks);
                     head = (int32_t)quotient(start - at, of_head);
                     at += head * of_head;
@@ -688,7 +709,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                                     some = false;
                                     break;
                                 }
-                                sq = load_seq(seq);
+                                sq = get_seq(seq);
                             } while (sq.blocks == 0);
                         }
                     }
@@ -713,9 +734,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             bool fine = true;
             deal(0);
             for (uint32_t n = 0; fine && next(n, it); ++n) {
-                deal(n + 1);
                 const int32_t tiles = tiles_of(it), first = span(it, 0).first;
-                if (lane == 0) {
                     auto load_q = [&](int t) {
                         if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase >> t & 1u, stop))) return;
                         q_phase ^= 1u << t;
@@ -743,13 +762,20 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                         raw_phase ^= look ? bit : 0;
                         if (++slot == P::kStages) slot = 0, free_phase ^= 1;
                     };
+                    auto load_v = [&](int32_t j) {
+                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (it.from + j + 1) * kKeys > first);
+                    };
+                if (lane == 0) {
                     if (span(it, 0).tiles) load_q(0);
                     if (tiles) load(&mk, 0, NB == 2 && tiles > 1 ? 1 : -1, false);
                     for (uint32_t t = 1; t < NT; ++t)
                         if (span(it, (int)t).tiles) load_q((int)t);
-                    for (int32_t j = 0; j < tiles && fine; ++j)
-                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (it.from + j + 1) * kKeys > first);
+                    if (tiles) load_v(0);
                 }
+                __syncwarp();
+                deal(n + 1);
+                if (lane == 0)
+                    for (int32_t j = 1; j < tiles && fine; ++j) load_v(j);
                 fine = __shfl_sync(0xffffffffu, fine, 0);
             }
             // copies in flight land before the CTA ends (they have, unless a wait ran out)
@@ -879,11 +905,13 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                         else {
                             const uint4 x = *w;
                             const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+                            // an exponent of ones carries into the sign's place
+                            constexpr uint32_t kCarry = (0x8000u - E) | (0x8000u - E) << 16;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) found |= (y[k] & E) == E || (y[k] >> 16 & E) == E;
+                            for (int k = 0; k < 4; ++k) found |= (y[k] & 0x7fff7fffu) + kCarry;
                         }
                     }
-                    if (__any_sync(0xffffffffu, found)) {
+                    if (__any_sync(0xffffffffu, found & 0x80008000u)) {
                         __syncwarp();
                         for (uint32_t d = lane; d < (uint32_t)D; d += 32) {
                             for (int32_t k = 0; k < rows; ++k) {
