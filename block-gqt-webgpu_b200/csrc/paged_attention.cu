@@ -45,7 +45,7 @@ struct Shape {
     static constexpr int kRow = F == F_INT4 ? D / 2 : F == F_INT8 ? D : 2 * D;  // bytes
     static constexpr int kGroups = F == F_INT4 ? D / 32 : F == F_INT8 ? 1 : 0;
     static constexpr int kTokens = kRow >= 256 ? 16 : kRow >= 128 ? 32 : 64;  // of a unit: 8 KB, or 4 KB
-    static constexpr int kStages = kRow >= 64 ? 3 : 4;
+    static constexpr int kStages = 3;
     static constexpr int kPart = kTokens * kRow;                 // K or V rows of a unit
     static constexpr int kScale = kTokens * kGroups * 2;         // K or V scales of a unit
     static constexpr int kStage = 2 * (kPart + kScale);
@@ -143,7 +143,7 @@ struct Cursor {
     uint32_t at, end;  // the units of it that are this CTA's (quads: all or none)
 };
 // What an item costs beside its units, in units: its queries, the join of the warps, its output.
-constexpr uint32_t kItemCost = 6;
+constexpr uint32_t kItemCost = 10;
 
 template <int F, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendArgs a) {
@@ -287,12 +287,22 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
     Cursor pre = cur;
     uint32_t pre_unit = unit0(pre);
     bool more = true;
-    int32_t page_reg = -1;
-    auto settle = [&]() {  // moves `pre` to the warp's next unit, if there is one, and loads its page indices
+    // Page indices of the warp's next units of the item, `span` to a unit: one load brings a window of them, a
+    // second one the window after it while this one is used.
+    const uint32_t span_shift = (uint32_t)T > (1u << shift) ? 31 - __clz(T) - shift : 0, span = 1u << span_shift;
+    const uint32_t window = 32 >> span_shift;
+    int32_t pages_now = -1, pages_next = -1;
+    uint32_t used = 0;  // units of this window that are done with
+    auto fetch_pages = [&](uint32_t unit) {  // for the units from `unit` on, in the warp's step
+        const uint32_t u = unit + (lane >> span_shift) * step_of(pre), t = u * T + ((lane & (span - 1)) << shift);
+        return u < pre.end && t < (uint32_t)pre.len ? __ldg(a.table + (int64_t)pre.b * a.table_stride + (t >> shift)) : -1;
+    };
+    auto settle = [&](bool fresh) {  // moves `pre` to the warp's next unit, if there is one, and sees to its page indices
         while (more && pre_unit >= pre.end) {
             more = next_item(pre);
             if (!more) break;
             pre_unit = unit0(pre);
+            fresh = true;
             // its queries, which are loaded when the ring gets there
             const uint32_t p = pair_of(pre), h = p % blocks * S::kHeads + lane / 2;
             if (p < pairs && lane / 2 < (uint32_t)S::kHeads && h < a.group) {
@@ -301,20 +311,24 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                 asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
             }
         }
-        if (more) {
-            const uint32_t t = pre_unit * T + (lane << shift);
-            page_reg = t < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T)
-                           ? __ldg(a.table + (int64_t)pre.b * a.table_stride + (t >> shift)) : -1;
+        if (!more) return;
+        if (fresh) {
+            used = 0;
+            pages_now = fetch_pages(pre_unit);
+            pages_next = fetch_pages(pre_unit + window * step_of(pre));
+        } else if (++used == window) {
+            used = 0;
+            pages_now = pages_next;
+            pages_next = fetch_pages(pre_unit + window * step_of(pre));
         }
     };
-    settle();
+    settle(true);
     auto fill = [&](uint32_t stage) {
         if (more) {
             const uint32_t t0 = pre_unit * T, kh = pair_of(pre) / blocks;
-            const int32_t page = page_reg;
-            const bool wrong = (uint32_t)page >= a.c.pages;
-            const bool asked = t0 + (lane << shift) < (uint32_t)pre.len && (lane == 0 || lane << shift < (uint32_t)T);
-            const uint32_t bad = __ballot_sync(0xffffffffu, wrong && asked);
+            const int32_t page = __shfl_sync(0xffffffffu, pages_now, (used << span_shift) + (lane & (span - 1)));
+            const bool asked = lane < span && t0 + (lane << shift) < (uint32_t)pre.len;
+            const uint32_t bad = __ballot_sync(0xffffffffu, asked && (uint32_t)page >= a.c.pages);
             if (bad && lane == 0) atomicOr(a.status, kStatusBadSlot);
             if (lane == 0) flags[warp * 4 + stage] = bad;
             const uint32_t dst = ring_at + stage * S::kStage;
@@ -349,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                 }
             }
             pre_unit += step_of(pre);
-            settle();
+            settle(false);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -568,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                 uint32_t big = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < (T * S::kGroups + 31) / 32; ++i) {
-                    const uint32_t x = vsc[i * 32 + lane];
+                    const uint32_t x = T * S::kGroups % 32 == 0 || lane < T * S::kGroups ? vsc[i * 32 + lane] : 0;
                     big = max(big, x < 0x7f80u ? x : 0u);
                 }
                 big = __reduce_max_sync(0xffffffffu, big);
@@ -784,21 +798,37 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
             __syncthreads();
             if (flags[kWarps * 4]) {
                 __threadfence();
-                for (uint32_t i = threadIdx.x; i < heads * (D / 2); i += kThreads) {
-                    const uint32_t head = i / (D / 2), d = 2 * (i % (D / 2));
-                    float big = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
-                    for (uint32_t c = c_first; c <= c_last; ++c) {
-                        const float *p = parts + (2ull * c + (c == c_first ? 1 : 0)) * S::kPartFloats;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + S::kHeads * D + 2 * head));
-                        const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + head * D + d));
-                        const float now = fmaxf(big, ml.x), ref = now == -INFINITY ? 0.0f : now;
-                        const float f = ex2(big - ref), g = ex2(ml.x - ref);
+                for (uint32_t i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
+                    const uint32_t head = i / (D / 4), d = 4 * (i % (D / 4));
+                    float big = -INFINITY, sum = 0.0f, x[4] = {};
+                    // kBatch parts at a time, so that their loads are in flight together
+                    constexpr uint32_t kBatch = 8;
+                    for (uint32_t c0 = c_first; c0 <= c_last; c0 += kBatch) {
+                        float2 ml[kBatch];
+                        float4 v[kBatch];
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const uint32_t c = min(c0 + k, c_last);
+                            const float *p = parts + (2ull * c + (c == c_first ? 1 : 0)) * S::kPartFloats;
+                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(p + S::kHeads * D + 2 * head));
+                            v[k] = __ldcg(reinterpret_cast<const float4 *>(p + head * D + d));
+                        }
+                        float now = big;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) now = fmaxf(now, ml[k].x);
+                        const float ref = now == -INFINITY ? 0.0f : now, f = ex2(big - ref);
                         big = now;
-                        sum = sum * f + ml.y * g;
-                        x = x * f + v.x * g;
-                        y = y * f + v.y * g;
+                        sum *= f, x[0] *= f, x[1] *= f, x[2] *= f, x[3] *= f;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const float g = c0 + k <= c_last ? ex2(ml[k].x - ref) : 0.0f;
+                            sum = fmaf(ml[k].y, g, sum);
+                            x[0] = fmaf(v[k].x, g, x[0]), x[1] = fmaf(v[k].y, g, x[1]);
+                            x[2] = fmaf(v[k].z, g, x[2]), x[3] = fmaf(v[k].w, g, x[3]);
+                        }
                     }
-                    write_out(head, d, x, y, big, sum);
+                    write_out(head, d, x[0], x[1], big, sum);
+                    write_out(head, d + 2, x[2], x[3], big, sum);
                 }
             }
         }
