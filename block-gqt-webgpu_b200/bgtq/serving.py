@@ -20,7 +20,8 @@ import torch
 from . import _lib
 
 _DTYPE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
-# format: (code, element type, elements of a row per dimension, dimensions per scale)
+_HALF = {torch.float16: "f16", torch.bfloat16: "bf16"}
+# format: (code, element type)
 _FORMATS = {"f16": (_lib.PAGES_F16, torch.float16), "bf16": (_lib.PAGES_BF16, torch.bfloat16),
             "int8": (_lib.PAGES_INT8, torch.int8), "int4": (_lib.PAGES_INT4, torch.uint8)}
 
@@ -80,43 +81,53 @@ class PagedCache:
                                          self.v.data_ptr(), *(None if t is None else t.data_ptr()
                                                               for t in (self.k_scales, self.v_scales)))
         self._ref = C.byref(self._desc)
+        self._on = self.k.device
         self._workspace = {}
+        library = _lib.lib()
+        self._write, self._read = library.bgtq_paged_write, library.bgtq_paged_read
+        self._attend = library.bgtq_paged_attend
 
-    def _slots(self, slots):
-        if (not slots.is_cuda or slots.device.index != self.device or slots.dtype != torch.int64 or slots.dim() != 1
-                or not slots.is_contiguous()):
+    def _check_slots(self, slots) -> None:
+        if slots.dtype != torch.int64 or slots.device != self._on or slots.dim() != 1 or not slots.is_contiguous():
             _refuse("Paged cache: slots must be a contiguous one-dimensional int64 tensor on the cache's device")
-        return slots
 
     def write(self, k, v, slots) -> None:
         """Store rows k, v [tokens, kv_heads, dim] (float16, bfloat16 or float32; any strides with
         a contiguous last dimension) at ``slots`` [tokens].  Negative slots are padding."""
-        slots = self._slots(slots)
+        self._check_slots(slots)
         shape = (slots.shape[0], self.kv_heads, self.dim)
-        if tuple(k.shape) != shape or tuple(v.shape) != shape:
+        if k.shape != shape or v.shape != shape:
             _refuse("Paged write: K and V must be [tokens, kv_heads, dim] with one slot a token")
-        if k.dtype != v.dtype or k.dtype not in _DTYPE:
+        dtype = _DTYPE.get(k.dtype)
+        if dtype is None or v.dtype != k.dtype:
             _refuse("Paged write: K and V must both be float16, bfloat16 or float32")
-        if not k.is_cuda or k.device != slots.device or v.device != slots.device:
+        if k.device != self._on or v.device != self._on:
             _refuse("Paged write: K and V must be on the cache's device")
-        if k.stride(2) != 1 or v.stride(2) != 1:
+        k0, k1, k2 = k.stride()
+        v0, v1, v2 = v.stride()
+        if k2 != 1 or v2 != 1:
             _refuse("Paged write: the last dimension must be contiguous")
-        _lib.call("bgtq_paged_write", self._ref, k.data_ptr(), v.data_ptr(), _DTYPE[k.dtype], shape[0], k.stride(0),
-                  k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), _stream(self.device))
+        status = self._write(self._ref, k.data_ptr(), v.data_ptr(), dtype, shape[0], k0, k1, v0, v1, slots.data_ptr(),
+                             _stream(self.device))
+        if status:
+            _lib.check(status)
 
     def read(self, slots, dtype=None):
         """(k, v) [tokens, kv_heads, dim]: the values that the rows at ``slots`` stand for, as
         dtype (default: the pages' own type, bfloat16 for 8- and 4-bit pages); zeros for
         negative slots."""
-        slots = self._slots(slots)
+        self._check_slots(slots)
         if dtype is None:
             dtype = torch.float16 if self.format == "f16" else torch.bfloat16
-        if dtype not in _DTYPE:
+        code = _DTYPE.get(dtype)
+        if code is None:
             _refuse("Paged read: dtype must be float16, bfloat16 or float32")
-        k = torch.empty((slots.shape[0], self.kv_heads, self.dim), dtype=dtype, device=slots.device)
+        n = slots.shape[0]
+        k = slots.new_empty((n, self.kv_heads, self.dim), dtype=dtype)
         v = torch.empty_like(k)
-        _lib.call("bgtq_paged_read", self._ref, slots.data_ptr(), slots.shape[0], k.data_ptr(), v.data_ptr(),
-                  _DTYPE[dtype], _stream(self.device))
+        status = self._read(self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code, _stream(self.device))
+        if status:
+            _lib.check(status)
         return k, v
 
     def attend(self, q, table, lengths, scale: float | None = None, out=None, lse: bool = False):
@@ -124,57 +135,68 @@ class PagedCache:
         pages' type over 16-bit pages) over the first ``lengths`` [batch] (int32) tokens of the
         pages in ``table`` [batch, width] (int32).  Returns out [batch, q_heads, dim], with
         ``lse`` also the log sums [batch, q_heads] (float32).  scale: 1 / sqrt(dim) if None."""
-        if q.dim() != 3 or q.shape[2] != self.dim or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.dim or shape[1] < 1 or shape[1] % self.kv_heads:
             _refuse("Paged attention: Q must be [batch, q_heads, dim], q_heads a multiple of kv_heads")
-        batch, heads = q.shape[0], q.shape[1]
-        if q.dtype not in (torch.float16, torch.bfloat16) or self.format in ("f16", "bf16") and q.dtype != self.k.dtype:
+        batch, heads, _ = shape
+        dtype = q.dtype
+        if dtype not in _HALF or self.format in _HALF.values() and self.format != _HALF[dtype]:
             _refuse("Paged attention: Q must be float16 or bfloat16, and of the type of 16-bit pages")
-        if not q.is_cuda or q.device.index != self.device or q.stride(2) != 1:
+        q0, q1, q2 = q.stride()
+        if q.device != self._on or q2 != 1:
             _refuse("Paged attention: Q must be on the cache's device with a contiguous last dimension")
-        if (table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32 or table.device != q.device
+        if (table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32 or table.device != self._on
                 or (table.shape[1] > 1 and table.stride(1) != 1)):
             _refuse("Paged attention: the table must be int32 [batch, width] on the cache's device")
         if (lengths.dim() != 1 or lengths.shape[0] != batch or lengths.dtype != torch.int32
-                or lengths.device != q.device or (batch > 1 and lengths.stride(0) != 1)):
+                or lengths.device != self._on or (batch > 1 and lengths.stride(0) != 1)):
             _refuse("Paged attention: lengths must be int32 [batch] on the cache's device")
         if scale is not None and not 0.0 < scale < float("inf"):
             _refuse("Paged attention: scale must be positive and finite")
         if out is None:
-            out = torch.empty((batch, heads, self.dim), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            out = q.new_empty(shape)
+        elif out.shape != shape or out.dtype != dtype or out.device != self._on or not out.is_contiguous():
             _refuse("Paged attention: out must be contiguous, of Q's shape, type and device")
-        sums = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if lse else None
+        sums = q.new_empty((batch, heads), dtype=torch.float32) if lse else None
         st = _stream(self.device)
-        work = self._work(heads, st)
-        _lib.call("bgtq_paged_attend", self._ref, q.data_ptr(), _DTYPE[q.dtype], batch, heads, q.stride(0), q.stride(1),
-                  table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-                  0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr(),
-                  work.data_ptr(), work.numel(), st)
+        work = self._workspace.get((st, heads)) or self._work(heads, st)
+        status = self._attend(self._ref, q.data_ptr(), _DTYPE[dtype], batch, heads, q0, q1, table.data_ptr(),
+                              table.stride(0), table.shape[1], lengths.data_ptr(), 0.0 if scale is None else scale,
+                              out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1], st)
+        if status:
+            _lib.check(status)
         return (out, sums) if lse else out
 
     def _work(self, heads: int, stream: int):
-        """The stream's own workspace (calls on different streams may overlap)."""
-        have = self._workspace.get((stream, heads))
-        if have is None:
-            need = C.c_size_t()
-            _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
-            have = torch.zeros(need.value, dtype=torch.uint8, device=self.k.device)
-            self._workspace[stream, heads] = have
-        return have
+        """The stream's own workspace (calls on different streams may overlap): address, bytes, tensor."""
+        need = C.c_size_t()
+        _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
+        have = torch.zeros(need.value, dtype=torch.uint8, device=self._on)
+        self._workspace[stream, heads] = have.data_ptr(), need.value, have
+        return self._workspace[stream, heads]
 
 
 _prompt_work = {}
 
 
-def _prompt_workspace(device: int, dim: int, stream: int):
-    """The stream's own workspace (calls on different streams may overlap)."""
-    have = _prompt_work.get((device, dim, stream))
-    if have is None:
-        need = C.c_size_t()
-        _lib.call("bgtq_prompt_workspace", device, dim, C.byref(need))
-        have = torch.zeros(need.value, dtype=torch.uint8, device=torch.device("cuda", device))
-        _prompt_work[device, dim, stream] = have
-    return have
+def _prompt_workspace(device, dim: int, stream: int):
+    """The stream's own workspace (calls on different streams may overlap): address, bytes, tensor."""
+    need = C.c_size_t()
+    _lib.call("bgtq_prompt_workspace", device.index, dim, C.byref(need))
+    have = torch.zeros(need.value, dtype=torch.uint8, device=device)
+    _prompt_work[device.index, dim, stream] = have.data_ptr(), need.value, have
+    return _prompt_work[device.index, dim, stream]
+
+
+def _even(t):
+    """t, or a packed copy of it where the kernels' loads cannot follow its strides or address, and its
+    token and head strides (that of a dimension of one element is never used)."""
+    s0, s1, s2 = t.stride()
+    n0, n1, _ = t.shape
+    if s2 != 1 or n0 > 1 and (s0 <= 0 or s0 % 8) or n1 > 1 and (s1 <= 0 or s1 % 8) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, _ = t.stride()
+    return t, s0 if n0 > 1 else 8, s1 if n1 > 1 else 8
 
 
 def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scale: float | None = None, out=None,
@@ -188,43 +210,41 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
     contiguous last dimension; a tensor whose strides or address are not multiples of 16
     bytes is copied.  Returns out [tokens, q_heads, dim], with ``lse`` also the log sums
     [tokens, q_heads] (float32)."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+    shape, keys = q.shape, k.shape
+    if len(shape) != 3 or len(keys) != 3 or v.shape != keys or shape[2] != keys[2]:
         _refuse("Prompt attention: Q must be [tokens, q_heads, dim], K and V [key tokens, kv_heads, dim]")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype, on = q.dtype, q.device
+    if dtype not in _HALF or k.dtype != dtype or v.dtype != dtype:
         _refuse("Prompt attention: Q, K and V must all be float16 or all bfloat16")
-    if not q.is_cuda or k.device != q.device or v.device != q.device:
+    if on.type != "cuda" or k.device != on or v.device != on:
         _refuse("Prompt attention: Q, K and V must be CUDA tensors on one device")
-    if q.shape[2] not in (64, 128) or k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+    tokens, heads, dim = shape
+    if dim not in (64, 128) or keys[1] < 1 or heads < 1 or heads % keys[1]:
         _refuse("Prompt attention: head dim must be 64 or 128 and q_heads a multiple of kv_heads")
-    for s in (starts, key_starts):
-        if s is not None and (s.dim() != 1 or s.shape[0] != starts.shape[0] or s.shape[0] < 1 or s.dtype != torch.int32
-                              or s.device != q.device or not s.is_contiguous()):
+    for s in (starts,) if key_starts is None else (starts, key_starts):
+        if (s.dim() != 1 or s.shape[0] != starts.shape[0] or s.shape[0] < 1 or s.dtype != torch.int32 or s.device != on
+                or not s.is_contiguous()):
             _refuse("Prompt attention: starts must be int32 [sequences + 1] on Q's device")
-    if key_starts is None and k.shape[0] != q.shape[0]:
+    if key_starts is None and keys[0] != tokens:
         _refuse("Prompt attention: key_starts are needed when K has other tokens than Q")
     if scale is not None and not 0.0 < scale < float("inf"):
         _refuse("Prompt attention: scale must be positive and finite")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype or out.device != on or not out.is_contiguous():
         _refuse("Prompt attention: out must be contiguous, of Q's shape, type and device")
-    sums = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if lse else None
-
-    def even(t):
-        # a stride of a dimension of one element is never used
-        steps = [t.stride(i) for i in (0, 1) if t.shape[i] > 1]
-        if t.stride(2) != 1 or any(s % 8 or s == 0 for s in steps) or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t, t.stride(0) if t.shape[0] > 1 else 8, t.stride(1) if t.shape[1] > 1 else 8
-
-    (q, *sq), (k, *sk), (v, *sv) = even(q), even(k), even(v)
-    dev = q.device.index
+    sums = q.new_empty((tokens, heads), dtype=torch.float32) if lse else None
+    q, q0, q1 = _even(q)
+    k, k0, k1 = _even(k)
+    v, v0, v1 = _even(v)
+    dev = on.index
     st = _stream(dev)
-    work = _prompt_workspace(dev, q.shape[2], st)
-    p = _lib.PromptDesc(dev, _DTYPE[q.dtype], starts.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2], q.shape[0],
-                        k.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), *sq, *sk, *sv, starts.data_ptr(),
-                        None if key_starts is None else key_starts.data_ptr(), int(bool(causal)),
-                        0.0 if scale is None else scale, out.data_ptr(), None if sums is None else sums.data_ptr(),
-                        work.data_ptr(), work.numel())
-    _lib.call("bgtq_prompt_attend", C.byref(p), st)
+    work = _prompt_work.get((dev, dim, st)) or _prompt_workspace(on, dim, st)
+    p = _lib.PromptDesc(dev, _DTYPE[dtype], starts.shape[0] - 1, heads, keys[1], dim, tokens, keys[0], q.data_ptr(),
+                        k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, starts.data_ptr(),
+                        None if key_starts is None else key_starts.data_ptr(), 1 if causal else 0,
+                        0.0 if scale is None else scale, out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1])
+    status = _lib.lib().bgtq_prompt_attend(C.byref(p), st)
+    if status:
+        _lib.check(status)
     return (out, sums) if lse else out

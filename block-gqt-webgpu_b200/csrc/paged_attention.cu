@@ -840,10 +840,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
 
 // CTAs of a launch at most: the workspace holds two parts of each.
 uint32_t most_ctas() {
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return (uint32_t)sms * 4;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess ? (uint32_t)sm_count(dev) * 4 : 0;
 }
 uint32_t counter_bytes() { return (most_ctas() * 4 + 15) / 16 * 16; }
 
@@ -863,9 +861,8 @@ cudaError_t run(const PagedAttendArgs &a, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         resident[dev] = n < 1 ? 1 : n > 4 ? 4 : n;
     }
-    int sms = 0;
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
+    const int sms = sm_count(dev);
+    if (!sms) return cudaErrorInvalidDevice;
     PagedAttendArgs b = a;
     b.counters = counter_bytes();
     b.q_even = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_batch % 8 == 0 && a.q_head % 8 == 0;

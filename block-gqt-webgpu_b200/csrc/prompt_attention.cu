@@ -983,10 +983,11 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
     using P = Plan<D>;
     if (!encoder()) return cudaErrorNotSupported;
     auto kernel = prompt_kernel<D, BF>;
-    int dev = 0, sms = 0;
+    int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    if (e != cudaSuccess) return e;
+    const int sms = sm_count(dev);
+    if (!sms) return cudaErrorInvalidDevice;
     static bool ready[64] = {};
     if (!ready[dev]) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kTotal);
@@ -1017,9 +1018,9 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
 }  // namespace
 
 size_t prompt_workspace(uint32_t dim) {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
+    int dev = 0;
+    const int sms = cudaGetDevice(&dev) == cudaSuccess ? sm_count(dev) : 0;
+    if (!sms) return 0;
     const uint32_t tiles = dim == 64 ? Plan<64>::kTiles : Plan<128>::kTiles;
     return prompt_counters(sms, tiles) + 2ull * sms * tiles * kRows * (dim + 2) * 4;
 }

@@ -89,4 +89,15 @@ cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t s);
 size_t prompt_workspace(uint32_t dim);
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s);
 
+// SMs of a device (0: no such device), asked for once.
+inline int sm_count(int device) {
+    static int known[64] = {};  // (threads that race here write the same value)
+    if (device < 0 || device >= 64) return 0;
+    if (!known[device] && cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        known[device] = 0;
+        cudaGetLastError();
+    }
+    return known[device];
+}
+
 }  // namespace bgtq
