@@ -14,16 +14,17 @@ from .attention import AttentionEngine, AttentionSession, GroupedAttention, Opti
 __all__ = ["BGTQError", "DeviceError", "LayoutError", "RangeError", "StateError", "LIB_PATH", "lib",
            "BlockGTQParameters", "allocate_bits", "build_tables", "haar_rotation", "optimal_centroids", "tables", "validate_layout", "CompressedKeys", "FP16Keys", "append_kv",
            "PackedKeys", "Values", "AttentionEngine", "AttentionSession", "GroupedAttention", "OptimizedAttention",
-           "PagedCache", "prompt_attention",
+           "PagedCache", "prompt_attention", "PagedDecoder",
            "device_status", "set_layout_jit", "layout_jit_stats",
            "layout_jit_counts", "layout_jit_wait"]
 
 
 def __getattr__(name):
     # the serving operators work on torch tensors: torch is imported with their first use
-    if name in ("PagedCache", "prompt_attention"):
-        from . import serving
-        globals().update(PagedCache=serving.PagedCache, prompt_attention=serving.prompt_attention)
+    if name in ("PagedCache", "prompt_attention", "PagedDecoder"):
+        from . import paged_model, serving
+        globals().update(PagedCache=serving.PagedCache, prompt_attention=serving.prompt_attention,
+                         PagedDecoder=paged_model.PagedDecoder)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 

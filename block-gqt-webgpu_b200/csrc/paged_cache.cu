@@ -2,7 +2,7 @@
 // reading them back.
 //
 // A group of a row (the whole row in 8 bits, 32 dimensions in 4) has one scale, stored in BF16:
-//     s = bf16(max|x| / top),  c = clamp(round(x / s), -top, top),  x' = c s,   top = 127 or 7,
+//     s = bf16(max|x| (1 / top)),  c = clamp(round(x / s), -top, top),  x' = c s,   top = 127 or 7,
 // c = 0 where s = 0.  The scale keeps BF16's 8 bits because its exponent range is FP32's (no
 // input of any source type overflows it), and because the codes are computed against the
 // rounded scale, so that its rounding moves the step by 0.4 % at most and adds no error of its
@@ -97,7 +97,10 @@ __device__ __forceinline__ void put(unsigned char *rows, uint16_t *scales, uint6
 #pragma unroll
         for (uint32_t w = 1; w < kLanes; w <<= 1) m = max(m, __shfl_xor_sync(lanes, m, w));
         const bool fine = m < 0x7f800000u;
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(m), kTop));
+        // one product with the rounded 1 / top: at most an ulp of FP32 from the quotient, and the scale keeps 8 bits
+        // of it (about one scale in 2^17 lands on the other side of a BF16 tie; every code and value goes by the
+        // scale that is stored)
+        const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__uint_as_float(m), 1.0f / kTop));
         const float s = __bfloat162float(sb);
         // x / s, correctly rounded: one correctly rounded reciprocal y, then q = q0 + (x - s q0) y with q0 = x y
         // (Markstein, IBM J. Res. Dev. 34(1), 1990: q is the IEEE quotient where nothing over- or underflows;

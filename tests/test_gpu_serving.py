@@ -8,10 +8,11 @@ product and the result rounded once, is within u |o| + u A of the exact value, A
 relative on a probability) add at most 3e-5 A; an FP16 probability below 2^-14 is held to
 2^-25 absolute, which adds 2^-25 sum |v_t| / l, l = sum exp(s_t - max) >= 1.  The log sum is
 FP32 throughout: 3e-5 absolute.
-Stored rows are exact: the formula's steps are FP32 with IEEE rounding, which a 64-bit
-computation of the scale (rounded to FP32 before BF16) reproduces, and a code can differ from
-the 64-bit one only where x / s falls on a half within an FP32 rounding; those places are
-counted, and a code there may differ by one.
+Stored rows are exact: the formula's steps are FP32 with IEEE rounding; a 64-bit computation of
+the scale (rounded to FP32 before BF16) gives the same one but for about one group in 2^17, whose
+maximum / top is within an FP32 rounding of a BF16 tie (none of these inputs has one), and a code
+can differ from the 64-bit one only where x / s falls on a half within an FP32 rounding; those
+places are counted, and a code there may differ by one.
 """
 import math
 import subprocess
