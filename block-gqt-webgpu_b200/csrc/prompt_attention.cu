@@ -42,7 +42,8 @@ constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_interna
 constexpr uint32_t kDeal = 4;            // items dealt ahead
 constexpr int64_t kItemCost = 384;       // what an item costs beside its keys, in keys: queries, outputs, joining
 constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while where items are few
-constexpr int32_t kWhole = 512;          // an item of no more keys than that is not split: joining costs as much
+constexpr int32_t kWhole = 1024;         // an item of no more keys than that is not split: joining costs as much
+constexpr int kJoin = 2;                 // parts of an item that are joined at a time
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
 // ---- device helpers -----------------------------------------------------------------------
@@ -185,7 +186,8 @@ struct Plan {
     static constexpr uint32_t kKeys = 64;                          // of a K or V tile
     static constexpr uint32_t kColO = kTiles * kBufs * kKeys;      // the first column of the outputs
     static constexpr uint32_t kThreads = 128 * kTiles + 128;
-    // Registers: kThreads x kAll at launch, 128 kTiles x kSoft + 128 x kRest afterwards, 61440 or 64512 in all.
+    // Registers: kThreads x 96 (head dim 64) or 168 at launch, 128 kTiles x kSoft + 128 x kRest afterwards: 61440
+    // or 64512 in all.  More does not fit beside the tiles; the softmax threads hold 64 logits and little else.
     static constexpr uint32_t kSoft = D == 64 ? 104 : 216, kRest = D == 64 ? 64 : 72;
     static constexpr int kFma = D == 64 ? 2 : 6;                   // exponentials of 16 on the FMA pipe
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
@@ -455,16 +457,16 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     float *mine = part_of((int32_t)blockIdx.x);
                     __stcg(mine + D * 32, sp.tiles ? ref : -INFINITY);
                     __stcg(mine + (D + 1) * 32, sp.tiles ? sum : 0.0f);
-                    if (sp.tiles) {
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16] = {};
+                        if (sp.tiles) {
                             tm_load16(to + 16 * c, o);
                             tc_wait_ld();
                             if (flagged) overlay(o, 16 * c, std::integral_constant<int, 16>());
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]));
                         }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]));
                     }
                     tc_before();
                     __threadfence();
@@ -481,10 +483,23 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     }
                     __threadfence();
                     ref = -INFINITY, sum = 0.0f;
-                    for (int32_t c = it.part; c < it.part + it.parts; ++c) ref = max_nan(ref, __ldcg(part_of(c) + D * 32));
-                    const float base_ref = ref == -INFINITY ? 0.0f : ref;
-                    for (int32_t c = it.part; c < it.part + it.parts; ++c)
-                        sum = fmaf(ex2(__ldcg(part_of(c) + D * 32) - base_ref), __ldcg(part_of(c) + (D + 1) * 32), sum);
+                    const int32_t after = it.part + it.parts;
+                    for (int32_t c = it.part; c < after; c += kJoin) {
+                        float m[kJoin], l[kJoin];
+#pragma unroll
+                        for (int b = 0; b < kJoin; ++b) {
+                            m[b] = c + b < after ? __ldcg(part_of(c + b) + D * 32) : -INFINITY;
+                            l[b] = c + b < after ? __ldcg(part_of(c + b) + (D + 1) * 32) : 0.0f;
+                        }
+                        float top = ref;
+#pragma unroll
+                        for (int b = 0; b < kJoin; ++b) top = max_nan(top, m[b]);
+                        const float from = top == -INFINITY ? 0.0f : top;
+                        sum *= ex2(ref - from);
+#pragma unroll
+                        for (int b = 0; b < kJoin; ++b) sum = fmaf(ex2(m[b] - from), l[b], sum);
+                        ref = top;
+                    }
                 }
                 const bool none = sees == 0;
                 const float inv = none ? 0.0f : 1.0f / sum;
@@ -500,20 +515,28 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 }
                 // 16-byte chunk c of row r: a phase of eight lanes meets 128 different bytes, writing and reading
                 auto chunk = [&](uint32_t r, uint32_t c) { return turn + r * 2 * kW + ((c ^ r / (8 / kL) % kL) << 4); };
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D / kW; ++c) {
                     uint32_t o[kW];
                     if (!whole) {
 #pragma unroll
                         for (int i = 0; i < kW; ++i) o[i] = 0;
-                        for (int32_t q = it.part; q < it.part + it.parts; ++q) {
-                            const float *from = part_of(q);
-                            const float m = __ldcg(from + D * 32);
-                            if (m == -INFINITY) continue;  // no K tile of this row tile
-                            const float f = ex2(m - ref);
+                        const int32_t after = it.part + it.parts;
+                        for (int32_t q = it.part; q < after; q += kJoin) {  // their loads in flight together
+                            float f[kJoin], x[kJoin][kW];
 #pragma unroll
-                            for (int i = 0; i < kW; ++i)
-                                o[i] = __float_as_uint(fmaf(f, __ldcg(from + (kW * c + i) * 32), __uint_as_float(o[i])));
+                            for (int b = 0; b < kJoin; ++b) {
+                                const float *from = part_of(q + b);
+                                f[b] = q + b < after ? __ldcg(from + D * 32) : -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < kW; ++i) x[b][i] = q + b < after ? __ldcg(from + (kW * c + i) * 32) : 0.0f;
+                            }
+#pragma unroll
+                            for (int b = 0; b < kJoin; ++b) {
+                                const float e = ex2(f[b] - ref);  // 0 for a part of no K tile that this row sees
+#pragma unroll
+                                for (int i = 0; i < kW; ++i) o[i] = __float_as_uint(fmaf(e, x[b][i], __uint_as_float(o[i])));
+                            }
                         }
                     } else if (sp.tiles) {
                         if constexpr (kW == 32) tm_load(to + kW * c, o);
@@ -612,17 +635,20 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             };
             int64_t total = __shfl_sync(0xffffffffu, own_upto, 31);
             uint32_t blocks = (uint32_t)mine.blocks;
+            int32_t longest = mine.blocks ? mine.nk : 0;
             if (a.sequences > 32) {
                 int64_t rest = 0;
                 for (uint32_t s = lane + 32; s < a.sequences; s += 32) {
                     const Seq q = load_seq(s);
                     rest += a.kv_heads * price(q, q.blocks);
                     blocks += (uint32_t)q.blocks;
+                    longest = max(longest, q.blocks ? q.nk : 0);
                 }
                 total += __shfl_sync(0xffffffffu, scan(rest), 31);
             }
             const int64_t all = (int64_t)__reduce_add_sync(0xffffffffu, blocks) * a.kv_heads;
-            const int64_t ctas = min(min((int64_t)gridDim.x, max((int64_t)1, total / kKeys)), max(all, total / kPiece));
+            int64_t ctas = min((int64_t)gridDim.x, max((int64_t)1, total / kKeys));
+            if (__reduce_max_sync(0xffffffffu, longest) > kWhole) ctas = min(ctas, max(all, total / kPiece));
             bool some = ctas > 0 && (int64_t)blockIdx.x < ctas;
             const int64_t each = some ? quotient(total, ctas) : 1, over = some ? total - each * ctas : 0;
             const int64_t start = blockIdx.x * each + min((int64_t)blockIdx.x, over);
@@ -735,36 +761,36 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             deal(0);
             for (uint32_t n = 0; fine && next(n, it); ++n) {
                 const int32_t tiles = tiles_of(it), first = span(it, 0).first;
-                    auto load_q = [&](int t) {
-                        if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase >> t & 1u, stop))) return;
-                        q_phase ^= 1u << t;
-                        q_issued |= 1u << t;
-                        bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
+                auto load_q = [&](int t) {
+                    if (!(fine = fine && bar_wait(bar(B_QFREE + t), q_phase >> t & 1u, stop))) return;
+                    q_phase ^= 1u << t;
+                    q_issued |= 1u << t;
+                    bar_expect(bar(B_QFULL + t), P::kChunks * per * a.group * 128u);
+                    for (uint32_t c = 0; c < P::kChunks; ++c)
+                        tma3(base + P::kQ + t * P::kQTile + c * P::kQChunk, &mq, bar(B_QFULL + t), 64 * c,
+                             it.head * (int32_t)a.group, it.token + t * (int32_t)per);
+                };
+                // first the K tiles that logits run ahead by, then V j and K j + NB: rows of tiles, -1 for none
+                auto load = [&](const CUtensorMap *map, int32_t one, int32_t two, bool look) {
+                    if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
+                    const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
+                    bar_expect(on, P::kTile * (two < 0 ? 1u : 2u));
+                    const uint32_t dst = base + P::kRing + slot * 2 * P::kTile;
+                    for (uint32_t c = 0; c < P::kChunks; ++c)
+                        tma3(dst + c * P::kChunk, map, on, 64 * c, it.head, it.key + (it.from + one) * kKeys);
+                    if (two >= 0)
                         for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(base + P::kQ + t * P::kQTile + c * P::kQChunk, &mq, bar(B_QFULL + t), 64 * c,
-                                 it.head * (int32_t)a.group, it.token + t * (int32_t)per);
-                    };
-                    // first the K tiles that logits run ahead by, then V j and K j + NB: rows of tiles, -1 for none
-                    auto load = [&](const CUtensorMap *map, int32_t one, int32_t two, bool look) {
-                        if (!(fine = fine && bar_wait(bar(B_FREE + slot), free_phase, stop))) return;
-                        const uint32_t on = bar((look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
-                        bar_expect(on, P::kTile * (two < 0 ? 1u : 2u));
-                        const uint32_t dst = base + P::kRing + slot * 2 * P::kTile;
-                        for (uint32_t c = 0; c < P::kChunks; ++c)
-                            tma3(dst + c * P::kChunk, map, on, 64 * c, it.head, it.key + (it.from + one) * kKeys);
-                        if (two >= 0)
-                            for (uint32_t c = 0; c < P::kChunks; ++c)
-                                tma3(dst + P::kTile + c * P::kChunk, &mk, on, 64 * c, it.head,
-                                     it.key + (it.from + two) * kKeys);
-                        issued |= bit;
-                        raw = look ? raw | bit : raw & ~bit;
-                        full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
-                        raw_phase ^= look ? bit : 0;
-                        if (++slot == P::kStages) slot = 0, free_phase ^= 1;
-                    };
-                    auto load_v = [&](int32_t j) {
-                        load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (it.from + j + 1) * kKeys > first);
-                    };
+                            tma3(dst + P::kTile + c * P::kChunk, &mk, on, 64 * c, it.head,
+                                 it.key + (it.from + two) * kKeys);
+                    issued |= bit;
+                    raw = look ? raw | bit : raw & ~bit;
+                    full_phase = (full_phase & ~bit) | (free_phase ^ 1u) << slot;
+                    raw_phase ^= look ? bit : 0;
+                    if (++slot == P::kStages) slot = 0, free_phase ^= 1;
+                };
+                auto load_v = [&](int32_t j) {
+                    load(&mv, j, j + (int32_t)NB < tiles ? j + (int32_t)NB : -1, (it.from + j + 1) * kKeys > first);
+                };
                 if (lane == 0) {
                     if (span(it, 0).tiles) load_q(0);
                     if (tiles) load(&mk, 0, NB == 2 && tiles > 1 ? 1 : -1, false);
@@ -992,6 +1018,11 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
     if (!ready[dev]) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kTotal);
         if (e != cudaSuccess) return e;
+        // the warps hand registers to each other: more than the launch has would be waited for
+        cudaFuncAttributes f;
+        e = cudaFuncGetAttributes(&f, kernel);
+        if (e != cudaSuccess) return e;
+        if ((uint32_t)f.numRegs * P::kThreads < 128 * P::kTiles * P::kSoft + 128 * P::kRest) return cudaErrorNotSupported;
         ready[dev] = true;
     }
     PromptArgs a = args;
@@ -1008,8 +1039,7 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
     auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.sequences - 1); };
     a.tiles = P::kTiles;
     while (a.tiles > 1 && 2 * items(a.tiles) <= (uint64_t)sms) a.tiles /= 2;
-    const uint64_t most = items(a.tiles), pieces = most * (a.k_tokens + kItemCost) / kPiece + 1;
-    const uint64_t ctas = most > pieces ? most : pieces;
+    const uint64_t ctas = items(a.tiles) * (a.k_tokens + kItemCost) / P::kKeys + 1;
     a.counters = prompt_counters(sms, P::kTiles);
     kernel<<<(uint32_t)(ctas < (uint64_t)sms ? ctas : sms), P::kThreads, P::kTotal, s>>>(a, mq, mk, mv);
     return cudaGetLastError();
