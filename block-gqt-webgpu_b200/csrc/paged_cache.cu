@@ -7,11 +7,13 @@
 // input of any source type overflows it), and because the codes are computed against the
 // rounded scale, so that its rounding moves the step by 0.4 % at most and adds no error of its
 // own.  A group with an infinity or a NaN in it has no step: its scale is stored as NaN and the
-// whole group reads back as NaN.  All of it is FP32 arithmetic with IEEE divisions.
+// whole group reads back as NaN.  All of it is FP32 arithmetic with IEEE rounding.
 //
-// Both directions move each row once and compute little, so HBM bounds them.  A thread takes eight
-// dimensions of a row (16-byte loads and stores of 16-bit elements); the lanes of a row, or of a
-// 4-bit group, agree on the maximum by shuffles.
+// Both directions move each row once.  A thread takes eight dimensions of a row (16-byte loads and
+// stores of 16-bit elements); the lanes of a row, or of a 4-bit group, agree on the maximum by
+// shuffles.  16K tokens of 8 heads of 128 in 4 bits, written and read back: 51 us for 172 MB,
+// 3.4 TB/s, half a copy's rate: writing is bound by its arithmetic (six instructions an element for
+// the quotient and its code), reading by its stores.  16 tokens of 3 heads: 3.8 us, two launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

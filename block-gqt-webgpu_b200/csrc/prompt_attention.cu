@@ -6,13 +6,15 @@
 // A work item is a block of consecutive positions of one sequence with all query heads of one
 // KV head: 128 rows a tile, floor(128 / group) positions x group heads, up to four tiles (head
 // dim 64) or two (128), which share every K and V tile of 64 keys.  Tensor memory sets these
-// numbers: logits and outputs of all row tiles fill its 512 columns, 4 x (64 + 64) at head dim 64,
-// 2 x (2 x 64 + 128) at 128, where the logits are double-buffered instead.  A CTA takes items
-// until none is left.  Its warps have roles:
+// numbers: logits and outputs of all row tiles fill its 512 columns, 4 x (64 + 64) at head dim
+// 64, 2 x (2 x 64 + 128) at 128, where the logits are double-buffered instead.  One CTA an SM
+// takes an equal range of the items' keys, computed on the device from the lengths; an item
+// across two ranges is done in parts, which its last CTA joins.  The warps have roles:
 //   softmax     four warps a row tile, a thread a row: logits out of tensor memory, mask, running
 //               maximum, probabilities back into tensor memory (as 16-bit pairs in the columns
 //               where the logits were), and the outputs at the end
-//   deal, loads one warp: this CTA's share of the items, and the TMA loads of Q, K and V (128-byte swizzle) into a ring of stages
+//   deal, loads one warp: this CTA's share of the items, and the TMA loads of Q, K and V (128-byte
+//               swizzle) into a ring of stages
 //   products    two warps, each for half of the row tiles: S = Q K^T (operands in shared memory)
 //               ahead of softmax and O += P V (P in tensor memory, V as it lies), FP32
 //               accumulators in tensor memory.  The warp stays together and one lane issues, so
@@ -22,9 +24,21 @@
 //               multiplied: rows past the end (another sequence's, or nothing) are zeroed, and an
 //               infinity or a NaN, which the zero probability of a row that does not see it would
 //               turn into a NaN, is taken out and given to the rows that do see it
+//
+// What bounds it.  A K tile of 64 keys costs a row tile 512 (head dim 128) or 256 clocks of
+// tensor arithmetic; the logits' products, which read both operands from shared memory, take 48
+// clocks an instruction for 32 of arithmetic, so products alone come to 640 or 320.  Its 8192
+// exponentials take 512 clocks at 16 a clock, so some go to the FMA pipe (kFma).  At head dim 128
+// products are the longer: four prompts of 3500 to 4096 tokens, 32 / 8 heads, causal, run at 1.04
+// to 1.14 PFLOP/s (415 to 455 us, with the power limit's clock).  At 64 it is exponentials with
+// the rest of softmax: two prompts of 8192 tokens, 14 / 2 heads, 283 us, 850 TFLOP/s.  Short
+// prompts are bound by their chain of latencies: 37 tokens take 8.3 us.  The tails (outputs,
+// joining) are short loops on purpose: unrolled, their instruction fetches cost 10 us a call.
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time: until then probabilities are taken relative to the older maximum, so they stay
-// below 2^8, and P is FP16 or BF16 (the inputs' type) with the same relative error.
+// below 2^8, and P is FP16 or BF16 (the inputs' type) with the same relative error: their rounding
+// is the formula's one beside the outputs' own, and sums take them before it.  (Rescaling at every
+// growth: three prompts of 300 to 512 tokens after 3500, 32 / 8 heads of 128, 120 us for 83.)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,10 +54,16 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kRows = 128;
 constexpr uint32_t kStatusTimeout = 1u;  // a bounded wait ran out (bgtq_internal.h's kStatusWaitTimeout)
 constexpr uint32_t kDeal = 4;            // items dealt ahead
-constexpr int64_t kItemCost = 384;       // what an item costs beside its keys, in keys: queries, outputs, joining
-constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while where items are few
-constexpr int32_t kWhole = 1024;         // an item of no more keys than that is not split: joining costs as much
-constexpr int kJoin = 2;                 // parts of an item that are joined at a time
+// What an item costs beside its keys, in keys: queries, outputs, joining.  (None: 12 prompts of 1 to 2047 tokens,
+// 14 / 2 heads of 64, 51 us for 42, two of 8192 tokens 345 us for 293; 200 and 600 are within 5 % of 384.)
+constexpr int64_t kItemCost = 384;
+// Items of no more keys are not split: joining costs as much as they do.  (512: 700 tokens of 32 heads of 64, 28.5 us
+// for 20.9; 2048: 64 tokens after 2000, 32 / 8 heads of 128, 42 us for 25.)
+constexpr int32_t kWhole = 1024;
+// Keys that make a CTA worth its while where items are few and long.  (16 tokens after 8000, 14 / 2 heads of 64:
+// 28.2 us with 512, 29.0 with 1024, 38.5 with 2048; 64 tokens after 2000 as above: 25.0, 26.4, 49.)
+constexpr int64_t kPiece = 512;
+constexpr int kJoin = 2;                 // parts of an item that are joined at a time (1: 2 % slower, 4: 5 %)
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 
 // ---- device helpers -----------------------------------------------------------------------
@@ -189,13 +209,15 @@ struct Plan {
     // Registers: kThreads x 96 (head dim 64) or 168 at launch, 128 kTiles x kSoft + 128 x kRest afterwards: 61440
     // or 64512 in all.  More does not fit beside the tiles; the softmax threads hold 64 logits and little else.
     static constexpr uint32_t kSoft = D == 64 ? 104 : 216, kRest = D == 64 ? 64 : 72;
-    static constexpr int kFma = D == 64 ? 2 : 6;                   // exponentials of 16 on the FMA pipe
+    // Exponentials of 16 on the FMA pipe.  Head dim 64, two prompts of 8192 tokens: none 319 us, 2 293, 4 297;
+    // 128, three of 300 to 512 after 3500: none 88.6 us, 2 88.5, 4 86.9, 6 83.6, 10 90.6.
+    static constexpr int kFma = D == 64 ? 2 : 6;
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
     static constexpr uint32_t kStages = D == 128 ? 4 : 7;          // of two K or V tiles in the ring
     static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kAfter = kRing + kStages * 2 * kTile;
-    static constexpr int kTurn = D == 64 ? 16 : 32;                // dimensions of an output row stored at a time (registers)
+    static constexpr int kTurn = D == 64 ? 16 : 32;                // dimensions of an output row stored at a time: what registers hold
     static constexpr uint32_t kOut = kAfter;                       // [softmax warps][32 rows][kTurn] outputs
     static constexpr uint32_t kBad = kOut + 4 * kTiles * 64 * kTurn;                    // [kDeal items][3 kinds][D] first keys
     static constexpr uint32_t kItems = kBad + kDeal * 3 * D * 2;   // [kDeal] Item
@@ -393,7 +415,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     const float f = grown ? ex2(ref - top) : 1.0f;
                     if (grown) ref = top;
                     sum *= f;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
                         tm_load16(to + 16 * c, o);
@@ -580,7 +602,8 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
             // An item's price is its keys, as its last row sees them, and kItemCost.  Items stand in order - sequences,
             // KV heads, blocks - on a line as long as their prices, K tile j of one at kItemCost + 64 j of its stretch,
             // and the line is cut into equal ranges, one a CTA, none shorter than a tile: whatever the
-            // lengths are, all CTAs end together, and where items are few, their keys are split.
+            // lengths are, all CTAs end together, and where items are few, their keys are split.  An item of up to kWhole
+            // keys is the CTA's in whose range it begins.
             const int32_t block = (int32_t)(a.tiles * per);
             struct Seq {
                 int32_t q0, k0, nq, nk, blocks, shift;
@@ -1034,8 +1057,9 @@ cudaError_t run(const PromptArgs &args, cudaStream_t s) {
         !make_map(&mk, BF, keys ? a.k : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.k_head, a.k_token, 1, P::kKeys) ||
         !make_map(&mv, BF, keys ? a.v : a.q, D, a.kv_heads, keys ? a.k_tokens : 1, a.v_head, a.v_token, 1, P::kKeys))
         return cudaErrorInvalidValue;
-    // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as possible,
-    // while that makes half as many items as there are SMs.
+    // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as possible, while
+    // that makes half as many items as there are SMs.  (512 tokens, 14 / 2 heads of 64: one tile 15.4 us, four 20.0;
+    // 700 tokens of 32 heads: one 32.9 us, two 30.5, four 35.3; two prompts of 8192: one 717 us, four 293.)
     auto items = [&](uint32_t tiles) { return a.kv_heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.sequences - 1); };
     a.tiles = P::kTiles;
     while (a.tiles > 1 && 2 * items(a.tiles) <= (uint64_t)sms) a.tiles /= 2;
