@@ -34,6 +34,7 @@ struct PagedWriteArgs {
     uint64_t tokens;
     bgtq_dtype dtype;
     uint32_t *status;
+    uint32_t head_mul, head_shift;  // row / heads = row * head_mul >> (32 + head_shift), for the kernels
 };
 
 struct PagedReadArgs {
@@ -43,6 +44,7 @@ struct PagedReadArgs {
     uint64_t tokens;
     bgtq_dtype dtype;
     uint32_t *status;
+    uint32_t head_mul, head_shift;
 };
 
 struct PagedAttendArgs {
