@@ -284,6 +284,65 @@ def test_prompt_in_a_graph(cuda):
     assert torch.equal(out, prompt_attention(q, k, v, st))
 
 
+@pytest.mark.parametrize("dtype,dim,hq,hk", [("f16", 64, 14, 2), ("bf16", 128, 4, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_items_done_in_parts(cuda, dtype, dim, hq, hk, causal):
+    """Few items over long keys: several CTAs have keys of one, and the last of them joins."""
+    nq, nk = [5, 200, 0, 700], [5003, 1300, 64, 3001]
+    q = randn(4, sum(nq), hq, dim, dtype=dtype)
+    k, v = (randn(s, sum(nk), hk, dim, dtype=dtype) for s in (5, 6))
+    check_prompt(q, k, v, nq, nk, causal, dtype)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_prompt_parts_with_values_not_every_row_sees(cuda, bad):
+    """Infinities and NaN in the last keys of a long item: they reach the rows that see them, from
+    whichever part holds them, and no others."""
+    import torch
+    n, m = 70, 4000
+    q = randn(1, n, 4, 64, dtype="f16")
+    k, v = (randn(s, m, 1, 64, dtype="f16") for s in (2, 3))
+    clean, _ = check_prompt(q, k, v, [n], [m], True, "f16")
+    v[m - 30, 0, 7] = bad
+    k[m - 1, 0, 0] = math.nan          # the last row alone sees it
+    from bgtq import prompt_attention
+    out = prompt_attention(q, k, v, starts_of([n]), starts_of([m]))
+    sees = torch.arange(n, device="cuda") >= n - 30
+    want = clean.clone()
+    want[sees, :, 7] = bad
+    want[n - 1] = math.nan
+    assert torch.equal(out.nan_to_num(nan=7.0, posinf=8.0), want.nan_to_num(nan=7.0, posinf=8.0))
+
+
+def test_prompt_many_sequences_and_one_long(cuda):
+    rng = np.random.default_rng(3)
+    n = [int(x) for x in rng.integers(0, 60, 70)] + [2500] + [int(x) for x in rng.integers(0, 9, 20)]
+    q = randn(4, sum(n), 6, 64, dtype="bf16")
+    k, v = (randn(s, sum(n), 2, 64, dtype="bf16") for s in (5, 6))
+    check_prompt(q, k, v, n, n, True, "bf16", seqs=[0, 3, 31, 32, 33, 69, 70, 71, 90])
+
+
+@pytest.mark.parametrize("dim,hq,hk", [(64, 14, 2), (128, 8, 2)])
+def test_prompt_repeated_over_changing_lengths(cuda, dim, hq, hk):
+    """Calls that follow each other without a pause, items whole and in parts in turn, give the bits
+    of a call alone."""
+    import torch
+    from bgtq import device_status, prompt_attention
+    lengths = [[1, 700, 33, 257], [2100], [64] * 40, [5, 1025, 900]]
+    calls = []
+    for i, n in enumerate(lengths):
+        q = randn(10 + i, sum(n), hq, dim, dtype="f16")
+        k, v = (randn(s + i, sum(n), hk, dim, dtype="f16") for s in (20, 30))
+        calls.append((q, k, v, starts_of(n)))
+    want = []
+    for c in calls:
+        want.append(prompt_attention(*c))
+        torch.cuda.synchronize()
+    got = [prompt_attention(*calls[i % 4]) for i in range(80)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 4]) for i, g in enumerate(got)) and device_status() == 0
+
+
 # ---- the paged cache --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("fmt", ["f16", "bf16", "int8", "int4"])
@@ -609,3 +668,43 @@ print("fine")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                        cwd=ROOT / "block-gqt-webgpu_b200")
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_python_refusals_on_the_device(cuda):
+    import ctypes as C
+    import torch
+    from bgtq import PagedCache, prompt_attention
+    c = PagedCache(2, 64, 4, 16, "f16")
+    x = randn(1, 3, 2, 64, dtype="f16")
+    slots = torch.arange(3, device="cuda")
+    for k, v, s, message in [(x, x, slots.int(), "int64"), (x, x, slots.cpu(), "cache's device"), (x, x, slots[:2], "one slot"),
+                             (x, x.float(), slots, "both be"), (x, x.cpu(), slots, "device"), (x.long(), x.long(), slots, "both be"),
+                             (x.transpose(0, 2).contiguous().transpose(0, 2), x, slots, "contiguous")]:
+        with pytest.raises(_lib.RangeError, match=message):
+            c.write(k, v, s)
+    with pytest.raises(_lib.RangeError, match="dtype"):
+        c.read(slots, torch.float64)
+    q = randn(1, 2, 4, 64, dtype="f16")
+    table, lengths = torch.zeros((2, 2), dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for args, message in [((q[:, :3], table, lengths), "multiple"), ((q.bfloat16(), table, lengths), "16-bit pages"),
+                          ((q, table.long(), lengths), "table"), ((q, table[:1], lengths), "table"),
+                          ((q, table, lengths.long()), "lengths"), ((q, table, lengths.cpu()), "lengths"),
+                          ((q.cpu(), table, lengths), "device"), ((q, table, lengths, -1.0), "scale"),
+                          ((q, table, lengths, None, q.float()), "out")]:
+        with pytest.raises(_lib.RangeError, match=message):
+            c.attend(*args)
+    st = starts_of([2])
+    k = randn(2, 2, 2, 64, dtype="f16")
+    for args, message in [((q, k, k, st.long()), "starts"), ((q, k.bfloat16(), k, st), "float16"), ((q, k[:1], k[:1], st), "key_starts"),
+                          ((q, k, k, st, starts_of([1, 1])), "starts"), ((q[:, :3], k, k, st), "multiple")]:
+        with pytest.raises(_lib.RangeError, match=message):
+            prompt_attention(*args)
+    # a workspace that is too small, or none
+    need = C.c_size_t()
+    _lib.call("bgtq_prompt_workspace", 0, 64, C.byref(need))
+    room = torch.zeros(need.value + 128, dtype=torch.uint8, device="cuda")
+    for address, size in ((None, need.value), (room.data_ptr(), need.value - 1), (room.data_ptr() + 4, need.value)):
+        p = _lib.PromptDesc(0, _lib.F16, 1, 4, 2, 64, 2, 2, q.data_ptr(), k.data_ptr(), k.data_ptr(), 256, 64, 128, 64, 128, 64,
+                            st.data_ptr(), None, 1, 0.0, torch.empty_like(q).data_ptr(), None, address, size)
+        with pytest.raises(_lib.RangeError, match="workspace"):
+            _lib.call("bgtq_prompt_attend", C.byref(p), None)

@@ -113,6 +113,11 @@ def test_prompt_without_work():
     _lib.call("bgtq_prompt_attend", C.byref(prompt(sequences=0)), None)
 
 
+def test_prompt_workspace_refusals():
+    refused("head dim", "bgtq_prompt_workspace", 0, 80, C.byref(C.c_size_t()))
+    refused("null|invalid|head dim", "bgtq_prompt_workspace", 0, 64, None)
+
+
 def test_python_refusals():
     import torch
     from bgtq import PagedCache, prompt_attention
