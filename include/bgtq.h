@@ -480,7 +480,7 @@ typedef struct bgtq_paged_cache {
  * k[t * k_token_stride + h * k_head_stride + i] (elements of dtype F16, BF16 or F32), v the
  * same.  slots[t] = page * page_size + row; a negative slot is padding and is not stored.
  * Slots of one call are distinct.  A slot past the last page is not stored and sets a bit of
- * the device status word.  A scale is max|x| / 127 (8 bits) or / 7 (4 bits) rounded to BF16,
+ * the device status word.  A scale is max|x| times FP32 1 / 127 (8 bits) or 1 / 7 (4 bits), rounded to BF16,
  * a code is x / scale rounded to the nearest, ties to even; rows (groups) with an infinity
  * or a NaN in them read back as NaN. */
 bgtq_status bgtq_paged_write(const bgtq_paged_cache *c, const void *k, const void *v, bgtq_dtype dtype,
