@@ -3,8 +3,9 @@
 //
 // What bounds it is the one pass over K and V: 2 row_bytes a token and KV head, against 2 D
 // multiply-adds for each query head, so the work is laid out for the memory system.  128 requests
-// of 16K to 32K tokens, 9 / 3 heads of 64 in 8 bits: 345 us, 6.7 TB/s, a little above a plain
-// copy's rate.  Few tokens are bound by latencies instead (the deal, the first pages' way through
+// of 16K to 32K tokens, 9 / 3 heads of 64 in 16 bits: 345 us, 6.7 TB/s, a little above a plain
+// copy's rate; in 8 bits 242 us, 5.0 TB/s, in 4 bits 258 us, 2.5 TB/s, where turning codes into
+// operands costs as many instructions for half the bytes.  Few tokens are bound by latencies instead (the deal, the first pages' way through
 // the table, the join), about 10 us: one request of 4096 tokens 10.3 us, 48 of 1 to 8191, 32 / 8
 // heads of 128, 33 us (3.0 TB/s), eight of 20K to 32K, 14 / 2 heads of 64 in 4 bits, 21 us.
 //   * The (request, KV head, block of query heads) pairs are cut into units of kTokens tokens,
