@@ -4,10 +4,10 @@
 // What bounds it is the one pass over K and V: 2 row_bytes a token and KV head, against 2 D
 // multiply-adds for each query head, so the work is laid out for the memory system.  128 requests
 // of 16K to 32K tokens, 9 / 3 heads of 64 in 16 bits: 345 us, 6.7 TB/s, a little above a plain
-// copy's rate; in 8 bits 242 us, 5.0 TB/s, in 4 bits 258 us, 2.5 TB/s, where turning codes into
+// copy's rate; in 8 bits 225 us, 5.3 TB/s, in 4 bits 248 us, 2.6 TB/s, where turning codes into
 // operands costs as many instructions for half the bytes.  Few tokens are bound by latencies instead (the deal, the first pages' way through
 // the table, the join), about 10 us: one request of 4096 tokens 10.3 us, 48 of 1 to 8191, 32 / 8
-// heads of 128, 33 us (3.0 TB/s), eight of 20K to 32K, 14 / 2 heads of 64 in 4 bits, 21 us.
+// heads of 128, 32 us (3.1 TB/s), eight of 20K to 32K, 14 / 2 heads of 64 in 4 bits, 21 us.
 //   * The (request, KV head, block of query heads) pairs are cut into units of kTokens tokens,
 //     and the units, in order, are dealt to the CTAs in equal ranges, whatever the lengths
 //     are: a range covers the end of one pair, whole pairs, and the start of another.  The
@@ -50,7 +50,9 @@ template <int F, int D, int NT>
 struct Shape {
     static constexpr int kRow = F == F_INT4 ? D / 2 : F == F_INT8 ? D : 2 * D;  // bytes
     static constexpr int kGroups = F == F_INT4 ? D / 32 : F == F_INT8 ? 1 : 0;
-    static constexpr int kTokens = kRow >= 256 ? 16 : kRow >= 128 ? 32 : 64;  // of a unit: 8 KB, or 4 KB
+    // Tokens of a unit: what three stages for each of eight warps of an SM hold, 64 at most.  (128 requests of 16K to 32K
+    // tokens, 9 / 3 heads of 64: in 8 bits 32 tokens 299 us, 64 240; in 4 bits 32 tokens 311 us, 64 253, 128 289.)
+    static constexpr int kTokens = kRow >= 256 ? 16 : kRow >= 128 ? 32 : 64;
     static constexpr int kStages = 3;
     static constexpr int kPart = kTokens * kRow;                 // K or V rows of a unit
     static constexpr int kScale = kTokens * kGroups * 2;         // K or V scales of a unit
@@ -152,6 +154,8 @@ struct Cursor {
 // (None: 48 requests of 1 to 8191 tokens, 32 / 8 heads of 128, 44 us for 33.)
 constexpr uint32_t kItemCost = 10;
 
+// (Two CTAs an SM for their registers; three of 168, with units of 32 tokens, take 269 us for 240 in 8 bits and 296 for
+// 257 in 4, of the requests above.)
 template <int F, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendArgs a) {
     using S = Shape<F, D, NT>;
@@ -340,15 +344,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
             if (bad && lane == 0) atomicOr(a.status, kStatusBadSlot);
             if (lane == 0) flags[warp * 4 + stage] = bad;
             const uint32_t dst = ring_at + stage * S::kStage;
+            const int32_t left = pre.len - (int32_t)t0;
+            // the cache row of this KV head with which the lane's page begins (span > 1: rows are counted from there),
+            // or of the unit's first token; page 0 stands for one that is not there, of which nothing is copied
+            const uint32_t in_page = (1u << shift) - 1;
+            const uint64_t begin = ((uint64_t)((uint32_t)page < a.c.pages ? (uint32_t)page : 0u) * H + kh << shift) + (t0 & in_page);
             constexpr uint32_t CH = S::kRow / 16;
 #pragma unroll
             for (uint32_t i = 0; i < T * CH / 32; ++i) {
                 const uint32_t idx = i * 32 + lane, r = idx / CH, c = idx % CH;
                 const uint32_t pi = r >> shift;
-                const int32_t pg = __shfl_sync(0xffffffffu, page, pi);
-                const bool ok = t0 + r < (uint32_t)pre.len && !(bad >> pi & 1u);
-                const uint64_t at = ((uint64_t)(ok ? (uint32_t)pg : 0u) * H + kh << shift) + ((t0 + r) & ((1u << shift) - 1));
-                const uint64_t off = ok ? at * S::kRow + c * 16 : 0;
+                const bool ok = (int32_t)r < left && !(bad >> pi & 1u);
+                const uint64_t off = (__shfl_sync(0xffffffffu, begin, pi) + (r & in_page)) * S::kRow + c * 16;
                 const uint32_t to = place<S::kRow>(r, c);
                 copy16(dst + to, a.c.k + off, ok ? 16u : 0u);
                 copy16(dst + S::kPart + to, a.c.v + off, ok ? 16u : 0u);
@@ -358,12 +365,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
 #pragma unroll
                 for (uint32_t i = 0; i < (N + 31) / 32; ++i) {
                     const uint32_t idx = i * 32 + lane, r = idx * PER, pi = min(r >> shift, 31u);
-                    const int32_t pg = __shfl_sync(0xffffffffu, page, pi);
-                    const int32_t left = pre.len - (int32_t)(t0 + r);
-                    const bool ok = left > 0 && !(bad >> pi & 1u);
-                    const uint64_t at = ((uint64_t)(ok ? (uint32_t)pg : 0u) * H + kh << shift) + ((t0 + r) & ((1u << shift) - 1));
-                    const uint64_t off = ok ? at * S::kGroups : 0;
-                    const uint32_t bytes = ok ? min(16u, (uint32_t)left * S::kGroups * 2u) : 0u;
+                    const bool ok = (int32_t)r < left && !(bad >> pi & 1u);
+                    const uint64_t off = (__shfl_sync(0xffffffffu, begin, pi) + (r & in_page)) * S::kGroups;
+                    const uint32_t bytes = ok ? min(16u, (uint32_t)(left - (int32_t)r) * S::kGroups * 2u) : 0u;
                     if (N % 32 == 0 || idx < N) {
                         copy16(dst + 2 * S::kPart + idx * 16, a.c.ks + off, bytes);
                         copy16(dst + 2 * S::kPart + S::kScale + idx * 16, a.c.vs + off, bytes);
