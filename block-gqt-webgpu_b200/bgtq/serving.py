@@ -10,6 +10,10 @@ tensors out, ordered on the current stream of the tensors' device; nothing synch
 Indices that only the GPU sees (slots, page tables, lengths, starts) are checked there: what
 lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
 length or starts).
+
+Attention keeps a zeroed workspace for every stream that it has been called on.  A CUDA graph
+recorded on such a stream uses that one, so it is not replayed at the same time as calls there;
+recorded on a stream without one, it has its own.
 """
 from __future__ import annotations
 
@@ -172,8 +176,10 @@ class PagedCache:
         need = C.c_size_t()
         _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
         have = torch.zeros(need.value, dtype=torch.uint8, device=self._on)
-        self._workspace[stream, heads] = have.data_ptr(), need.value, have
-        return self._workspace[stream, heads]
+        work = have.data_ptr(), need.value, have
+        if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
+            self._workspace[stream, heads] = work
+        return work
 
 
 _prompt_work = {}
@@ -184,8 +190,10 @@ def _prompt_workspace(device, dim: int, stream: int):
     need = C.c_size_t()
     _lib.call("bgtq_prompt_workspace", device.index, dim, C.byref(need))
     have = torch.zeros(need.value, dtype=torch.uint8, device=device)
-    _prompt_work[device.index, dim, stream] = have.data_ptr(), need.value, have
-    return _prompt_work[device.index, dim, stream]
+    work = have.data_ptr(), need.value, have
+    if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
+        _prompt_work[device.index, dim, stream] = work
+    return work
 
 
 def _even(t):

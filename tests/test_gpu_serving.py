@@ -708,3 +708,32 @@ def test_python_refusals_on_the_device(cuda):
                             st.data_ptr(), None, 1, 0.0, torch.empty_like(q).data_ptr(), None, address, size)
         with pytest.raises(_lib.RangeError, match="workspace"):
             _lib.call("bgtq_prompt_attend", C.byref(p), None)
+
+
+def test_first_call_of_a_stream_inside_a_recording(cuda):
+    """The graph has a workspace of its own; a call on that stream before any replay has another."""
+    import torch
+    from bgtq import PagedCache, prompt_attention
+    c = PagedCache(2, 64, 300, 16, "int8")
+    n = 4000
+    slots = torch.arange(n, device="cuda")
+    k, v = randn(1, n, 2, 64, dtype="f16"), randn(2, n, 2, 64, dtype="f16")
+    c.write(k, v, slots)
+    table = torch.arange(300, dtype=torch.int32, device="cuda")[None]
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q1, q2 = randn(3, 1, 14, 64, dtype="f16"), randn(4, 16, 14, 64, dtype="f16")
+    st, ks = starts_of([16]), starts_of([n])
+    want = c.attend(q1, table, lengths), prompt_attention(q2, k, v, st, ks)   # in several parts, both
+    out = torch.zeros_like(want[0]), torch.zeros_like(want[1])
+    torch.cuda.synchronize()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.attend(q1, table, lengths, out=out[0])
+        prompt_attention(q2, k, v, st, ks, out=out[1])
+    with torch.cuda.stream(side):
+        got = c.attend(q1, table, lengths), prompt_attention(q2, k, v, st, ks)
+        for _ in range(3):
+            g.replay()
+    torch.cuda.synchronize()
+    for a, b, w in zip(got, out, want):
+        assert torch.equal(a, w) and torch.equal(b, w)
