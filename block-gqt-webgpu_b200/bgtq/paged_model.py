@@ -19,6 +19,9 @@ from .model import ModelGeometry
 from .serving import PagedCache, prompt_attention, _refuse
 
 
+_RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width
+
+
 class PagedDecoder:
     """pages: pages of page_size tokens that all requests share (one pool a layer, one table
     for all).  format: "f16" / "bf16" (dtype's own), "int8" or "int4" pages.  dtype: float16 or
@@ -55,6 +58,7 @@ class PagedDecoder:
         self._free = list(range(pages))[::-1]
         self._held = {}        # request: [its pages in order, its tokens]
         self._next = 0
+        self._steps, self._side = {}, torch.cuda.Stream(self.dev)
 
     # ---- requests and pages ----
     def open(self) -> int:
@@ -138,24 +142,47 @@ class PagedDecoder:
         return self._forward(self._to(flat, torch.int64), positions, attention, self._to(ends - 1, torch.int64))
 
     def step(self, requests, tokens):
-        """One token of each request: logits [requests, vocab] (FP32)."""
+        """One token of each request: logits [requests, vocab] (FP32).  Replays a CUDA graph,
+        recorded at the first step of so many requests and pages (up to a power of two)."""
         tokens = np.asarray(tokens.cpu() if torch.is_tensor(tokens) else tokens, np.int64).reshape(-1)
         if len(tokens) != len(requests):
             _refuse("Paged decoder: one token for every request")
-        flat = self._vocabulary(tokens)
+        self._vocabulary(tokens)
         held, before = self._grow(requests, [1] * len(tokens))
-        slots = self._to([h[0][b // self.page_size] * self.page_size + b % self.page_size
-                          for h, b in zip(held, before)], torch.int64)
-        table = np.zeros((len(held), max(len(h[0]) for h in held)), np.int32)
+        width = 1 << max(4, (max(len(h[0]) for h in held) - 1).bit_length())
+        table = np.zeros((len(held), width), np.int32)
         for row, h in zip(table, held):
             row[:len(h[0])] = h[0]
-        table, lengths = self._to(table, torch.int32), self._to([h[1] for h in held], torch.int32)
+        slots = [h[0][b // self.page_size] * self.page_size + b % self.page_size for h, b in zip(held, before)]
+        graph, inputs, logits = self._steps.get((len(held), width)) or self._record(len(held), width)
+        for buffer, values in zip(inputs, (tokens, before, slots, table, [h[1] for h in held])):
+            buffer.copy_(torch.as_tensor(np.asarray(values), dtype=buffer.dtype))
+        graph.replay()
+        return logits.clone()
+
+    def _record(self, batch: int, width: int):
+        """A step of batch requests over tables of width pages: graph, inputs, logits."""
+        tokens, positions, slots, table, lengths = inputs = (
+            self._to(np.zeros(batch), torch.int64), self._to(np.zeros(batch), torch.float32),
+            self._to(np.full(batch, -1), torch.int64), self._to(np.zeros((batch, width)), torch.int32),
+            self._to(np.zeros(batch), torch.int32))
 
         def attention(cache, q, k, v):
             cache.write(k, v, slots)
             return cache.attend(q.to(self.dtype), table, lengths)
 
-        return self._forward(self._to(flat, torch.int64), self._to(before, torch.float32), attention, None)
+        # once beside the recording, for what is set up at first calls: no row is written, none is read
+        self._side.wait_stream(torch.cuda.current_stream(self.dev))
+        with torch.cuda.stream(self._side):
+            self._forward(tokens, positions, attention, None)
+        torch.cuda.current_stream(self.dev).wait_stream(self._side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=self._side):
+            logits = self._forward(tokens, positions, attention, None)
+        if len(self._steps) == _RECORDED:
+            del self._steps[next(iter(self._steps))]
+        self._steps[batch, width] = graph, inputs, logits
+        return self._steps[batch, width]
 
     def generate(self, prompts, count: int):
         """Greedy: count tokens after each of prompts (sequences of tokens), as an int64 array

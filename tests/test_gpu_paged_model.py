@@ -218,3 +218,31 @@ def test_refusals_change_nothing(cuda):
     dec.step([r], [1])
     dec.close(r)
     assert dec.free_pages == 2
+
+
+def test_steps_of_changing_batches_and_widths(cuda):
+    """Recorded steps of other batches and table widths, more of them than are kept, on another stream
+    too, follow the requests."""
+    import torch
+    from bgtq import PagedDecoder, paged_model
+    g = SMALL["llama"]
+    w = weights_of(g, "f16")
+    dec = PagedDecoder(w, g, pages=64, page_size=16, format="int8", dtype=types()["f16"])
+    rng = np.random.default_rng(2)
+    held = [dec.open() for _ in range(18)]
+    plain = {r: Plain(w, dec, r, BOUND["f16"]) for r in held}
+    lengths = [250] + [3 + i for i in range(17)]     # the first grows past 16 pages, to tables of 32
+    tokens = [rng.integers(0, g.vocab, n) for n in lengths]
+    for row, r, t in zip(dec.prompt(held, tokens), held, tokens):
+        assert off(row, plain[r].forward(t, False)) < BOUND["f16"], r
+    side = torch.cuda.Stream()
+    for batch in [*range(1, 19), 1, 2, 1]:
+        some = held[:batch]
+        t = rng.integers(0, g.vocab, batch)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if batch % 2 else torch.cuda.current_stream()):
+            got = dec.step(some, t)
+        torch.cuda.synchronize()
+        for row, r, x in zip(got, some, t):
+            assert off(row, plain[r].forward([x], True)) < BOUND["f16"], (batch, r)
+    assert len(dec._steps) <= paged_model._RECORDED
