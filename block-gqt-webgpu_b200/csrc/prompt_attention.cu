@@ -170,13 +170,14 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one of t
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
     return r;
 }
-// 2^y of two values on the FMA pipe, y below 2^20 (from -126 down: about 2^-126, NaN: NaN): adding 1.5 * 2^23
-// rounds y to a whole number n in the low mantissa bits, and 2^f of the rest, -1/2 <= f <= 1/2, is
-// the polynomial of degree 4 with the least largest relative error on that interval (Remez
-// exchange): 2.7e-6 in FP32, 4e-8 on average.
+// 2^y of two values on the FMA pipe, y below 2^20: adding 1.5 * 2^23 rounds y to a whole number n in the low
+// mantissa bits, and 2^f of the rest, -1/2 <= f <= 1/2, is the polynomial of degree 4 with the least
+// largest relative error on that interval (Remez exchange): 2.7e-6 in FP32, 4e-8 on average.  From
+// -126.5 down, -infinity with it, it is zero: -127 is the n whose 2^n has the bits of zero, and in
+// BF16 any floor above that is a weight that a large value shows.  NaN: NaN.
 __device__ __forceinline__ float2 ex2_fma(float2 y) {
     constexpr float kRound = 12582912.0f;
-    y = make_float2(max_nan(y.x, -126.0f), max_nan(y.y, -126.0f));
+    y = make_float2(max_nan(y.x, -127.0f), max_nan(y.y, -127.0f));
     const float2 t = __fadd2_rn(y, make_float2(kRound, kRound));
     const float2 f = __ffma2_rn(__fadd2_rn(t, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), y);
     float2 p = __ffma2_rn(f, make_float2(0.0095701022f, 0.0095701022f), make_float2(0.055917859f, 0.055917859f));
@@ -524,7 +525,8 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     }
                 }
                 const bool none = sees == 0;
-                const float inv = none ? 0.0f : 1.0f / sum;
+                const float ref0 = ref == -INFINITY ? 0.0f : ref;
+                const float inv = none || sum == 0.0f ? 0.0f : 1.0f / sum;  // (0: every logit is -infinity)
                 // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
                 constexpr int kW = P::kTurn, kL = kW / 8;
                 unsigned char *turn = sm + P::kOut + warp * 64 * kW;
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                             }
 #pragma unroll
                             for (int b = 0; b < kJoin; ++b) {
-                                const float e = ex2(f[b] - ref);  // 0 for a part of no K tile that this row sees
+                                const float e = ex2(f[b] - ref0);  // 0 for a part of no K tile that this row sees
 #pragma unroll
                                 for (int i = 0; i < kW; ++i) o[i] = __float_as_uint(fmaf(e, x[b][i], __uint_as_float(o[i])));
                             }
