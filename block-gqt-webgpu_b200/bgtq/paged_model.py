@@ -11,6 +11,8 @@ its request's pages (`PagedCache.attend`).  Geometry, weights, RoPE and norms ar
 """
 from __future__ import annotations
 
+import contextlib
+
 import numpy as np
 import torch
 import torch.nn.functional as F
@@ -85,19 +87,29 @@ class PagedDecoder:
             _refuse("Paged decoder: no such request")
         return self._held[request]
 
-    def _grow(self, requests, counts):
-        """Pages for counts[i] more tokens of requests[i]: all of them, or a refusal that changes nothing."""
+    @contextlib.contextmanager
+    def _grown(self, requests, counts):
+        """Pages for counts[i] more tokens of requests[i], all of them or a refusal: what each holds now and
+        its length before.  A body that fails has written no rows to count on, so it leaves lengths and
+        pages as they were."""
         if not requests or len(set(requests)) < len(requests):
             _refuse("Paged decoder: requests must be one or more, each once")
         held = [self._request(r) for r in requests]
         need = [-(-(h[1] + n) // self.page_size) - len(h[0]) for h, n in zip(held, counts)]
         if sum(need) > len(self._free):
             _refuse(f"Paged decoder: {sum(need)} pages wanted, {len(self._free)} free")
-        starts = [h[1] for h in held]
+        before = [h[1] for h in held]
         for h, n, more in zip(held, counts, need):
             h[0] += [self._free.pop() for _ in range(more)]
             h[1] += n
-        return held, starts
+        try:
+            yield held, before
+        except BaseException:
+            for h, start, more in reversed(list(zip(held, before, need))):
+                self._free += h[0][len(h[0]) - more:][::-1]
+                del h[0][len(h[0]) - more:]
+                h[1] = start
+            raise
 
     def _slots(self, pages, first: int, upto: int):
         t = np.arange(first, upto)
@@ -115,7 +127,10 @@ class PagedDecoder:
             _refuse("Paged decoder: one or more tokens for every request")
         flat = self._vocabulary(np.concatenate(tokens)) if tokens else None
         counts = [len(t) for t in tokens]
-        held, before = self._grow(requests, counts)
+        with self._grown(requests, counts) as (held, before):
+            return self._prompt(flat, counts, held, before)
+
+    def _prompt(self, flat, counts, held, before):
         ends = np.cumsum(counts)
         slots = self._to(np.concatenate([self._slots(h[0], b, h[1]) for h, b in zip(held, before)]), torch.int64)
         positions = self._to(np.concatenate([np.arange(b, h[1]) for h, b in zip(held, before)]), torch.float32)
@@ -148,7 +163,10 @@ class PagedDecoder:
         if len(tokens) != len(requests):
             _refuse("Paged decoder: one token for every request")
         self._vocabulary(tokens)
-        held, before = self._grow(requests, [1] * len(tokens))
+        with self._grown(requests, [1] * len(tokens)) as (held, before):
+            return self._step(tokens, held, before)
+
+    def _step(self, tokens, held, before):
         width = 1 << max(4, (max(len(h[0]) for h in held) - 1).bit_length())
         table = np.zeros((len(held), width), np.int32)
         for row, h in zip(table, held):
