@@ -36,8 +36,9 @@
 // joining) are short loops on purpose: unrolled, their instruction fetches cost 10 us a call.
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time: until then probabilities are taken relative to the older maximum, so they stay
-// below 2^8, and P is FP16 or BF16 (the inputs' type) with the same relative error: their rounding
-// is the formula's one beside the outputs' own, and sums take them before it.  (Rescaling at every
+// below 2^8.  P is FP16 or BF16, the inputs' type, and its rounding is the formula's one beside the outputs'
+// own; sums take probabilities before it.  In FP16 they are multiplied by 2^7, and the sums with them:
+// what is above 2^-21 of a row's largest keeps 11 bits, what is below is held to 2^-32 of it.  (Rescaling at every
 // growth: three prompts of 300 to 512 tokens after 3500, 32 / 8 heads of 128, 120 us for 83.)
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -65,6 +66,9 @@ constexpr int32_t kWhole = 1024;
 constexpr int64_t kPiece = 512;
 constexpr int kJoin = 2;                 // parts of an item that are joined at a time (1: 2 % slower, 4: 5 %)
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
+// log2 of what probabilities are multiplied by: with kLazy, what FP16 holds.  (Less growth and more of this, in FP16:
+// 2^4 and 2^11 take 3 % more for three prompts of 300 to 512 tokens after 3500, 8 % for four of 3500 to 4096.)
+template <bool BF> constexpr float kUp = BF ? 0.0f : 15.0f - kLazy;
 
 // ---- device helpers -----------------------------------------------------------------------
 
@@ -426,7 +430,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                         tm_store16(to + 16 * c, o);
                     }
                 }
-                const float from = ref == -INFINITY ? 0.0f : ref;
+                const float from = (ref == -INFINITY ? 0.0f : ref) - kUp<BF>;
                 const float2 scale2 = make_float2(a.scale, a.scale), from2 = make_float2(-from, -from);
                 float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                     }
                     __syncwarp();
                 }
-                if (live && a.lse) a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref + __log2f(sum)) * kLn2;
+                if (live && a.lse) a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - kUp<BF> + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;

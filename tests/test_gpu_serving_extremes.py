@@ -10,7 +10,7 @@ import math
 import pytest
 
 from bgtq import device_status
-from test_gpu_serving import randn, starts_of, types
+from test_gpu_serving import U, attention64, randn, starts_of, types
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,39 @@ def test_prompt_rows_whose_logits_are_all_minus_infinity(cuda, dtype, dim, nq, n
     assert torch.equal(out[:, 0], want[:, 0]) and torch.equal(lse[:, 0], want_lse[:, 0])
     assert not out[:, 1].any() and bool((lse[:, 1] == -math.inf).all())
     assert device_status(0) == 0
+
+
+# What FP16 holds of a probability at least: half its last place, 2^-25, over what it is multiplied by
+LEAST = {"prompt": 2.0 ** -25 / 2 ** 7, "token": 2.0 ** -25 / 2 ** 12}
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind", ["prompt", "token"])
+@pytest.mark.parametrize("n", [900, 8193])                 # prompts: an item as a whole, and one in parts
+@pytest.mark.parametrize("gap", [14.0, 16.8, 17.4, 18.5])  # nats: 2^-20 to 2^-27
+def test_many_small_probabilities_beside_a_large_one(cuda, kind, dim, n, gap):
+    """One key has nearly all of the weight and a value of zero; what the others, each of them small,
+    add up to is the answer.  Tolerance: the roundings of an output and its probabilities, 3e-5 of them
+    for FP32, and what FP16 drops of a small probability."""
+    import torch
+    from bgtq import PagedCache, prompt_attention
+    q = torch.zeros((1, 2, dim), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    k = torch.zeros((n, 1, dim), dtype=torch.float16, device="cuda")
+    k[5, 0, 0] = gap
+    k[:, 0, 1:] = 0.0
+    v = (64 + 16 * randn(3, n, 1, dim)).half()     # outputs above 2^-14, where FP16 rounds by 2^-11
+    v[5] = 0
+    if kind == "prompt":
+        out, lse = prompt_attention(q, k, v, starts_of([1]), starts_of([n]), scale=1.0, lse=True)
+    else:
+        pages = (n + 15) // 16
+        cache = PagedCache(1, dim, pages, 16, "f16")
+        cache.write(k, v, torch.arange(n, device="cuda"))
+        out, lse = cache.attend(q, torch.arange(pages, dtype=torch.int32, device="cuda")[None],
+                                torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0, lse=True)
+    for h in range(2):
+        want, want_lse, mag, small = attention64(q[:, h], k[:, 0], v[:, 0], torch.ones((1, n), dtype=torch.bool, device="cuda"), 1.0)
+        tol = U["f16"] * want.abs() + (U["f16"] + 3e-5) * mag + LEAST[kind] * small
+        assert bool(((out[:, h].double() - want).abs() <= tol).all()), float(((out[:, h].double() - want).abs() / tol).max())
+        assert float((lse[:, h].double() - want_lse).abs().max()) <= 3e-5
