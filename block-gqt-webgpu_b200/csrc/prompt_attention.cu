@@ -23,7 +23,9 @@
 //   ends        one warp: V tiles at a sequence's end or on the diagonal, before they are
 //               multiplied: rows past the end (another sequence's, or nothing) are zeroed, and an
 //               infinity or a NaN, which the zero probability of a row that does not see it would
-//               turn into a NaN, is taken out and given to the rows that do see it
+//               turn into a NaN, is taken out and added to the rows that do see it.  (In
+//               a tile that every row sees an infinity is multiplied like any value: by zero, which
+//               makes a NaN, where its probability is below what P's type holds)
 //
 // What bounds it.  A K tile of 64 keys costs a row tile 512 (head dim 128) or 256 clocks of
 // tensor arithmetic; the logits' products, which read both operands from shared memory, take 48
@@ -461,7 +463,8 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 if (!fine) break;
                 tc_after();
                 const uint32_t flagged = bad_flag[n % kDeal];
-                // infinities and NaN among the values of the kW dimensions from d0 on that this row sees
+                // infinities and NaN among the values of the dimensions from d0 on that this row sees, added to
+                // what the other keys came to, which may be an infinity or a NaN of their own
                 auto overlay = [&](uint32_t *o, int d0, auto width) {
                     // keys from `key0` on were looked through
                     const int32_t key0 = max(0, span(it, 0).first / kKeys) * kKeys;
@@ -469,8 +472,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
 #pragma unroll
                     for (int i = 0; i < decltype(width)::value; ++i) {
                         const bool up = key0 + first[i] < sees, down = key0 + first[D + i] < sees;
-                        if (key0 + first[2 * D + i] < sees || (up && down)) o[i] = 0x7fc00000u;
-                        else if (up || down) o[i] = up ? 0x7f800000u : 0xff800000u;
+                        const bool nan = key0 + first[2 * D + i] < sees;
+                        const float x = nan || up == down ? __uint_as_float(0x7fc00000u) : up ? INFINITY : -INFINITY;
+                        if (nan || up || down) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
                     }
                 };
                 // Parts of an item go to the workspace, [warp][dimension, maximum, sum][lane], and the warp that

@@ -101,3 +101,25 @@ def test_many_small_probabilities_beside_a_large_one(cuda, kind, dim, n, gap):
         tol = U["f16"] * want.abs() + (U["f16"] + 3e-5) * mag + LEAST[kind] * small
         assert bool(((out[:, h].double() - want).abs() <= tol).all()), float(((out[:, h].double() - want).abs() / tol).max())
         assert float((lse[:, h].double() - want_lse).abs().max()) <= 3e-5
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nq,nk", [(300, 300), (40, 4000)])    # items as a whole, and one in parts
+@pytest.mark.parametrize("early,late,both", [(math.nan, math.inf, math.nan), (-math.inf, math.inf, math.nan),
+                                             (math.inf, -math.inf, math.nan), (math.inf, math.inf, math.inf)])
+def test_prompt_infinities_and_nan_of_far_and_near_keys_add_up(cuda, dtype, dim, nq, nk, early, late, both):
+    """One value is in a tile that every row sees, one where only the later rows see it."""
+    import torch
+    from bgtq import prompt_attention
+    q, k, v = (randn(s, n, 2, dim, dtype=dtype) for s, n in ((1, nq), (2, nk), (3, nk)))
+    st, ks = starts_of([nq]), starts_of([nk])
+    want = prompt_attention(q, k, v, st, ks)
+    v[3, :, 5], v[nk - 10, :, 5] = early, late
+    out = prompt_attention(q, k, v, st, ks)
+    rest = [i for i in range(dim) if i != 5]
+    assert torch.equal(out[..., rest], want[..., rest])
+    row = torch.arange(nq, device="cuda") + nk - nq          # the last key that each row sees
+    expect = torch.where(row >= nk - 10, both, torch.where(row >= 3, early, 0.0))[:, None].expand(nq, 2)
+    got = torch.where(row[:, None] >= 3, out[..., 5].float(), 0.0)
+    assert torch.equal(got.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), expect.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
