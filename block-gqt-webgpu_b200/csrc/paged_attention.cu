@@ -29,10 +29,14 @@
 //     BF16 pages, BF16.
 //   * 8-bit pages: a key's scale multiplies its logit, a value's scale its probability before
 //     the rounding.  4-bit pages: the logit is the sum of scale x partial product over groups
-//     of 32 dimensions; the values are multiplied in registers (code x scale has 11 bits, so
-//     FP16 holds it exactly).  Value scales are taken relative to a running power of two of
-//     the largest seen, and queries to one of their row's largest, so that FP16's exponent
-//     range holds any BF16 scale or query that matters beside the largest.
+//     of 32 dimensions; the values are multiplied in registers by their scales over their
+//     token's power of two (code x scale has 11 bits, so FP16 holds it exactly), and that
+//     power multiplies the probability.  FP16's exponent range does not hold such products
+//     of any scale: they are taken relative to the largest of each head, so that a value of
+//     any size whose weight is next to nothing leaves the others as they are.  What is
+//     rounded away is 2^-35 of the largest.  Queries are taken relative to a power of two
+//     of their row's largest; FP16 drops 2^-38 of it.  (128 requests of 16K to 32K
+//     tokens, 9 / 3 heads of 64 in 8 bits, 230 us for 225 with one power for all heads.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -44,7 +48,10 @@ namespace {
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWarps = 4, kThreads = 32 * kWarps;
 enum { F_F16, F_BF16, F_INT8, F_INT4 };
-constexpr int kLeastExp = -100;  // value scales below 2^-100 count as that in the running power of two
+// Over 8- and 4-bit pages (powers of two, as logarithms): value scales below kLeast count as that; how far a unit's largest
+// contribution may pass the largest before it, 10 + kRoom + 1 being what FP16 holds; how far apart the heads of a
+// KV head may be in contribution over probability.
+constexpr float kLeast = -100.0f, kRoom = 4.0f, kApart = 100.0f;
 
 template <int F, int D, int NT>
 struct Shape {
@@ -121,6 +128,11 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float least(float x) {  // of x and 2^127, NaN if x is
+    float y;
+    asm("min.NaN.f32 %0, %1, 0f7F000000;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float from_bf16(uint32_t bits) { return __uint_as_float(bits << 16); }
@@ -479,15 +491,21 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
         float m[NT][2], l[NT][2] = {};
 #pragma unroll
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
-        int vexp = kLeastExp;  // 2^vexp: the running power of two of the value scales
+        // Over 8- and 4-bit pages exponentials and sums are taken relative to 2^ref, outputs to 2^(ref + common); that is
+        // each head's largest contribution (exp(logit) x value scale) up to the last unit that passed it by kRoom.
+        float ref[NT][2], peak[NT][2], common = kLeast;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ref[n][h] = F >= F_INT8 ? -3.4e38f : 0.0f, peak[n][h] = -INFINITY;
 
         for (uint32_t unit = unit0(cur); unit < cur.end; unit += step_of(cur)) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
             __syncwarp();
             const unsigned char *buf = ring + stage * S::kStage;
             const uint32_t buf_at = ring_at + stage * S::kStage;
-            const uint16_t *ksc = reinterpret_cast<const uint16_t *>(buf + 2 * S::kPart);
-            const uint16_t *vsc = ksc + S::kScale / 2;
+            uint16_t *ksc = reinterpret_cast<uint16_t *>(ring + stage * S::kStage + 2 * S::kPart);
+            uint16_t *vsc = ksc + S::kScale / 2;
             const uint32_t bad = flags[warp * 4 + stage];
             const int32_t left = cur.len - (int32_t)(unit * T);  // tokens of the unit that exist
             // ---- S^T = K Q^T ----
@@ -573,8 +591,47 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                             top[n][h] = fmaxf(top[n][h], x);
                         }
                 }
+            // ---- value scales: the exponent of the unit's largest; in 4 bits, of each token's largest ----
+            float *tok = reinterpret_cast<float *>(ksc);  // 4 bits: powers of two of the tokens
+            float e_unit = kLeast;
+            if constexpr (F == F_INT8) {
+                uint32_t big = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < (T + 31) / 32; ++i) {
+                    const uint32_t x = T % 32 == 0 || lane < T ? vsc[i * 32 + lane] : 0;
+                    big = max(big, x < 0x7f80u ? x : 0u);
+                }
+                e_unit = (float)((int)(__reduce_max_sync(0xffffffffu, big) >> 7) - 127);
+            }
+            if constexpr (F == F_INT4) {
+                // a token's scales become FP16 over its power of two (times 2^10: code x scale has 11 bits, so FP16 holds
+                // it exactly, of any scale down to 2^-24 of the token's largest), which goes to its probability
+                static_assert(T % 32 == 0 && T * 4 <= S::kScale, "the powers lie where the key scales were");
+                constexpr int W = S::kGroups / 2;
+                __syncwarp();
+                uint32_t all = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < T / 32; ++i) {
+                    uint32_t *at = reinterpret_cast<uint32_t *>(vsc) + (i * 32 + lane) * W, w[W], big = 0;
+#pragma unroll
+                    for (int k = 0; k < W; ++k) {
+                        w[k] = at[k];
+                        const uint32_t a0 = w[k] & 0xffffu, a1 = w[k] >> 16;
+                        big = max(big, max(a0 < 0x7f80u ? a0 : 0u, a1 < 0x7f80u ? a1 : 0u));
+                    }
+                    const uint32_t e = max(big >> 7, (uint32_t)(127 + (int)kLeast));
+                    const float f = __uint_as_float((264 - e) << 23);  // 2^(10 - exponent)
+#pragma unroll
+                    for (int k = 0; k < W; ++k) at[k] = pack<false>(from_bf16(w[k] & 0xffffu) * f, from_bf16(w[k] >> 16) * f);
+                    tok[i * 32 + lane] = __uint_as_float(e << 23);
+                    all = max(all, e);
+                }
+                e_unit = (float)((int)__reduce_max_sync(0xffffffffu, all) - 127);
+                __syncwarp();
+            }
             bool moved = false;
-            float alpha[NT][2];
+            float alpha[NT][2], beta[NT][2];  // 2^alpha: what sums are multiplied by, 2^beta: outputs
+            const float above = fmaxf(e_unit, common - (kApart + 5.0f)) - kRoom - common;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -584,64 +641,80 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     const float now = fmaxf(m[n][h], x);
-                    moved |= now > m[n][h];
-                    alpha[n][h] = now == -INFINITY ? 1.0f : ex2(m[n][h] - now);
+                    if constexpr (F >= F_INT8) moved |= x + above > ref[n][h];
+                    else {
+                        moved |= now > m[n][h];
+                        alpha[n][h] = beta[n][h] = now == -INFINITY ? 0.0f : m[n][h] - now;
+                        ref[n][h] = now == -INFINITY ? 0.0f : now;
+                    }
                     m[n][h] = now;
                 }
-            // ---- value scales: the running power of two ----
-            float vmul = 4096.0f;  // of a probability (FP16 and 8-bit pages) or a value scale (4 bits)
-            if constexpr (F >= F_INT8) {
-                uint32_t big = 0;
+            if (__any_sync(0xffffffffu, moved)) {
+                if constexpr (F >= F_INT8) {
+                    // the largest contributions, by every token's logit and exponent
 #pragma unroll
-                for (uint32_t i = 0; i < (T * S::kGroups + 31) / 32; ++i) {
-                    const uint32_t x = T * S::kGroups % 32 == 0 || lane < T * S::kGroups ? vsc[i * 32 + lane] : 0;
-                    big = max(big, x < 0x7f80u ? x : 0u);
-                }
-                big = __reduce_max_sync(0xffffffffu, big);
-                const int e = min((int)(big >> 7) - 127, 126);
-                if (e > vexp) {
-                    const float f = __uint_as_float((uint32_t)max(vexp - e + 127, 0) << 23);
+                    for (int c = 0; c < C16; ++c)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t t = 16 * c + row4 + 8 * k;
+                            uint32_t b;
+                            if constexpr (F == F_INT8) b = vsc[t] < 0x7f80u ? vsc[t] >> 7 : 0u;
+                            else b = __float_as_uint(tok[t]) >> 23;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) peak[n][h] = fmaxf(peak[n][h], s[c][n][2 * k + h] + fmaxf((float)((int)b - 127), kLeast));
+                        }
+                    const float before = common;
+                    common = kLeast;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < KS; ++i)
+                        for (int h = 0; h < 2; ++h) {
+                            peak[n][h] = fmaxf(peak[n][h], __shfl_xor_sync(0xffffffffu, peak[n][h], 4));
+                            peak[n][h] = fmaxf(peak[n][h], __shfl_xor_sync(0xffffffffu, peak[n][h], 8));
+                            peak[n][h] = fmaxf(peak[n][h], __shfl_xor_sync(0xffffffffu, peak[n][h], 16));
+                            // (no token yet: NaN, passed over; a column without a head has equal weights for all tokens)
+                            if (n * 8 + 2 * col4 + h < heads) common = fmaxf(common, ceilf(peak[n][h] - m[n][h]));
+                        }
+                    common = fmaxf(common, __shfl_xor_sync(0xffffffffu, common, 1));
+                    common = fmaxf(common, __shfl_xor_sync(0xffffffffu, common, 2));
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) o[i][n][k] *= f;
-                    vexp = e;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float now = fmaxf(fmaxf(peak[n][h] - common, m[n][h] - kApart), -3.4e38f);
+                            alpha[n][h] = ref[n][h] - now;
+                            beta[n][h] = alpha[n][h] + (before - common);
+                            ref[n][h] = now;
+                        }
                 }
-                vmul = __uint_as_float((uint32_t)(127 - vexp) << 23);  // 2^-vexp
-                vmul *= F == F_INT8 ? 4096.0f : 128.0f;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    l[n][0] *= alpha[n][0];
-                    l[n][1] *= alpha[n][1];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        o[i][n][0] *= alpha[n][0];
-                        o[i][n][1] *= alpha[n][1];
-                        o[i][n][2] *= alpha[n][0];
-                        o[i][n][3] *= alpha[n][1];
+                    for (int h = 0; h < 2; ++h) {
+                        const float f = ex2(alpha[n][h]), g = F >= F_INT8 ? ex2(beta[n][h]) : f;
+                        l[n][h] *= f;
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) {
+                            o[i][n][h] *= g;
+                            o[i][n][2 + h] *= g;
+                        }
                     }
-                }
             }
+            const float vmul = F == F_BF16 ? 1.0f : F == F_F16 ? 4096.0f : __uint_as_float((uint32_t)(137 - (int)common) << 23);
             // ---- probabilities, O^T += V^T P^T ----
 #pragma unroll
             for (int c = 0; c < C16; ++c) {
                 uint32_t p[NT][2];
                 float w0 = vmul, w1 = vmul;
-                if constexpr (F == F_BF16) w0 = w1 = 1.0f;
-                if constexpr (F == F_INT4) w0 = w1 = 4096.0f;
-                if constexpr (F == F_INT8) {
-                    w0 = from_bf16(vsc[16 * c + row4]) * vmul;
-                    w1 = from_bf16(vsc[16 * c + row4 + 8]) * vmul;
-                }
+                // (at most 2^127: what a token of more weighs is below 2^-111, and zero times infinity is not zero)
+                if constexpr (F == F_INT8) w0 = least(from_bf16(vsc[16 * c + row4]) * vmul), w1 = least(from_bf16(vsc[16 * c + row4 + 8]) * vmul);
+                if constexpr (F == F_INT4) w0 = least(tok[16 * c + row4] * vmul), w1 = least(tok[16 * c + row4 + 8] * vmul);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float r0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], r1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
-                    const float e0 = ex2(s[c][n][0] - r0), e1 = ex2(s[c][n][1] - r1);
-                    const float e2 = ex2(s[c][n][2] - r0), e3 = ex2(s[c][n][3] - r1);
+                    const float e0 = ex2(s[c][n][0] - ref[n][0]), e1 = ex2(s[c][n][1] - ref[n][1]);
+                    const float e2 = ex2(s[c][n][2] - ref[n][0]), e3 = ex2(s[c][n][3] - ref[n][1]);
                     l[n][0] += e0 + e2;
                     l[n][1] += e1 + e3;
                     p[n][0] = turn(pack<BF>(e0 * w0, e1 * w0));
@@ -689,11 +762,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                     } else {
                         // D / 8 dimensions lie in one group: scales of the four tokens as two FP16 pairs
                         const uint32_t g = row4 * (D / 8) / 32, t = 16 * c + 2 * col4;
-                        const float f0 = from_bf16(vsc[t * S::kGroups + g]) * vmul;
-                        const float f1 = from_bf16(vsc[(t + 1) * S::kGroups + g]) * vmul;
-                        const float f2 = from_bf16(vsc[(t + 8) * S::kGroups + g]) * vmul;
-                        const float f3 = from_bf16(vsc[(t + 9) * S::kGroups + g]) * vmul;
-                        const uint32_t sa = pack<false>(f0, f1), sb = pack<false>(f2, f3);
+                        const uint32_t sa = vsc[t * S::kGroups + g] | (uint32_t)vsc[(t + 1) * S::kGroups + g] << 16;
+                        const uint32_t sb = vsc[(t + 8) * S::kGroups + g] | (uint32_t)vsc[(t + 9) * S::kGroups + g] << 16;
 #pragma unroll
                         for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -722,15 +792,19 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
         // ---- the warp's part, in the ring slot that it read last (the next fill comes after a unit more) ----
         float *mine_o = reinterpret_cast<float *>(ring + (stage == 0 ? S::kStages - 1 : stage - 1) * S::kStage);
         {
-            float unit_out = 1.0f;
-            if constexpr (F != F_BF16) unit_out = 1.0f / 4096.0f;
-            if constexpr (F == F_INT4) unit_out *= 1.0f / 128.0f;
-            if constexpr (F >= F_INT8) unit_out *= __uint_as_float((uint32_t)(vexp + 127) << 23);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float x = l[n][h];
+                    float unit_out = 1.0f, x = l[n][h];
+                    if constexpr (F == F_F16) unit_out = 1.0f / 4096.0f;
+                    if constexpr (F >= F_INT8) unit_out = 1.0f / 1024.0f;
+                    if constexpr (F == F_INT4) unit_out *= 1.0f / 1024.0f;
+                    if constexpr (F >= F_INT8) {  // relative to the maximum, like the other formats'
+                        const float past = m[n][h] == -INFINITY ? 0.0f : ref[n][h] - m[n][h];
+                        x *= ex2(past);
+                        unit_out *= ex2(past + common);
+                    }
                     x += __shfl_xor_sync(0xffffffffu, x, 4);
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);

@@ -123,3 +123,91 @@ def test_prompt_infinities_and_nan_of_far_and_near_keys_add_up(cuda, dtype, dim,
     expect = torch.where(row >= nk - 10, both, torch.where(row >= 3, early, 0.0))[:, None].expand(nq, 2)
     got = torch.where(row[:, None] >= 3, out[..., 5].float(), 0.0)
     assert torch.equal(got.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), expect.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+
+
+def pages_of(k, v, fmt):
+    """A cache that holds rows k, v [tokens, heads, dim], its table, and the rows as they stand there."""
+    import torch
+    from bgtq import PagedCache
+    n = k.shape[0]
+    pages = (n + 15) // 16
+    cache = PagedCache(k.shape[1], k.shape[2], pages, 16, fmt)
+    slots = torch.arange(n, device="cuda")
+    cache.write(k, v, slots)
+    table, length = torch.arange(pages, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+    return cache, table, length, cache.read(slots, torch.float32)
+
+
+def check_quantised(cache, q, table, length, rows, dtype, scale):
+    """Tolerance: the roundings of an output and of its probabilities, 3e-5 of them for FP32, and for every
+    token FP16's half of a last place, 2^-25 / 2^10 of the head's largest contribution.  A contribution is a
+    probability x a scale in 8 bits, whose codes are up to the row's largest / scale; in 4 bits a probability x a
+    power of two of at least half the token's largest scale, with codes x scales up to 16 of it: with the row's
+    largest, 7 scales or more, that is 2^-35 and 16 x 2^-35 / 7 of probability x row at most, 2^-33 for both."""
+    import torch
+    out, lse = cache.attend(q, table, length, scale=scale, lse=True)
+    k, v = (x[:, 0].double() for x in rows)
+    s = (q[0].double() @ k.T) * scale
+    p = torch.softmax(s, -1)
+    want = p @ v
+    least = k.shape[0] * 2.0 ** -33 * (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+    tol = U[dtype] * want.abs() + (U[dtype] + 3e-5) * (p @ v.abs()) + least
+    off = (out[0].double() - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+    assert float((lse[0].double() - torch.logsumexp(s, -1)).abs().max()) <= 3e-5 * max(1.0, float(s.abs().max()) / 64)
+    return out
+
+
+@pytest.mark.parametrize("fmt,dtype", [("int8", "f16"), ("int8", "bf16"), ("int4", "f16"), ("int4", "bf16")])
+@pytest.mark.parametrize("dim,heads", [(64, 2), (64, 14), (128, 3), (128, 16)])
+@pytest.mark.parametrize("big", [1e5, 1e12, 1e30, 3e38])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "half"])
+def test_token_large_values_without_weight(cuda, fmt, dtype, dim, heads, big, where):
+    """Rows of large values that no head gives weight to leave the others as they are."""
+    import torch
+    n = 700
+    far = torch.zeros(n, dtype=torch.bool, device="cuda")
+    if where == "half":
+        far[1::2] = True
+    else:
+        far[{"first": 0, "middle": 333, "last": n - 1}[where]] = True
+    k, v = randn(1, n, 1, dim), randn(2, n, 1, dim) + 0.5
+    k[:, 0, 0] = 0
+    k[far] = 0
+    k[far, 0, 0] = -2400.0                     # logits of -300: weights below 2^-420
+    v[far] = big
+    q = randn(3, 1, heads, dim, dtype=dtype)
+    q[..., 0] = 1.0
+    cache, table, length, rows = pages_of(k, v, fmt)
+    check_quantised(cache, q, table, length, rows, dtype, 1.0 / 8)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("big", [1e6, 1e25])
+def test_token_heads_that_see_values_of_different_size(cuda, fmt, dim, big):
+    """Of the heads of a KV head some give all their weight to large values, some to small ones."""
+    import torch
+    n = 600
+    k, v = randn(1, n, 1, dim, spread=0.5), randn(2, n, 1, dim) + 0.5
+    k[:, 0, 0] = torch.where(torch.arange(n, device="cuda") % 7 == 3, 30.0, -30.0)
+    v[k[:, 0, 0] > 0] *= big
+    q = randn(3, 1, 10, dim, dtype="bf16")
+    q[0, :, 0] = torch.where(torch.arange(10, device="cuda") % 3 == 0, 16.0, -16.0).bfloat16()
+    cache, table, length, rows = pages_of(k, v, fmt)
+    check_quantised(cache, q, table, length, rows, "bf16", 1.0 / 8)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+def test_token_climbing_logits_after_a_large_value(cuda, fmt):
+    """The large value leads at first; by the end of a slow climb its weight is 2^-115."""
+    import torch
+    n = 3000
+    k = torch.zeros((n, 1, 64), device="cuda")
+    k[:, 0, 0] = torch.linspace(-40, 40, n, device="cuda")
+    v = randn(2, n, 1, 64) + 0.5
+    v[0] = 1e20
+    q = torch.zeros((1, 4, 64), device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    cache, table, length, rows = pages_of(k, v, fmt)
+    check_quantised(cache, q, table, length, rows, "bf16", 1.0)
