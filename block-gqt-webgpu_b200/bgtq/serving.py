@@ -28,6 +28,7 @@ _HALF = {torch.float16: "f16", torch.bfloat16: "bf16"}
 # format: (code, element type)
 _FORMATS = {"f16": (_lib.PAGES_F16, torch.float16), "bf16": (_lib.PAGES_BF16, torch.bfloat16),
             "int8": (_lib.PAGES_INT8, torch.int8), "int4": (_lib.PAGES_INT4, torch.uint8)}
+_LEAST_SCALE = 2.0 ** -149  # the least FP32: a zero stands for the default at the C ABI
 
 
 def _refuse(message: str):
@@ -165,7 +166,7 @@ class PagedCache:
         st = _stream(self.device)
         work = self._workspace.get((st, heads)) or self._work(heads, st)
         status = self._attend(self._ref, q.data_ptr(), _DTYPE[dtype], batch, heads, q0, q1, table.data_ptr(),
-                              table.stride(0), table.shape[1], lengths.data_ptr(), 0.0 if scale is None else scale,
+                              table.stride(0), table.shape[1], lengths.data_ptr(), 0.0 if scale is None else max(scale, _LEAST_SCALE),
                               out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1], st)
         if status:
             _lib.check(status)
@@ -251,7 +252,7 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
     p = _lib.PromptDesc(dev, _DTYPE[dtype], starts.shape[0] - 1, heads, keys[1], dim, tokens, keys[0], q.data_ptr(),
                         k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, starts.data_ptr(),
                         None if key_starts is None else key_starts.data_ptr(), 1 if causal else 0,
-                        0.0 if scale is None else scale, out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1])
+                        0.0 if scale is None else max(scale, _LEAST_SCALE), out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1])
     status = _lib.lib().bgtq_prompt_attend(C.byref(p), st)
     if status:
         _lib.check(status)

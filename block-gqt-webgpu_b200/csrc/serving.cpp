@@ -68,9 +68,9 @@ bgtq_status view(const bgtq_paged_cache *c, PageView &v) {
 
 // scale of the logits in log2 units; 0 stands for 1 / sqrt(dim)
 bool logit_scale(float scale, uint32_t dim, float &out) {
-    if (!(scale >= 0.0f) || !std::isfinite(scale)) return false;
+    if (!(scale >= 0.0f)) return false;
     out = (scale == 0.0f ? 1.0f / std::sqrt((float)dim) : scale) * kLog2e;
-    return true;
+    return std::isfinite(out);
 }
 
 size_t width_of(bgtq_dtype t) { return t == BGTQ_F32 ? 4 : 2; }

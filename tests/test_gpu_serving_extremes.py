@@ -211,3 +211,19 @@ def test_token_climbing_logits_after_a_large_value(cuda, fmt):
     q[..., 0] = 1.0
     cache, table, length, rows = pages_of(k, v, fmt)
     check_quantised(cache, q, table, length, rows, "bf16", 1.0)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-46, 1e-44])
+def test_scales_below_fp32(cuda, scale):
+    """A scale of next to nothing gives equal weights, not the default scale."""
+    import torch
+    from bgtq import prompt_attention
+    n = 50
+    q, k, v = (randn(s, n, 1, 64, dtype="f16") for s in (1, 2, 3))
+    want = v[:, 0].double().mean(0)
+    tol = U["f16"] * want.abs() + (U["f16"] + 3e-5) * v[:, 0].double().abs().mean(0)
+    out = prompt_attention(q, k, v, starts_of([n]), causal=False, scale=scale)
+    assert bool(((out[:, 0].double() - want).abs() <= tol).all())
+    cache, table, length, _ = pages_of(k, v, "f16")
+    out = cache.attend(q[:1], table, length, scale=scale)
+    assert bool(((out[0, 0].double() - want).abs() <= tol).all())
