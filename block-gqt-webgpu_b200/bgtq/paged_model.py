@@ -21,7 +21,12 @@ from .model import ModelGeometry
 from .serving import PagedCache, prompt_attention, _refuse
 
 
-_RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width
+_RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width, both rounded up
+
+
+def _places(requests: int) -> int:
+    """The places of the recorded step that so many requests take: powers of two up to 16, then multiples of 16."""
+    return 1 << (requests - 1).bit_length() if requests <= 16 else min(-(-requests // 16) * 16, max(requests, 65535))
 
 
 class PagedDecoder:
@@ -60,7 +65,7 @@ class PagedDecoder:
         self._free = list(range(pages))[::-1]
         self._held = {}        # request: [its pages in order, its tokens]
         self._next = 0
-        self._steps, self._side = {}, torch.cuda.Stream(self.dev)
+        self._steps, self._side, self._pool = {}, torch.cuda.Stream(self.dev), torch.cuda.graph_pool_handle()
 
     # ---- requests and pages ----
     def open(self) -> int:
@@ -157,8 +162,9 @@ class PagedDecoder:
         return self._forward(self._to(flat, torch.int64), positions, attention, self._to(ends - 1, torch.int64))
 
     def step(self, requests, tokens):
-        """One token of each request: logits [requests, vocab] (FP32).  Replays a CUDA graph,
-        recorded at the first step of so many requests and pages (up to a power of two)."""
+        """One token of each request: logits [requests, vocab] (FP32).  Replays a CUDA graph that is
+        recorded at the first step of about so many requests and pages; of the places that are
+        left over, nothing is written or read.  The graphs used last are kept."""
         tokens = np.asarray(tokens.cpu() if torch.is_tensor(tokens) else tokens, np.int64).reshape(-1)
         if len(tokens) != len(requests):
             _refuse("Paged decoder: one token for every request")
@@ -167,23 +173,28 @@ class PagedDecoder:
             return self._step(tokens, held, before)
 
     def _step(self, tokens, held, before):
+        n, places = len(held), _places(len(held))
         width = 1 << max(4, (max(len(h[0]) for h in held) - 1).bit_length())
-        table = np.zeros((len(held), width), np.int32)
+        key = places, width
+        graph, inputs, logits = self._steps[key] = self._steps.pop(key, None) or self._record(places, width)
+        slots = [h[0][b // self.page_size] * self.page_size + b % self.page_size for h, b in zip(held, before)]
+        for buffer, values, rest in zip(inputs, (tokens, before, slots, [h[1] for h in held]), (0, 0, -1, 0)):
+            row = np.full(places, rest, np.float32 if buffer.is_floating_point() else np.int64)
+            row[:n] = values
+            buffer.copy_(torch.as_tensor(row).to(buffer.dtype))
+        table = np.zeros((places, width), np.int32)
         for row, h in zip(table, held):
             row[:len(h[0])] = h[0]
-        slots = [h[0][b // self.page_size] * self.page_size + b % self.page_size for h, b in zip(held, before)]
-        graph, inputs, logits = self._steps.get((len(held), width)) or self._record(len(held), width)
-        for buffer, values in zip(inputs, (tokens, before, slots, table, [h[1] for h in held])):
-            buffer.copy_(torch.as_tensor(np.asarray(values), dtype=buffer.dtype))
+        inputs[-1].copy_(torch.as_tensor(table))
         graph.replay()
-        return logits.clone()
+        return logits[:n].clone()
 
     def _record(self, batch: int, width: int):
         """A step of batch requests over tables of width pages: graph, inputs, logits."""
-        tokens, positions, slots, table, lengths = inputs = (
+        tokens, positions, slots, lengths, table = inputs = (
             self._to(np.zeros(batch), torch.int64), self._to(np.zeros(batch), torch.float32),
-            self._to(np.full(batch, -1), torch.int64), self._to(np.zeros((batch, width)), torch.int32),
-            self._to(np.zeros(batch), torch.int32))
+            self._to(np.full(batch, -1), torch.int64), self._to(np.zeros(batch), torch.int32),
+            self._to(np.zeros((batch, width)), torch.int32))
 
         def attention(cache, q, k, v):
             cache.write(k, v, slots)
@@ -195,12 +206,12 @@ class PagedDecoder:
             self._forward(tokens, positions, attention, None)
         torch.cuda.current_stream(self.dev).wait_stream(self._side)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=self._side):
+        # one pool for all: a replay's logits are copied before the next one, whichever it is
+        with torch.cuda.graph(graph, pool=self._pool, stream=self._side):
             logits = self._forward(tokens, positions, attention, None)
-        if len(self._steps) == _RECORDED:
+        while len(self._steps) >= _RECORDED:
             del self._steps[next(iter(self._steps))]
-        self._steps[batch, width] = graph, inputs, logits
-        return self._steps[batch, width]
+        return graph, inputs, logits
 
     def generate(self, prompts, count: int):
         """Greedy: count tokens after each of prompts (sequences of tokens), as an int64 array
