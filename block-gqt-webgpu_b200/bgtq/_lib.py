@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libbgtq.so"
 OK, EINVAL, ECAPACITY, ENONFINITE, EBUSY, ELAYOUT, ETIMEOUT, ECUDA, ENOMEM = range(9)
 F16, F32, BF16 = 1, 2, 3
 PAGES_F16, PAGES_BF16, PAGES_INT8, PAGES_INT4 = 1, 2, 3, 4
+WORKSPACE_ZEROED = 65536
 KEYS_PACKED, KEYS_FP16, KEYS_COMPRESSED = 1, 2, 3
 
 

@@ -11,7 +11,7 @@ Indices that only the GPU sees (slots, page tables, lengths, starts) are checked
 lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
 length or starts).
 
-Attention keeps a zeroed workspace for every stream that it has been called on.  A CUDA graph
+Attention keeps a workspace for every stream that it has been called on.  A CUDA graph
 recorded on such a stream uses that one, so it is not replayed at the same time as calls there;
 recorded on a stream without one, it has its own.
 """
@@ -33,6 +33,13 @@ _LEAST_SCALE = 2.0 ** -149  # the least FP32: a zero stands for the default at t
 
 def _refuse(message: str):
     raise _lib.RangeError(_lib.EINVAL, message)
+
+
+def _room(size: int, device):
+    """A workspace, its counters zeroed: address, bytes, tensor."""
+    have = torch.empty(size, dtype=torch.uint8, device=device)
+    have[:_lib.WORKSPACE_ZEROED].zero_()
+    return have.data_ptr(), size, have
 
 
 def _stream(device: int) -> int:
@@ -176,8 +183,7 @@ class PagedCache:
         """The stream's own workspace (calls on different streams may overlap): address, bytes, tensor."""
         need = C.c_size_t()
         _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
-        have = torch.zeros(need.value, dtype=torch.uint8, device=self._on)
-        work = have.data_ptr(), need.value, have
+        work = _room(need.value, self._on)
         if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
             self._workspace[stream, heads] = work
         return work
@@ -190,8 +196,7 @@ def _prompt_workspace(device, dim: int, stream: int):
     """The stream's own workspace (calls on different streams may overlap): address, bytes, tensor."""
     need = C.c_size_t()
     _lib.call("bgtq_prompt_workspace", device.index, dim, C.byref(need))
-    have = torch.zeros(need.value, dtype=torch.uint8, device=device)
-    work = have.data_ptr(), need.value, have
+    work = _room(need.value, device)
     if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
         _prompt_work[device.index, dim, stream] = work
     return work

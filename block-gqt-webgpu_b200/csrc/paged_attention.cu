@@ -968,6 +968,7 @@ cudaError_t by_shape(const PagedAttendArgs &a, cudaStream_t s) {
 
 }  // namespace
 
+// (The counters of any device with less than 4096 SMs are within the bytes that start from zero.)
 size_t paged_attend_workspace(uint32_t q_heads, uint32_t kv_heads, uint32_t dim) {
     return counter_bytes() + 2ull * most_ctas() * (q_heads / kv_heads <= 8 ? 8u : 16u) * (dim + 2) * 4;
 }

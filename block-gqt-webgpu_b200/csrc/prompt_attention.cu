@@ -1034,7 +1034,8 @@ bool make_map(CUtensorMap *m, bool bf16, const void *p, uint32_t dim, uint32_t h
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Bytes of the workspace's counters: one for every softmax warp of every CTA.
+// Bytes of the workspace's counters: one for every softmax warp of every CTA.  (Those of any device with up to 1024 SMs
+// are within BGTQ_WORKSPACE_ZEROED.)
 uint32_t prompt_counters(int sms, uint32_t tiles) { return ((uint32_t)sms * tiles * 16 + 127) / 128 * 128; }
 
 template <int D, bool BF>

@@ -491,6 +491,9 @@ bgtq_status bgtq_paged_write(const bgtq_paged_cache *c, const void *k, const voi
  * the status bit), give zeros. */
 bgtq_status bgtq_paged_read(const bgtq_paged_cache *c, const int64_t *slots, uint64_t tokens, void *k_out,
                             void *v_out, bgtq_dtype dtype, void *stream);
+/* Of a workspace only the counters at its front have to start from zero: these bytes, or all if
+ * it has fewer. */
+#define BGTQ_WORKSPACE_ZEROED 65536
 /* Bytes of workspace that bgtq_paged_attend needs for this head count, whatever the batch. */
 bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t q_heads, size_t *bytes);
 /* One new token per request: out[b][h] = sum over t < lengths[b] of softmax(scale q.k_t) v_t.
@@ -505,8 +508,8 @@ bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t q_he
  *   scale    of the logits, positive (0: 1 / sqrt(dim))
  *   out      dense [batch][q_heads][dim] of dtype; lse [batch][q_heads] FP32 natural log of
  *            the sum of exponentials (-inf for length 0), or null
- *   workspace  zero-filled before its first use; every call leaves it ready for the next.
- *            Calls that may overlap on the GPU need workspaces of their own. */
+ *   workspace  its first BGTQ_WORKSPACE_ZEROED bytes zero before its first use; every call leaves
+ *            it ready for the next.  Calls that may overlap on the GPU need workspaces of their own. */
 bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dtype dtype, uint32_t batch,
                               uint32_t q_heads, int64_t q_batch_stride, int64_t q_head_stride, const int32_t *table,
                               int64_t table_stride, uint32_t table_width, const int32_t *lengths, float scale,
@@ -533,8 +536,9 @@ typedef struct bgtq_prompt {
     float scale;  /* of the logits, positive (0: 1 / sqrt(dim)) */
     void *out;    /* dense [q_tokens][q_heads][dim] of dtype */
     float *lse;   /* [q_tokens][q_heads] FP32, or null */
-    void *workspace; /* 128-byte aligned, zero-filled before its first use; every call leaves it
-                        ready for the next.  Calls that may overlap need their own. */
+    void *workspace; /* 128-byte aligned, its first BGTQ_WORKSPACE_ZEROED bytes zero before its first
+                        use; every call leaves it ready for the next.  Calls that may overlap
+                        need their own. */
     size_t workspace_bytes;
 } bgtq_prompt;
 /* Bytes of workspace that bgtq_prompt_attend needs for a head dim, whatever the batch. */
