@@ -67,9 +67,13 @@ def layout_jit_wait(timeout_s: float = 300.0) -> bool:
 
 
 def device_status(device: int = 0) -> int:
-    """Device status word (0 = no kernel reported a timeout or bad length)."""
+    """Device status word (0 = no kernel reported a timeout or bad length).  Where a wait ran out
+    (bit 1), the prompt workspaces are made ready again, whose last call may have left them otherwise."""
     import ctypes as C
+    import sys
     from . import _lib
     v = C.c_uint32()
     _lib.call("bgtq_device_status", device, C.byref(v))
+    if v.value & 1 and __name__ + ".serving" in sys.modules:
+        sys.modules[__name__ + ".serving"]._ready_again(device)
     return v.value

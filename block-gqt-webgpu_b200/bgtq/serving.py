@@ -202,6 +202,16 @@ def _prompt_workspace(device, dim: int, stream: int):
     return work
 
 
+def _ready_again(device: int):
+    """Zeroes the counters of the device's prompt workspaces: a call whose wait ran out ends without its joins.
+    (One-token attention waits for nothing, and a graph's own workspace is zeroed by its replays.)"""
+    torch.cuda.synchronize(device)
+    for (on, _, _), work in _prompt_work.items():
+        if on == device:
+            work[2][:_lib.WORKSPACE_ZEROED].zero_()
+    torch.cuda.synchronize(device)
+
+
 def _even(t):
     """t, or a packed copy of it where the kernels' loads cannot follow its strides or address, and its
     token and head strides (that of a dimension of one element is never used)."""

@@ -537,8 +537,9 @@ typedef struct bgtq_prompt {
     void *out;    /* dense [q_tokens][q_heads][dim] of dtype */
     float *lse;   /* [q_tokens][q_heads] FP32, or null */
     void *workspace; /* 128-byte aligned, its first BGTQ_WORKSPACE_ZEROED bytes zero before its first
-                        use; every call leaves it ready for the next.  Calls that may overlap
-                        need their own. */
+                        use; every call leaves it ready for the next, but for one whose wait
+                        ran out (device status bit 1): zero them again.  Calls that may
+                        overlap need their own. */
     size_t workspace_bytes;
 } bgtq_prompt;
 /* Bytes of workspace that bgtq_prompt_attend needs for a head dim, whatever the batch. */

@@ -73,3 +73,28 @@ def test_a_recording_on_a_new_stream_zeroes_the_front_alone(cuda):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_workspace_is_ready_again_after_a_wait_that_ran_out(cuda, monkeypatch):
+    """The status is made up, and so are the counters that such a call leaves; they stay within the launch's parts."""
+    import torch
+    import bgtq
+    from bgtq import prompt_attention, serving
+    c = case()
+    run = lambda: prompt_attention(c["q2"], c["k"], c["v"], c["starts"], c["keys"])
+    want = run()
+    torch.cuda.synchronize()
+    work = serving._prompt_work[0, 64, torch.cuda.current_stream().cuda_stream][2]
+    assert not work[:_lib.WORKSPACE_ZEROED // 8].any()
+    work.view(torch.int32)[:64] = 1
+    real = _lib.call
+
+    def call(name, *args):
+        real(name, *args)
+        if name == "bgtq_device_status":
+            args[1]._obj.value |= 1
+
+    monkeypatch.setattr(_lib, "call", call)
+    assert bgtq.device_status() & 1
+    assert torch.equal(run(), want)
+    assert not work[:_lib.WORKSPACE_ZEROED // 8].any()
