@@ -44,6 +44,8 @@ class PagedDecoder:
         self.dtype, self.page_size = dtype, int(page_size)
         self.dev = torch.device("cuda", device)
         self.caches = [PagedCache(g.kv_heads, g.head_dim, pages, page_size, format, device) for _ in range(g.layers)]
+        for c in self.caches[1:]:  # the layers follow each other on one stream: one workspace serves all
+            c._workspace = self.caches[0]._workspace
         w = {k: v.to(self.dev, dtype) for k, v in weights.items()}
         self.emb, self.final_norm = w["model.embed_tokens.weight"], w["model.norm.weight"].float()
         self.layers = []

@@ -98,3 +98,13 @@ def test_a_workspace_is_ready_again_after_a_wait_that_ran_out(cuda, monkeypatch)
     assert bgtq.device_status() & 1
     assert torch.equal(run(), want)
     assert not work[:_lib.WORKSPACE_ZEROED // 8].any()
+
+
+def test_the_layers_of_a_decoder_share_a_workspace(cuda):
+    import numpy as np
+    from test_gpu_paged_decoder_failures import decoder
+    dec = decoder()
+    r = dec.open()
+    dec.prompt([r], [np.arange(20)])
+    dec.step([r], [3])
+    assert len({work[0] for cache in dec.caches for work in cache._workspace.values()}) == 1
