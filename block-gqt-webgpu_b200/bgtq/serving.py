@@ -42,6 +42,11 @@ def _room(size: int, device):
     return have.data_ptr(), size, have
 
 
+def _recording(device) -> bool:
+    with torch.cuda.device(device):  # the tensors' device need not be the current one
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -184,7 +189,7 @@ class PagedCache:
         need = C.c_size_t()
         _lib.call("bgtq_paged_attend_workspace", self._ref, heads, C.byref(need))
         work = _room(need.value, self._on)
-        if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
+        if not _recording(self._on):  # a graph's own is zeroed by its replays alone
             self._workspace[stream, heads] = work
         return work
 
@@ -197,7 +202,7 @@ def _prompt_workspace(device, dim: int, stream: int):
     need = C.c_size_t()
     _lib.call("bgtq_prompt_workspace", device.index, dim, C.byref(need))
     work = _room(need.value, device)
-    if not torch.cuda.is_current_stream_capturing():  # a graph's own is zeroed by its replays alone
+    if not _recording(device):  # a graph's own is zeroed by its replays alone
         _prompt_work[device.index, dim, stream] = work
     return work
 
