@@ -14,14 +14,28 @@ from .attention import AttentionEngine, AttentionSession, GroupedAttention, Opti
 __all__ = ["BGTQError", "DeviceError", "LayoutError", "RangeError", "StateError", "LIB_PATH", "lib",
            "BlockGTQParameters", "allocate_bits", "build_tables", "haar_rotation", "optimal_centroids", "tables", "validate_layout", "CompressedKeys", "FP16Keys", "append_kv",
            "PackedKeys", "Values", "AttentionEngine", "AttentionSession", "GroupedAttention", "OptimizedAttention",
-           "PagedCache", "prompt_attention", "PagedDecoder",
            "device_status", "set_layout_jit", "layout_jit_stats",
            "layout_jit_counts", "layout_jit_wait"]
 
+# the serving operators work on torch tensors: torch is imported with their first use, and they are among
+# the names of a star import where there is one
+_SERVING = ("PagedCache", "prompt_attention", "PagedDecoder")
+
+
+def _torch_is_there() -> bool:
+    import importlib.util
+    try:
+        return importlib.util.find_spec("torch") is not None
+    except (ImportError, ValueError):
+        return False
+
+
+if _torch_is_there():
+    __all__ += _SERVING
+
 
 def __getattr__(name):
-    # the serving operators work on torch tensors: torch is imported with their first use
-    if name in ("PagedCache", "prompt_attention", "PagedDecoder"):
+    if name in _SERVING:
         from . import paged_model, serving
         globals().update(PagedCache=serving.PagedCache, prompt_attention=serving.prompt_attention,
                          PagedDecoder=paged_model.PagedDecoder)
