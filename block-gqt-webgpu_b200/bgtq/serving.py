@@ -6,14 +6,15 @@
                        ``attend`` runs one new token of every request over its own pages
 
 No counterpart in the reference, whose stores hold one sequence each.  CUDA tensors in, CUDA
-tensors out, ordered on the current stream of the tensors' device; nothing synchronises.
+tensors out, ordered on the current stream of the tensors' device; nothing synchronises, and
+nothing is differentiated: results do not require gradients, whatever the arguments do.
 Indices that only the GPU sees (slots, page tables, lengths, starts) are checked there: what
 lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
 length or starts).
 
 Attention keeps a workspace for every stream that it has been called on.  A CUDA graph
-recorded on such a stream uses that one, so it is not replayed at the same time as calls there;
-recorded on a stream without one, it has its own.
+recorded on such a stream uses that one, so it is not replayed at the same time as calls there or
+other graphs that were recorded there; recorded on a stream without one, it has its own.
 """
 from __future__ import annotations
 
@@ -235,7 +236,8 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
     is query rows starts[s] .. starts[s + 1] and key rows key_starts[s] .. key_starts[s + 1]
     (int32 [sequences + 1]; key_starts None: the same as starts).  Causal rows see their
     sequence's keys up to their own, counted from the end, so a chunk whose prefix is cached
-    passes more keys than queries.  Rows that see nothing are zeros.  Any strides with a
+    passes more keys than queries.  Rows that see nothing are zeros; rows that no sequence holds are
+    not written (of a new output they are whatever its memory held).  Any strides with a
     contiguous last dimension; a tensor whose strides or address are not multiples of 16
     bytes is copied.  Returns out [tokens, q_heads, dim], with ``lse`` also the log sums
     [tokens, q_heads] (float32)."""

@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) prompt_kernel(const __gr
                 m0 = max3(m0, s[kKeys - 4], s[kKeys - 3]);
                 m1 = max3(m1, s[kKeys - 2], s[kKeys - 1]);
                 const float top = fmaxf(max3(m0, m1, m2), m3) * a.scale;
-                const bool grown = top > ref + kLazy;  // each row for itself: no result depends on a neighbour
+                const bool grown = top > ref + kLazy;  // each row for itself, not by the others of the warp
                 if (j == 0) ref = top;
                 else if (__any_sync(0xffffffffu, grown)) {
                     // not under a product that is still adding to the outputs: the other buffer's next logits

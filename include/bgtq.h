@@ -506,7 +506,8 @@ bgtq_status bgtq_paged_attend_workspace(const bgtq_paged_cache *c, uint32_t q_he
  *            there and sets a status bit; tokens of a page index past the last page are left
  *            out and set one
  *   scale    of the logits, positive (0: 1 / sqrt(dim))
- *   out      dense [batch][q_heads][dim] of dtype; lse [batch][q_heads] FP32 natural log of
+ *   out      dense [batch][q_heads][dim] of dtype (an infinity among the values of 16-bit pages
+ *            gives infinity, or NaN where its probability is below what 16 bits hold); lse [batch][q_heads] FP32 natural log of
  *            the sum of exponentials (-inf for length 0), or null
  *   workspace  its first BGTQ_WORKSPACE_ZEROED bytes zero before its first use; every call leaves
  *            it ready for the next.  Calls that may overlap on the GPU need workspaces of their own. */
@@ -521,7 +522,8 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
  * key_starts[s + 1] (device int32, ascending; null: the same as starts).  Causal: row i of a
  * sequence sees its keys j <= i + (keys - queries), so prompts whose earlier tokens are
  * cached pass more keys than queries.  Rows that see nothing give zeros and -inf; query rows
- * that no sequence holds are not written.  Starts that fall or pass the token counts set a
+ * that no sequence holds are not written.  An infinity in V gives infinity to the rows that see it,
+ * or NaN where its probability is below what 16 bits hold.  Starts that fall or pass the token counts set a
  * status bit and their sequence is skipped.
  * Pointers are 16-byte aligned, strides positive multiples of 8 elements; q_heads / kv_heads <= 128. */
 typedef struct bgtq_prompt {
