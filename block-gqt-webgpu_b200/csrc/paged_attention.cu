@@ -35,8 +35,7 @@
 //     of any scale: they are taken relative to the largest of each head, so that a value of
 //     any size whose weight is next to nothing leaves the others as they are.  What is
 //     rounded away is 2^-35 of the largest.  Queries are taken relative to a power of two
-//     of their row's largest; FP16 drops 2^-38 of it, and FP32 holds their products with key
-//     scales up to 2^99.  (128 requests of 16K to 32K
+//     of their row's largest; FP16 drops 2^-38 of it.  (128 requests of 16K to 32K
 //     tokens, 9 / 3 heads of 64 in 8 bits, 230 us for 225 with one power for all heads.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,6 +52,7 @@ enum { F_F16, F_BF16, F_INT8, F_INT4 };
 // contribution may pass the largest before it, 10 + kRoom + 1 being what FP16 holds; how far apart the heads of a
 // KV head may be in contribution over probability.
 constexpr float kLeast = -100.0f, kRoom = 4.0f, kApart = 100.0f;
+constexpr float kSmall = 1.0f / 65536.0f;  // of 4-bit pages' key scales, given back with the query's power
 
 template <int F, int D, int NT>
 struct Shape {
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
 #pragma unroll
                         for (int k = 0; k < 4; ++k) x[n][s][k] *= g;
                 }
-                f *= a.scale;
+                f *= F == F_INT4 ? a.scale * (1.0f / kSmall) : a.scale;
                 qs[n][0] = __shfl_sync(0xffffffffu, f, col4 * 8);
                 qs[n][1] = __shfl_sync(0xffffffffu, f, col4 * 8 + 4);
 #pragma unroll
@@ -540,12 +540,13 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                         }
                     }
                     const float k0 = from_bf16(ksc[r0]), k1 = from_bf16(ksc[r0 + 8]);
+                    // (by the query's power first: a product of up to 2^28 with a large key scale may pass FP32)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        s[c][n][0] *= k0;
-                        s[c][n][1] *= k0;
-                        s[c][n][2] *= k1;
-                        s[c][n][3] *= k1;
+                        s[c][n][0] *= k0 * qs[n][0];
+                        s[c][n][1] *= k0 * qs[n][1];
+                        s[c][n][2] *= k1 * qs[n][0];
+                        s[c][n][3] *= k1 * qs[n][1];
                     }
                 } else {
 #pragma unroll
@@ -561,8 +562,19 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
                             x >>= 8;
                             y >>= 8;
                         }
-                        const float k0 = from_bf16(ksc[r0 * S::kGroups + g]);
-                        const float k1 = from_bf16(ksc[(r0 + 8) * S::kGroups + g]);
+                        // (products of up to 2^22 with a large key scale may pass FP32)
+                        float k0, k1;
+                        if constexpr (D == 64) {  // both groups' scales of a token by one load (252 us for 257; at 128 it costs 1 %)
+                            const uint32_t kx = reinterpret_cast<const uint32_t *>(ksc)[r0];
+                            const uint32_t ky = reinterpret_cast<const uint32_t *>(ksc)[r0 + 8];
+                            k0 = g ? __uint_as_float(kx & 0xffff0000u) : from_bf16(kx);
+                            k1 = g ? __uint_as_float(ky & 0xffff0000u) : from_bf16(ky);
+                        } else {
+                            k0 = from_bf16(ksc[r0 * S::kGroups + g]);
+                            k1 = from_bf16(ksc[(r0 + 8) * S::kGroups + g]);
+                        }
+                        k0 *= kSmall;
+                        k1 *= kSmall;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             s[c][n][0] = fmaf(p[n][0], k0, s[c][n][0]);
@@ -588,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const PagedAttendAr
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float &x = s[c][n][2 * e + h];
-                            x = in ? x * qs[n][h] : -INFINITY;
+                            x = in ? (F == F_INT8 ? x : x * qs[n][h]) : -INFINITY;
                             top[n][h] = fmaxf(top[n][h], x);
                         }
                 }

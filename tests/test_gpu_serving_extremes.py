@@ -227,3 +227,14 @@ def test_scales_below_fp32(cuda, scale):
     cache, table, length, _ = pages_of(k, v, "f16")
     out = cache.attend(q[:1], table, length, scale=scale)
     assert bool(((out[0, 0].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dim,heads", [(64, 3), (128, 10)])
+@pytest.mark.parametrize("q_size,k_size", [(1.0, 1e36), (1e36, 1.0), (1e-30, 1e32), (1e32, 1e-30)])
+def test_token_large_queries_and_keys(cuda, fmt, dim, heads, q_size, k_size):
+    """Logits that FP32 holds, from queries or keys near the ends of BF16."""
+    k, v = randn(1, 300, 1, dim) * k_size, randn(2, 300, 1, dim) + 0.5
+    q = (randn(3, 1, heads, dim) * q_size).bfloat16()
+    cache, table, length, rows = pages_of(k, v, fmt)
+    check_quantised(cache, q, table, length, rows, "bf16", 1.0 / 8)
