@@ -46,7 +46,7 @@ class PagedDecoder:
         self.caches = [PagedCache(g.kv_heads, g.head_dim, pages, page_size, format, device) for _ in range(g.layers)]
         for c in self.caches[1:]:  # the layers follow each other on one stream: one workspace serves all
             c._workspace = self.caches[0]._workspace
-        w = {k: v.to(self.dev, dtype) for k, v in weights.items()}
+        w = {k: v.detach().to(self.dev, dtype) for k, v in weights.items()}  # (attention has no gradient)
         self.emb, self.final_norm = w["model.embed_tokens.weight"], w["model.norm.weight"].float()
         self.layers = []
         for layer in range(g.layers):

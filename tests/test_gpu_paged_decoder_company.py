@@ -1,4 +1,5 @@
-"""What a request of the paged decoder answers does not depend on whom it is served with, up to rounding."""
+"""What a request of the paged decoder answers does not depend on whom it is served with, up to rounding, nor
+on whether its weights are a training program's."""
 import math
 
 import numpy as np
@@ -27,3 +28,18 @@ def test_every_token_of_company_is_one_that_the_request_alone_would_choose(cuda,
             logits = dec.step([r], [t])[0]
         dec.close(r)
     assert dec.free_pages == 32
+
+
+def test_weights_that_require_gradients(cuda):
+    """Logits carry no graph, which would leave attention out, and no step's memory is kept for one."""
+    import torch
+    from bgtq import PagedDecoder
+    g = SMALL["llama"]
+    w = weights_of(g, "f16")
+    answers = []
+    for weights in (w, {k: v.clone().requires_grad_() for k, v in w.items()}):
+        dec = PagedDecoder(weights, g, pages=8, page_size=16, format="int8", dtype=torch.float16)
+        r = dec.open()
+        answers.append((dec.prompt([r], [np.arange(20)]), dec.prompt([r], [[4, 5]]), dec.step([r], [6])))
+    for a, b in zip(*answers):
+        assert not b.requires_grad and torch.equal(a, b)
