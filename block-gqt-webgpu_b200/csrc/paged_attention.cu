@@ -4,8 +4,9 @@
 // What bounds it is the one pass over K and V: 2 row_bytes a token and KV head, against 2 D
 // multiply-adds for each query head, so the work is laid out for the memory system.  128 requests
 // of 16K to 32K tokens, 9 / 3 heads of 64 in 16 bits: 345 us, 6.7 TB/s, a little above a plain
-// copy's rate; in 8 bits 225 us, 5.3 TB/s, in 4 bits 248 us, 2.6 TB/s, where turning codes into
-// operands costs as many instructions for half the bytes.  Few tokens are bound by latencies instead (the deal, the first pages' way through
+// copy's rate; in 8 bits 232 us, 5.1 TB/s, in 4 bits 248 us, 2.6 TB/s, where turning codes into
+// operands costs as many instructions for half the bytes (they issue in 57 and 63 % of all cycles, the
+// integer pipe is busy in 51 and 55 %).  Few tokens are bound by latencies instead (the deal, the first pages' way through
 // the table, the join), about 10 us: one request of 4096 tokens 10.3 us, 48 of 1 to 8191, 32 / 8
 // heads of 128, 32 us (3.1 TB/s), eight of 20K to 32K, 14 / 2 heads of 64 in 4 bits, 21 us.
 //   * The (request, KV head, block of query heads) pairs are cut into units of kTokens tokens,
@@ -36,7 +37,7 @@
 //     any size whose weight is next to nothing leaves the others as they are.  What is
 //     rounded away is 2^-35 of the largest.  Queries are taken relative to a power of two
 //     of their row's largest; FP16 drops 2^-38 of it.  (128 requests of 16K to 32K
-//     tokens, 9 / 3 heads of 64 in 8 bits, 230 us for 225 with one power for all heads.)
+//     tokens, 9 / 3 heads of 64 in 8 bits, 232 us for 225 with one power for all heads.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

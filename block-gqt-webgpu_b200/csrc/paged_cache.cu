@@ -12,8 +12,9 @@
 // Both directions move each row once.  A thread takes eight dimensions of a row (16-byte loads and
 // stores of 16-bit elements); the lanes of a row, or of a 4-bit group, agree on the maximum by
 // shuffles.  16K tokens of 8 heads of 128 in 4 bits, written (21 us) and read back (16 us): 42 us
-// with the second launch, 172 MB, 4.1 TB/s of a copy's 6.5: instructions bound both (both issue in 2
-// of 3 cycles; about twelve instructions an element, half of them the quotient and its code).
+// with the second launch, 172 MB, 4.1 TB/s of a copy's 6.5.  Loads' latency bounds both first (5 and 9 warps wait
+// for one at each issue), then issue (2 of 3 cycles; about twelve instructions an element, half of them the
+// quotient and its code).
 // 16 tokens of 3 heads: 3.3 us, two launches' latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

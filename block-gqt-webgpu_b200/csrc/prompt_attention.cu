@@ -31,10 +31,12 @@
 // tensor arithmetic; the logits' products, which read both operands from shared memory, take 48
 // clocks an instruction for 32 of arithmetic, so products alone come to 640 or 320.  Its 8192
 // exponentials take 512 clocks at 16 a clock, so some go to the FMA pipe (kFma).  At head dim 128
-// products are the longer: four prompts of 3500 to 4096 tokens, 32 / 8 heads, causal, run at 1.04
-// to 1.14 PFLOP/s (415 to 455 us, with the power limit's clock).  At 64 it is exponentials with
-// the rest of softmax: two prompts of 8192 tokens, 14 / 2 heads, 283 us, 850 TFLOP/s.  Short
-// prompts are bound by their chain of latencies: 37 tokens take 8.3 us.  The tails (outputs,
+// products are the longer: four prompts of 3500 to 4096 tokens, 32 / 8 heads, causal, run at 1.03
+// to 1.12 PFLOP/s (425 to 460 us, with the power limit's clock).  At 64 it is softmax: two prompts
+// of 8192 tokens, 14 / 2 heads, 279 to 290 us, 830 to 860 TFLOP/s, with the exponential pipe 57 % full and
+// the tensor pipe 32 %, so neither is the limit by itself; most waits are for tensor memory, in each row's
+// chain of logits, maximum, exponentials and probabilities.  Short prompts are bound by their chain
+// of latencies: 37 tokens take 8.3 us.  The tails (outputs,
 // joining) are short loops on purpose: unrolled, their instruction fetches cost 10 us a call.
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the
 // last time: until then probabilities are taken relative to the older maximum, so they stay
