@@ -99,6 +99,7 @@ class PagedDecoder:
         """Pages for counts[i] more tokens of requests[i], all of them or a refusal: what each holds now and
         its length before.  A body that fails has written no rows to count on, so it leaves lengths and
         pages as they were."""
+        requests = requests.tolist() if hasattr(requests, "tolist") else list(requests)
         if not requests or len(set(requests)) < len(requests):
             _refuse("Paged decoder: requests must be one or more, each once")
         held = [self._request(r) for r in requests]

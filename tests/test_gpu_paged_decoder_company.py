@@ -43,3 +43,15 @@ def test_weights_that_require_gradients(cuda):
         answers.append((dec.prompt([r], [np.arange(20)]), dec.prompt([r], [[4, 5]]), dec.step([r], [6])))
     for a, b in zip(*answers):
         assert not b.requires_grad and torch.equal(a, b)
+
+
+def test_requests_in_an_array(cuda):
+    """Requests may stand in an array or a tensor, like tokens."""
+    import torch
+    from test_gpu_paged_decoder_failures import decoder
+    dec, same = decoder(), decoder()
+    held = [d.open() for d in (dec, same) for _ in range(2)][:2]
+    for wrap in (np.array, torch.tensor):
+        tokens = [np.arange(5), np.arange(9)]
+        assert torch.equal(dec.prompt(wrap(held), tokens), same.prompt(held, tokens))
+        assert torch.equal(dec.step(wrap(held), [3, 4]), same.step(held, [3, 4]))
