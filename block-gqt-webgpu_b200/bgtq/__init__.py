@@ -19,7 +19,7 @@ __all__ = ["BGTQError", "DeviceError", "LayoutError", "RangeError", "StateError"
 
 # the serving operators work on torch tensors: torch is imported with their first use, and they are among
 # the names of a star import where there is one
-_SERVING = ("PagedCache", "prompt_attention", "PagedDecoder")
+_SERVING = ("PagedCache", "prompt_attention", "adjust_logits", "PagedDecoder")
 
 
 def _torch_is_there() -> bool:
@@ -38,7 +38,7 @@ def __getattr__(name):
     if name in _SERVING:
         from . import paged_model, serving
         globals().update(PagedCache=serving.PagedCache, prompt_attention=serving.prompt_attention,
-                         PagedDecoder=paged_model.PagedDecoder)
+                         adjust_logits=serving.adjust_logits, PagedDecoder=paged_model.PagedDecoder)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 

@@ -83,6 +83,36 @@ class PromptDesc(C.Structure):
         ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class AppendDesc(C.Structure):
+    """bgtq_append: new tokens into the pages, rotated on the way."""
+    _fields_ = [("dtype", C.c_int), ("q_heads", C.c_uint32), ("tokens", C.c_uint64)] + [
+        (n, C.c_void_p) for n in ("q", "k", "v")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                 "v_token_stride", "v_head_stride")] + [
+        ("slots", C.c_void_p), ("rotary", C.c_void_p), ("rotary_rows", C.c_uint64), ("positions", C.c_void_p),
+        ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("out_dtype", C.c_int),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p)]
+
+
+class ChunkDesc(C.Structure):
+    """bgtq_chunk: new tokens of every request over its pages."""
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_uint32), ("q_heads", C.c_uint32), ("q_tokens", C.c_uint64),
+                ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("starts", C.c_void_p),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_uint32),
+                ("lengths", C.c_void_p), ("scale", C.c_float), ("window", C.c_uint32), ("sinks", C.c_uint32),
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LogitsDesc(C.Structure):
+    """bgtq_logits: penalties, biases and a mask on logits."""
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("batch", C.c_uint32), ("vocab", C.c_uint32),
+                ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("tokens", C.c_void_p),
+                ("tokens_stride", C.c_int64), ("width", C.c_uint32), ("id_bytes", C.c_uint32)] + [
+        (n, C.c_void_p) for n in ("lengths", "repetition", "presence", "frequency", "bias_ids", "bias")] + [
+        ("bias_stride", C.c_int64), ("entries", C.c_uint32), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
 # (name, restype, argtypes) for every exported symbol declared in include/bgtq.h
 P, U32, U64, I32, I64, SZ = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_int64, C.c_size_t
 SIGNATURES = {
@@ -156,6 +186,10 @@ SIGNATURES = {
     "bgtq_paged_attend": (I32, [P, P, I32, U32, U32, I64, I64, P, I64, U32, P, C.c_float, P, P, P, SZ, P]),
     "bgtq_prompt_workspace": (I32, [C.c_int, U32, P]),
     "bgtq_prompt_attend": (I32, [P, P]),
+    "bgtq_paged_append": (I32, [P, P, P]),
+    "bgtq_paged_chunk_workspace": (I32, [P, U32, P]),
+    "bgtq_paged_attend_chunk": (I32, [P, P, P]),
+    "bgtq_adjust_logits": (I32, [P, P]),
 }
 
 _lib = None

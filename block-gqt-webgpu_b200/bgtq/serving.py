@@ -2,8 +2,12 @@
 
     prompt_attention   a whole batch of prompts, packed one after the other, in one call
     PagedCache         K and V of every request in the pages of one pool, in 16, 8 or 4 bits:
-                       ``write`` quantises new rows, ``read`` gives back what rows stand for,
-                       ``attend`` runs one new token of every request over its own pages
+                       ``write`` quantises new rows, ``append`` rotates them (and norms their
+                       heads) on the way, ``read`` gives back what rows stand for, ``attend`` runs
+                       one new token of every request over its own pages, ``attend_chunk`` any
+                       number of them; both over all tokens or a window and the first few
+    adjust_logits      penalties for repeated tokens, biases and grammar masks, before a token is
+                       chosen
 
 No counterpart in the reference, whose stores hold one sequence each.  CUDA tensors in, CUDA
 tensors out, ordered on the current stream of the tensors' device; nothing synchronises, and
@@ -104,6 +108,7 @@ class PagedCache:
         library = _lib.lib()
         self._write, self._read = library.bgtq_paged_write, library.bgtq_paged_read
         self._attend = library.bgtq_paged_attend
+        self._append, self._chunk = library.bgtq_paged_append, library.bgtq_paged_attend_chunk
 
     def _check_slots(self, slots) -> None:
         if slots.dtype != torch.int64 or slots.device != self._on or slots.dim() != 1 or not slots.is_contiguous():
@@ -148,11 +153,74 @@ class PagedCache:
             _lib.check(status)
         return k, v
 
-    def attend(self, q, table, lengths, scale: float | None = None, out=None, lse: bool = False):
+    def append(self, q, k, v, slots, rotary, positions=None, q_norm=None, k_norm=None, eps: float = 1e-6, dtype=None,
+               keys: bool = False):
+        """New tokens in one pass: heads of q [tokens, q_heads, dim] and k [tokens, kv_heads, dim] are
+        normed, where q_norm / k_norm [dim] (float32) are given (x norm / sqrt(mean(x^2) + eps)), and rotated;
+        k and v [tokens, kv_heads, dim] are stored at ``slots`` [tokens] as ``write`` stores them.  All
+        three are float16, bfloat16 or float32, of any strides with a contiguous last dimension.
+        Dimension i < dim / 2 is rotated with dimension i + dim / 2 by the token's row of ``rotary``
+        [rows, dim] (float32: dim / 2 cosines, then sines), row positions[t] (int64) or, without
+        positions, row t.  Negative slots are padding: nothing is stored of them.  A token whose
+        position is outside the table is not stored and its results are zeros.
+        Returns the queries, as dtype (default: q's own), with ``keys`` also the keys."""
+        self._check_slots(slots)
+        n, shape = slots.shape[0], q.shape
+        if len(shape) != 3 or shape[0] != n or shape[1] < 1 or shape[2] != self.dim:
+            _refuse("Paged append: Q must be [tokens, q_heads, dim] with one slot a token")
+        if k.shape != (n, self.kv_heads, self.dim) or v.shape != k.shape:
+            _refuse("Paged append: K and V must be [tokens, kv_heads, dim] with one slot a token")
+        code = _DTYPE.get(q.dtype)
+        if code is None or k.dtype != q.dtype or v.dtype != q.dtype:
+            _refuse("Paged append: Q, K and V must all be float16, bfloat16 or float32")
+        to = q.dtype if dtype is None else dtype
+        out = _DTYPE.get(to)
+        if out is None:
+            _refuse("Paged append: dtype must be float16, bfloat16 or float32")
+        on = self._on
+        if q.device != on or k.device != on or v.device != on:
+            _refuse("Paged append: Q, K and V must be on the cache's device")
+        q0, q1, q2 = q.stride()
+        k0, k1, k2 = k.stride()
+        v0, v1, v2 = v.stride()
+        if q2 != 1 or k2 != 1 or v2 != 1:
+            _refuse("Paged append: the last dimension must be contiguous")
+        if (rotary.dim() != 2 or rotary.shape[1] != self.dim or rotary.dtype != torch.float32 or rotary.device != on
+                or not rotary.is_contiguous()):
+            _refuse("Paged append: rotary must be a contiguous float32 tensor [rows, dim] on the cache's device")
+        if positions is None:
+            if rotary.shape[0] < n:
+                _refuse("Paged append: without positions rotary must have a row for every token")
+        elif positions.shape != (n,) or positions.dtype != torch.int64 or positions.device != on or not positions.is_contiguous():
+            _refuse("Paged append: positions must be a contiguous int64 tensor [tokens] on the cache's device")
+        for w in (q_norm, k_norm):
+            if w is not None and (w.shape != (self.dim,) or w.dtype != torch.float32 or w.device != on
+                                  or not w.is_contiguous()):
+                _refuse("Paged append: norms must be contiguous float32 tensors [dim] on the cache's device")
+        if not 0.0 <= eps < float("inf"):
+            _refuse("Paged append: eps must be nonnegative and finite")
+        q_out = q.new_empty(shape, dtype=to)
+        k_out = q.new_empty(k.shape, dtype=to) if keys else None
+        p = _lib.AppendDesc(code, shape[1], n, q.data_ptr(), k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1,
+                            slots.data_ptr(), rotary.data_ptr(), rotary.shape[0],
+                            None if positions is None else positions.data_ptr(),
+                            None if q_norm is None else q_norm.data_ptr(),
+                            None if k_norm is None else k_norm.data_ptr(), eps, out, q_out.data_ptr(),
+                            k_out.data_ptr() if keys else None)
+        status = self._append(self._ref, C.byref(p), _stream(self.device))
+        if status:
+            _lib.check(status)
+        return (q_out, k_out) if keys else q_out
+
+    def attend(self, q, table, lengths, scale: float | None = None, out=None, lse: bool = False,
+               window: int | None = None, sinks: int = 0):
         """One new token of every request: q [batch, q_heads, dim] (float16 or bfloat16, the
         pages' type over 16-bit pages) over the first ``lengths`` [batch] (int32) tokens of the
-        pages in ``table`` [batch, width] (int32).  Returns out [batch, q_heads, dim], with
+        pages in ``table`` [batch, width] (int32), with ``window`` only over the last of them and
+        the first ``sinks`` (as `attend_chunk` does it).  Returns out [batch, q_heads, dim], with
         ``lse`` also the log sums [batch, q_heads] (float32).  scale: 1 / sqrt(dim) if None."""
+        if window is not None:
+            return self.attend_chunk(q, None, table, lengths, scale, window, sinks, out, lse)
         shape = q.shape
         if len(shape) != 3 or shape[2] != self.dim or shape[1] < 1 or shape[1] % self.kv_heads:
             _refuse("Paged attention: Q must be [batch, q_heads, dim], q_heads a multiple of kv_heads")
@@ -194,8 +262,62 @@ class PagedCache:
             self._workspace[stream, heads] = work
         return work
 
+    def attend_chunk(self, q, starts, table, lengths, scale: float | None = None, window: int | None = None,
+                     sinks: int = 0, out=None, lse: bool = False):
+        """Any number of new tokens of every request over its pages, which hold their rows already:
+        q [tokens, q_heads, dim] (float16 or bfloat16, the pages' type over 16-bit pages), rows
+        starts[b] .. starts[b + 1] (int32 [batch + 1]) the last tokens of the ``lengths`` [batch]
+        (int32) that the pages in ``table`` [batch, width] (int32) hold of request b; starts None: one
+        row each.  A row sees the tokens up to its own, with ``window`` the last so many of them, its own
+        included, and the first ``sinks``.  Rows that see nothing are zeros; rows that no
+        request holds are not written (of a new output they are whatever its memory held).  Any
+        strides of q with a contiguous last dimension; one whose strides or address are not
+        multiples of 16 bytes is copied.  Returns out [tokens, q_heads, dim], with ``lse`` also the
+        log sums [tokens, q_heads] (float32).  scale: 1 / sqrt(dim) if None."""
+        shape = q.shape
+        if len(shape) != 3 or shape[2] != self.dim or shape[1] < 1 or shape[1] % self.kv_heads:
+            _refuse("Chunk attention: Q must be [tokens, q_heads, dim], q_heads a multiple of kv_heads")
+        tokens, heads, _ = shape
+        if heads // self.kv_heads > 128:
+            _refuse("Chunk attention: at most 128 query heads for a KV head")
+        dtype, on = q.dtype, self._on
+        if dtype not in _HALF or self.format in _HALF.values() and self.format != _HALF[dtype]:
+            _refuse("Chunk attention: Q must be float16 or bfloat16, and of the type of 16-bit pages")
+        if q.device != on:
+            _refuse("Chunk attention: Q must be on the cache's device")
+        batch = tokens if starts is None else starts.shape[0] - 1 if starts.dim() == 1 else -1
+        if starts is not None and (batch < 0 or starts.dtype != torch.int32 or starts.device != on
+                                   or not starts.is_contiguous()):
+            _refuse("Chunk attention: starts must be int32 [batch + 1] on the cache's device")
+        if (table.dim() != 2 or table.shape[0] != batch or table.dtype != torch.int32 or table.device != on
+                or (table.shape[1] > 1 and table.stride(1) != 1)):
+            _refuse("Chunk attention: the table must be int32 [batch, width] on the cache's device")
+        if (lengths.dim() != 1 or lengths.shape[0] != batch or lengths.dtype != torch.int32 or lengths.device != on
+                or (batch > 1 and lengths.stride(0) != 1)):
+            _refuse("Chunk attention: lengths must be int32 [batch] on the cache's device")
+        if scale is not None and not 0.0 < scale < float("inf"):
+            _refuse("Chunk attention: scale must be positive and finite")
+        if window is not None and not 1 <= window < 2**31 or not 0 <= sinks < 2**31:
+            _refuse("Chunk attention: window must be positive and sinks nonnegative, both below 2^31")
+        if out is None:
+            out = q.new_empty(shape)
+        elif out.shape != shape or out.dtype != dtype or out.device != on or not out.is_contiguous():
+            _refuse("Chunk attention: out must be contiguous, of Q's shape, type and device")
+        sums = q.new_empty((tokens, heads), dtype=torch.float32) if lse else None
+        q, q0, q1 = _even(q)
+        st = _stream(self.device)
+        work = _chunk_work.get((self.device, self.dim, st)) or _chunk_workspace(self, heads, st)
+        p = _lib.ChunkDesc(_DTYPE[dtype], batch, heads, tokens, q.data_ptr(), q0, q1,
+                           None if starts is None else starts.data_ptr(), table.data_ptr(), table.stride(0),
+                           table.shape[1], lengths.data_ptr(), 0.0 if scale is None else max(scale, _LEAST_SCALE),
+                           window or 0, sinks, out.data_ptr(), sums.data_ptr() if lse else None, work[0], work[1])
+        status = self._chunk(self._ref, C.byref(p), st)
+        if status:
+            _lib.check(status)
+        return (out, sums) if lse else out
 
-_prompt_work = {}
+
+_prompt_work, _chunk_work = {}, {}
 
 
 def _prompt_workspace(device, dim: int, stream: int):
@@ -208,11 +330,21 @@ def _prompt_workspace(device, dim: int, stream: int):
     return work
 
 
+def _chunk_workspace(cache, heads: int, stream: int):
+    """The same for chunks over pages: one for all caches of a device and head dim."""
+    need = C.c_size_t()
+    _lib.call("bgtq_paged_chunk_workspace", cache._ref, heads, C.byref(need))
+    work = _room(need.value, cache._on)
+    if not _recording(cache._on):
+        _chunk_work[cache.device, cache.dim, stream] = work
+    return work
+
+
 def _ready_again(device: int):
-    """Zeroes the counters of the device's prompt workspaces: a call whose wait ran out ends without its joins.
-    (One-token attention waits for nothing, and a graph's own workspace is zeroed by its replays.)"""
+    """Zeroes the counters of the device's prompt and chunk workspaces: a call whose wait ran out ends without its
+    joins.  (One-token attention waits for nothing, and a graph's own workspace is zeroed by its replays.)"""
     torch.cuda.synchronize(device)
-    for (on, _, _), work in _prompt_work.items():
+    for (on, _, _), work in (*_prompt_work.items(), *_chunk_work.items()):
         if on == device:
             work[2][:_lib.WORKSPACE_ZEROED].zero_()
     torch.cuda.synchronize(device)
@@ -279,3 +411,92 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
     if status:
         _lib.check(status)
     return (out, sums) if lse else out
+
+
+def _per_row(x, batch: int, device, name: str):
+    """A penalty as float32 [batch]: a tensor as it is, a number filled in; None stays."""
+    if x is None:
+        return None
+    if not torch.is_tensor(x):
+        if not -float("inf") < x < float("inf") or name == "repetition" and x <= 0.0:
+            _refuse(f"Logits: {name} must be finite" + (" and positive" if name == "repetition" else ""))
+        return torch.full((batch,), float(x), dtype=torch.float32, device=device)
+    if x.shape != (batch,) or x.dtype != torch.float32 or x.device != device or not x.is_contiguous():
+        _refuse(f"Logits: {name} must be a number or a contiguous float32 tensor [batch] on the logits' device")
+    return x
+
+
+def _rows(t, batch: int, device, name: str, shape: str):
+    """The row stride of [batch or 1, n] (one row for all: 0)."""
+    if t.dim() != 2 or t.shape[0] not in (1, batch) or t.device != device or t.shape[1] > 1 and t.stride(1) != 1:
+        _refuse(f"Logits: {name} must be {shape} on the logits' device, with a contiguous last dimension")
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def adjust_logits(logits, tokens=None, lengths=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                  bias=None, mask=None, out=None):
+    """Penalties for repeated tokens, biases and a grammar's mask on logits [batch, vocab] (float16, bfloat16 or
+    float32), in this order, where they are given; FP32 within, rounded once:
+
+        repetition   x / repetition if x > 0, else x * repetition   for tokens of the row's history
+        presence     x - presence                                   for tokens of the row's history
+        frequency    x - frequency * (how often the history has the token)
+        bias         x + bias[b, j] for token bias_ids[b, j]        (one that comes twice is added twice)
+        mask         -inf where bit v % 32 of mask[b, v // 32] is not set
+
+    The history of row b is the first lengths[b] (int32 [batch]; None: all) of tokens [batch, width] (int32 or
+    int64), negative ones left out.  Penalties are numbers or float32 [batch]; repetition is positive.  bias_ids (int32) and bias
+    (float32) are [batch, n] or, for all rows alike, [1, n]; mask (int32, the bits of 32 tokens a word) [batch,
+    ceil(vocab / 32)] or [1, ...].  Token ids past the vocabulary are left out and set bit 4 of `device_status`, lengths
+    outside 0 .. width are cut and set bit 8.  Returns the result, a new tensor or ``out`` (which may be logits)."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        _refuse("Logits: logits must be a CUDA tensor [batch, vocab] with a contiguous last dimension")
+    batch, vocab = logits.shape
+    dtype, on = _DTYPE.get(logits.dtype), logits.device
+    if dtype is None:
+        _refuse("Logits: logits must be float16, bfloat16 or float32")
+    tokens_stride = width = 0
+    if tokens is not None:
+        if (tokens.dim() != 2 or tokens.shape[0] != batch or tokens.dtype not in (torch.int32, torch.int64)
+                or tokens.device != on or tokens.shape[1] > 1 and tokens.stride(1) != 1):
+            _refuse("Logits: tokens must be int32 or int64 [batch, width] on the logits' device, with a contiguous "
+                    "last dimension")
+        tokens_stride, width = tokens.stride(0), tokens.shape[1]
+    if lengths is not None and (tokens is None or lengths.shape != (batch,) or lengths.dtype != torch.int32
+                                or lengths.device != on or not lengths.is_contiguous()):
+        _refuse("Logits: lengths must be a contiguous int32 tensor [batch] on the logits' device, with tokens")
+    if tokens is None and not repetition is presence is frequency is None:
+        _refuse("Logits: penalties need tokens")
+    repetition, presence, frequency = (_per_row(x, batch, on, n) for x, n in (
+        (repetition, "repetition"), (presence, "presence"), (frequency, "frequency")))
+    bias_stride = mask_stride = entries = 0
+    if (bias is None) != (bias_ids is None):
+        _refuse("Logits: bias and bias_ids come together")
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias_ids.dtype != torch.int32 or bias.shape != bias_ids.shape:
+            _refuse("Logits: bias must be float32 and bias_ids int32, of one shape")
+        bias_stride = _rows(bias, batch, on, "bias", "[batch, n] or [1, n]")
+        if _rows(bias_ids, batch, on, "bias_ids", "[batch, n] or [1, n]") != bias_stride:
+            bias, bias_ids = bias.contiguous(), bias_ids.contiguous()
+            bias_stride = bias.shape[1] if bias.shape[0] > 1 else 0
+        entries = bias.shape[1]
+    if mask is not None:
+        mask_stride = _rows(mask, batch, on, "mask", "[batch, ceil(vocab / 32)] or [1, ceil(vocab / 32)]")
+        if mask.dtype != torch.int32 or mask.shape[1] != (vocab + 31) // 32:
+            _refuse("Logits: mask must be int32, a bit for each token of the vocabulary")
+    if out is None:
+        out = logits.new_empty((batch, vocab))
+    elif (out.shape != logits.shape or out.dtype != logits.dtype or out.device != on
+          or out.stride(1) != 1 and vocab > 1 or batch > 1 and out.stride(0) < vocab):
+        _refuse("Logits: out must be of the logits' shape, type and device, with a contiguous last dimension")
+    p = _lib.LogitsDesc(on.index, dtype, batch, vocab, logits.data_ptr(), logits.stride(0),
+                        None if tokens is None else tokens.data_ptr(), tokens_stride, width,
+                        8 if tokens is not None and tokens.dtype == torch.int64 else 4,
+                        *(None if t is None else t.data_ptr()
+                          for t in (lengths, repetition, presence, frequency, bias_ids, bias)),
+                        bias_stride, entries, None if mask is None else mask.data_ptr(), mask_stride, out.data_ptr(),
+                        out.stride(0))
+    status = _lib.lib().bgtq_adjust_logits(C.byref(p), _stream(on.index))
+    if status:
+        _lib.check(status)
+    return out

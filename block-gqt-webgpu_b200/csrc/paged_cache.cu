@@ -16,73 +16,12 @@
 // for one at each issue), then issue (2 of 3 cycles; about twelve instructions an element, half of them the
 // quotient and its code).
 // 16 tokens of 3 heads: 3.3 us, two launches' latency.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "serving.h"
+#include "paged_rows.cuh"
 
 namespace bgtq {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-
-template <int F> struct Format {  // a stored row
-    static constexpr bool kCodes = F == BGTQ_PAGES_INT8 || F == BGTQ_PAGES_INT4;
-    static constexpr int kBytes = F == BGTQ_PAGES_INT4 ? 4 : F == BGTQ_PAGES_INT8 ? 8 : 16;  // of eight dimensions
-};
-template <int T> struct Element {
-    static constexpr int kBytes = T == BGTQ_F32 ? 4 : 2;
-};
-
-template <int T>
-__device__ __forceinline__ float to_float(uint32_t bits) {
-    if constexpr (T == BGTQ_F32) return __uint_as_float(bits);
-    else if constexpr (T == BGTQ_F16) return __half2float(__ushort_as_half((unsigned short)bits));
-    else return __uint_as_float(bits << 16);
-}
-template <int T>
-__device__ __forceinline__ uint32_t from_float(float x) {
-    if constexpr (T == BGTQ_F32) return __float_as_uint(x);
-    else if constexpr (T == BGTQ_F16) return __half_as_ushort(__float2half_rn(x));
-    else return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-}
-
-// Eight elements of type T as they lie in memory; V: loaded by 16 bytes.
-template <int T> struct Eight {
-    static constexpr int kWords = Element<T>::kBytes / 2;
-    uint4 w[kWords];
-    template <bool V>
-    __device__ __forceinline__ void load(const void *p) {
-        if constexpr (V) {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = __ldg(static_cast<const uint4 *>(p) + i);
-        } else {
-            uint32_t *u = reinterpret_cast<uint32_t *>(w);
-#pragma unroll
-            for (int i = 0; i < 4 * kWords; ++i) {
-                if constexpr (T == BGTQ_F32) u[i] = static_cast<const uint32_t *>(p)[i];
-                else u[i] = static_cast<const uint16_t *>(p)[2 * i] | (uint32_t)static_cast<const uint16_t *>(p)[2 * i + 1] << 16;
-            }
-        }
-    }
-    __device__ __forceinline__ void floats(float (&x)[8]) const {
-        const uint32_t *u = reinterpret_cast<const uint32_t *>(w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_float<T>(T == BGTQ_F32 ? u[i] : u[i / 2] >> 16 * (i & 1) & 0xffffu);
-    }
-};
-template <int T>
-__device__ __forceinline__ void store8(void *p, const float (&x)[8]) {
-    constexpr int N = Element<T>::kBytes / 2;
-    uint32_t u[4 * N];
-#pragma unroll
-    for (int i = 0; i < 4 * N; ++i) {
-        if constexpr (T == BGTQ_F32) u[i] = from_float<T>(x[i]);
-        else u[i] = from_float<T>(x[2 * i]) | from_float<T>(x[2 * i + 1]) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) static_cast<uint4 *>(p)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-}
 
 // Eight dimensions of a row into the pages.  All lanes of a row come here together.
 template <int F, int D, int T>
@@ -94,7 +33,6 @@ __device__ __forceinline__ void put(unsigned char *rows, uint16_t *scales, uint6
     if constexpr (!Format<F>::kCodes) {
         store8<F == BGTQ_PAGES_F16 ? BGTQ_F16 : BGTQ_BF16>(dst, x);
     } else {
-        constexpr float kTop = F == BGTQ_PAGES_INT4 ? 7.0f : 127.0f;
         constexpr uint32_t kLanes = F == BGTQ_PAGES_INT4 ? kInt4Group / 8 : D / 8;  // that share a scale
         // as bits, |x| orders like a whole number with NaN above infinity, so the maximum keeps both; elements of 16
         // bits go two at a time
@@ -112,50 +50,8 @@ __device__ __forceinline__ void put(unsigned char *rows, uint16_t *scales, uint6
             for (uint32_t w = 1; w < kLanes; w <<= 1) m = __vmaxs2(m, __shfl_xor_sync(lanes, m, w));
             m = __float_as_uint(to_float<T>(max(m & 0xffffu, m >> 16)));
         }
-        const bool fine = m < 0x7f800000u;
-        // one product with the rounded 1 / top: at most an ulp of FP32 from the quotient, and the scale keeps 8 bits
-        // of it (about one scale in 2^17 lands on the other side of a BF16 tie; every code and value goes by the
-        // scale that is stored)
-        const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__uint_as_float(m), 1.0f / kTop));
-        const float s = __bfloat162float(sb);
-        // Codes in the low bits of q + 1.5 * 2^23, which rounds q to the nearest whole number, ties to even (the
-        // conversion instructions run at a quarter of the rate).
-        constexpr uint32_t kRound = 0x4b400000u;
-        uint32_t c[8];
-        if (fine && s > 1e-30f && s < 1e30f) {
-            // x / s, correctly rounded: one correctly rounded reciprocal y, then q = q0 + (x - s q0) y with q0 = x y
-            // (Markstein, IBM J. Res. Dev. 34(1), 1990: q is the IEEE quotient where nothing over- or underflows;
-            // quotients are below 128 here).  |q| <= top (1 + 2^-8) rounds to top at most: no clamp.
-            const float2 y = make_float2(__frcp_rn(s), __frcp_rn(s)), minus = make_float2(-s, -s);
-            const float2 round = make_float2(__uint_as_float(kRound), __uint_as_float(kRound));
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float2 v = make_float2(x[i], x[i + 1]), q = __fmul2_rn(v, y);
-                const float2 z = __fadd2_rn(__ffma2_rn(__ffma2_rn(minus, q, v), y, q), round);
-                c[i] = __float_as_uint(z.x), c[i + 1] = __float_as_uint(z.y);
-            }
-        } else {  // scales near the ends of the exponent range, zero and NaN
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float q = fine && s > 0.0f ? fminf(fmaxf(__fdiv_rn(x[i], s), -kTop), kTop) : 0.0f;
-                c[i] = __float_as_uint(__fadd_rn(q, __uint_as_float(kRound)));
-            }
-        }
-        // The codes' places are added up: a word starts with the codes' offset (8 or 128, which makes them
-        // nonnegative) in every place, less what kRound adds up to.
-        constexpr uint32_t kBits = F == BGTQ_PAGES_INT4 ? 4 : 8, kEach = 32 / kBits;
-        constexpr uint32_t kOffsets = F == BGTQ_PAGES_INT4 ? 0x88888888u : 0x80808080u;
-        constexpr uint32_t kStart = kOffsets - kRound * (1u + (1u << kBits) + (1u << 2 * kBits));  // further places shift it out
-        uint32_t u[8 / kEach];
-#pragma unroll
-        for (uint32_t w = 0; w < 8 / kEach; ++w) {
-            u[w] = kStart;
-#pragma unroll
-            for (uint32_t i = 0; i < kEach; ++i) u[w] += c[kEach * w + i] << kBits * i;
-        }
-        if constexpr (F == BGTQ_PAGES_INT4) *reinterpret_cast<uint32_t *>(dst) = u[0];
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(u[0] ^ kOffsets, u[1] ^ kOffsets);
-        if (part % kLanes == 0) scales[(r * (D / 8) + part) / kLanes] = fine ? __bfloat16_as_ushort(sb) : 0x7fffu;
+        const uint32_t sb = encode<F>(dst, x, m);
+        if (part % kLanes == 0) scales[(r * (D / 8) + part) / kLanes] = (uint16_t)sb;
     }
 }
 // Eight dimensions of a stored row as the values that they stand for (2^23 + u is 0x4b000000 | u).
@@ -235,22 +131,16 @@ __global__ void __launch_bounds__(kThreads) read_rows_kernel(const PagedReadArgs
     if constexpr (kBoth) store8<T>(static_cast<char *>(a.v) + i * 8 * B, v);
 }
 
-bool even(const void *p, int64_t token, int64_t head, int bytes) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && token * bytes % 16 == 0 && head * bytes % 16 == 0;
-}
 // From about a wave of threads on, a thread takes K and V, and shares the slot and the address between them (16K
 // tokens of 8 heads of 128 in 4 bits, written and read: 42.3 us, 50.4 with threads of their own); below it, threads
 // of their own end sooner (4999 tokens of 2 heads of 64 in 8 bits from FP32: 5.8 us, 6.2 with both).
 constexpr uint64_t kMany = 1u << 18;
 
-// row / heads by one product: m = ceil(2^(31 + l) / heads), 2^l >= heads, is exact for rows below 2^31, which the
-// entry points see to.  One head needs none.
 template <typename Args>
 Args divided(Args a) {
-    uint32_t l = 0;
-    while (1u << l < a.c.heads) ++l;
-    a.head_mul = l ? (uint32_t)(((1ull << (31 + l)) + a.c.heads - 1) / a.c.heads) : 0;
-    a.head_shift = l ? l - 1 : 0;
+    const Divisor d = divisor(a.c.heads);
+    a.head_mul = d.mul;
+    a.head_shift = d.shift;
     return a;
 }
 

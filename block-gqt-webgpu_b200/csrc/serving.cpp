@@ -1,5 +1,5 @@
-// C ABI of the serving operators (paged cache, one-token attention over its pages, packed
-// prompt attention): argument checks before anything is launched, then one launcher each.
+// C ABI of the serving operators (paged cache, one-token and chunk attention over its pages, packed
+// prompt attention, what is put on logits): argument checks before anything is launched, then one launcher each.
 #include <cmath>
 #include <string>
 
@@ -174,6 +174,158 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
     a.width = table_width;
     a.dtype = dtype;
     return launched(launch_paged_attend(a, static_cast<cudaStream_t>(stream)), "Paged attention");
+}
+
+bgtq_status bgtq_paged_append(const bgtq_paged_cache *c, const bgtq_append *p, void *stream) {
+    AppendArgs a{};
+    if (bgtq_status s = view(c, a.c)) return s;
+    if (!p) return refuse("Paged append: null");
+    if (p->dtype < BGTQ_F16 || p->dtype > BGTQ_BF16) return refuse("Paged append: source must be FP16, BF16 or FP32");
+    if (p->out_dtype < BGTQ_F16 || p->out_dtype > BGTQ_BF16) return refuse("Paged append: output must be FP16, BF16 or FP32");
+    if (p->q_heads < 1 || p->q_heads > 65535u) return refuse("Paged append: invalid head count");
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return refuse("Paged append: eps must be nonnegative and finite");
+    if (p->tokens == 0) return BGTQ_OK;
+    if (!p->q || !p->k || !p->v || !p->slots || !p->rotary || !p->q_out) return refuse("Paged append: null argument");
+    const size_t w = width_of(p->dtype);
+    if (!aligned(p->q, w) || !aligned(p->k, w) || !aligned(p->v, w) || !aligned(p->slots, 8) || !aligned(p->positions, 8) ||
+        !aligned(p->rotary, 16) || !aligned(p->q_norm, 16) || !aligned(p->k_norm, 16) || !aligned(p->q_out, 16) ||
+        !aligned(p->k_out, 16))
+        return refuse("Paged append: misaligned argument");
+    if (p->tokens > 0x7fffffffull / (p->q_heads + 2 * c->kv_heads)) return refuse("Paged append: too many rows in one call");
+    if (p->rotary_rows > 0x7fffffffull || (!p->positions && p->rotary_rows < p->tokens))
+        return refuse("Paged append: a row of cosines and sines for every token, 2^31 - 1 at most");
+    OnDevice on(c->device);
+    a.status = on.ok ? device_status_word(c->device) : nullptr;
+    if (!a.status) return launched(cudaErrorInvalidDevice, "Paged append");
+    a.q = p->q;
+    a.k = p->k;
+    a.v = p->v;
+    a.q_token = p->q_token_stride;
+    a.q_head = p->q_head_stride;
+    a.k_token = p->k_token_stride;
+    a.k_head = p->k_head_stride;
+    a.v_token = p->v_token_stride;
+    a.v_head = p->v_head_stride;
+    a.slots = p->slots;
+    a.positions = p->positions;
+    a.rotary = p->rotary;
+    a.rotary_rows = p->rotary_rows;
+    a.q_norm = p->q_norm;
+    a.k_norm = p->k_norm;
+    a.tokens = p->tokens;
+    a.q_out = p->q_out;
+    a.k_out = p->k_out;
+    a.eps = p->eps;
+    a.q_heads = p->q_heads;
+    a.dtype = p->dtype;
+    a.out_dtype = p->out_dtype;
+    return launched(launch_append(a, static_cast<cudaStream_t>(stream)), "Paged append");
+}
+
+bgtq_status bgtq_paged_chunk_workspace(const bgtq_paged_cache *c, uint32_t q_heads, size_t *bytes) {
+    PageView v{};
+    if (bgtq_status s = view(c, v)) return s;
+    if (!bytes || !q_heads || q_heads % c->kv_heads || q_heads / c->kv_heads > 128)
+        return refuse("Chunk attention: invalid head count");
+    OnDevice on(c->device);
+    const size_t need = on.ok ? chunk_workspace(v, q_heads) : 0;
+    if (!need) return launched(cudaErrorInvalidDevice, "Chunk attention");
+    *bytes = need;
+    return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_attend_chunk(const bgtq_paged_cache *c, const bgtq_chunk *p, void *stream) {
+    ChunkArgs a{};
+    if (bgtq_status s = view(c, a.c)) return s;
+    if (!p) return refuse("Chunk attention: null");
+    if (p->dtype != BGTQ_F16 && p->dtype != BGTQ_BF16) return refuse("Chunk attention: queries must be FP16 or BF16");
+    if ((c->format == BGTQ_PAGES_F16 && p->dtype != BGTQ_F16) || (c->format == BGTQ_PAGES_BF16 && p->dtype != BGTQ_BF16))
+        return refuse("Chunk attention: queries must have the type of 16-bit pages");
+    if (!p->q_heads || p->q_heads % c->kv_heads || p->q_heads / c->kv_heads > 128)
+        return refuse("Chunk attention: invalid head count");
+    if (!logit_scale(p->scale, c->dim, a.scale)) return refuse("Chunk attention: scale must be positive and finite");
+    if (p->window > 0x7fffffffu || p->sinks > 0x7fffffffu) return refuse("Chunk attention: window and sinks must be below 2^31");
+    if (p->batch > 65535u || p->q_tokens > 0x7fffffffull / p->q_heads)
+        return refuse("Chunk attention: too many requests or tokens in one call");
+    if (!p->starts && p->q_tokens != p->batch) return refuse("Chunk attention: one query row for every request without starts");
+    if (p->batch == 0 || p->q_tokens == 0) return BGTQ_OK;
+    if (!p->q || !p->lengths || !p->out || (!p->table && p->table_width)) return refuse("Chunk attention: null argument");
+    if ((uint64_t)p->table_width * c->page_size > 0x7fffffffull)
+        return refuse("Chunk attention: a table row must cover fewer than 2^31 tokens");
+    if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->starts, 4) || !aligned(p->table, 4) ||
+        !aligned(p->lengths, 4) || !aligned(p->lse, 4))
+        return refuse("Chunk attention: misaligned argument");
+    for (int64_t s : {p->q_token_stride, p->q_head_stride})
+        if (s <= 0 || s % 8 || s >= (int64_t)1 << 39)
+            return refuse("Chunk attention: strides must be positive multiples of 16 bytes");
+    OnDevice on(c->device);
+    a.status = on.ok ? device_status_word(c->device) : nullptr;
+    if (!a.status) return launched(cudaErrorInvalidDevice, "Chunk attention");
+    const size_t need = chunk_workspace(a.c, p->q_heads);
+    if (!need) return launched(cudaErrorInvalidDevice, "Chunk attention");
+    if (!p->workspace || p->workspace_bytes < need || !aligned(p->workspace, 128))
+        return refuse("Chunk attention: the workspace is too small or misaligned");
+    a.q = p->q;
+    a.q_token = p->q_token_stride;
+    a.q_head = p->q_head_stride;
+    a.starts = p->starts;
+    a.table = p->table;
+    a.table_stride = p->table_stride;
+    a.lengths = p->lengths;
+    a.out = p->out;
+    a.lse = p->lse;
+    a.workspace = p->workspace;
+    a.q_tokens = p->q_tokens;
+    a.batch = p->batch;
+    a.q_heads = p->q_heads;
+    a.group = p->q_heads / c->kv_heads;
+    a.width = p->table_width;
+    a.window = p->window;
+    a.sinks = p->sinks;
+    a.dtype = p->dtype;
+    return launched(launch_chunk(a, static_cast<cudaStream_t>(stream)), "Chunk attention");
+}
+
+bgtq_status bgtq_adjust_logits(const bgtq_logits *p, void *stream) {
+    if (!p) return refuse("Logits: null");
+    if (p->dtype < BGTQ_F16 || p->dtype > BGTQ_BF16) return refuse("Logits: logits must be FP16, BF16 or FP32");
+    if (p->vocab < 1 || p->vocab > 0x7fffffffu) return refuse("Logits: invalid vocabulary");
+    if (p->batch > 65535u) return refuse("Logits: too many rows in one call");
+    if (p->width > 0x7fffffffu || p->entries > 0x7fffffffu) return refuse("Logits: too many tokens or biases in a row");
+    if (p->tokens && p->id_bytes != 4 && p->id_bytes != 8) return refuse("Logits: token ids must have 4 or 8 bytes");
+    if (p->batch == 0) return BGTQ_OK;
+    if (!p->logits || !p->out || (!p->bias) != (!p->bias_ids)) return refuse("Logits: null argument");
+    const size_t w = width_of(p->dtype);
+    if (!aligned(p->logits, w) || !aligned(p->out, w) || !aligned(p->tokens, p->tokens ? p->id_bytes : 1) ||
+        !aligned(p->lengths, 4) || !aligned(p->repetition, 4) || !aligned(p->presence, 4) || !aligned(p->frequency, 4) ||
+        !aligned(p->bias_ids, 4) || !aligned(p->bias, 4) || !aligned(p->mask, 4))
+        return refuse("Logits: misaligned argument");
+    OnDevice on(p->device);
+    LogitsArgs a{};
+    a.status = on.ok ? device_status_word(p->device) : nullptr;
+    if (!a.status) return launched(cudaErrorInvalidDevice, "Logits");
+    a.logits = p->logits;
+    a.logits_stride = p->logits_stride;
+    a.tokens = p->width ? p->tokens : nullptr;
+    a.tokens_stride = p->tokens_stride;
+    a.width = p->width;
+    a.id_bytes = p->id_bytes;
+    a.lengths = p->lengths;
+    a.repetition = p->repetition;
+    a.presence = p->presence;
+    a.frequency = p->frequency;
+    a.bias_ids = p->entries ? p->bias_ids : nullptr;
+    a.bias = p->entries ? p->bias : nullptr;
+    a.bias_stride = p->bias_stride;
+    a.entries = p->entries;
+    a.mask = p->mask;
+    a.mask_stride = p->mask_stride;
+    a.out = p->out;
+    a.out_stride = p->out_stride;
+    a.batch = p->batch;
+    a.vocab = p->vocab;
+    a.dtype = p->dtype;
+    return launched(launch_logits(a, static_cast<cudaStream_t>(stream)), "Logits");
 }
 
 bgtq_status bgtq_prompt_workspace(int device, uint32_t dim, size_t *bytes) {

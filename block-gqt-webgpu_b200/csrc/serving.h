@@ -1,5 +1,6 @@
-// Kernel arguments and launchers of the serving operators: the paged cache's write and read,
-// one-token attention over its pages, and packed prompt attention.
+// Kernel arguments and launchers of the serving operators: the paged cache's write and read, new
+// tokens rotated into it, one-token and chunk attention over its pages, packed prompt attention,
+// and what is put on logits.
 #pragma once
 
 #include <cstddef>
@@ -82,6 +83,53 @@ struct PromptArgs {
     uint32_t *status;
 };
 
+struct AppendArgs {
+    PageView c;
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // element strides
+    const int64_t *slots, *positions;                            // positions nullable
+    const float *rotary, *q_norm, *k_norm;                       // norms nullable
+    uint64_t rotary_rows, tokens;
+    void *q_out, *k_out;  // dense; k_out nullable
+    float eps;
+    uint32_t q_heads;
+    bgtq_dtype dtype, out_dtype;
+    uint32_t *status;
+    uint32_t rows_mul, rows_shift;  // the launcher's: row / (q_heads + 2 heads), for the kernels
+};
+
+struct ChunkArgs {
+    PageView c;
+    const void *q;
+    int64_t q_token, q_head;  // element strides
+    const int32_t *starts;    // [batch + 1]; null: one row each
+    const int32_t *table;
+    int64_t table_stride;
+    const int32_t *lengths;
+    void *out;
+    float *lse;  // nullable
+    void *workspace;
+    uint64_t q_tokens;
+    uint32_t batch, q_heads, group, width;
+    uint32_t window, sinks;  // window 0: none
+    float scale;             // of the logits, times log2(e)
+    bgtq_dtype dtype;
+    uint32_t *status;
+};
+
+struct LogitsArgs {
+    const void *logits, *tokens;
+    const int32_t *lengths, *bias_ids;
+    const float *repetition, *presence, *frequency, *bias;
+    const uint32_t *mask;
+    void *out;
+    int64_t logits_stride, tokens_stride, bias_stride, mask_stride, out_stride;
+    uint32_t batch, vocab, width, id_bytes, entries;
+    uint32_t slice;  // the launcher's: ids of a CTA
+    bgtq_dtype dtype;
+    uint32_t *status;
+};
+
 cudaError_t launch_paged_write(const PagedWriteArgs &a, cudaStream_t s);
 cudaError_t launch_paged_read(const PagedReadArgs &a, cudaStream_t s);
 // Bytes of the workspace that launch_paged_attend needs (counters first, zero between calls).
@@ -90,6 +138,12 @@ cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t s);
 // Bytes of the workspace that launch_prompt needs (counters first, zero between calls).
 size_t prompt_workspace(uint32_t dim);
 cudaError_t launch_prompt(const PromptArgs &a, cudaStream_t s);
+
+cudaError_t launch_append(const AppendArgs &a, cudaStream_t s);
+// Bytes of the workspace that launch_chunk needs (counters first, zero between calls).
+size_t chunk_workspace(const PageView &c, uint32_t q_heads);
+cudaError_t launch_chunk(const ChunkArgs &a, cudaStream_t s);
+cudaError_t launch_logits(const LogitsArgs &a, cudaStream_t s);
 
 // SMs of a device (0: no such device), asked for once.
 inline int sm_count(int device) {

@@ -516,6 +516,70 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
                               int64_t table_stride, uint32_t table_width, const int32_t *lengths, float scale,
                               void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
+/* New tokens into the pages, rotated on the way.  Of queries q and keys k every head x is, in this order,
+ *   normed    where q_norm / k_norm is given: x_i norm[i] / sqrt(mean(x^2) + eps)
+ *   rotated   (x_i, x_{i + dim/2}) -> (x_i c_i - x_{i + dim/2} s_i, x_{i + dim/2} c_i + x_i s_i), c and s the
+ *             first and the second half of the token's row of `rotary`
+ * and keys and values are stored at the token's slot as bgtq_paged_write stores rows, queries (and, where k_out is
+ * given, keys) written to dense outputs.  Element (t, h, i) of q is at q[t * q_token_stride + h * q_head_stride + i]
+ * of dtype (F16, BF16 or F32), k and v the same.  Rows of 8- and 4-bit pages are normed and rotated in 64 bits and
+ * rounded to FP32 once before they are quantised, so their codes are the formula's; all else is FP32.  A negative
+ * slot is padding: its outputs are written, its rows are not stored.  Slots of one call are distinct.  A slot past the
+ * last page is not stored; a token whose position is outside the table is not stored and its outputs are zeros; both
+ * set a bit of the device status word. */
+typedef struct bgtq_append {
+    bgtq_dtype dtype;
+    uint32_t q_heads; /* any number, 1 to 65535 */
+    uint64_t tokens;
+    const void *q, *k, *v;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int64_t *slots;     /* [tokens] */
+    const float *rotary;      /* [rotary_rows][dim], 16-byte aligned: cosines, then sines, of dim / 2 pairs */
+    uint64_t rotary_rows;
+    const int64_t *positions; /* [tokens] rows of rotary; null: token t has row t */
+    const float *q_norm, *k_norm; /* [dim], 16-byte aligned, or null */
+    float eps;                /* nonnegative */
+    bgtq_dtype out_dtype;     /* F16, BF16 or F32 */
+    void *q_out;              /* dense [tokens][q_heads][dim] of out_dtype, 16-byte aligned */
+    void *k_out;              /* dense [tokens][kv_heads][dim] of out_dtype, 16-byte aligned, or null */
+} bgtq_append;
+bgtq_status bgtq_paged_append(const bgtq_paged_cache *c, const bgtq_append *p, void *stream);
+
+/* A chunk of new tokens of every request over its pages, which hold their rows already:
+ *     out[i][h] = sum_t softmax_t(scale q[i][h].k_t) v_t
+ * Request b has query rows starts[b] .. starts[b + 1] (device int32 [batch + 1], ascending; null: row b is its only
+ * one) and its pages lengths[b] tokens, of which its n query rows are the last n: row i of them is at position
+ * p = lengths[b] - n + i and sees the tokens t <= p, with a window only those of p - window < t and those of
+ * t < sinks.  A row that sees nothing gives zeros and -inf; query rows that no request holds are not written.  Starts
+ * that fall or pass q_tokens set a status bit and their request is skipped.  dtype, table, lengths, scale, out and lse
+ * are bgtq_paged_attend's; of the table only entries of tokens that a row sees are followed (others may be read, and
+ * need only be readable).  An infinity among the values of 16-bit pages gives infinity to rows that see it, or NaN where
+ * its probability is below what 16 bits hold.  Pointers to q and out are 16-byte aligned, q's strides positive
+ * multiples of 8 elements; q_heads / kv_heads <= 128. */
+typedef struct bgtq_chunk {
+    bgtq_dtype dtype;
+    uint32_t batch, q_heads;
+    uint64_t q_tokens;
+    const void *q;
+    int64_t q_token_stride, q_head_stride;
+    const int32_t *starts;
+    const int32_t *table;   /* [batch] rows of table_width page indices, table_stride apart */
+    int64_t table_stride;
+    uint32_t table_width;
+    const int32_t *lengths; /* [batch] */
+    float scale;            /* of the logits, positive (0: 1 / sqrt(dim)) */
+    uint32_t window;        /* tokens that a row sees up to its own, at most 2^31 - 1; 0: all */
+    uint32_t sinks;         /* first tokens that a window leaves visible, at most 2^31 - 1 */
+    void *out;              /* dense [q_tokens][q_heads][dim] of dtype */
+    float *lse;             /* [q_tokens][q_heads] FP32, or null */
+    void *workspace;        /* 128-byte aligned; as for bgtq_prompt */
+    size_t workspace_bytes;
+} bgtq_chunk;
+/* Bytes of workspace that bgtq_paged_attend_chunk needs: the same for all caches of a head dim, whatever the head
+ * count and the batch. */
+bgtq_status bgtq_paged_chunk_workspace(const bgtq_paged_cache *c, uint32_t q_heads, size_t *bytes);
+bgtq_status bgtq_paged_attend_chunk(const bgtq_paged_cache *c, const bgtq_chunk *p, void *stream);
+
 /* Packed prompts: queries q_tokens x q_heads x dim, keys and values k_tokens x kv_heads x
  * dim, all of dtype (F16 or BF16), element (t, h, i) at t * token_stride + h * head_stride
  * + i.  Sequence s holds query rows starts[s] .. starts[s + 1] and key rows key_starts[s] ..
@@ -547,6 +611,39 @@ typedef struct bgtq_prompt {
 /* Bytes of workspace that bgtq_prompt_attend needs for a head dim, whatever the batch. */
 bgtq_status bgtq_prompt_workspace(int device, uint32_t dim, size_t *bytes);
 bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream);
+
+/* Penalties, biases and a mask on logits, before a token is chosen.  Of row b and token v, with c the number of
+ * times that v is among the first lengths[b] tokens of the row's history, x = logits[b][v] becomes, in FP32,
+ *   x / repetition if x > 0, else x * repetition       where c > 0
+ *   x - presence                                       where c > 0
+ *   x - frequency * c
+ *   x + bias[j] for every j with bias_ids[b][j] = v, in their order
+ *   -inf                                               where bit v % 32 of mask[b][v / 32] is 0
+ * each step where its arguments are given (null arrays and a repetition of 1, a presence and a frequency of 0 leave x as
+ * it is), and is rounded to dtype once.  Token ids are int32 or int64 (id_bytes 4 or 8); negative ones are padding, ones
+ * past the vocabulary are left out and set a bit of the device status word, as does a length below 0 or past width,
+ * which is cut.  out may be logits. */
+typedef struct bgtq_logits {
+    int device;
+    bgtq_dtype dtype;       /* F16, BF16 or F32 */
+    uint32_t batch, vocab;
+    const void *logits;     /* [batch][vocab], rows logits_stride elements apart */
+    int64_t logits_stride;
+    const void *tokens;     /* [batch][width] ids, rows tokens_stride elements apart, or null */
+    int64_t tokens_stride;
+    uint32_t width, id_bytes;
+    const int32_t *lengths; /* [batch], or null: width */
+    const float *repetition, *presence, *frequency; /* [batch], or null: 1, 0, 0 */
+    const int32_t *bias_ids; /* [batch][entries], rows bias_stride elements apart (0: one row for all), or null */
+    const float *bias;
+    int64_t bias_stride;
+    uint32_t entries;
+    const uint32_t *mask;   /* [batch][(vocab + 31) / 32], rows mask_stride words apart (0: one row for all), or null */
+    int64_t mask_stride;
+    void *out;              /* [batch][vocab] of dtype, rows out_stride elements apart */
+    int64_t out_stride;
+} bgtq_logits;
+bgtq_status bgtq_adjust_logits(const bgtq_logits *p, void *stream);
 
 /* Device status word written by kernels (0 = fine); reading it synchronises. */
 bgtq_status bgtq_device_status(int device, uint32_t *status_out);
