@@ -112,6 +112,7 @@ struct ChunkArgs {
     uint64_t q_tokens;
     uint32_t batch, q_heads, group, width;
     uint32_t window, sinks;  // window 0: none
+    uint32_t counters;       // the launcher's: bytes of the workspace's counters
     float scale;             // of the logits, times log2(e)
     bgtq_dtype dtype;
     uint32_t *status;
