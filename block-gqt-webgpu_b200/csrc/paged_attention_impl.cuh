@@ -1119,7 +1119,8 @@ cudaError_t run(const std::conditional_t<C, ChunkArgs, PagedAttendArgs> &a, cuda
     const int sms = sm_count(dev);
     if (!sms) return cudaErrorInvalidDevice;
     auto b = a;
-    b.counters = counter_bytes();
+    // (chunks share their workspace with the kernel of many rows: both keep their counters in the bytes that start from zero)
+    b.counters = C ? BGTQ_WORKSPACE_ZEROED : counter_bytes();
     // queries by 16 bytes where they lie so, else by elements (32 requests of 4096 tokens, 16 / 1 heads: 29.5, 30.7 us)
     if constexpr (!C) b.q_even = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_batch % 8 == 0 && a.q_head % 8 == 0;
     kernel<<<(uint32_t)(sms * resident[dev]), kThreads, S::kSmem, s>>>(b);

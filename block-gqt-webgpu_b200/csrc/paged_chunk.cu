@@ -14,11 +14,15 @@ cudaError_t by_shape(const ChunkArgs &a, cudaStream_t s) {
 
 }  // namespace
 
-size_t chunk_workspace(const PageView &c, uint32_t) { return counter_bytes() + 2ull * most_ctas() * 16u * (c.dim + 2) * 4; }
+size_t chunk_workspace(const PageView &c, uint32_t) {
+    const size_t few = BGTQ_WORKSPACE_ZEROED + 2ull * most_ctas() * 16u * (c.dim + 2) * 4, many = paged_prompt_workspace(c.dim);
+    return !many ? 0 : few > many ? few : many;
+}
 
 cudaError_t launch_chunk(const ChunkArgs &args, cudaStream_t s) {
     ChunkArgs a = args;
     if (a.window >= (uint64_t)a.width << a.c.page_shift) a.window = 0;  // all tokens that the table holds
+    if (a.q_tokens * a.group > 16ull * a.batch) return launch_paged_prompt(a, s);
     switch (a.c.format) {
         case BGTQ_PAGES_F16: return by_shape<F_F16>(a, s);
         case BGTQ_PAGES_BF16: return by_shape<F_BF16>(a, s);

@@ -113,6 +113,7 @@ struct ChunkArgs {
     uint32_t batch, q_heads, group, width;
     uint32_t window, sinks;  // window 0: none
     uint32_t counters;       // the launcher's: bytes of the workspace's counters
+    uint32_t tiles;          // the launcher's: row tiles of a work item (many rows)
     float scale;             // of the logits, times log2(e)
     bgtq_dtype dtype;
     uint32_t *status;
@@ -144,6 +145,9 @@ cudaError_t launch_append(const AppendArgs &a, cudaStream_t s);
 // Bytes of the workspace that launch_chunk needs (counters first, zero between calls).
 size_t chunk_workspace(const PageView &c, uint32_t q_heads);
 cudaError_t launch_chunk(const ChunkArgs &a, cudaStream_t s);
+// The kernel of many rows (paged_prompt.cu), which launch_chunk calls, and the bytes of its workspace.
+size_t paged_prompt_workspace(uint32_t dim);
+cudaError_t launch_paged_prompt(const ChunkArgs &a, cudaStream_t s);
 cudaError_t launch_logits(const LogitsArgs &a, cudaStream_t s);
 
 // SMs of a device (0: no such device), asked for once.
