@@ -19,9 +19,12 @@
 //               16-bit operands ahead of the products.  Keys stay exact, so that logits are FP32's: 8-bit codes in the
 //               queries' type, 4-bit codes times their scale over a power of two of their token (11 bits) in FP16; what
 //               is left of the scales multiplies the logits, in softmax.  (BF16 queries go to FP16 for 4-bit keys, over a
-//               power of two of their row, which loses what is below 2^-37 of the row's largest.)  Values are rounded
-//               to BF16, as they are read back by default, and probabilities too: half a step of an 8-bit row
-//               is 2^-8 of its largest value already, which is what BF16 keeps of each
+//               power of two of their row, which loses what is below 2^-37 of the row's largest.)  Values are exact in
+//               FP16 in the same two ways, and what is left of their scales multiplies the probabilities, before the
+//               rounding to FP16.  Its exponent range does not hold such products of any scale: they are taken relative
+//               to the row's largest (exp(logit) x value scale) so far, in steps of at least 2^kRoom, so that a value of any
+//               size whose weight is next to nothing leaves the others as they are.  What is rounded away is
+//               2^-34 of the largest
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -36,6 +39,9 @@ constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while
 constexpr int kJoin = 2;                 // parts of an item that are joined at a time
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 template <bool BF> constexpr float kUp = BF ? 0.0f : 15.0f - kLazy;  // log2 of what probabilities are multiplied by
+// Over 8- and 4-bit pages (powers of two, as logarithms): how far a tile's largest probability x value scale may pass the
+// largest before it; what such products are multiplied by; how far they may be below their probability.
+constexpr float kRoom = 4.0f, kUpCodes = 10.0f, kApart = 100.0f;
 
 enum { F_F16, F_BF16, F_INT8, F_INT4 };
 
@@ -58,16 +64,18 @@ struct Plan {
     // 8- and 4-bit pages: tiles as they lie in the pages, and their scales
     static constexpr uint32_t kRow = F == F_INT8 ? D : D / 2, kGroups = F == F_INT8 ? 1 : D / 32;
     static constexpr uint32_t kRawTile = kKeys * kRow, kRawScale = kKeys * kGroups * 2;
-    static constexpr uint32_t kRawStage = 2 * (kRawTile + kRawScale), kRawStages = kCodes ? (kRow == 128 ? 2 : 4) : 0;
+    // (two tiles, the scales of both, and where they are K tiles those of the same tokens' values)
+    static constexpr uint32_t kRawStage = 2 * kRawTile + 4 * kRawScale, kRawStages = kCodes ? (D == 128 ? 2 : 4) : 0;
     // What softmax has to know of the K tiles in a stage is kept until that stage's logits are done with, which is sure
     // when the load warp has gone all stages and the logits' lead further.
-    static constexpr uint32_t kMeta = 16;
-    static_assert(kMeta >= kRawStages + kStages + kBufs + 1, "");
+    static constexpr uint32_t kMeta = kRawStages + kStages + kBufs + 1 <= 8 ? 8 : 16;
     static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kRaw = kRing + kStages * 2 * kTile;
     static constexpr int kTurn = NT == 4 ? 16 : 32;                // dimensions of an output row stored at a time
     static constexpr uint32_t kOut = kRaw + kRawStages * kRawStage;                     // [softmax warps][32 rows][kTurn] outputs
-    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][kKeys] what logits are multiplied by
-    static constexpr uint32_t kBadPages = kScales + (kCodes ? kMeta * 2 * kKeys * 4 : 0);  // [kMeta][2] pieces without a page
+    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][2][kKeys] what logits, and
+                                                                                        // probabilities, are multiplied by
+    static constexpr uint32_t kLargest = kScales + (kCodes ? kMeta * 4 * kKeys * 4 : 0);   // [kMeta][2] exponent of the latter's largest
+    static constexpr uint32_t kBadPages = kLargest + (kCodes ? kMeta * 8 : 0);             // [kMeta][2] pieces without a page
     static constexpr uint32_t kItems = kBadPages + kMeta * 8;      // [kDeal] Item
     static constexpr uint32_t kBars = kItems + kDeal * 64;
     static constexpr uint32_t kBarCount = 3 * kStages + 2 * kRawStages + 3 * kTiles + 3 * kTiles * kBufs + 2 * kDeal + 2;
@@ -111,10 +119,6 @@ __device__ __forceinline__ uint32_t sub_b(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ uint32_t mul_b(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 // Two signed bytes as two whole numbers: in FP16 1024 + (byte + 128) is 0x6400 | (byte ^ 128), less 1152; in BF16 128 +
 // (the low seven bits) is 0x4300 | them, less 128, or 256 where the sign bit, which falls on the exponent, is set.
 template <bool BF>
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
     constexpr bool kCodes = P::kCodes;
     constexpr bool kQTurn = F == F_INT4 && QBF;              // queries go from BF16 to FP16
     constexpr bool S_BF = F == F_INT4 ? false : QBF;         // the logits' operands
-    constexpr bool P_BF = kCodes ? true : QBF;               // the probabilities and values
+    constexpr bool P_BF = kCodes ? false : QBF;              // the probabilities and values
     constexpr int32_t kKeys = (int32_t)P::kKeys;
     constexpr uint32_t NB = P::kBufs;
     extern __shared__ unsigned char raw_smem[];
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             bar_init(bar(B_FREE + i), 2);
             bar_init(bar(B_RAW + i), 1);
         }
-        for (uint32_t i = 0; i < P::kRawStages; ++i) {
+        for (int i = 0; i < (int)P::kRawStages; ++i) {
             bar_init(bar(B_CODES + i), 1);
             bar_init(bar(B_TURNED + i), P::kEnds);
         }
@@ -314,6 +318,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
             }
             float ref = -INFINITY, sum = 0.0f;  // the maximum that probabilities are relative to (log2 units)
+            float unit = -INFINITY;             // codes: what their products with value scales are relative to
             for (int32_t j = 0; j < tiles; ++j) {
                 const uint32_t buf = j % NB, ts = tmem + lanes + (NB * t + buf) * kKeys;
                 if (!(fine = all_wait(bar(B_S + NB * t + buf), phase >> buf & 1u))) break;
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
                 if constexpr (kCodes) {
-                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (kKeys / 4);
+                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
 #pragma unroll
                     for (int i = 0; i < kKeys; i += 4) {
                         const float4 f = by[i / 4];
@@ -374,8 +379,44 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 c1 = max3(c1, s[kKeys - 2], s[kKeys - 1]);
                 const float top = fmaxf(max3(c0, c1, c2), c3) * (kCodes ? 1.0f : a.scale);
                 const bool grown = top > ref + kLazy;  // each row for itself, not by the others of the warp
-                if (j == 0) ref = top;
-                else if (__any_sync(0xffffffffu, grown)) {
+                float alpha = 0.0f, beta = 0.0f;       // 2^alpha: what sums are multiplied by, 2^beta: outputs
+                bool moved = j != 0 && grown;
+                if constexpr (kCodes) {
+                    const float4 *weights = reinterpret_cast<const float4 *>(sm + P::kScales) + (meta * 2 + 1) * (kKeys / 4);
+                    // no product is larger than the largest probability x the largest scale; if that is too large, look
+                    const bool wide = top + reinterpret_cast<const float *>(sm + P::kLargest)[meta] > unit + kRoom;
+                    const float before = ref;
+                    if (j == 0 || grown) ref = top;
+                    if (__any_sync(0xffffffffu, wide || grown)) {
+                        float peak = -INFINITY;
+                        if (__any_sync(0xffffffffu, wide)) {
+#pragma unroll
+                            for (int i = 0; i < kKeys; i += 4) {
+                                const float4 w = weights[i / 4];
+                                auto exponent = [](float y) {  // as a number: 2^23 + n is 0x4b000000 | n
+                                    return __uint_as_float(0x4b000000u | (__float_as_uint(y) >> 23 & 255u)) - (8388608.0f + 127.0f);
+                                };
+                                peak = max3(peak, s[i] + exponent(w.x), s[i + 1] + exponent(w.y));
+                                peak = max3(peak, s[i + 2] + exponent(w.z), s[i + 3] + exponent(w.w));
+                            }
+                        }
+                        float now = peak > unit + kRoom ? peak : unit;
+                        now = fmaxf(now, ref - kApart);
+                        if (j != 0) {
+                            alpha = grown ? before - ref : 0.0f;
+                            beta = now > unit ? unit - now : 0.0f;
+                            moved = alpha != 0.0f || beta != 0.0f;
+                        }
+                        unit = now;
+                    }
+                } else {
+                    if (j == 0) ref = top;
+                    else if (grown) {
+                        alpha = beta = ref - top;
+                        ref = top;
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
                     // not under a product that is still adding to the outputs: the other buffer's next logits
                     // come after it, or nothing does (with one buffer, these logits did)
                     if (NB == 2) {
@@ -384,9 +425,8 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         if (!fine) break;
                         tc_after();
                     }
-                    const float f = grown ? ex2(ref - top) : 1.0f;
-                    if (grown) ref = top;
-                    sum *= f;
+                    const float f = kCodes ? ex2(beta) : ex2(alpha);
+                    sum *= kCodes ? ex2(alpha) : f;
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
@@ -397,16 +437,34 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         tm_store16(to + 16 * c, o);
                     }
                 }
-                const float from = (ref == -INFINITY ? 0.0f : ref) - kUp<P_BF>;
+                const float from = (ref == -INFINITY ? 0.0f : ref) - (kCodes ? 0.0f : kUp<P_BF>);
                 const float2 scale2 = make_float2(a.scale, a.scale), from2 = make_float2(-from, -from);
                 float2 total = make_float2(0.0f, 0.0f);
+                if constexpr (kCodes) {
+                    const float4 *weights = reinterpret_cast<const float4 *>(sm + P::kScales) + (meta * 2 + 1) * (kKeys / 4);
+                    const float g = unit == -INFINITY ? 0.0f : ex2(ref - unit + kUpCodes);
+                    const float2 g2 = make_float2(g, g);
 #pragma unroll
-                for (int i = 0; i < kKeys; i += 2) {
-                    const float2 y = make_float2(s[i], s[i + 1]);
-                    const float2 v = kCodes ? __fadd2_rn(y, from2) : __ffma2_rn(y, scale2, from2);
-                    const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
-                    total = __fadd2_rn(total, e);
-                    x[i / 2] = pack<P_BF>(e.x, e.y);
+                    for (int i = 0; i < kKeys; i += 4) {
+                        const float4 w = weights[i / 4];
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            const float2 v = __fadd2_rn(make_float2(s[i + k], s[i + k + 1]), from2);
+                            const float2 e = (i + k) % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
+                            total = __fadd2_rn(total, e);
+                            // (by the scale last: the other way round a large one without weight may pass FP32)
+                            const float2 y = __fmul2_rn(__fmul2_rn(e, g2), k ? make_float2(w.z, w.w) : make_float2(w.x, w.y));
+                            x[(i + k) / 2] = pack<P_BF>(y.x, y.y);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 2) {
+                        const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
+                        const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
+                        total = __fadd2_rn(total, e);
+                        x[i / 2] = pack<P_BF>(e.x, e.y);
+                    }
                 }
                 sum += total.x + total.y;
                 tm_store(ts, x);
@@ -430,6 +488,8 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 if (!fine) break;
                 tc_after();
                 const uint32_t flagged = bad_flag[n % kDeal];
+                // what outputs are multiplied by to be relative to the probabilities' maximum
+                const float back = !kCodes ? 1.0f : unit == -INFINITY ? 0.0f : ex2(unit - ref - kUpCodes);
                 // infinities and NaN among the values of the dimensions from d0 on that this row sees in tiles that were
                 // looked through, added to what the other tokens came to, which may be an infinity or a NaN of their own
                 auto overlay = [&](uint32_t *o, int d0, auto width) {
@@ -484,7 +544,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                             if (flagged) overlay(o, 16 * c, std::integral_constant<int, 16>());
                         }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]));
+                        for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]) * back);
                     }
                     tc_before();
                     __threadfence();
@@ -521,7 +581,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
                 const bool none = at < 0 || it.keys == 0;
                 const float ref0 = ref == -INFINITY ? 0.0f : ref;
-                const float inv = none || sum == 0.0f ? 0.0f : 1.0f / sum;  // (0: every logit is -infinity)
+                const float inv = none || sum == 0.0f ? 0.0f : whole ? back / sum : 1.0f / sum;  // (0: every logit is -infinity)
                 // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
                 constexpr int kW = P::kTurn, kL = kW / 8;
                 unsigned char *turn = sm + P::kOut + warp * 64 * kW;
@@ -599,7 +659,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     __syncwarp();
                 }
                 if (live && a.lse)
-                    a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - kUp<P_BF> + __log2f(sum)) * kLn2;
+                    a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - (kCodes ? 0.0f : kUp<P_BF>) + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;
@@ -796,7 +856,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             // ---- loads ----
             // Stage 0 of an item is the K tiles that logits run ahead by, stage k + 1 is V k and K k + NB.  Lanes 0 to 7
             // load the first tile of a stage, 8 to 15 the second: four pieces x two columns of 64 dimensions (16 bits), or
-            // x codes and scales.  A stage that the last warp looks through (16 bits) lands on its raw barrier, and that
+            // x codes and scales (then lanes 16 to 31 those of a K tile's tokens' values).  A stage that the last warp looks through (16 bits) lands on its raw barrier, and that
             // warp arrives on the full one when it is done with it; codes land in stages of their own.
             constexpr uint32_t kRing = kCodes ? P::kRawStages : P::kStages;
             uint32_t slot = 0, free_phase = 1, q_phase = (1u << NT) - 1, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
@@ -822,7 +882,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 // the tile of stage k that this lane has a piece of; -1: none
                 auto unit_of = [&](int32_t k) -> int32_t {
                     const int32_t j = k == 0 ? (int32_t)sel : sel ? k - 1 + (int32_t)NB : k - 1;
-                    return lane < 16 && piece < pieces && j < (k == 0 ? min(tiles, (int32_t)NB) : tiles) ? j : -1;
+                    return (lane < 16 || (kCodes && half && (k == 0 || sel))) && piece < pieces && j < (k == 0 ? min(tiles, (int32_t)NB) : tiles) ? j : -1;
                 };
                 auto token_of = [&](int32_t k) {
                     const int32_t j = unit_of(k);
@@ -837,7 +897,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const int32_t ahead = k < tiles ? page_of(k + 1) : 0;
                     const int32_t token = token_of(k);
                     const bool there = (uint32_t)page < a.c.pages;
-                    const uint32_t bad = __ballot_sync(0xffffffffu, token < it.keys && !there && half == 0);
+                    const uint32_t bad = __ballot_sync(0xffffffffu, token < it.keys && !there && half == 0 && lane < 16);
                     if (!(fine = fine && all_wait(bar((kCodes ? B_TURNED : B_FREE) + slot), free_phase))) return;
                     const bool two = k == 0 ? NB == 2 && tiles > 1 : k - 1 + (int32_t)NB < tiles;
                     const bool look = !kCodes && k && !plain(it, first_of(it, k - 1));
@@ -846,11 +906,12 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         if (bad) atomicOr(a.status, kStatusBadSlot);
                         bad_pages[stage_no % P::kMeta * 2] = bad & 15u;
                         bad_pages[stage_no % P::kMeta * 2 + 1] = bad >> 8 & 15u;
-                        bar_expect(on, (kCodes ? P::kRawTile + P::kRawScale : P::kTile) * (two ? 2u : 1u));
+                        bar_expect(on, kCodes ? (P::kRawTile + P::kRawScale) * (two ? 2u : 1u) + P::kRawScale * ((k == 0 ? 1u : 0u) + (two ? 1u : 0u))
+                                              : P::kTile * (two ? 2u : 1u));
                     }
                     __syncwarp();
                     if (unit_of(k) >= 0) {
-                        const bool value = k && !sel;
+                        const bool value = lane >= 16 || (k && !sel);
                         const int32_t in_page = token & (int32_t)(a.c.page_size - 1);
                         // (past the cache's last page: zeros)
                         const int32_t z = there ? page : (int32_t)a.c.pages;
@@ -864,7 +925,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                                 tma4(dst + sel * P::kRawTile + (piece << piece_shift) * P::kRow, value ? &mv : &mk, on, 0, in_page, it.head, z);
                             else {
                                 const uint64_t r = there ? ((uint64_t)page * a.c.heads + it.head << a.c.page_shift) + in_page : 0;
-                                bulk(dst + 2 * P::kRawTile + sel * P::kRawScale + (piece << piece_shift) * P::kGroups * 2,
+                                bulk(dst + 2 * P::kRawTile + (lane >= 16 ? 2 + sel : sel) * P::kRawScale + (piece << piece_shift) * P::kGroups * 2,
                                      (value ? a.c.vs : a.c.ks) + r * P::kGroups, piece_rows * P::kGroups * 2, on);
                             }
                         }
@@ -1049,76 +1110,91 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             };
             // (columns of 64 dimensions begin at one bank: their chunks are written in another order)
             auto order = [](uint32_t c, uint32_t k) { return k ^ (c * kOut / 8 % kOut); };
-            auto turn_keys = [&](const unsigned char *codes, const uint16_t *scales, unsigned char *tile, float *by) {
+            // exponent of the largest finite scale of a token, at least that of 2^-100
+            auto largest = [](const uint16_t *scales) {
+                uint32_t big = 0;
+#pragma unroll
+                for (uint32_t g = 0; g < G; ++g) {
+                    const uint32_t s = scales[g] & 0x7fffu;
+                    big = max(big, s < 0x7f80u ? s : 0u);
+                }
+                return max(big >> 7, 27u);
+            };
+            // a token's scale over that power of two, times 2^10
+            auto scaled = [](uint32_t scale, uint32_t e) {
+                const float f = from_bf16(scale) * __uint_as_float((264 - e) << 23);
+                return pack<false>(f, f);
+            };
+            // 16 bytes of 4-bit codes x a scale in FP16, into the operand
+            auto put4 = [&](unsigned char *tile, uint32_t r, uint32_t c, const uint32_t (&w)[4], uint32_t s2) {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b)  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
+                        h[b] = mul_h(sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u), s2);
+                    put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
+                }
+            };
+            // 16 bytes of 8-bit codes, into the operand
+            auto put8 = [&](unsigned char *tile, uint32_t r, uint32_t c, const uint32_t (&w)[4], auto bf) {
+                constexpr bool BF = decltype(bf)::value;
+                uint4 v[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    v[k] = make_uint4(codes8<BF>(w[2 * k], 0x4140), codes8<BF>(w[2 * k], 0x4342), codes8<BF>(w[2 * k + 1], 0x4140),
+                                      codes8<BF>(w[2 * k + 1], 0x4342));
+                const uint32_t first = order(c, 0);
+                put(tile, r, c, first, first ? v[1] : v[0]);
+                put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
+            };
+            // what logits and probabilities of a K tile's tokens are multiplied by: the first of these warps
+            auto weigh = [&](const uint16_t *keys, const uint16_t *values, uint32_t slot_of, uint32_t rows, bool look, uint32_t bad, uint32_t n) {
+                float *by = reinterpret_cast<float *>(sm + P::kScales) + slot_of * 2 * kKeys;
+                uint32_t top = 0;
+#pragma unroll
+                for (uint32_t r = lane; r < P::kKeys; r += 32) {
+                    float k, v;
+                    if constexpr (F == F_INT8) {
+                        k = from_bf16(keys[r]);
+                        uint32_t s = values[r];
+                        if (r >= rows || bad >> (r >> piece_shift) & 1u) s = 0;
+                        else if (look && (s & 0x7f80u) == 0x7f80u) s = 0, bad_flag[n % kDeal] = 1;
+                        v = from_bf16(s);
+                    } else {
+                        k = __uint_as_float((largest(keys + r * G) - 10) << 23);
+                        v = r >= rows ? 0.0f : __uint_as_float((largest(values + r * G) - 10) << 23);
+                    }
+                    by[r] = k * a.scale;
+                    by[kKeys + r] = v;
+                    top = max(top, __float_as_uint(v) >> 23 & 255u);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) reinterpret_cast<float *>(sm + P::kLargest)[slot_of] = (float)top - 127.0f;
+            };
+            auto turn_keys = [&](const unsigned char *codes, const uint16_t *scales, unsigned char *tile) {
                 for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
                     const uint32_t r = i / kPer, c = i % kPer;
                     const uint4 x = reinterpret_cast<const uint4 *>(codes)[i];
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    if constexpr (F == F_INT8) {
-                        uint4 v[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            v[k] = make_uint4(codes8<QBF>(w[2 * k], 0x4140), codes8<QBF>(w[2 * k], 0x4342),
-                                              codes8<QBF>(w[2 * k + 1], 0x4140), codes8<QBF>(w[2 * k + 1], 0x4342));
-                        const uint32_t first = order(c, 0);
-                        put(tile, r, c, first, first ? v[1] : v[0]);
-                        put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
-                        if (c == 0) by[r] = from_bf16(scales[r]) * a.scale;
-                    } else {
-                        // the token's largest scale to [2^10, 2^11)
-                        uint32_t big = 0;
-#pragma unroll
-                        for (uint32_t g = 0; g < G; ++g) {
-                            const uint32_t s = scales[r * G + g] & 0x7fffu;
-                            big = max(big, s < 0x7f80u ? s : 0u);
-                        }
-                        const uint32_t e = max(big >> 7, 27u);
-                        const float f = from_bf16(scales[r * G + c]) * __uint_as_float((264 - e) << 23);
-                        const uint32_t s2 = pack<false>(f, f);
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            uint32_t h[4];
-#pragma unroll
-                            for (uint32_t b = 0; b < 4; ++b)  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
-                                h[b] = mul_h(sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u), s2);
-                            put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
-                        }
-                        if (c == 0) by[r] = __uint_as_float((e - 10) << 23) * a.scale;
-                    }
+                    if constexpr (F == F_INT8) put8(tile, r, c, w, std::integral_constant<bool, QBF>());
+                    else put4(tile, r, c, w, scaled(scales[r * G + c], largest(scales + r * G)));
                 }
             };
-            // values in BF16; of a tile that is looked through, what is past the request's tokens is zero, and so is what
-            // has a NaN for a scale
+            // (8-bit codes are finite, and what is left out has no weight.  In 4 bits what is past the request's tokens, and
+            // in a tile that is looked through what has a NaN for a scale, is zero.)
             auto turn_values = [&](const unsigned char *codes, const uint16_t *scales, unsigned char *tile, uint32_t rows, bool look, uint32_t bad) {
                 uint32_t found = 0;
                 for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
                     const uint32_t r = i / kPer, c = i % kPer;
                     const uint4 x = reinterpret_cast<const uint4 *>(codes)[i];
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    uint32_t s = scales[r * G + (G == 1 ? 0 : c)];
-                    bool zero = r >= rows || bad >> (r >> piece_shift) & 1u;
-                    if (look && !zero && (s & 0x7f80u) == 0x7f80u) zero = true, found = 1;
-                    if (zero) s = 0;  // (a code times zero)
-                    const uint32_t s2 = s | s << 16;
-                    if constexpr (F == F_INT8) {
-                        uint4 v[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            v[k] = make_uint4(mul_b(codes8<true>(w[2 * k], 0x4140), s2), mul_b(codes8<true>(w[2 * k], 0x4342), s2),
-                                              mul_b(codes8<true>(w[2 * k + 1], 0x4140), s2), mul_b(codes8<true>(w[2 * k + 1], 0x4342), s2));
-                        const uint32_t first = order(c, 0);
-                        put(tile, r, c, first, first ? v[1] : v[0]);
-                        put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
-                    } else {
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const uint32_t lo = w[k], hi = w[k] >> 4;
-                            uint32_t h[4];
-#pragma unroll
-                            for (uint32_t b = 0; b < 4; ++b)  // 128 + code + 8 in both halves
-                                h[b] = mul_b(sub_b((__byte_perm(lo, hi, b * 0x11u | (4 + b) * 0x1100u) & 0x000f000fu) | 0x43004300u, 0x43084308u), s2);
-                            put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
-                        }
+                    if constexpr (F == F_INT8) put8(tile, r, c, w, std::false_type());
+                    else {
+                        uint32_t s = scales[r * G + c];
+                        const bool zero = r >= rows || bad >> (r >> piece_shift) & 1u, nan = look && (s & 0x7f80u) == 0x7f80u;
+                        if (nan && !zero) found = 1;
+                        put4(tile, r, c, w, zero || nan ? 0u : scaled(s, largest(scales + r * G)));
                     }
                 }
                 return found;
@@ -1130,16 +1206,23 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     if (!(fine = all_wait(bar(B_FREE + slot), free_phase))) break;
                     const unsigned char *codes = sm + P::kRaw + from * P::kRawStage;
                     const uint16_t *scales = reinterpret_cast<const uint16_t *>(codes + 2 * P::kRawTile);
+                    constexpr uint32_t kNext = P::kRawScale / 2;
                     unsigned char *tile = sm + P::kRing + slot * 2 * P::kTile;
-                    float *by = reinterpret_cast<float *>(sm + P::kScales) + stage_no % P::kMeta * 2 * kKeys;
-                    if (k == 0) turn_keys(codes, scales, tile, by);
-                    else {
-                        const int32_t k0 = first_of(it, k - 1);
-                        const uint32_t rows = (uint32_t)min(kKeys, it.keys - k0);
-                        if (turn_values(codes, scales, tile, rows, !plain(it, k0), bad_pages[stage_no % P::kMeta * 2])) bad_flag[n % kDeal] = 1;
+                    const uint32_t meta = stage_no % P::kMeta * 2;
+                    auto rows_of = [&](int32_t j) { return (uint32_t)min(kKeys, it.keys - first_of(it, j)); };
+                    auto look_of = [&](int32_t j) { return !plain(it, first_of(it, j)); };
+                    if (k == 0) {
+                        if (warp == W_ENDS) weigh(scales, scales + 2 * kNext, meta, rows_of(0), look_of(0), bad_pages[meta], n);
+                        turn_keys(codes, scales, tile);
+                    } else if (turn_values(codes, scales, tile, rows_of(k - 1), look_of(k - 1), bad_pages[meta])) {
+                        bad_flag[n % kDeal] = 1;
                     }
-                    if (k == 0 ? NB == 2 && tiles > 1 : k - 1 + (int32_t)NB < tiles)
-                        turn_keys(codes + P::kRawTile, scales + P::kRawScale / 2, tile + P::kTile, by + kKeys);
+                    const int32_t ahead = k == 0 ? 1 : k - 1 + (int32_t)NB;
+                    if (k == 0 ? NB == 2 && tiles > 1 : ahead < tiles) {
+                        if (warp == W_ENDS)
+                            weigh(scales + kNext, scales + 3 * kNext, meta + 1, rows_of(ahead), look_of(ahead), bad_pages[meta + 1], n);
+                        turn_keys(codes + P::kRawTile, scales + kNext, tile + P::kTile);
+                    }
                     fence_async();
                     __syncwarp();
                     if (lane == 0) {

@@ -7,9 +7,10 @@ append   a rotated value is three FP32 roundings of a c and b s, of at most |a| 
          a root, a quotient and two products: 24 u in all.  32 u (|a| + |b|) holds both, and the result is
          rounded once.  Rows that become codes are 64-bit and rounded to FP32 once: their codes are those
          of the 64-bit row, but for ties.
-chunk    over 16-bit pages what test_gpu_serving says: u |o| + (u + 3e-5) A, A = sum p_t |v_t|.  Over 8- and
-         4-bit pages probabilities and values may both be rounded to BF16 before their product: 2 u + u^2 of
-         BF16 in place of u.  The log sum is FP32 throughout: 3e-5 absolute.
+chunk    what test_gpu_serving says: u |o| + (u + 3e-5) A, A = sum p_t |v_t|, for the roundings of probabilities
+         and outputs; over 8- and 4-bit pages probabilities are rounded to FP16, whatever the queries' type, and
+         held to 2^-34 of the row's largest product with a value scale, times a code of at most 2^4 of it (4 bits)
+         or 2^7 (8 bits): 2^-25 (A + 1) covers it for rows of one size.  The log sum is FP32 throughout: 3e-5 absolute.
 logits   every step is one FP32 rounding of what it gives: 5 u of the sum of the steps' magnitudes.
 """
 import math
@@ -253,10 +254,10 @@ def seen_of(n, length, window, sinks):
 def close_chunk(out, lse, ref, dtype, fmt):
     import torch
     want, want_lse, mag, small = ref
-    u = U[dtype] if fmt in ("f16", "bf16") else 2 * U["bf16"] + U["bf16"] ** 2
+    u = U[dtype] if fmt in ("f16", "bf16") else U["f16"]
     tol = U[dtype] * want.abs() + (u + 3e-5) * mag + 1e-30
-    if dtype == "f16":
-        tol = tol + 2.0 ** -25 * (small + 1)
+    if dtype == "f16" or fmt not in ("f16", "bf16"):
+        tol = tol + 2.0 ** -25 * (small + mag + (1 if dtype == "f16" else 0))
     off = (out.double() - want).abs()
     bad = ~(off <= tol) & ~(torch.isnan(want) & torch.isnan(out)) & ~(torch.isinf(want) & (out.double() == want))
     assert not bool(bad.any()), (int(bad.sum()), float((off / tol).nan_to_num(0).max()))
