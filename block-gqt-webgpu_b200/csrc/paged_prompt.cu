@@ -16,15 +16,17 @@
 //               row that does not see it would turn into a NaN, is taken out; the rows that see it look the tile
 //               through once more, in the pages, when they are written
 //   codes       (8- and 4-bit pages) codes and scales are loaded as they are, and warps of their own turn a tile into
-//               16-bit operands ahead of the products.  Keys stay exact, so that logits are FP32's: 8-bit codes in the
-//               queries' type, 4-bit codes times their scale over a power of two of their token (11 bits) in FP16; what
-//               is left of the scales multiplies the logits, in softmax.  (BF16 queries go to FP16 for 4-bit keys, over a
-//               power of two of their row, which loses what is below 2^-37 of the row's largest.)  Values are exact in
-//               FP16 in the same two ways, and what is left of their scales multiplies the probabilities, before the
-//               rounding to FP16.  Its exponent range does not hold such products of any scale: they are taken relative
-//               to the row's largest (exp(logit) x value scale) so far, in steps of at least 2^kRoom, so that a value of any
-//               size whose weight is next to nothing leaves the others as they are.  What is rounded away is
-//               2^-34 of the largest
+//               FP16 operands ahead of the products: codes x scales over a power of two of the tile's largest scale, which
+//               multiplies the tile's logits as the scale of all logits does, and its probabilities as an addend of their
+//               exponents, so that softmax does no more than over 16-bit pages.  A key stays exact, so that
+//               logits are FP32's: 4-bit codes x scales have 11 bits, 8-bit ones have 15, of which a second operand
+//               holds the last four, multiplied by the same queries into the same logits.  (BF16 queries go to FP16
+//               over a power of two of their row, which loses what is below 2^-38 of the row's largest.)  A value in 8 bits is
+//               rounded to 11 bits, a sixteenth of the step that its code was rounded to.  Where the scales of a
+//               tile are more than 2^16 apart, as next to rows of 1e30, powers of two of each token take their place
+//               and multiply each logit, or each probability.  Probabilities x value scales are taken relative to
+//               the row's largest so far, in steps of at least 2^kRoom, so that values of any size whose weight is next
+//               to nothing leave the others as they are; what is rounded away is 2^-34 of the largest
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -40,8 +42,10 @@ constexpr int kJoin = 2;                 // parts of an item that are joined at 
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 template <bool BF> constexpr float kUp = BF ? 0.0f : 15.0f - kLazy;  // log2 of what probabilities are multiplied by
 // Over 8- and 4-bit pages (powers of two, as logarithms): how far a tile's largest probability x value scale may pass the
-// largest before it; what such products are multiplied by; how far they may be below their probability.
+// largest before it; what such products are multiplied by; how far they may be below their probability; how far apart
+// the scales of a tile may be that has one power of two.
 constexpr float kRoom = 4.0f, kUpCodes = 10.0f, kApart = 100.0f;
+constexpr uint32_t kNear = 16;
 
 enum { F_F16, F_BF16, F_INT8, F_INT4 };
 
@@ -60,23 +64,26 @@ struct Plan {
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
-    static constexpr uint32_t kStages = D == 128 ? (kCodes ? 3 : 4) : (kCodes ? 5 : 7);  // of two K or V tiles in the ring
+    static constexpr bool kLow = F == F_INT8;                      // keys have a second operand
+    static constexpr uint32_t kStageBytes = (kLow ? 3 : 2) * kTile;  // a V tile and a K tile
+    static constexpr uint32_t kStages = D == 128 ? (kLow ? 2 : kCodes ? 3 : 4) : (kLow ? 4 : kCodes ? 5 : 7);
     // 8- and 4-bit pages: tiles as they lie in the pages, and their scales
     static constexpr uint32_t kRow = F == F_INT8 ? D : D / 2, kGroups = F == F_INT8 ? 1 : D / 32;
     static constexpr uint32_t kRawTile = kKeys * kRow, kRawScale = kKeys * kGroups * 2;
-    // (two tiles, the scales of both, and where they are K tiles those of the same tokens' values)
-    static constexpr uint32_t kRawStage = 2 * kRawTile + 4 * kRawScale, kRawStages = kCodes ? (D == 128 ? 2 : 4) : 0;
-    // What softmax has to know of the K tiles in a stage is kept until that stage's logits are done with, which is sure
+    // (the two tiles, the scales of both, and those of the K tile's tokens' values)
+    static constexpr uint32_t kRawStage = 2 * kRawTile + 3 * kRawScale, kRawStages = kCodes ? (D == 128 ? 2 : 4) : 0;
+    static constexpr int kUpTile = F == F_INT8 ? 7 : 10;           // log2 of what a tile's largest scale goes to
+    // What softmax has to know of the K tile in a stage is kept until that tile's logits are done with, which is sure
     // when the load warp has gone all stages and the logits' lead further.
-    static constexpr uint32_t kMeta = kRawStages + kStages + kBufs + 1 <= 8 ? 8 : 16;
-    static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kRaw = kRing + kStages * 2 * kTile;
+    static constexpr uint32_t kMeta = kRawStages + kStages + kBufs <= 8 ? 8 : 16;
+    static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kRaw = kRing + kStages * kStageBytes;
     static constexpr int kTurn = NT == 4 ? 16 : 32;                // dimensions of an output row stored at a time
     static constexpr uint32_t kOut = kRaw + kRawStages * kRawStage;                     // [softmax warps][32 rows][kTurn] outputs
-    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][2][kKeys] what logits, and
+    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][kKeys] what logits, and
                                                                                         // probabilities, are multiplied by
-    static constexpr uint32_t kLargest = kScales + (kCodes ? kMeta * 4 * kKeys * 4 : 0);   // [kMeta][2] exponent of the latter's largest
-    static constexpr uint32_t kBadPages = kLargest + (kCodes ? kMeta * 8 : 0);             // [kMeta][2] pieces without a page
-    static constexpr uint32_t kItems = kBadPages + kMeta * 8;      // [kDeal] Item
+    static constexpr uint32_t kAbout = kScales + (kCodes ? kMeta * 2 * kKeys * 4 : 0);     // [kMeta] About
+    static constexpr uint32_t kBadPages = kAbout + (kCodes ? kMeta * 16 : 0);              // [kMeta] pieces without a page: K, V
+    static constexpr uint32_t kItems = kBadPages + kMeta * 4;      // [kDeal] Item
     static constexpr uint32_t kBars = kItems + kDeal * 64;
     static constexpr uint32_t kBarCount = 3 * kStages + 2 * kRawStages + 3 * kTiles + 3 * kTiles * kBufs + 2 * kDeal + 2;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
@@ -98,6 +105,13 @@ struct TileSpan {
     int32_t count, tiles;  // rows, units of this piece
 };
 
+// Of a K tile of codes: what its logits are multiplied by, the exponent of the largest scale among its tokens' values,
+// and whether (bits 0, 1) logits, and probabilities, have a factor for each token instead.
+struct About {
+    float mul, top;
+    uint32_t each, pad;
+};
+
 __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
                  "[%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -115,20 +129,10 @@ __device__ __forceinline__ uint32_t mul_h(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ uint32_t sub_b(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+__device__ __forceinline__ uint32_t rest_h(uint32_t a, uint32_t b, uint32_t c) {  // a b - c, rounded once
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b),
+                              __hneg2(*reinterpret_cast<const __half2 *>(&c)));
     return *reinterpret_cast<const uint32_t *>(&r);
-}
-// Two signed bytes as two whole numbers: in FP16 1024 + (byte + 128) is 0x6400 | (byte ^ 128), less 1152; in BF16 128 +
-// (the low seven bits) is 0x4300 | them, less 128, or 256 where the sign bit, which falls on the exponent, is set.
-template <bool BF>
-__device__ __forceinline__ uint32_t codes8(uint32_t w, uint32_t sel) {
-    if constexpr (BF) {
-        const uint32_t p = __byte_perm(w, 0x43434343u, sel);
-        return sub_b(p & 0xff7fff7fu, p & 0xff80ff80u);
-    } else {
-        return sub_h(__byte_perm(w ^ 0x80808080u, 0x64646464u, sel), 0x64806480u);
-    }
 }
 
 template <int D, int NT, int F, bool QBF>
@@ -138,9 +142,8 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                                                                     const __grid_constant__ CUtensorMap mv) {
     using P = Plan<D, NT, F>;
     constexpr bool kCodes = P::kCodes;
-    constexpr bool kQTurn = F == F_INT4 && QBF;              // queries go from BF16 to FP16
-    constexpr bool S_BF = F == F_INT4 ? false : QBF;         // the logits' operands
-    constexpr bool P_BF = kCodes ? false : QBF;              // the probabilities and values
+    constexpr bool kQTurn = kCodes && QBF;          // queries go from BF16 to FP16
+    constexpr bool BF = kCodes ? false : QBF;       // the operands
     constexpr int32_t kKeys = (int32_t)P::kKeys;
     constexpr uint32_t NB = P::kBufs;
     extern __shared__ unsigned char raw_smem[];
@@ -251,8 +254,9 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
         return k0 + kKeys <= min(it.keys, it.place + 1) &&
                (!a.window || it.place + it.count - 1 - k0 < (int32_t)a.window || (uint32_t)(k0 + kKeys) <= a.sinks);
     };
-    // stages that an item takes
-    auto stages_of = [](int32_t tiles) { return (uint32_t)(tiles ? tiles + 1 : 0); };
+    // stages that an item takes: K tiles that logits run ahead by, then V j with K j + NB
+    auto lead_of = [](int32_t tiles) { return min(tiles, (int32_t)NB); };
+    auto stages_of = [&](int32_t tiles) { return (uint32_t)(tiles + lead_of(tiles)); };
 
     if (warp < 4 * NT) {
         // ---- softmax: thread = row of tile t ----
@@ -328,22 +332,23 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 tm_load(ts, x);
                 tm_load(ts + 32, x + 32);
                 // where the K tile lay
-                const uint32_t meta = (stage_no + (j < (int32_t)NB ? 0u : 1u + (uint32_t)j - NB)) % P::kMeta * 2 + (j < (int32_t)NB ? (uint32_t)j : 1u);
+                const uint32_t meta = (stage_no + (uint32_t)j) % P::kMeta;
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
+                float mul = a.scale, largest = 0.0f;
+                uint32_t each = 0;
                 if constexpr (kCodes) {
-                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
+                    const About &about = reinterpret_cast<const About *>(sm + P::kAbout)[meta];
+                    // (not 0, which minus infinity is not multiplied by: such logits are next to nothing)
+                    mul = fmaxf(about.mul * q_mul, 1.2e-38f), largest = about.top, each = about.each;
+                    if (each & 1u) {
+                        const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
 #pragma unroll
-                    for (int i = 0; i < kKeys; i += 4) {
-                        const float4 f = by[i / 4];
-                        float2 f0 = make_float2(f.x, f.y), f1 = make_float2(f.z, f.w);
-                        if constexpr (kQTurn) {  // first, as a product of up to 2^35 with a large key scale may pass FP32
-                            f0 = __fmul2_rn(f0, make_float2(q_mul, q_mul));
-                            f1 = __fmul2_rn(f1, make_float2(q_mul, q_mul));
+                        for (int i = 0; i < kKeys; i += 4) {  // (with the queries' power first: a product of up to 2^35 may pass FP32)
+                            const float4 f = by[i / 4];
+                            s[i] *= f.x * q_mul, s[i + 1] *= f.y * q_mul, s[i + 2] *= f.z * q_mul, s[i + 3] *= f.w * q_mul;
                         }
-                        f0 = __fmul2_rn(make_float2(s[i], s[i + 1]), f0);
-                        f1 = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), f1);
-                        s[i] = f0.x, s[i + 1] = f0.y, s[i + 2] = f1.x, s[i + 3] = f1.y;
+                        mul = 1.0f;
                     }
                 }
                 {
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const int32_t place = it.place, keys = it.keys;
                     const bool full = k0 + kKeys <= min(keys, place + 1) &&
                                       (!a.window || place + it.count - 1 - k0 < (int32_t)a.window || (uint32_t)(k0 + kKeys) <= a.sinks);
-                    const uint32_t bad = bad_pages[meta];
+                    const uint32_t bad = bad_pages[meta] & 15u;
                     if (__any_sync(0xffffffffu, !full || bad)) {
                         uint64_t m = mask_of(place + t * (int32_t)per + (int32_t)p, keys, k0);
                         if (bad)
@@ -377,38 +382,29 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
                 c0 = max3(c0, s[kKeys - 4], s[kKeys - 3]);
                 c1 = max3(c1, s[kKeys - 2], s[kKeys - 1]);
-                const float top = fmaxf(max3(c0, c1, c2), c3) * (kCodes ? 1.0f : a.scale);
+                const float top = fmaxf(max3(c0, c1, c2), c3) * mul;
                 const bool grown = top > ref + kLazy;  // each row for itself, not by the others of the warp
                 float alpha = 0.0f, beta = 0.0f;       // 2^alpha: what sums are multiplied by, 2^beta: outputs
                 bool moved = j != 0 && grown;
                 if constexpr (kCodes) {
-                    const float4 *weights = reinterpret_cast<const float4 *>(sm + P::kScales) + (meta * 2 + 1) * (kKeys / 4);
-                    // no product is larger than the largest probability x the largest scale; if that is too large, look
-                    const bool wide = top + reinterpret_cast<const float *>(sm + P::kLargest)[meta] > unit + kRoom;
-                    const float before = ref;
-                    if (j == 0 || grown) ref = top;
-                    if (__any_sync(0xffffffffu, wide || grown)) {
-                        float peak = -INFINITY;
-                        if (__any_sync(0xffffffffu, wide)) {
-#pragma unroll
-                            for (int i = 0; i < kKeys; i += 4) {
-                                const float4 w = weights[i / 4];
-                                auto exponent = [](float y) {  // as a number: 2^23 + n is 0x4b000000 | n
-                                    return __uint_as_float(0x4b000000u | (__float_as_uint(y) >> 23 & 255u)) - (8388608.0f + 127.0f);
-                                };
-                                peak = max3(peak, s[i] + exponent(w.x), s[i + 1] + exponent(w.y));
-                                peak = max3(peak, s[i + 2] + exponent(w.z), s[i + 3] + exponent(w.w));
-                            }
-                        }
-                        float now = peak > unit + kRoom ? peak : unit;
-                        now = fmaxf(now, ref - kApart);
-                        if (j != 0) {
-                            alpha = grown ? before - ref : 0.0f;
-                            beta = now > unit ? unit - now : 0.0f;
-                            moved = alpha != 0.0f || beta != 0.0f;
-                        }
-                        unit = now;
+                    if (j == 0 || grown) {
+                        alpha = j == 0 ? 0.0f : ref - top;
+                        ref = top;
                     }
+                    // no product is larger than the largest probability x the largest scale; where scales are far apart, look
+                    float peak = top + largest;
+                    if (each & 2u && __any_sync(0xffffffffu, peak > unit + kRoom)) {
+                        const float *weights = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
+                        peak = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i)  // (an exponent as a number: 2^23 + n is 0x4b000000 | n)
+                            peak = fmaxf(peak, fmaf(s[i], mul, __uint_as_float(0x4b000000u | __float_as_uint(weights[i]) >> 23) - (8388608.0f + 127.0f)));
+                    }
+                    const float now = fmaxf(peak > unit + kRoom ? peak : unit, ref - kApart);
+                    beta = j != 0 && now > unit ? unit - now : 0.0f;
+                    unit = now;
+                    sum *= ex2(alpha);
+                    moved = beta != 0.0f;
                 } else {
                     if (j == 0) ref = top;
                     else if (grown) {
@@ -425,8 +421,8 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         if (!fine) break;
                         tc_after();
                     }
-                    const float f = kCodes ? ex2(beta) : ex2(alpha);
-                    sum *= kCodes ? ex2(alpha) : f;
+                    const float f = ex2(beta);
+                    if (!kCodes) sum *= f;
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
@@ -437,36 +433,38 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         tm_store16(to + 16 * c, o);
                     }
                 }
-                const float from = (ref == -INFINITY ? 0.0f : ref) - (kCodes ? 0.0f : kUp<P_BF>);
-                const float2 scale2 = make_float2(a.scale, a.scale), from2 = make_float2(-from, -from);
-                float2 total = make_float2(0.0f, 0.0f);
+                // probabilities; over codes, times the largest scale of the tile's values, relative to 2^unit
+                float from = ref - kUp<BF>, give = 1.0f;  // give: what their sum is multiplied by
+                bool apart = false;
                 if constexpr (kCodes) {
-                    const float4 *weights = reinterpret_cast<const float4 *>(sm + P::kScales) + (meta * 2 + 1) * (kKeys / 4);
-                    const float g = unit == -INFINITY ? 0.0f : ex2(ref - unit + kUpCodes);
-                    const float2 g2 = make_float2(g, g);
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 4) {
-                        const float4 w = weights[i / 4];
-#pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
-                            const float2 v = __fadd2_rn(make_float2(s[i + k], s[i + k + 1]), from2);
-                            const float2 e = (i + k) % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
-                            total = __fadd2_rn(total, e);
-                            // (by the scale last: the other way round a large one without weight may pass FP32)
-                            const float2 y = __fmul2_rn(__fmul2_rn(e, g2), k ? make_float2(w.z, w.w) : make_float2(w.x, w.y));
-                            x[(i + k) / 2] = pack<P_BF>(y.x, y.y);
-                        }
-                    }
-                } else {
+                    from = unit - largest - kUpCodes;
+                    apart = __any_sync(0xffffffffu, (each & 2u) || from - ref > kApart);
+                    give = ex2(from - ref);
+                }
+                if (ref == -INFINITY) from = 0.0f, give = 1.0f;
+                float2 total = make_float2(0.0f, 0.0f);
+                if (kCodes && apart) {
+                    const float *weights = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
+                    const float g = unit == -INFINITY ? 0.0f : ex2(ref - unit + kUpCodes), all = ex2(largest), base = ref == -INFINITY ? 0.0f : ref;
+                    give = 1.0f;
 #pragma unroll
                     for (int i = 0; i < kKeys; i += 2) {
-                        const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), scale2, from2);
+                        const float e0 = ex2(fmaf(s[i], mul, -base)), e1 = ex2(fmaf(s[i + 1], mul, -base));
+                        total.x += e0, total.y += e1;
+                        // (by the scale last: the other way round a large one without weight may pass FP32)
+                        x[i / 2] = pack<BF>(e0 * g * (each & 2u ? weights[i] : all), e1 * g * (each & 2u ? weights[i + 1] : all));
+                    }
+                } else {
+                    const float2 mul2 = make_float2(mul, mul), from2 = make_float2(-from, -from);
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 2) {
+                        const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), mul2, from2);
                         const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
                         total = __fadd2_rn(total, e);
-                        x[i / 2] = pack<P_BF>(e.x, e.y);
+                        x[i / 2] = pack<BF>(e.x, e.y);
                     }
                 }
-                sum += total.x + total.y;
+                sum = kCodes ? fmaf(total.x + total.y, give, sum) : sum + (total.x + total.y);
                 tm_store(ts, x);
                 tc_wait_st();
                 tc_before();
@@ -489,7 +487,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 tc_after();
                 const uint32_t flagged = bad_flag[n % kDeal];
                 // what outputs are multiplied by to be relative to the probabilities' maximum
-                const float back = !kCodes ? 1.0f : unit == -INFINITY ? 0.0f : ex2(unit - ref - kUpCodes);
+                const float back = !kCodes ? 1.0f : unit == -INFINITY ? 0.0f : ex2(unit - ref - kUpCodes - P::kUpTile);
                 // infinities and NaN among the values of the dimensions from d0 on that this row sees in tiles that were
                 // looked through, added to what the other tokens came to, which may be an infinity or a NaN of their own
                 auto overlay = [&](uint32_t *o, int d0, auto width) {
@@ -659,7 +657,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     __syncwarp();
                 }
                 if (live && a.lse)
-                    a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - (kCodes ? 0.0f : kUp<P_BF>) + __log2f(sum)) * kLn2;
+                    a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - (kCodes ? 0.0f : kUp<BF>) + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;
@@ -854,14 +852,15 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 __syncwarp();
             };
             // ---- loads ----
-            // Stage 0 of an item is the K tiles that logits run ahead by, stage k + 1 is V k and K k + NB.  Lanes 0 to 7
-            // load the first tile of a stage, 8 to 15 the second: four pieces x two columns of 64 dimensions (16 bits), or
-            // x codes and scales (then lanes 16 to 31 those of a K tile's tokens' values).  A stage that the last warp looks through (16 bits) lands on its raw barrier, and that
-            // warp arrives on the full one when it is done with it; codes land in stages of their own.
+            // The first stages of an item are the K tiles that logits run ahead by, then come V j and K j + NB.  Lanes in
+            // fours, one for each piece of a tile: two columns of 64 dimensions of V, and of K; over codes V's codes and
+            // scales, K's codes and scales, and the scales of the values of K's tokens.  A stage that the last warp looks
+            // through (16 bits) lands on its raw barrier, and that warp arrives on the full one when it is done with it;
+            // codes land in stages of their own.
             constexpr uint32_t kRing = kCodes ? P::kRawStages : P::kStages;
             uint32_t slot = 0, free_phase = 1, q_phase = (1u << NT) - 1, issued = 0, full_phase = 0, raw = 0, raw_phase = 0;
             uint32_t q_issued = 0, stage_no = 0;
-            const uint32_t sel = lane >> 3 & 1u, half = lane >> 2 & 1u, piece = lane & 3u;
+            const uint32_t what = lane >> 2, half = what & 1u, piece = lane & 3u;
             Item it;
             bool fine = true;
             deal(0);
@@ -880,9 +879,10 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     __syncwarp();
                 };
                 // the tile of stage k that this lane has a piece of; -1: none
+                const int32_t lead = lead_of(tiles);
                 auto unit_of = [&](int32_t k) -> int32_t {
-                    const int32_t j = k == 0 ? (int32_t)sel : sel ? k - 1 + (int32_t)NB : k - 1;
-                    return (lane < 16 || (kCodes && half && (k == 0 || sel))) && piece < pieces && j < (k == 0 ? min(tiles, (int32_t)NB) : tiles) ? j : -1;
+                    const int32_t j = what < 2 ? k - lead : k;
+                    return what < (kCodes ? 5u : 4u) && piece < pieces && j >= 0 && j < tiles ? j : -1;
                 };
                 auto token_of = [&](int32_t k) {
                     const int32_t j = unit_of(k);
@@ -894,39 +894,37 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 };
                 int32_t page = tiles ? page_of(0) : 0;
                 auto load = [&](int32_t k) {
-                    const int32_t ahead = k < tiles ? page_of(k + 1) : 0;
+                    const int32_t ahead = k + 1 < tiles + lead ? page_of(k + 1) : 0;
                     const int32_t token = token_of(k);
                     const bool there = (uint32_t)page < a.c.pages;
-                    const uint32_t bad = __ballot_sync(0xffffffffu, token < it.keys && !there && half == 0 && lane < 16);
+                    const uint32_t bad = __ballot_sync(0xffffffffu, token < it.keys && !there);
                     if (!(fine = fine && all_wait(bar((kCodes ? B_TURNED : B_FREE) + slot), free_phase))) return;
-                    const bool two = k == 0 ? NB == 2 && tiles > 1 : k - 1 + (int32_t)NB < tiles;
-                    const bool look = !kCodes && k && !plain(it, first_of(it, k - 1));
+                    const bool values = k >= lead, keys = k < tiles;
+                    const bool look = !kCodes && values && !plain(it, first_of(it, k - lead));
                     const uint32_t on = bar((kCodes ? B_CODES : look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
                     if (lane == 0) {
                         if (bad) atomicOr(a.status, kStatusBadSlot);
-                        bad_pages[stage_no % P::kMeta * 2] = bad & 15u;
-                        bad_pages[stage_no % P::kMeta * 2 + 1] = bad >> 8 & 15u;
-                        bar_expect(on, kCodes ? (P::kRawTile + P::kRawScale) * (two ? 2u : 1u) + P::kRawScale * ((k == 0 ? 1u : 0u) + (two ? 1u : 0u))
-                                              : P::kTile * (two ? 2u : 1u));
+                        bad_pages[stage_no % P::kMeta] = (bad >> 8 & 15u) | (bad & 15u) << 4;
+                        bar_expect(on, kCodes ? (values ? P::kRawTile + P::kRawScale : 0u) + (keys ? P::kRawTile + 2 * P::kRawScale : 0u)
+                                              : (values ? P::kTile : 0u) + (keys ? P::kTile : 0u));
                     }
                     __syncwarp();
                     if (unit_of(k) >= 0) {
-                        const bool value = lane >= 16 || (k && !sel);
                         const int32_t in_page = token & (int32_t)(a.c.page_size - 1);
                         // (past the cache's last page: zeros)
                         const int32_t z = there ? page : (int32_t)a.c.pages;
                         if constexpr (!kCodes) {
                             if (half < P::kChunks)
-                                tma4(base + P::kRing + slot * 2 * P::kTile + sel * P::kTile + half * P::kChunk + (piece << piece_shift) * 128,
-                                     value ? &mv : &mk, on, 64 * half, in_page, it.head, z);
+                                tma4(base + P::kRing + slot * P::kStageBytes + (what >> 1) * P::kTile + half * P::kChunk + (piece << piece_shift) * 128,
+                                     what < 2 ? &mv : &mk, on, 64 * half, in_page, it.head, z);
                         } else {
                             const uint32_t dst = base + P::kRaw + slot * P::kRawStage;
-                            if (half == 0)
-                                tma4(dst + sel * P::kRawTile + (piece << piece_shift) * P::kRow, value ? &mv : &mk, on, 0, in_page, it.head, z);
+                            if (what == 0 || what == 2)
+                                tma4(dst + (what >> 1) * P::kRawTile + (piece << piece_shift) * P::kRow, what == 0 ? &mv : &mk, on, 0, in_page, it.head, z);
                             else {
                                 const uint64_t r = there ? ((uint64_t)page * a.c.heads + it.head << a.c.page_shift) + in_page : 0;
-                                bulk(dst + 2 * P::kRawTile + (lane >= 16 ? 2 + sel : sel) * P::kRawScale + (piece << piece_shift) * P::kGroups * 2,
-                                     (value ? a.c.vs : a.c.ks) + r * P::kGroups, piece_rows * P::kGroups * 2, on);
+                                bulk(dst + 2 * P::kRawTile + (what >> 1) * P::kRawScale + (piece << piece_shift) * P::kGroups * 2,
+                                     (what == 3 ? a.c.ks : a.c.vs) + r * P::kGroups, piece_rows * P::kGroups * 2, on);
                             }
                         }
                     }
@@ -945,7 +943,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     if (span(it, (int)t).tiles && fine) load_q((int)t);
                 if (tiles && fine) load(1);
                 deal(n + 1);
-                for (int32_t k = 2; k <= tiles && fine; ++k) load(k);
+                for (int32_t k = 2; k < tiles + lead && fine; ++k) load(k);
             }
             // copies in flight land before the CTA ends (they have, unless a wait ran out)
             if (lane == 0 && *stop) {
@@ -964,7 +962,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             // ---- products of every second row tile: the warp stays together, one lane issues ----
             const uint32_t half = warp - W_MMA;
             uint32_t slot = 0, full_phase = 0, q_phase = 0, p_phase = 0;  // p_phase: a bit for each buffer of every tile
-            constexpr uint32_t ID_S = product(S_BF, 0, P::kKeys), ID_O = product(P_BF, 1, D), MINE = NT / 2;
+            constexpr uint32_t ID_S = product(BF, 0, P::kKeys), ID_O = product(BF, 1, D), MINE = NT / 2;
             Item it;
             bool fine = true;
             for (uint32_t n = 0; fine && next(n, it); ++n) {
@@ -984,38 +982,41 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const uint32_t q = operand(base + P::kQ + t * P::kQTile, 0), key = operand(k_at, 0);
                     const uint32_t d = tmem + (NB * t + j % NB) * kKeys;
 #pragma unroll
-                    for (uint32_t c = 0; c < P::kChunks; ++c)
+                    for (uint32_t l = 0; l < (P::kLow ? 2u : 1u); ++l)
 #pragma unroll
-                        for (uint32_t s = 0; s < 4; ++s)
-                            mma_ss(d, q + (c * P::kQChunk + 32 * s) / 16, key + (c * P::kChunk + 32 * s) / 16, ID_S, c | s);
+                        for (uint32_t c = 0; c < P::kChunks; ++c)
+#pragma unroll
+                            for (uint32_t s = 0; s < 4; ++s)
+                                mma_ss(d, q + (c * P::kQChunk + 32 * s) / 16, key + (l * P::kTile + c * P::kChunk + 32 * s) / 16, ID_S, l | c | s);
                 };
                 // logits run NB tiles ahead of the outputs
-                if (!(fine = all_wait(bar(B_FULL + slot), full_phase))) break;
+                for (int32_t j = 0; j < lead_of(tiles); ++j) {
+                    const uint32_t at = base + P::kRing + slot * P::kStageBytes + P::kTile;
+                    if (!(fine = all_wait(bar(B_FULL + slot), full_phase))) break;
 #pragma unroll
-                for (uint32_t i = 0; i < MINE; ++i) {
-                    if (!mine[i]) continue;
-                    const uint32_t t = half + 2 * i;
-                    if (!(fine = all_wait(bar((kQTurn ? B_QREADY : B_QFULL) + t), q_phase >> t & 1u))) break;
-                    q_phase ^= 1u << t;
-                    tc_after();
-                    if (elect()) {
-                        const uint32_t at = base + P::kRing + slot * 2 * P::kTile;
-                        logits(t, at, 0);
-                        tc_commit(bar(B_S + NB * t));
-                        if (NB == 2 && mine[i] > 1) {
-                            logits(t, at + P::kTile, 1);
-                            tc_commit(bar(B_S + NB * t + 1));
+                    for (uint32_t i = 0; i < MINE; ++i) {
+                        if (j >= mine[i]) continue;
+                        const uint32_t t = half + 2 * i;
+                        if (j == 0) {
+                            if (!(fine = all_wait(bar((kQTurn ? B_QREADY : B_QFULL) + t), q_phase >> t & 1u))) break;
+                            q_phase ^= 1u << t;
                         }
-                        if (mine[i] <= (int32_t)NB) tc_commit(bar(B_QFREE + t));
+                        tc_after();
+                        if (elect()) {
+                            logits(t, at, j);
+                            tc_commit(bar(B_S + NB * t + j));
+                            if (j + 1 == mine[i]) tc_commit(bar(B_QFREE + t));
+                        }
+                        __syncwarp();
                     }
+                    if (!fine) break;
+                    if (elect()) tc_commit(bar(B_FREE + slot));
                     __syncwarp();
+                    advance();
                 }
                 if (!fine) break;
-                if (elect()) tc_commit(bar(B_FREE + slot));
-                __syncwarp();
-                advance();
                 for (int32_t j = 0; j < tiles; ++j) {
-                    const uint32_t v = slot, at = base + P::kRing + v * 2 * P::kTile;
+                    const uint32_t v = slot, at = base + P::kRing + v * P::kStageBytes;
                     if (!(fine = all_wait(bar(B_FULL + v), full_phase))) break;
                     advance();
 #pragma unroll
@@ -1059,10 +1060,10 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 for (int32_t j = 0; j < tiles; ++j) {
                     const int32_t k0 = first_of(it, j);
                     if (plain(it, k0)) continue;
-                    const uint32_t v = (slot + 1 + (uint32_t)j) % P::kStages;  // past the stage of the first K tiles
+                    const uint32_t v = (slot + (uint32_t)(lead_of(tiles) + j)) % P::kStages;
                     if (!(fine = all_wait(bar(B_RAW + v), raw_phase >> v & 1u))) break;
                     raw_phase ^= 1u << v;
-                    unsigned char *tile = sm + P::kRing + v * 2 * P::kTile;
+                    unsigned char *tile = sm + P::kRing + v * P::kStageBytes;
                     const int32_t rows = min(kKeys, it.keys - k0);
                     uint32_t found = 0;
                     constexpr uint32_t E = QBF ? 0x7f80u : 0x7c00u;
@@ -1110,6 +1111,27 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             };
             // (columns of 64 dimensions begin at one bank: their chunks are written in another order)
             auto order = [](uint32_t c, uint32_t k) { return k ^ (c * kOut / 8 % kOut); };
+            // Exponents (biased, at least that of 2^-100) of the largest and the smallest scale of a tile's tokens that are
+            // there; finite ones, and the smallest of those that are not zero.
+            struct Sizes {
+                uint32_t top, least;
+                __device__ bool apart() const { return least + kNear < top; }
+            };
+            auto sizes = [&](const uint16_t *scales, uint32_t rows, uint32_t bad) {
+                uint32_t top = 27, least = 255;
+#pragma unroll
+                for (uint32_t i = lane; i < P::kKeys * G / 2; i += 32) {
+                    const uint32_t r = 2 * i / G, w = reinterpret_cast<const uint32_t *>(scales)[i];
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const uint32_t token = G == 1 ? r + k : r, e = w >> 16 * k >> 7 & 255u;
+                        const bool counts = e != 255u && token < rows && !(bad >> (token >> piece_shift) & 1u);
+                        top = max(top, counts ? e : 0u);
+                        least = min(least, counts && e ? e : 255u);
+                    }
+                }
+                return Sizes{__reduce_max_sync(0xffffffffu, top), __reduce_min_sync(0xffffffffu, least)};
+            };
             // exponent of the largest finite scale of a token, at least that of 2^-100
             auto largest = [](const uint16_t *scales) {
                 uint32_t big = 0;
@@ -1120,108 +1142,107 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
                 return max(big >> 7, 27u);
             };
-            // a token's scale over that power of two, times 2^10
-            auto scaled = [](uint32_t scale, uint32_t e) {
-                const float f = from_bf16(scale) * __uint_as_float((264 - e) << 23);
+            // what codes are multiplied by, twice: their scale over the power of two of the tile or the token, times 2^kUpTile
+            auto factor = [&](const uint16_t *scales, uint32_t r, uint32_t c, const Sizes &z, bool there) {
+                const uint32_t scale = scales[r * G + (G == 1 ? 0 : c)];
+                uint32_t e = z.top;
+                float f = from_bf16(scale);
+                if (z.apart()) {
+                    if constexpr (F == F_INT8) f = (scale & 0x7f80u) == 0x7f80u ? f : 1.0f, e = 127;
+                    else e = largest(scales + r * G);
+                }
+                f = there ? f * __uint_as_float((254 + P::kUpTile - e) << 23) : 0.0f;
                 return pack<false>(f, f);
             };
-            // 16 bytes of 4-bit codes x a scale in FP16, into the operand
-            auto put4 = [&](unsigned char *tile, uint32_t r, uint32_t c, const uint32_t (&w)[4], uint32_t s2) {
+            // 16 bytes of codes times their factor, into the operand; what FP16 leaves of a product, into `low`
+            auto turn = [&](const uint4 &codes, unsigned char *tile, unsigned char *low, uint32_t r, uint32_t c, uint32_t s2) {
+                const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+                if constexpr (F == F_INT8) {
+                    uint4 v[2], l[2];
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    uint32_t h[4];
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t h[4], g[4];
 #pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b)  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
-                        h[b] = mul_h(sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u), s2);
-                    put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
-                }
-            };
-            // 16 bytes of 8-bit codes, into the operand
-            auto put8 = [&](unsigned char *tile, uint32_t r, uint32_t c, const uint32_t (&w)[4], auto bf) {
-                constexpr bool BF = decltype(bf)::value;
-                uint4 v[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    v[k] = make_uint4(codes8<BF>(w[2 * k], 0x4140), codes8<BF>(w[2 * k], 0x4342), codes8<BF>(w[2 * k + 1], 0x4140),
-                                      codes8<BF>(w[2 * k + 1], 0x4342));
-                const uint32_t first = order(c, 0);
-                put(tile, r, c, first, first ? v[1] : v[0]);
-                put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
-            };
-            // what logits and probabilities of a K tile's tokens are multiplied by: the first of these warps
-            auto weigh = [&](const uint16_t *keys, const uint16_t *values, uint32_t slot_of, uint32_t rows, bool look, uint32_t bad, uint32_t n) {
-                float *by = reinterpret_cast<float *>(sm + P::kScales) + slot_of * 2 * kKeys;
-                uint32_t top = 0;
-#pragma unroll
-                for (uint32_t r = lane; r < P::kKeys; r += 32) {
-                    float k, v;
-                    if constexpr (F == F_INT8) {
-                        k = from_bf16(keys[r]);
-                        uint32_t s = values[r];
-                        if (r >= rows || bad >> (r >> piece_shift) & 1u) s = 0;
-                        else if (look && (s & 0x7f80u) == 0x7f80u) s = 0, bad_flag[n % kDeal] = 1;
-                        v = from_bf16(s);
-                    } else {
-                        k = __uint_as_float((largest(keys + r * G) - 10) << 23);
-                        v = r >= rows ? 0.0f : __uint_as_float((largest(values + r * G) - 10) << 23);
+                        for (int b = 0; b < 4; ++b) {  // 1024 + code + 128
+                            const uint32_t code = sub_h(__byte_perm(w[2 * k + b / 2] ^ 0x80808080u, 0x64646464u, b % 2 ? 0x4342 : 0x4140), 0x64806480u);
+                            h[b] = mul_h(code, s2);
+                            g[b] = low ? rest_h(code, s2, h[b]) : 0u;
+                        }
+                        v[k] = make_uint4(h[0], h[1], h[2], h[3]);
+                        l[k] = make_uint4(g[0], g[1], g[2], g[3]);
                     }
-                    by[r] = k * a.scale;
-                    by[kKeys + r] = v;
-                    top = max(top, __float_as_uint(v) >> 23 & 255u);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                if (lane == 0) reinterpret_cast<float *>(sm + P::kLargest)[slot_of] = (float)top - 127.0f;
-            };
-            auto turn_keys = [&](const unsigned char *codes, const uint16_t *scales, unsigned char *tile) {
-                for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
-                    const uint32_t r = i / kPer, c = i % kPer;
-                    const uint4 x = reinterpret_cast<const uint4 *>(codes)[i];
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    if constexpr (F == F_INT8) put8(tile, r, c, w, std::integral_constant<bool, QBF>());
-                    else put4(tile, r, c, w, scaled(scales[r * G + c], largest(scales + r * G)));
-                }
-            };
-            // (8-bit codes are finite, and what is left out has no weight.  In 4 bits what is past the request's tokens, and
-            // in a tile that is looked through what has a NaN for a scale, is zero.)
-            auto turn_values = [&](const unsigned char *codes, const uint16_t *scales, unsigned char *tile, uint32_t rows, bool look, uint32_t bad) {
-                uint32_t found = 0;
-                for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
-                    const uint32_t r = i / kPer, c = i % kPer;
-                    const uint4 x = reinterpret_cast<const uint4 *>(codes)[i];
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    if constexpr (F == F_INT8) put8(tile, r, c, w, std::false_type());
-                    else {
-                        uint32_t s = scales[r * G + c];
-                        const bool zero = r >= rows || bad >> (r >> piece_shift) & 1u, nan = look && (s & 0x7f80u) == 0x7f80u;
-                        if (nan && !zero) found = 1;
-                        put4(tile, r, c, w, zero || nan ? 0u : scaled(s, largest(scales + r * G)));
+                    const uint32_t first = order(c, 0);
+                    put(tile, r, c, first, first ? v[1] : v[0]);
+                    put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
+                    if (low) {
+                        put(low, r, c, first, first ? l[1] : l[0]);
+                        put(low, r, c, first ^ 1u, first ? l[0] : l[1]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (uint32_t b = 0; b < 4; ++b)  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
+                            h[b] = mul_h(sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u), s2);
+                        put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
                     }
                 }
-                return found;
+            };
+            // what softmax has to know of a K tile: the first of these warps writes it
+            auto weigh = [&](const uint16_t *keys, const uint16_t *values, const Sizes &zk, const Sizes &zv, uint32_t meta, uint32_t rows) {
+                if (lane == 0) {
+                    About &about = reinterpret_cast<About *>(sm + P::kAbout)[meta];
+                    about.mul = __uint_as_float((zk.top - P::kUpTile) << 23) * a.scale;
+                    about.top = (float)zv.top - 127.0f;
+                    about.each = (zk.apart() ? 1u : 0u) | (zv.apart() ? 2u : 0u);
+                }
+                float *by = reinterpret_cast<float *>(sm + P::kScales) + meta * 2 * kKeys;
+                if (zk.apart())
+                    for (uint32_t r = lane; r < P::kKeys; r += 32) {
+                        if constexpr (F == F_INT8) by[r] = from_bf16(keys[r]) * (1.0f / 128.0f) * a.scale;
+                        else by[r] = __uint_as_float((largest(keys + r * G) - P::kUpTile) << 23) * a.scale;
+                    }
+                if (zv.apart())  // (0 for what has no scale, whose weight or values are zero)
+                    for (uint32_t r = lane; r < P::kKeys; r += 32) {
+                        if constexpr (F == F_INT8) by[kKeys + r] = r < rows && (values[r] & 0x7f80u) != 0x7f80u ? from_bf16(values[r]) : 0.0f;
+                        else by[kKeys + r] = r < rows ? __uint_as_float(largest(values + r * G) << 23) : 0.0f;
+                    }
             };
             for (uint32_t n = 0; fine && next(n, it); ++n) {
-                const int32_t tiles = tiles_of(it);
-                for (int32_t k = 0; tiles && k <= tiles; ++k) {
+                const int32_t tiles = tiles_of(it), lead = lead_of(tiles);
+                for (int32_t k = 0; k < tiles + lead; ++k) {
                     if (!(fine = all_wait(bar(B_CODES + from), from_phase))) break;
                     if (!(fine = all_wait(bar(B_FREE + slot), free_phase))) break;
-                    const unsigned char *codes = sm + P::kRaw + from * P::kRawStage;
-                    const uint16_t *scales = reinterpret_cast<const uint16_t *>(codes + 2 * P::kRawTile);
+                    const uint4 *codes = reinterpret_cast<const uint4 *>(sm + P::kRaw + from * P::kRawStage);
+                    const uint16_t *scales = reinterpret_cast<const uint16_t *>(codes + 2 * P::kRawTile / 16);
                     constexpr uint32_t kNext = P::kRawScale / 2;
-                    unsigned char *tile = sm + P::kRing + slot * 2 * P::kTile;
-                    const uint32_t meta = stage_no % P::kMeta * 2;
-                    auto rows_of = [&](int32_t j) { return (uint32_t)min(kKeys, it.keys - first_of(it, j)); };
-                    auto look_of = [&](int32_t j) { return !plain(it, first_of(it, j)); };
-                    if (k == 0) {
-                        if (warp == W_ENDS) weigh(scales, scales + 2 * kNext, meta, rows_of(0), look_of(0), bad_pages[meta], n);
-                        turn_keys(codes, scales, tile);
-                    } else if (turn_values(codes, scales, tile, rows_of(k - 1), look_of(k - 1), bad_pages[meta])) {
-                        bad_flag[n % kDeal] = 1;
+                    unsigned char *tile = sm + P::kRing + slot * P::kStageBytes;
+                    const uint32_t meta = stage_no % P::kMeta, bad = bad_pages[meta];
+                    if (k >= lead) {
+                        // values; of a tile that is looked through, what has a NaN for a scale is zero
+                        const int32_t k0 = first_of(it, k - lead);
+                        const uint32_t rows = (uint32_t)min(kKeys, it.keys - k0);
+                        const bool look = !plain(it, k0);
+                        const Sizes z = sizes(scales, rows, bad >> 4);
+                        uint32_t found = 0;
+                        for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
+                            const uint32_t r = i / kPer, c = i % kPer;
+                            bool there = r < rows && !(bad >> 4 >> (r >> piece_shift) & 1u);
+                            if (look && there && (scales[r * G + (G == 1 ? 0 : c)] & 0x7f80u) == 0x7f80u) there = false, found = 1;
+                            turn(codes[i], tile, nullptr, r, c, factor(scales, r, c, z, there));
+                        }
+                        if (found) bad_flag[n % kDeal] = 1;
                     }
-                    const int32_t ahead = k == 0 ? 1 : k - 1 + (int32_t)NB;
-                    if (k == 0 ? NB == 2 && tiles > 1 : ahead < tiles) {
-                        if (warp == W_ENDS)
-                            weigh(scales + kNext, scales + 3 * kNext, meta + 1, rows_of(ahead), look_of(ahead), bad_pages[meta + 1], n);
-                        turn_keys(codes + P::kRawTile, scales + kNext, tile + P::kTile);
+                    if (k < tiles) {
+                        const uint32_t rows = (uint32_t)min(kKeys, it.keys - first_of(it, k));
+                        const Sizes z = sizes(scales + kNext, rows, bad);
+                        if (warp == W_ENDS) weigh(scales + kNext, scales + 2 * kNext, z, sizes(scales + 2 * kNext, rows, bad), meta, rows);
+                        for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
+                            const uint32_t r = i / kPer, c = i % kPer;
+                            const bool there = r < rows && !(bad >> (r >> piece_shift) & 1u);
+                            turn(codes[P::kRawTile / 16 + i], tile + P::kTile, P::kLow ? tile + 2 * P::kTile : nullptr, r, c, factor(scales + kNext, r, c, z, there));
+                        }
                     }
                     fence_async();
                     __syncwarp();

@@ -8,9 +8,10 @@ append   a rotated value is three FP32 roundings of a c and b s, of at most |a| 
          rounded once.  Rows that become codes are 64-bit and rounded to FP32 once: their codes are those
          of the 64-bit row, but for ties.
 chunk    what test_gpu_serving says: u |o| + (u + 3e-5) A, A = sum p_t |v_t|, for the roundings of probabilities
-         and outputs; over 8- and 4-bit pages probabilities are rounded to FP16, whatever the queries' type, and
-         held to 2^-34 of the row's largest product with a value scale, times a code of at most 2^4 of it (4 bits)
-         or 2^7 (8 bits): 2^-25 (A + 1) covers it for rows of one size.  The log sum is FP32 throughout: 3e-5 absolute.
+         and outputs; over 8- and 4-bit pages probabilities are rounded to FP16, whatever the queries' type, and values
+         in 8 bits too (2 u + u^2 of FP16 in place of u), and products are held to 2^-34 of the row's largest
+         probability x value scale, times a code of at most 2^4 of it (4 bits) or 2^7 (8 bits): 2^-25 (A + 1) covers it
+         for rows of one size.  The log sum is FP32 throughout: 3e-5 absolute.
 logits   every step is one FP32 rounding of what it gives: 5 u of the sum of the steps' magnitudes.
 """
 import math
@@ -254,7 +255,7 @@ def seen_of(n, length, window, sinks):
 def close_chunk(out, lse, ref, dtype, fmt):
     import torch
     want, want_lse, mag, small = ref
-    u = U[dtype] if fmt in ("f16", "bf16") else U["f16"]
+    u = U[dtype] if fmt in ("f16", "bf16") else U["f16"] if fmt == "int4" else 2 * U["f16"] + U["f16"] ** 2
     tol = U[dtype] * want.abs() + (u + 3e-5) * mag + 1e-30
     if dtype == "f16" or fmt not in ("f16", "bf16"):
         tol = tol + 2.0 ** -25 * (small + mag + (1 if dtype == "f16" else 0))
@@ -552,6 +553,48 @@ def test_chunk_sizes_of_rows(cuda, fmt, n):
     for dtype, by in (("bf16", 1.0), ("bf16", 1e-6), ("f16", 1e-2)):
         cache.write(randn(1, length, 1, 64) * small / by, randn(2, length, 1, 64) * (size if dtype == "bf16" else small), torch.arange(length, device="cuda"))
         check_chunk(cache, (randn(3, n, 3, 64) * by).to(types()[dtype]), [n], table, lens, dtype)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("int8", "f16"), ("int8", "bf16"), ("int4", "f16"), ("int4", "bf16")])
+@pytest.mark.parametrize("dim,hq", [(64, 2), (64, 7), (128, 3), (128, 16)])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("big", [1e5, 1e12, 1e30])
+@pytest.mark.parametrize("where", ["first", "last", "half"])
+def test_chunk_large_values_without_weight(cuda, fmt, dtype, dim, hq, n, big, where):
+    """Rows of large values that no row gives weight to leave the others as they are, and so do keys that are next to
+    nothing beside them.  Tolerance: as test_gpu_serving_extremes derives it for one token, 2^-33 of the row's largest
+    probability x value for every token, and FP16's rounding of values in 8 bits."""
+    import torch
+    from bgtq import PagedCache
+    length = 700
+    far = torch.zeros(length, dtype=torch.bool, device="cuda")
+    if where == "half":
+        far[1::2] = True
+    else:
+        far[{"first": 0, "last": length - n}[where]] = True
+    k, v = randn(1, length, 1, dim), randn(2, length, 1, dim) + 0.5
+    k[::5] *= 1e-13
+    k[:, 0, 0] = 0
+    k[far] = 0
+    k[far, 0, 0] = -2400.0                     # logits of -300: weights below 2^-420
+    v[far] = big
+    q = randn(3, n, hq, dim, dtype=dtype)
+    q[..., 0] = 1.0
+    cache = PagedCache(1, dim, 44, 16, fmt)
+    t = torch.arange(length, device="cuda")
+    cache.write(k, v, t)
+    table = torch.arange(44, dtype=torch.int32, device="cuda")[None]
+    out, lse = cache.attend_chunk(q, starts_of([n]), table, torch.tensor([length], dtype=torch.int32, device="cuda"), scale=1.0 / 8, lse=True)
+    rk, rv = (x[:, 0].double() for x in cache.read(t, torch.float32))
+    for h in range(hq):
+        s = (q[:, h].double() @ rk.T / 8).masked_fill(~seen_of(n, length, None, 0), -math.inf)
+        p = torch.softmax(s, -1)
+        want, mag = p @ rv, p @ rv.abs()
+        least = length * 2.0 ** -33 * (p * rv.abs().amax(-1)).amax(-1, keepdim=True)
+        tol = U[dtype] * want.abs() + (2 * U["f16"] + 3e-5) * mag + least + (2.0 ** -25 if dtype == "f16" else 0)
+        off = (out[:, h].double() - want).abs()
+        assert bool((off <= tol).all()), float((off / tol).max())
+        assert float((lse[:, h].double() - torch.logsumexp(s, -1)).abs().max()) <= 3e-5
 
 
 def test_indices_outside_the_cache_are_left_out_and_reported(cuda):
