@@ -56,15 +56,16 @@ struct Plan {
     static constexpr uint32_t kBufs = NT == 4 ? 1 : 2;             // of logits, for each row tile
     static constexpr uint32_t kKeys = 64;                          // of a K or V tile
     static constexpr uint32_t kColO = kTiles * kBufs * kKeys;      // the first column of the outputs
-    static constexpr uint32_t kEnds = kCodes && NT == 2 ? 5 : 1;   // warps that look at, or turn, tiles
+    static constexpr uint32_t kEnds = kCodes ? (NT == 4 ? 5 : 9) : 1;  // warps that look at, or turn, tiles
     static constexpr uint32_t kThreads = 128 * NT + 32 * (3 + kEnds);
     // Registers after the hand-over, of softmax's warps and of the others: what the launch has, in all.
-    static constexpr uint32_t kSoft = NT == 4 ? 104 : kCodes ? 168 : 216, kRest = NT == 4 ? 64 : kCodes ? 88 : 72;
+    static constexpr uint32_t kSoft = NT == 4 ? (kCodes ? 96 : 104) : kCodes ? 128 : 216, kRest = NT == 4 ? (kCodes ? 48 : 64) : 72;
     static constexpr int kFma = D == 64 ? 2 : 6;                   // exponentials of 16 on the FMA pipe
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
-    static constexpr bool kLow = F == F_INT8;                      // keys have a second operand
+    static constexpr bool kOwn = F == F_INT8 && D == 128;          // every key's logits are multiplied by its own scale
+    static constexpr bool kLow = F == F_INT8 && D == 64;           // keys have a second operand
     static constexpr uint32_t kStageBytes = (kLow ? 3 : 2) * kTile;  // a V tile and a K tile
     static constexpr uint32_t kStages = D == 128 ? (kLow ? 2 : kCodes ? 3 : 4) : (kLow ? 4 : kCodes ? 5 : 7);
     // 8- and 4-bit pages: tiles as they lie in the pages, and their scales
@@ -72,15 +73,15 @@ struct Plan {
     static constexpr uint32_t kRawTile = kKeys * kRow, kRawScale = kKeys * kGroups * 2;
     // (the two tiles, the scales of both, and those of the K tile's tokens' values)
     static constexpr uint32_t kRawStage = 2 * kRawTile + 3 * kRawScale, kRawStages = kCodes ? (D == 128 ? 2 : 4) : 0;
-    static constexpr int kUpTile = F == F_INT8 ? 7 : 10;           // log2 of what a tile's largest scale goes to
+    static constexpr int kUpTile = F == F_INT8 ? 7 : 10, kUpKeys = kOwn ? 0 : kUpTile;  // log2 of what a tile's largest scale goes to
     // What softmax has to know of the K tile in a stage is kept until that tile's logits are done with, which is sure
     // when the load warp has gone all stages and the logits' lead further.
     static constexpr uint32_t kMeta = kRawStages + kStages + kBufs <= 8 ? 8 : 16;
     static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kRaw = kRing + kStages * kStageBytes;
     static constexpr int kTurn = NT == 4 ? 16 : 32;                // dimensions of an output row stored at a time
     static constexpr uint32_t kOut = kRaw + kRawStages * kRawStage;                     // [softmax warps][32 rows][kTurn] outputs
-    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][kKeys] what logits, and
-                                                                                        // probabilities, are multiplied by
+    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][kKeys] what logits, and, as
+                                                                                        // logarithms, probabilities are multiplied by
     static constexpr uint32_t kAbout = kScales + (kCodes ? kMeta * 2 * kKeys * 4 : 0);     // [kMeta] About
     static constexpr uint32_t kBadPages = kAbout + (kCodes ? kMeta * 16 : 0);              // [kMeta] pieces without a page: K, V
     static constexpr uint32_t kItems = kBadPages + kMeta * 4;      // [kDeal] Item
@@ -281,12 +282,17 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
         // (of an item only what the loop needs stays in registers; the rest is read again at its end)
         for (uint32_t n = 0;; ++n) {
             int32_t tiles, all_tiles;
+            int32_t full_from, full_upto;  // units of the piece that every row sees all of (but sinks)
             float q_mul = 1.0f;  // the power of two that this row's queries were divided by
             {
                 Item it;
                 if (!next(n, it)) break;
                 tiles = span(it, t).tiles;
                 all_tiles = tiles_of(it);
+                const int32_t last = it.place + it.count - 1;
+                full_from = a.window ? (max(0, last - (int32_t)a.window + 1) + kKeys - 1) / kKeys : 0;
+                full_upto = max(0, min(it.keys, it.place + 1)) / kKeys - it.gap - it.from;
+                full_from = max(full_from - it.gap, it.sunk) - it.from;
             }
             bool fine = true;
             if constexpr (kQTurn) {
@@ -333,42 +339,37 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 tm_load(ts + 32, x + 32);
                 // where the K tile lay
                 const uint32_t meta = (stage_no + (uint32_t)j) % P::kMeta;
-                tc_wait_ld();
-                float *s = reinterpret_cast<float *>(x);
+                const uint32_t bad = bad_pages[meta] & 15u;
                 float mul = a.scale, largest = 0.0f;
                 uint32_t each = 0;
                 if constexpr (kCodes) {
-                    const About &about = reinterpret_cast<const About *>(sm + P::kAbout)[meta];
+                    const float4 about = *reinterpret_cast<const float4 *>(sm + P::kAbout + meta * sizeof(About));
                     // (not 0, which minus infinity is not multiplied by: such logits are next to nothing)
-                    mul = fmaxf(about.mul * q_mul, 1.2e-38f), largest = about.top, each = about.each;
-                    if (each & 1u) {
-                        const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
+                    mul = fmaxf(about.x * q_mul, 1.2e-38f), largest = about.y, each = __float_as_uint(about.z);
+                }
+                tc_wait_ld();
+                float *s = reinterpret_cast<float *>(x);
+                if (kCodes && (P::kOwn || each & 1u)) {
+                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
 #pragma unroll
-                        for (int i = 0; i < kKeys; i += 4) {  // (with the queries' power first: a product of up to 2^35 may pass FP32)
-                            const float4 f = by[i / 4];
-                            s[i] *= f.x * q_mul, s[i + 1] *= f.y * q_mul, s[i + 2] *= f.z * q_mul, s[i + 3] *= f.w * q_mul;
-                        }
-                        mul = 1.0f;
+                    for (int i = 0; i < kKeys; i += 4) {
+                        const float4 f = by[i / 4];
+                        const float2 f0 = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y));
+                        const float2 f1 = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
+                        s[i] = f0.x, s[i + 1] = f0.y, s[i + 2] = f1.x, s[i + 3] = f1.y;
                     }
                 }
-                {
+                if (j < full_from || j >= full_upto || bad) {
                     const volatile Item &it = items[n % kDeal];
                     const int32_t u = it.from + j, k0 = (u < it.sunk ? u : u + it.gap) * kKeys;
-                    const int32_t place = it.place, keys = it.keys;
-                    const bool full = k0 + kKeys <= min(keys, place + 1) &&
-                                      (!a.window || place + it.count - 1 - k0 < (int32_t)a.window || (uint32_t)(k0 + kKeys) <= a.sinks);
-                    const uint32_t bad = bad_pages[meta] & 15u;
-                    if (__any_sync(0xffffffffu, !full || bad)) {
-                        uint64_t m = mask_of(place + t * (int32_t)per + (int32_t)p, keys, k0);
-                        if (bad)
-                            for (uint32_t c = 0; c < pieces; ++c)
-                                if (bad >> c & 1u) m &= ~((piece_rows == 64 ? ~0ull : (1ull << piece_rows) - 1) << (c << piece_shift));
-                        const uint32_t m0 = (uint32_t)m, m1 = (uint32_t)(m >> 32);
+                    uint64_t m = mask_of(it.place + t * (int32_t)per + (int32_t)p, it.keys, k0);
+                    for (uint32_t c = 0; c < pieces; ++c)
+                        if (bad >> c & 1u) m &= ~((piece_rows == 64 ? ~0ull : (1ull << piece_rows) - 1) << (c << piece_shift));
+                    const uint32_t m0 = (uint32_t)m, m1 = (uint32_t)(m >> 32);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (!(m0 >> i & 1u)) s[i] = -INFINITY;
-                            if (!(m1 >> i & 1u)) s[i + 32] = -INFINITY;
-                        }
+                    for (int i = 0; i < 32; ++i) {
+                        if (!(m0 >> i & 1u)) s[i] = -INFINITY;
+                        if (!(m1 >> i & 1u)) s[i + 32] = -INFINITY;
                     }
                 }
                 float c0 = max3(s[0], s[1], s[2]), c1 = max3(s[3], s[4], s[5]), c2 = max3(s[6], s[7], s[8]);
@@ -384,31 +385,49 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 c1 = max3(c1, s[kKeys - 2], s[kKeys - 1]);
                 const float top = fmaxf(max3(c0, c1, c2), c3) * mul;
                 const bool grown = top > ref + kLazy;  // each row for itself, not by the others of the warp
-                float alpha = 0.0f, beta = 0.0f;       // 2^alpha: what sums are multiplied by, 2^beta: outputs
+                float beta = 0.0f;                     // 2^beta: what outputs are multiplied by
+                float give = 1.0f;                     // codes: what the sum of the tile's probabilities is multiplied by
                 bool moved = j != 0 && grown;
                 if constexpr (kCodes) {
-                    if (j == 0 || grown) {
-                        alpha = j == 0 ? 0.0f : ref - top;
-                        ref = top;
-                    }
                     // no product is larger than the largest probability x the largest scale; where scales are far apart, look
-                    float peak = top + largest;
-                    if (each & 2u && __any_sync(0xffffffffu, peak > unit + kRoom)) {
-                        const float *weights = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
-                        peak = -INFINITY;
+                    const float most = unit - largest - (kApart + kUpCodes);
+                    bool slow = grown || top + largest > unit + kRoom || most > ref || each & 2u;
+                    moved = false;
+                    if (__any_sync(0xffffffffu, slow)) {
+                        if (j == 0 || grown) {
+                            sum *= j == 0 ? 1.0f : ex2(ref - top);
+                            ref = top;
+                        }
+                        const float *logs = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
+                        float peak = top + largest;
+                        if (each & 2u) {
+                            peak = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < kKeys; ++i)  // (an exponent as a number: 2^23 + n is 0x4b000000 | n)
-                            peak = fmaxf(peak, fmaf(s[i], mul, __uint_as_float(0x4b000000u | __float_as_uint(weights[i]) >> 23) - (8388608.0f + 127.0f)));
+                            for (int i = 0; i < kKeys; ++i) peak = fmaxf(peak, fmaf(s[i], mul, logs[i]));
+                        }
+                        const float now = fmaxf(peak > unit + kRoom ? peak : unit, ref - kApart);
+                        if (j != 0 && now > unit) beta = unit - now, moved = true;
+                        unit = now;
+                        if (__any_sync(0xffffffffu, (each & 2u) || unit - largest - (kApart + kUpCodes) > ref)) {
+                            // the sum for itself, and logits of the products
+                            const float from = ref == -INFINITY ? 0.0f : ref;
+                            float more = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < kKeys; ++i) {
+                                const float v = s[i] * mul;
+                                more += ex2(v - from);
+                                s[i] = each & 2u ? v + (logs[i] - largest) : v;
+                            }
+                            sum += more;
+                            mul = 1.0f, give = 0.0f;
+                        }
                     }
-                    const float now = fmaxf(peak > unit + kRoom ? peak : unit, ref - kApart);
-                    beta = j != 0 && now > unit ? unit - now : 0.0f;
-                    unit = now;
-                    sum *= ex2(alpha);
-                    moved = beta != 0.0f;
+                    give *= ex2(unit - largest - kUpCodes - ref);
+                    if (give != give) give = 0.0f;
                 } else {
                     if (j == 0) ref = top;
                     else if (grown) {
-                        alpha = beta = ref - top;
+                        beta = ref - top;
                         ref = top;
                     }
                 }
@@ -434,35 +453,15 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     }
                 }
                 // probabilities; over codes, times the largest scale of the tile's values, relative to 2^unit
-                float from = ref - kUp<BF>, give = 1.0f;  // give: what their sum is multiplied by
-                bool apart = false;
-                if constexpr (kCodes) {
-                    from = unit - largest - kUpCodes;
-                    apart = __any_sync(0xffffffffu, (each & 2u) || from - ref > kApart);
-                    give = ex2(from - ref);
-                }
-                if (ref == -INFINITY) from = 0.0f, give = 1.0f;
+                const float from = ref == -INFINITY ? 0.0f : kCodes ? unit - largest - kUpCodes : ref - kUp<BF>;
                 float2 total = make_float2(0.0f, 0.0f);
-                if (kCodes && apart) {
-                    const float *weights = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
-                    const float g = unit == -INFINITY ? 0.0f : ex2(ref - unit + kUpCodes), all = ex2(largest), base = ref == -INFINITY ? 0.0f : ref;
-                    give = 1.0f;
+                const float2 mul2 = make_float2(mul, mul), from2 = make_float2(-from, -from);
 #pragma unroll
-                    for (int i = 0; i < kKeys; i += 2) {
-                        const float e0 = ex2(fmaf(s[i], mul, -base)), e1 = ex2(fmaf(s[i + 1], mul, -base));
-                        total.x += e0, total.y += e1;
-                        // (by the scale last: the other way round a large one without weight may pass FP32)
-                        x[i / 2] = pack<BF>(e0 * g * (each & 2u ? weights[i] : all), e1 * g * (each & 2u ? weights[i + 1] : all));
-                    }
-                } else {
-                    const float2 mul2 = make_float2(mul, mul), from2 = make_float2(-from, -from);
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 2) {
-                        const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), mul2, from2);
-                        const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
-                        total = __fadd2_rn(total, e);
-                        x[i / 2] = pack<BF>(e.x, e.y);
-                    }
+                for (int i = 0; i < kKeys; i += 2) {
+                    const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), mul2, from2);
+                    const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
+                    total = __fadd2_rn(total, e);
+                    x[i / 2] = pack<BF>(e.x, e.y);
                 }
                 sum = kCodes ? fmaf(total.x + total.y, give, sum) : sum + (total.x + total.y);
                 tm_store(ts, x);
@@ -1098,19 +1097,29 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             }
         } else {
             // ---- codes into operands ----
-            const uint32_t me = (warp - W_ENDS) * 32 + lane;
-            constexpr uint32_t kMany = 32 * P::kEnds, G = P::kGroups;
+            // The first of these warps sees to what softmax has to know, the others turn.
+            constexpr uint32_t G = P::kGroups, kTurners = 32 * (P::kEnds - 1);
+            const uint32_t me = threadIdx.x - 32 * (W_ENDS + 1);  // (the first warp has none)
+            const bool weighs = warp == W_ENDS, turns = !weighs;
+            // 16 bytes of a row: in 8 bits 16 dimensions, two chunks of the operand; in 4 bits 32, four chunks.  A thread has
+            // kEach of them of one row, the q-th at q ^ twist(row): a phase of eight lanes then meets 128 different
+            // bytes, reading and writing (of 32-byte rows, every second one twice).
+            constexpr uint32_t kPer = P::kRow / 16, kOut = F == F_INT8 ? 2 : 4;
+            constexpr uint32_t kEach = P::kKeys * kPer / kTurners;
+            auto twist = [](uint32_t r) {
+                if constexpr (kPer == 8) return r & 7u;
+                else if constexpr (kPer == 2) return r >> 2 & 1u;
+                else if constexpr (F == F_INT4) return r >> 1 & 3u;
+                else return (r >> 2 & 1u) | ((r >> 1 ^ r >> 2) & 1u) << 1;
+            };
+            const uint32_t row = me & 63u;
+            auto place_of = [&](uint32_t q) { return ((me >> 6) * kEach + q) ^ twist(row); };
             uint32_t slot = 0, free_phase = 1, from = 0, from_phase = 0, stage_no = 0;
             Item it;
             bool fine = true;
-            // 16 bytes of a row: in 8 bits 16 dimensions, two chunks of the operand; in 4 bits 32, four chunks
-            constexpr uint32_t kPer = P::kRow / 16, kOut = F == F_INT8 ? 2 : 4;
-            auto put = [&](unsigned char *tile, uint32_t r, uint32_t c, uint32_t k, uint4 v) {
-                const uint32_t u = c * kOut + k;
+            auto put = [&](unsigned char *tile, uint32_t r, uint32_t u, uint4 v) {
                 *reinterpret_cast<uint4 *>(tile + u / 8 * P::kChunk + r * 128 + ((u % 8 ^ (r & 7u)) << 4)) = v;
             };
-            // (columns of 64 dimensions begin at one bank: their chunks are written in another order)
-            auto order = [](uint32_t c, uint32_t k) { return k ^ (c * kOut / 8 % kOut); };
             // Exponents (biased, at least that of 2^-100) of the largest and the smallest scale of a tile's tokens that are
             // there; finite ones, and the smallest of those that are not zero.
             struct Sizes {
@@ -1118,18 +1127,28 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 __device__ bool apart() const { return least + kNear < top; }
             };
             auto sizes = [&](const uint16_t *scales, uint32_t rows, uint32_t bad) {
+                const uint32_t *words = reinterpret_cast<const uint32_t *>(scales);
+                uint32_t w[G], big = 0, small = ~0u;
+#pragma unroll
+                for (uint32_t i = 0; i < G; ++i) {
+                    w[i] = words[lane + 32 * i];
+                    big = i ? __vmaxu2(big, w[i]) : w[i];
+                    small = i ? __vminu2(small, w[i]) : w[i];
+                }
+                big = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
+                small = __reduce_min_sync(0xffffffffu, min(small & 0xffffu, small >> 16));
+                // (all tokens there, no scale zero, negative or NaN: nearly always)
+                if (rows == P::kKeys && !bad && big < 0x7f80u && small >= 0x80u) return Sizes{max(big >> 7, 27u), small >> 7};
                 uint32_t top = 27, least = 255;
 #pragma unroll
-                for (uint32_t i = lane; i < P::kKeys * G / 2; i += 32) {
-                    const uint32_t r = 2 * i / G, w = reinterpret_cast<const uint32_t *>(scales)[i];
+                for (uint32_t i = 0; i < G; ++i)
 #pragma unroll
                     for (uint32_t k = 0; k < 2; ++k) {
-                        const uint32_t token = G == 1 ? r + k : r, e = w >> 16 * k >> 7 & 255u;
+                        const uint32_t token = (2 * (lane + 32 * i) + k) / G, e = w[i] >> 16 * k >> 7 & 255u;
                         const bool counts = e != 255u && token < rows && !(bad >> (token >> piece_shift) & 1u);
                         top = max(top, counts ? e : 0u);
                         least = min(least, counts && e ? e : 255u);
                     }
-                }
                 return Sizes{__reduce_max_sync(0xffffffffu, top), __reduce_min_sync(0xffffffffu, least)};
             };
             // exponent of the largest finite scale of a token, at least that of 2^-100
@@ -1154,102 +1173,108 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 f = there ? f * __uint_as_float((254 + P::kUpTile - e) << 23) : 0.0f;
                 return pack<false>(f, f);
             };
-            // 16 bytes of codes times their factor, into the operand; what FP16 leaves of a product, into `low`
-            auto turn = [&](const uint4 &codes, unsigned char *tile, unsigned char *low, uint32_t r, uint32_t c, uint32_t s2) {
+            // 16 bytes of codes times their factor, into the operand; what FP16 leaves of a product, into the second one
+            auto turn = [&](const uint4 &codes, unsigned char *tile, auto plain_codes, auto low, uint32_t r, uint32_t c, uint32_t s2) {
                 const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-                if constexpr (F == F_INT8) {
-                    uint4 v[2], l[2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        uint32_t h[4], g[4];
+                for (uint32_t k = 0; k < kOut; ++k) {
+                    uint32_t h[4], l[4];
 #pragma unroll
-                        for (int b = 0; b < 4; ++b) {  // 1024 + code + 128
-                            const uint32_t code = sub_h(__byte_perm(w[2 * k + b / 2] ^ 0x80808080u, 0x64646464u, b % 2 ? 0x4342 : 0x4140), 0x64806480u);
-                            h[b] = mul_h(code, s2);
-                            g[b] = low ? rest_h(code, s2, h[b]) : 0u;
-                        }
-                        v[k] = make_uint4(h[0], h[1], h[2], h[3]);
-                        l[k] = make_uint4(g[0], g[1], g[2], g[3]);
+                    for (uint32_t b = 0; b < 4; ++b) {
+                        uint32_t code;
+                        if constexpr (F == F_INT8)  // 1024 + code + 128
+                            code = sub_h(__byte_perm(w[2 * k + b / 2] ^ 0x80808080u, 0x64646464u, b % 2 ? 0x4342 : 0x4140), 0x64806480u);
+                        else  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
+                            code = sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u);
+                        h[b] = decltype(plain_codes)::value ? code : mul_h(code, s2);
+                        if constexpr (decltype(low)::value) l[b] = rest_h(code, s2, h[b]);
                     }
-                    const uint32_t first = order(c, 0);
-                    put(tile, r, c, first, first ? v[1] : v[0]);
-                    put(tile, r, c, first ^ 1u, first ? v[0] : v[1]);
-                    if (low) {
-                        put(low, r, c, first, first ? l[1] : l[0]);
-                        put(low, r, c, first ^ 1u, first ? l[0] : l[1]);
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (uint32_t b = 0; b < 4; ++b)  // 1024 + code + 8 in the low half, 64 + code + 8 in the high one
-                            h[b] = mul_h(sub_h((__byte_perm(w[k], 0, b | b << 8 | 0x4040u) & 0x00f0000fu) | 0x54006400u, 0x54806408u), s2);
-                        put(tile, r, c, k, make_uint4(h[0], h[1], h[2], h[3]));
-                    }
+                    put(tile, r, c * kOut + k, make_uint4(h[0], h[1], h[2], h[3]));
+                    if constexpr (decltype(low)::value) put(tile + P::kTile, r, c * kOut + k, make_uint4(l[0], l[1], l[2], l[3]));
                 }
             };
             // what softmax has to know of a K tile: the first of these warps writes it
             auto weigh = [&](const uint16_t *keys, const uint16_t *values, const Sizes &zk, const Sizes &zv, uint32_t meta, uint32_t rows) {
                 if (lane == 0) {
                     About &about = reinterpret_cast<About *>(sm + P::kAbout)[meta];
-                    about.mul = __uint_as_float((zk.top - P::kUpTile) << 23) * a.scale;
+                    about.mul = __uint_as_float((zk.top - P::kUpKeys) << 23) * a.scale;
                     about.top = (float)zv.top - 127.0f;
                     about.each = (zk.apart() ? 1u : 0u) | (zv.apart() ? 2u : 0u);
                 }
                 float *by = reinterpret_cast<float *>(sm + P::kScales) + meta * 2 * kKeys;
-                if (zk.apart())
+                if (P::kOwn || zk.apart())  // over the tile's largest
                     for (uint32_t r = lane; r < P::kKeys; r += 32) {
-                        if constexpr (F == F_INT8) by[r] = from_bf16(keys[r]) * (1.0f / 128.0f) * a.scale;
-                        else by[r] = __uint_as_float((largest(keys + r * G) - P::kUpTile) << 23) * a.scale;
+                        if constexpr (F == F_INT8) by[r] = from_bf16(keys[r]) * __uint_as_float((254 - zk.top) << 23);
+                        else by[r] = ex2((float)largest(keys + r * G) - (float)zk.top);
                     }
-                if (zv.apart())  // (0 for what has no scale, whose weight or values are zero)
+                if (zv.apart())  // (logarithms; what has no scale has no weight, or no values)
                     for (uint32_t r = lane; r < P::kKeys; r += 32) {
-                        if constexpr (F == F_INT8) by[kKeys + r] = r < rows && (values[r] & 0x7f80u) != 0x7f80u ? from_bf16(values[r]) : 0.0f;
-                        else by[kKeys + r] = r < rows ? __uint_as_float(largest(values + r * G) << 23) : 0.0f;
+                        if constexpr (F == F_INT8) by[kKeys + r] = r < rows && (values[r] & 0x7f80u) != 0x7f80u && values[r] ? __log2f(from_bf16(values[r])) : -150.0f;
+                        else by[kKeys + r] = r < rows ? (float)largest(values + r * G) - 127.0f : -150.0f;
                     }
+            };
+            // A tile's codes, and what they are multiplied by, in registers
+            struct Batch {
+                uint4 codes[kEach];
+                uint32_t s2[kEach];
+            };
+            // (of values in a tile that is looked through, what has a NaN for a scale is zero)
+            auto fetch = [&](Batch &b, const uint4 *codes, const uint16_t *scales, uint32_t rows, uint32_t bad, bool look) {
+#pragma unroll
+                for (uint32_t q = 0; q < kEach; ++q) b.codes[q] = codes[row * kPer + place_of(q)];
+                const Sizes z = sizes(scales, rows, bad);
+                uint32_t found = 0;
+                const bool there = row < rows && !(bad >> (row >> piece_shift) & 1u);
+#pragma unroll
+                for (uint32_t q = 0; q < kEach; ++q) {
+                    if (G == 1 && q) {
+                        b.s2[q] = b.s2[0];
+                        continue;
+                    }
+                    const uint32_t c = place_of(q);
+                    const bool nan = look && there && (scales[row * G + (G == 1 ? 0 : c)] & 0x7f80u) == 0x7f80u;
+                    found |= nan;
+                    b.s2[q] = factor(scales, row, c, z, there && !nan);
+                }
+                return found;
+            };
+            auto write = [&](const Batch &b, unsigned char *tile, auto plain_codes, auto low) {
+#pragma unroll
+                for (uint32_t q = 0; q < kEach; ++q) turn(b.codes[q], tile, plain_codes, low, row, place_of(q), b.s2[q]);
             };
             for (uint32_t n = 0; fine && next(n, it); ++n) {
                 const int32_t tiles = tiles_of(it), lead = lead_of(tiles);
                 for (int32_t k = 0; k < tiles + lead; ++k) {
                     if (!(fine = all_wait(bar(B_CODES + from), from_phase))) break;
-                    if (!(fine = all_wait(bar(B_FREE + slot), free_phase))) break;
                     const uint4 *codes = reinterpret_cast<const uint4 *>(sm + P::kRaw + from * P::kRawStage);
                     const uint16_t *scales = reinterpret_cast<const uint16_t *>(codes + 2 * P::kRawTile / 16);
                     constexpr uint32_t kNext = P::kRawScale / 2;
                     unsigned char *tile = sm + P::kRing + slot * P::kStageBytes;
                     const uint32_t meta = stage_no % P::kMeta, bad = bad_pages[meta];
-                    if (k >= lead) {
-                        // values; of a tile that is looked through, what has a NaN for a scale is zero
+                    const bool values = k >= lead, keys = k < tiles;
+                    const uint32_t key_rows = keys ? (uint32_t)min(kKeys, it.keys - first_of(it, k)) : 0;
+                    Batch of_keys, of_values;
+                    if (turns && values) {
                         const int32_t k0 = first_of(it, k - lead);
-                        const uint32_t rows = (uint32_t)min(kKeys, it.keys - k0);
-                        const bool look = !plain(it, k0);
-                        const Sizes z = sizes(scales, rows, bad >> 4);
-                        uint32_t found = 0;
-                        for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
-                            const uint32_t r = i / kPer, c = i % kPer;
-                            bool there = r < rows && !(bad >> 4 >> (r >> piece_shift) & 1u);
-                            if (look && there && (scales[r * G + (G == 1 ? 0 : c)] & 0x7f80u) == 0x7f80u) there = false, found = 1;
-                            turn(codes[i], tile, nullptr, r, c, factor(scales, r, c, z, there));
-                        }
-                        if (found) bad_flag[n % kDeal] = 1;
+                        if (fetch(of_values, codes, scales, (uint32_t)min(kKeys, it.keys - k0), bad >> 4, !plain(it, k0))) bad_flag[n % kDeal] = 1;
                     }
-                    if (k < tiles) {
-                        const uint32_t rows = (uint32_t)min(kKeys, it.keys - first_of(it, k));
-                        const Sizes z = sizes(scales + kNext, rows, bad);
-                        if (warp == W_ENDS) weigh(scales + kNext, scales + 2 * kNext, z, sizes(scales + 2 * kNext, rows, bad), meta, rows);
-                        for (uint32_t i = me; i < P::kKeys * kPer; i += kMany) {
-                            const uint32_t r = i / kPer, c = i % kPer;
-                            const bool there = r < rows && !(bad >> (r >> piece_shift) & 1u);
-                            turn(codes[P::kRawTile / 16 + i], tile + P::kTile, P::kLow ? tile + 2 * P::kTile : nullptr, r, c, factor(scales + kNext, r, c, z, there));
-                        }
+                    if (turns && keys) {
+                        if constexpr (P::kOwn) {  // (codes as they are)
+#pragma unroll
+                            for (uint32_t q = 0; q < kEach; ++q) of_keys.codes[q] = codes[P::kRawTile / 16 + row * kPer + place_of(q)], of_keys.s2[q] = 0;
+                        } else fetch(of_keys, codes + P::kRawTile / 16, scales + kNext, key_rows, bad & 15u, false);
                     }
+                    if (weighs && keys)
+                        weigh(scales + kNext, scales + 2 * kNext, sizes(scales + kNext, key_rows, bad & 15u), sizes(scales + 2 * kNext, key_rows, bad & 15u),
+                              meta, key_rows);
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar(B_TURNED + from));
+                    if (!(fine = all_wait(bar(B_FREE + slot), free_phase))) break;
+                    if (turns && values) write(of_values, tile, std::false_type(), std::false_type());
+                    if (turns && keys) write(of_keys, tile + P::kTile, std::bool_constant<P::kOwn>(), std::bool_constant<P::kLow>());
                     fence_async();
                     __syncwarp();
-                    if (lane == 0) {
-                        bar_arrive(bar(B_FULL + slot));
-                        bar_arrive(bar(B_TURNED + from));
-                    }
+                    if (lane == 0) bar_arrive(bar(B_FULL + slot));
                     if (++slot == P::kStages) slot = 0, free_phase ^= 1;
                     if (++from == P::kRawStages) from = 0, from_phase ^= 1;
                     ++stage_no;
