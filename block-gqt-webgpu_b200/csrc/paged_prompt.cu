@@ -60,7 +60,10 @@ struct Plan {
     static constexpr uint32_t kThreads = 128 * NT + 32 * (3 + kEnds);
     // Registers after the hand-over, of softmax's warps and of the others: what the launch has, in all.
     static constexpr uint32_t kSoft = NT == 4 ? (kCodes ? 96 : 104) : kCodes ? 128 : 216, kRest = NT == 4 ? (kCodes ? 48 : 64) : 72;
-    static constexpr int kFma = D == 64 ? 2 : 6;                   // exponentials of 16 on the FMA pipe
+    // Exponentials of 16 on the FMA pipe.  (Their code is long, and beside the code that turns codes the caches of
+    // instructions do not hold it: four chunks of 1024 after 8192, 32 / 8 heads of 128, with none 587 us in 8 bits and 662 in
+    // 4, with 6 of 16 612 and 714.)
+    static constexpr int kFma = D == 64 ? 2 : kCodes ? 0 : 6;
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
     static constexpr uint32_t kChunk = kKeys * 128, kTile = kChunks * kChunk;
@@ -400,10 +403,20 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         }
                         const float *logs = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
                         float peak = top + largest;
+                        // (seldom, and so short loops over tensor memory: unrolled over registers, their code costs what kFma says)
                         if (each & 2u) {
                             peak = -INFINITY;
+                            tm_store(ts, x);
+                            tm_store(ts + 32, x + 32);
+                            tc_wait_st();
+#pragma unroll 1
+                            for (int c = 0; c < kKeys; c += 16) {
+                                uint32_t y[16];
+                                tm_load16(ts + c, y);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < kKeys; ++i) peak = fmaxf(peak, fmaf(s[i], mul, logs[i]));
+                                for (int i = 0; i < 16; ++i) peak = fmaxf(peak, fmaf(__uint_as_float(y[i]), mul, logs[c + i]));
+                            }
                         }
                         const float now = fmaxf(peak > unit + kRoom ? peak : unit, ref - kApart);
                         if (j != 0 && now > unit) beta = unit - now, moved = true;
@@ -411,14 +424,26 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         if (__any_sync(0xffffffffu, (each & 2u) || unit - largest - (kApart + kUpCodes) > ref)) {
                             // the sum for itself, and logits of the products
                             const float from = ref == -INFINITY ? 0.0f : ref;
-                            float more = 0.0f;
+                            tm_store(ts, x);
+                            tm_store(ts + 32, x + 32);
+                            tc_wait_st();
+#pragma unroll 1
+                            for (int c = 0; c < kKeys; c += 16) {
+                                uint32_t y[16];
+                                tm_load16(ts + c, y);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < kKeys; ++i) {
-                                const float v = s[i] * mul;
-                                more += ex2(v - from);
-                                s[i] = each & 2u ? v + (logs[i] - largest) : v;
+                                for (int i = 0; i < 16; ++i) {
+                                    const float v = __uint_as_float(y[i]) * mul;
+                                    sum += ex2(v - from);
+                                    y[i] = __float_as_uint(each & 2u ? v + (logs[c + i] - largest) : v);
+                                }
+                                tm_store16(ts + c, y);
                             }
-                            sum += more;
+                            tc_wait_st();
+                            tm_load(ts, x);
+                            tm_load(ts + 32, x + 32);
+                            tc_wait_ld();
                             mul = 1.0f, give = 0.0f;
                         }
                     }
