@@ -1,6 +1,12 @@
-// Penalties for tokens that a request's text holds already, biases and a grammar's mask, on its logits.
-// A CTA takes a slice of the vocabulary of one row: it counts the history's tokens that fall into the slice and adds up
-// the biases of its ids in shared memory, then passes over the logits once.
+// Penalties for tokens that a request's text holds already, biases and a grammar's mask, on its logits:
+//     x -> x / r or x r where the token is in the text, by the sign of x;  x - presence - frequency count;  x + biases;
+//     -infinity where the mask has no bit
+//
+// One pass over the logits, which are what there is to move.  A CTA takes a slice of the vocabulary of one row; its first
+// loads - logits, mask words, the history's first tokens, biases - are all under way before it waits for one.  Counts of the
+// history's tokens that fall into the slice are gathered in shared memory beside them, by integer atomics, whose order
+// does not show; biases that fall into it are lined up there in the order of their entries, and each thread adds those
+// of its own ids.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -11,91 +17,247 @@
 namespace bgtq {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 256, kResident = 5;
+constexpr uint32_t kAhead = 2;  // times four tokens of the history that a thread loads before it knows the length
+constexpr uint64_t kEnough = 592;
 
+template <int T> struct Element {
+    static constexpr uint32_t kBytes = T == BGTQ_F32 ? 4 : 2, kEach = 16 / kBytes;  // logits in 16 bytes
+};
 template <int T>
-__device__ __forceinline__ float load(const void *p, int64_t i) {
-    if constexpr (T == BGTQ_F32) return static_cast<const float *>(p)[i];
-    else if constexpr (T == BGTQ_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    else return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+__device__ __forceinline__ float to_float(uint32_t bits) {
+    if constexpr (T == BGTQ_F32) return __uint_as_float(bits);
+    else if constexpr (T == BGTQ_F16) return __half2float(__ushort_as_half((unsigned short)bits));
+    else return __uint_as_float(bits << 16);
 }
 template <int T>
-__device__ __forceinline__ void store(void *p, int64_t i, float x) {
-    if constexpr (T == BGTQ_F32) static_cast<float *>(p)[i] = x;
-    else if constexpr (T == BGTQ_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ uint32_t from_float(float x) {
+    if constexpr (T == BGTQ_F32) return __float_as_uint(x);
+    else if constexpr (T == BGTQ_F16) return __half_as_ushort(__float2half_rn(x));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+}
+template <int T>
+__device__ __forceinline__ uint32_t load(const void *p, int64_t i) {
+    if constexpr (T == BGTQ_F32) return static_cast<const uint32_t *>(p)[i];
+    else return static_cast<const uint16_t *>(p)[i];
+}
+template <int T>
+__device__ __forceinline__ void store(void *p, int64_t i, uint32_t x) {
+    if constexpr (T == BGTQ_F32) static_cast<uint32_t *>(p)[i] = x;
+    else static_cast<uint16_t *>(p)[i] = (uint16_t)x;
 }
 
-template <int T>
-__global__ void __launch_bounds__(kThreads) logits_kernel(const LogitsArgs a) {
-    extern __shared__ uint32_t smem[];
-    uint32_t *counts = smem;
-    float *added = reinterpret_cast<float *>(smem + a.slice);
-    const uint32_t b = blockIdx.y, first = blockIdx.x * a.slice, n = min(a.slice, a.vocab - first);
-    const bool history = a.tokens != nullptr, biased = a.bias != nullptr;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) counts[i] = 0, added[i] = 0.0f;
-    __syncthreads();
-    if (history) {
-        int32_t len = a.lengths ? __ldg(a.lengths + b) : (int32_t)a.width;
-        if (len < 0 || (uint32_t)len > a.width) {
-            if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
-            len = len < 0 ? 0 : (int32_t)a.width;
-        }
-        for (int32_t i = threadIdx.x; i < len; i += kThreads) {
-            const int64_t at = (int64_t)b * a.tokens_stride + i;
-            const int64_t id = a.id_bytes == 8 ? __ldg(static_cast<const int64_t *>(a.tokens) + at)
-                                               : (int64_t)__ldg(static_cast<const int32_t *>(a.tokens) + at);
-            if (id >= (int64_t)a.vocab && blockIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
-            const uint64_t in = (uint64_t)(id - (int64_t)first);
-            if (in < n) atomicAdd(counts + in, 1u);
-        }
-    }
-    if (biased && threadIdx.x < 32) {  // one warp, so that the entries of an id are added in their order
-        for (uint32_t j = 0; j < a.entries; j += 32) {
-            const uint32_t e = j + threadIdx.x;
-            const int64_t at = (int64_t)b * a.bias_stride + e;
-            const int32_t id = e < a.entries ? __ldg(a.bias_ids + at) : -1;
-            if (id >= 0 && (uint32_t)id >= a.vocab && blockIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
-            const uint32_t in = id < 0 ? ~0u : (uint32_t)id - first;
-            const float x = in < n ? __ldg(a.bias + at) : 0.0f;
-            const uint32_t same = __match_any_sync(0xffffffffu, in < n ? in : ~0u);
-            float sum = 0.0f;
-            if (in < n) sum = added[in];
-            for (uint32_t l = 0; l < 32; ++l) {
-                const float y = __shfl_sync(0xffffffffu, x, l);
-                if (same >> l & 1u) sum += y;
+// U: 16 bytes of logits a thread; V: rows of logits and of results lie alike to 16 bytes.  Then a row's first 16 bytes may
+// begin before it.
+template <int T, int U, bool V>
+__global__ void __launch_bounds__(kThreads, kResident) logits_kernel(const LogitsArgs a) {
+    constexpr uint32_t E = Element<T>::kEach, kSlice = kThreads * U * E;
+    extern __shared__ __align__(16) uint32_t counts[];  // [kSlice], with a history
+    __shared__ uint32_t line_id[kThreads];
+    __shared__ float line_x[kThreads];
+    __shared__ uint32_t line[kThreads / 32];
+    const uint32_t b = blockIdx.y, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const char *row = static_cast<const char *>(a.logits) + (int64_t)b * a.logits_stride * Element<T>::kBytes;
+    char *to = static_cast<char *>(a.out) + (int64_t)b * a.out_stride * Element<T>::kBytes;
+    const int32_t vocab = (int32_t)a.vocab;
+    // the slice's first id; its ids are counted from there
+    const int32_t first = (int32_t)(blockIdx.x * kSlice) - (V ? (int32_t)(reinterpret_cast<uintptr_t>(row) % 16 / Element<T>::kBytes) : 0);
+    auto inside = [&](int32_t id) { return id >= 0 && id < vocab && (uint32_t)(id - first) < kSlice; };
+    // ---- loads ----
+    uint4 x[U];
+    uint32_t words[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int32_t i = first + (int32_t)((u * kThreads + threadIdx.x) * E);
+        x[u] = make_uint4(0, 0, 0, 0);
+        words[u] = ~0u;
+        if (i >= vocab) continue;
+        if (V && i >= 0 && i + (int32_t)E <= vocab) x[u] = *reinterpret_cast<const uint4 *>(row + (int64_t)i * Element<T>::kBytes);
+        else {
+            uint32_t *w = reinterpret_cast<uint32_t *>(&x[u]);
+#pragma unroll
+            for (int32_t k = 0; k < (int32_t)E; ++k) {
+                const uint32_t y = i + k >= 0 && i + k < vocab ? load<T>(row, i + k) : 0u;
+                if constexpr (T == BGTQ_F32) w[k] = y;
+                else w[k / 2] |= y << 16 * (k & 1);
             }
-            if (in < n) added[in] = sum;
-            __syncwarp();
+        }
+        if (a.mask) {
+            const uint32_t *mask = a.mask + (int64_t)b * a.mask_stride;
+            const int32_t last = min(i + (int32_t)E, vocab) - 1;
+            const uint32_t low = __ldg(mask + (max(i, 0) >> 5)), high = __ldg(mask + (last >> 5));
+            // (a row's first bit may come after i)
+            words[u] = i < 0 ? low << -i : __funnelshift_r(low, high, i & 31);
         }
     }
-    __syncthreads();
-    const float r = a.repetition ? __ldg(a.repetition + b) : 1.0f, p = a.presence ? __ldg(a.presence + b) : 0.0f;
-    const float f = a.frequency ? __ldg(a.frequency + b) : 0.0f;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const uint32_t v = first + i, c = counts[i];
-        float x = load<T>(a.logits, (int64_t)b * a.logits_stride + v);
-        if (c) {
-            x = x > 0.0f ? __fdiv_rn(x, r) : __fmul_rn(x, r);
-            x = __fsub_rn(__fsub_rn(x, p), __fmul_rn(f, (float)c));
+    // four tokens of the history from 4 v on; -1 past its width, and what no vocabulary holds for ids past 32 bits
+    auto tokens = [&](uint32_t v) -> int4 {
+        if (4 * v >= a.width) return make_int4(-1, -1, -1, -1);
+        const int64_t at = (int64_t)b * a.tokens_stride + 4 * v;
+        const bool whole = a.tokens_even && 4 * v + 4 <= a.width;
+        if (a.id_bytes == 4) {
+            const int32_t *from = static_cast<const int32_t *>(a.tokens) + at;
+            if (whole) return __ldg(reinterpret_cast<const int4 *>(from));
+            auto one = [&](uint32_t k) { return 4 * v + k < a.width ? __ldg(from + k) : -1; };
+            return make_int4(one(0), one(1), one(2), one(3));
         }
-        if (biased) x += added[i];
-        if (a.mask && !(__ldg(a.mask + (int64_t)b * a.mask_stride + v / 32) >> v % 32 & 1u)) x = -INFINITY;
-        store<T>(a.out, (int64_t)b * a.out_stride + v, x);
+        const int64_t *from = static_cast<const int64_t *>(a.tokens) + at;
+        auto narrow = [](int64_t id) { return id < 0 ? -1 : (int32_t)min(id, (int64_t)0x7fffffff); };
+        if (whole) {
+            const longlong2 y = __ldg(reinterpret_cast<const longlong2 *>(from)), z = __ldg(reinterpret_cast<const longlong2 *>(from) + 1);
+            return make_int4(narrow(y.x), narrow(y.y), narrow(z.x), narrow(z.y));
+        }
+        auto one = [&](uint32_t k) { return 4 * v + k < a.width ? narrow(__ldg(from + k)) : -1; };
+        return make_int4(one(0), one(1), one(2), one(3));
+    };
+    int4 ids[kAhead];
+    int32_t length = 0;
+    float r = 1.0f, p = 0.0f, f = 0.0f;
+    if (a.tokens) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) ids[k] = tokens(threadIdx.x + k * kThreads);
+        length = a.lengths ? __ldg(a.lengths + b) : (int32_t)a.width;
+        if (a.repetition) r = __ldg(a.repetition + b);
+        if (a.presence) p = __ldg(a.presence + b);
+        if (a.frequency) f = __ldg(a.frequency + b);
     }
+    int32_t bias_id = -1;
+    float bias = 0.0f;
+    auto entry = [&](uint32_t j) {
+        bias_id = j < a.entries ? __ldg(a.bias_ids + (int64_t)b * a.bias_stride + j) : -1;
+        bias = j < a.entries ? __ldg(a.bias + (int64_t)b * a.bias_stride + j) : 0.0f;
+    };
+    if (a.bias) entry(threadIdx.x);
+    // ---- counts ----
+    if (a.tokens) {
+#pragma unroll
+        for (uint32_t i = 0; i < kSlice / 4 / kThreads; ++i) reinterpret_cast<uint4 *>(counts)[i * kThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        if (length < 0 || (uint32_t)length > a.width) {
+            if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(a.status, kStatusBadExtent);
+            length = length < 0 ? 0 : (int32_t)a.width;
+        }
+        auto count = [&](const int4 &four, uint32_t v) {
+            const int32_t of[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                if (4 * v + k >= (uint32_t)length) break;
+                if (of[k] >= vocab && blockIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
+                if (inside(of[k])) atomicAdd(counts + (of[k] - first), 1u);
+            }
+        };
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) count(ids[k], threadIdx.x + k * kThreads);
+        for (uint32_t v = threadIdx.x + kAhead * kThreads; 4 * v < (uint32_t)length; v += 4 * kThreads) {
+            int4 more[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) more[k] = tokens(v + k * kThreads);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) count(more[k], v + k * kThreads);
+        }
+        __syncthreads();
+    }
+    // ---- the slice ----
+    float y[U][E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&x[u]);
+#pragma unroll
+        for (uint32_t k = 0; k < E; ++k) y[u][k] = to_float<T>(T == BGTQ_F32 ? w[k] : w[k / 2] >> 16 * (k & 1) & 0xffffu);
+        if (!a.tokens) continue;
+#pragma unroll
+        for (uint32_t q = 0; q < E / 4; ++q) {
+            const uint4 c = reinterpret_cast<const uint4 *>(counts + (u * kThreads + threadIdx.x) * E)[q];
+            if (!(c.x | c.y | c.z | c.w)) continue;
+            const uint32_t of[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (of[k]) {
+                    float &z = y[u][4 * q + k];
+                    z = z > 0.0f ? __fdiv_rn(z, r) : __fmul_rn(z, r);
+                    z = __fsub_rn(__fsub_rn(z, p), __fmul_rn(f, (float)of[k]));
+                }
+        }
+    }
+    for (uint32_t j = 0; j < a.entries; j += kThreads) {
+        if (j) {
+            __syncthreads();  // the line before this one has been read
+            entry(j + threadIdx.x);
+        }
+        if (bias_id >= vocab && blockIdx.x == 0) atomicOr(a.status, kStatusBadSlot);
+        const bool in = inside(bias_id);
+        const uint32_t here = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) line[warp] = __popc(here);
+        __syncthreads();
+        uint32_t at = __popc(here & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kThreads / 32; ++w) {
+            at += w < warp ? line[w] : 0;
+            all += line[w];
+        }
+        if (!all) continue;
+        if (in) line_id[at] = (uint32_t)(bias_id - first), line_x[at] = bias;
+        __syncthreads();
+        for (uint32_t k = 0; k < all; ++k) {
+            const uint32_t id = line_id[k];
+            if (id / E % kThreads != threadIdx.x) continue;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e)
+                    if (id == (u * kThreads + threadIdx.x) * E + e) y[u][e] += line_x[k];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int32_t i = first + (int32_t)((u * kThreads + threadIdx.x) * E);
+        if (i >= vocab) continue;
+        uint32_t w[4] = {};
+#pragma unroll
+        for (uint32_t k = 0; k < E; ++k) {
+            const uint32_t z = from_float<T>(words[u] >> k & 1u ? y[u][k] : -INFINITY);
+            if constexpr (T == BGTQ_F32) w[k] = z;
+            else w[k / 2] |= z << 16 * (k & 1);
+        }
+        if (V && i >= 0 && i + (int32_t)E <= vocab) *reinterpret_cast<uint4 *>(to + (int64_t)i * Element<T>::kBytes) = make_uint4(w[0], w[1], w[2], w[3]);
+        else {
+#pragma unroll
+            for (int32_t k = 0; k < (int32_t)E; ++k)
+                if (i + k >= 0 && i + k < vocab) store<T>(to, i + k, T == BGTQ_F32 ? w[k] : w[k / 2] >> 16 * (k & 1) & 0xffffu);
+        }
+    }
+}
+
+template <int T, int U, bool V>
+cudaError_t run(const LogitsArgs &a, cudaStream_t s) {
+    constexpr uint32_t kSlice = kThreads * U * Element<T>::kEach;
+    const uint32_t smem = a.tokens ? kSlice * 4 : 0, ids = a.vocab + (V ? Element<T>::kEach - 1 : 0);
+    logits_kernel<T, U, V><<<dim3((ids + kSlice - 1) / kSlice, a.batch), kThreads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+template <int T, int U>
+cudaError_t by_alignment(const LogitsArgs &a, cudaStream_t s) {
+    const bool v = (reinterpret_cast<uintptr_t>(a.logits) - reinterpret_cast<uintptr_t>(a.out)) % 16 == 0 &&
+                   (a.batch == 1 || (a.logits_stride - a.out_stride) * (int64_t)Element<T>::kBytes % 16 == 0);
+    return v ? run<T, U, true>(a, s) : run<T, U, false>(a, s);
+}
+// Slices of 16 KB of FP32 logits where that makes enough CTAs, else shorter ones.
+template <int T>
+cudaError_t by_size(const LogitsArgs &a, cudaStream_t s) {
+    constexpr uint32_t kOne = kThreads * Element<T>::kEach;
+    constexpr int kMost = T == BGTQ_F32 ? 4 : 2;
+    if ((uint64_t)a.batch * ((a.vocab + kMost * kOne - 1) / (kMost * kOne)) >= kEnough) return by_alignment<T, kMost>(a, s);
+    return by_alignment<T, 1>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_logits(const LogitsArgs &args, cudaStream_t s) {
     LogitsArgs a = args;
-    a.slice = 4096;
-    const dim3 grid((a.vocab + a.slice - 1) / a.slice, a.batch);
-    const size_t smem = a.slice * 8;
-    if (a.dtype == BGTQ_F32) logits_kernel<BGTQ_F32><<<grid, kThreads, smem, s>>>(a);
-    else if (a.dtype == BGTQ_F16) logits_kernel<BGTQ_F16><<<grid, kThreads, smem, s>>>(a);
-    else logits_kernel<BGTQ_BF16><<<grid, kThreads, smem, s>>>(a);
-    return cudaGetLastError();
+    a.tokens_even = reinterpret_cast<uintptr_t>(a.tokens) % 16 == 0 && a.tokens_stride * a.id_bytes % 16 == 0;
+    if (a.dtype == BGTQ_F32) return by_size<BGTQ_F32>(a, s);
+    if (a.dtype == BGTQ_F16) return by_size<BGTQ_F16>(a, s);
+    return by_size<BGTQ_BF16>(a, s);
 }
 
 }  // namespace bgtq

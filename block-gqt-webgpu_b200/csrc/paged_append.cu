@@ -1,8 +1,8 @@
 // New tokens into the pages of a cache: heads of queries and keys normed (where the model does), rotated by their
 // position, keys and values quantised and stored, queries written out, in one pass over the projections' output.
 //     y = x w / sqrt(mean(x^2) + eps),   (y_i, y_{i + D/2}) -> (y_i c_i - y_{i + D/2} s_i, y_{i + D/2} c_i + y_i s_i)
-// Rows that become codes are computed in 64 bits and rounded to FP32 once: a code is a step function of its row, and
-// so is the same whatever order the sums and products are taken in.  All else is FP32.
+// Rows that become codes are computed in pairs of FP32 numbers (a norm's factor in 64 bits) and rounded to FP32 once: a code is
+// a step function of its row, and so is the same whatever order sums and products are taken in.  All else is FP32.
 #include <type_traits>
 
 #include "paged_rows.cuh"
@@ -10,11 +10,35 @@
 namespace bgtq {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+// Small CTAs, and registers for ten of them an SM: what is slow here is waiting for loads.  (16384 tokens of 32 / 8 heads of 128
+// from BF16 into 8 bits: 256 threads and 58 registers 94 us, 128 and 48 79 us; into 4 bits with norms 116 and 102 us.)
+constexpr uint32_t kThreads = 128, kResident = 10;
+
+// Pairs of FP32 numbers and what their rounding left (Dekker's product by one fused multiply-add, Knuth's two-sum), two
+// at a time.
+struct Two {
+    float2 h, l;
+};
+__device__ __forceinline__ float2 minus(float2 x) { return make_float2(-x.x, -x.y); }
+__device__ __forceinline__ Two times(float2 a, float2 b) {
+    const float2 p = __fmul2_rn(a, b);
+    return {p, __ffma2_rn(a, b, minus(p))};
+}
+__device__ __forceinline__ Two times(const Two &a, float2 b) {
+    const Two p = times(a.h, b);
+    return {p.h, __ffma2_rn(a.l, b, p.l)};
+}
+// p - q, rounded once (but for 2^-24 of an ulp where nothing cancels); infinities and NaN as they come
+__device__ __forceinline__ float2 difference(const Two &p, const Two &q) {
+    const float2 h = __fadd2_rn(p.h, minus(q.h)), z = __fadd2_rn(h, minus(p.h));
+    const float2 e = __fadd2_rn(__fadd2_rn(p.h, minus(__fadd2_rn(h, minus(z)))), minus(__fadd2_rn(q.h, z)));
+    const float2 r = __fadd2_rn(h, __fadd2_rn(e, __fadd2_rn(p.l, minus(q.l))));
+    return make_float2(r.x == r.x ? r.x : h.x, r.y == r.y ? r.y : h.y);
+}
 
 // A thread takes eight dimensions of a row's first half and the eight of the second that they are rotated with.
-template <int F, int T, int D, bool V>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+template <int F, int T, int D, bool V, bool N>
+__global__ void __launch_bounds__(kThreads, kResident) append_kernel(const AppendArgs a) {
     constexpr uint32_t kLanes = D / 16;  // of a row
     constexpr bool kCodes = Format<F>::kCodes;
     const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -44,35 +68,68 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = y[k] = 0.0f;
     } else if (kind != 2) {
-        const float *norm = kind == 0 ? a.q_norm : a.k_norm;
-        auto turn = [&](auto zero) {
-            using R = decltype(zero);
-            R u[8], v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) u[k] = x[k], v[k] = y[k];
+        const float4 *rotary = reinterpret_cast<const float4 *>(a.rotary + pos * D + 8 * part);
+        const float *norm = N ? kind == 0 ? a.q_norm : a.k_norm : nullptr;
+        if (kCodes && kind == 1) {
+            float2 fh = make_float2(1.0f, 1.0f), fl = make_float2(0.0f, 0.0f);
             if (norm) {
-                R sum = 0;
+                double sum = 0.0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum += u[k] * u[k] + v[k] * v[k];
+                for (int k = 0; k < 8; ++k) sum = fma((double)x[k], (double)x[k], fma((double)y[k], (double)y[k], sum));
 #pragma unroll
                 for (uint32_t w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(lanes, sum, w);
-                const R f = R(1) / sqrt(sum / R(D) + R(a.eps));
+                const double f = 1.0 / sqrt(sum / D + (double)a.eps);
+                fh.x = fh.y = (float)f;
+                fl.x = fl.y = (float)(f - (double)fh.x);
+            }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    u[k] *= f * R(__ldg(norm + 8 * part + k));
-                    v[k] *= f * R(__ldg(norm + D / 2 + 8 * part + k));
+            for (int k = 0; k < 2; ++k) {
+                const float4 cs = __ldg(rotary + k), ss = __ldg(rotary + D / 8 + k);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const int e = 4 * k + 2 * m;
+                    const float2 c = m ? make_float2(cs.z, cs.w) : make_float2(cs.x, cs.y), s = m ? make_float2(ss.z, ss.w) : make_float2(ss.x, ss.y);
+                    Two u{make_float2(x[e], x[e + 1]), {}}, v{make_float2(y[e], y[e + 1]), {}};
+                    if (norm) {
+                        auto normed = [&](float2 z, const float *w) {
+                            const Two p = times(z, *reinterpret_cast<const float2 *>(w));
+                            Two r = times(p, fh);
+                            r.l = __ffma2_rn(p.h, fl, r.l);
+                            return r;
+                        };
+                        u = normed(u.h, norm + 8 * part + e);
+                        v = normed(v.h, norm + D / 2 + 8 * part + e);
+                    }
+                    const float2 p = difference(times(u, c), times(v, s)), q = difference(times(v, c), times(u, minus(s)));
+                    x[e] = p.x, x[e + 1] = p.y, y[e] = q.x, y[e + 1] = q.y;
                 }
             }
-            const float *rotary = a.rotary + pos * D + 8 * part;
+        } else {
+            if (norm) {
+                float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const R c = __ldg(rotary + k), s = __ldg(rotary + D / 2 + k);
-                x[k] = (float)(u[k] * c - v[k] * s);
-                y[k] = (float)(v[k] * c + u[k] * s);
+                for (int k = 0; k < 8; ++k) sum = fmaf(x[k], x[k], fmaf(y[k], y[k], sum));
+#pragma unroll
+                for (uint32_t w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(lanes, sum, w);
+                const float f = 1.0f / sqrtf(sum / D + a.eps);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[k] *= f * __ldg(norm + 8 * part + k);
+                    y[k] *= f * __ldg(norm + D / 2 + 8 * part + k);
+                }
             }
-        };
-        if (kCodes && kind == 1) turn(0.0);
-        else turn(0.0f);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float4 cs = __ldg(rotary + k), ss = __ldg(rotary + D / 8 + k);
+                const float c[4] = {cs.x, cs.y, cs.z, cs.w}, s[4] = {ss.x, ss.y, ss.z, ss.w};
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const float u = x[4 * k + m], v = y[4 * k + m];
+                    x[4 * k + m] = fmaf(u, c[m], -(v * s[m]));
+                    y[4 * k + m] = fmaf(v, c[m], u * s[m]);
+                }
+            }
+        }
     }
     auto write = [&](void *out, uint64_t r) {
         auto as = [&](auto type) {
@@ -127,18 +184,19 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     }
 }
 
-template <int F, int T, int D>
+template <int F, int T, int D, bool V>
 void append_rows(const AppendArgs &a, cudaStream_t s) {
     const uint64_t threads = a.tokens * (a.q_heads + 2 * a.c.heads) * (D / 16);
     const uint32_t blocks = (uint32_t)((threads + kThreads - 1) / kThreads);
-    constexpr int B = Element<T>::kBytes;
-    if (even(a.q, a.q_token, a.q_head, B) && even(a.k, a.k_token, a.k_head, B) && even(a.v, a.v_token, a.v_head, B))
-        append_kernel<F, T, D, true><<<blocks, kThreads, 0, s>>>(a);
-    else append_kernel<F, T, D, false><<<blocks, kThreads, 0, s>>>(a);
+    if (a.q_norm || a.k_norm) append_kernel<F, T, D, V, true><<<blocks, kThreads, 0, s>>>(a);
+    else append_kernel<F, T, D, V, false><<<blocks, kThreads, 0, s>>>(a);
 }
 template <int F, int T>
 void append_as(const AppendArgs &a, cudaStream_t s) {
-    a.c.dim == 64 ? append_rows<F, T, 64>(a, s) : append_rows<F, T, 128>(a, s);
+    constexpr int B = Element<T>::kBytes;
+    const bool v = even(a.q, a.q_token, a.q_head, B) && even(a.k, a.k_token, a.k_head, B) && even(a.v, a.v_token, a.v_head, B);
+    if (a.c.dim == 64) v ? append_rows<F, T, 64, true>(a, s) : append_rows<F, T, 64, false>(a, s);
+    else v ? append_rows<F, T, 128, true>(a, s) : append_rows<F, T, 128, false>(a, s);
 }
 template <int F>
 void append_from(const AppendArgs &a, cudaStream_t s) {

@@ -289,7 +289,7 @@ bgtq_status bgtq_paged_attend_chunk(const bgtq_paged_cache *c, const bgtq_chunk 
 bgtq_status bgtq_adjust_logits(const bgtq_logits *p, void *stream) {
     if (!p) return refuse("Logits: null");
     if (p->dtype < BGTQ_F16 || p->dtype > BGTQ_BF16) return refuse("Logits: logits must be FP16, BF16 or FP32");
-    if (p->vocab < 1 || p->vocab > 0x7fffffffu) return refuse("Logits: invalid vocabulary");
+    if (p->vocab < 1 || p->vocab > 0x7ffeffffu) return refuse("Logits: invalid vocabulary");
     if (p->batch > 65535u) return refuse("Logits: too many rows in one call");
     if (p->width > 0x7fffffffu || p->entries > 0x7fffffffu) return refuse("Logits: too many tokens or biases in a row");
     if (p->tokens && p->id_bytes != 4 && p->id_bytes != 8) return refuse("Logits: token ids must have 4 or 8 bytes");

@@ -127,7 +127,7 @@ struct LogitsArgs {
     void *out;
     int64_t logits_stride, tokens_stride, bias_stride, mask_stride, out_stride;
     uint32_t batch, vocab, width, id_bytes, entries;
-    uint32_t slice;  // the launcher's: ids of a CTA
+    uint32_t tokens_even;  // the launcher's: histories are 16-byte aligned
     bgtq_dtype dtype;
     uint32_t *status;
 };
