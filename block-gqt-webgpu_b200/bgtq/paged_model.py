@@ -5,9 +5,13 @@
 4-bit pages.  A call of `prompt` runs the new tokens of any number of requests as one packed
 batch: their rows are quantised into the pages (`PagedCache.write`), the rows of earlier calls
 are read back (`PagedCache.read`) in front of them, and `prompt_attention` runs over both.  A
-call of `step` runs one new token of each request: its row is written, then every head reads
-its request's pages (`PagedCache.attend`).  Geometry, weights, RoPE and norms are the ones of
-`model` (src/model/kernels.wgsl:11-54); the projections are plain GEMMs.
+call of `step` runs one new token of each request: it is rotated into the pages
+(`PagedCache.append`), then every head reads its request's pages (`PagedCache.attend`).  Over
+16-bit pages, which hold rows as they are, and with a window a prompt's chunk does the same
+(`PagedCache.attend_chunk`), and so does a call of `verify`, which answers for every one of a
+few drafted tokens what `step` would have answered one after the other.  `generate` chooses
+after penalties, biases and masks (`adjust_logits`).  Geometry, weights, RoPE and norms are the
+ones of `model` (src/model/kernels.wgsl:11-54); the projections are plain GEMMs.
 """
 from __future__ import annotations
 
@@ -18,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .model import ModelGeometry
-from .serving import PagedCache, prompt_attention, _refuse
+from .serving import PagedCache, adjust_logits, prompt_attention, _refuse
 
 
 _RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width, both rounded up
@@ -32,14 +36,20 @@ def _places(requests: int) -> int:
 class PagedDecoder:
     """pages: pages of page_size tokens that all requests share (one pool a layer, one table
     for all).  format: "f16" / "bf16" (dtype's own), "int8" or "int4" pages.  dtype: float16 or
-    bfloat16, the type of GEMMs and attention; the residual stream is FP32."""
+    bfloat16, the type of GEMMs and attention; the residual stream is FP32.  window, sinks: a
+    token sees the last `window` tokens, itself among them, and the first `sinks` of its request
+    (None: all); pages that no later token sees are given back when their request grows, so that a
+    request may become longer than the pool."""
 
     def __init__(self, weights, geometry: ModelGeometry, pages: int, page_size: int = 64, format: str = "int8",
-                 dtype=torch.bfloat16, device: int = 0):
+                 dtype=torch.bfloat16, device: int = 0, window: int | None = None, sinks: int = 0):
         if dtype not in (torch.float16, torch.bfloat16):
             _refuse("Paged decoder: dtype must be float16 or bfloat16")
         if format in ("f16", "bf16") and (format == "f16") != (dtype == torch.float16):
             _refuse("Paged decoder: 16-bit pages must be of dtype")
+        if window is not None and not 1 <= window < 2**31 or not 0 <= sinks < 2**31:
+            _refuse("Paged decoder: window must be positive and sinks nonnegative, both below 2^31")
+        self.window, self.sinks = window, int(sinks)
         g = self.g = geometry
         self.dtype, self.page_size = dtype, int(page_size)
         self.dev = torch.device("cuda", device)
@@ -78,8 +88,32 @@ class PagedDecoder:
 
     def close(self, request: int) -> None:
         """Ends a request; its pages are free for others."""
-        self._free += self._request(request)[0][::-1]
+        self._free += [p for p in self._request(request)[0][::-1] if p >= 0]
         del self._held[request]
+
+    def rewind(self, request: int, length: int) -> None:
+        """Takes back the last tokens of a request, so that `length` are left: what a draft was
+        verified to be wrong in.  Pages that are left over are free for others."""
+        pages, have = held = self._request(request)
+        if not 0 <= length <= have:
+            _refuse(f"Paged decoder: a length of 0 to {have} can be left")
+        keep = -(-length // self.page_size)
+        if length and -1 in pages[self._first(length) // self.page_size:keep]:
+            _refuse("Paged decoder: pages of tokens that would be seen again have been given back")
+        self._free += pages[keep:][::-1]
+        held[0], held[1] = pages[:keep], length
+
+    def _first(self, length: int) -> int:
+        """The first token that the next one sees, but for sinks."""
+        return 0 if self.window is None else max(0, length - self.window + 1)
+
+    def _release(self, held) -> None:
+        """Gives back the pages of tokens that no later one sees (-1 stands for them from then on)."""
+        pages, length = held
+        for i in range(-(-self.sinks // self.page_size), min(self._first(length) // self.page_size, len(pages))):
+            if pages[i] >= 0:
+                self._free.append(pages[i])
+                pages[i] = -1
 
     def length(self, request: int) -> int:
         """Tokens of a request whose rows the pages hold."""
@@ -103,6 +137,9 @@ class PagedDecoder:
         if not requests or len(set(requests)) < len(requests):
             _refuse("Paged decoder: requests must be one or more, each once")
         held = [self._request(r) for r in requests]
+        if self.window is not None:
+            for h in held:
+                self._release(h)
         need = [-(-(h[1] + n) // self.page_size) - len(h[0]) for h, n in zip(held, counts)]
         if sum(need) > len(self._free):
             _refuse(f"Paged decoder: {sum(need)} pages wanted, {len(self._free)} free")
@@ -123,6 +160,12 @@ class PagedDecoder:
         t = np.arange(first, upto)
         return np.asarray(pages, np.int64)[t // self.page_size] * self.page_size + t % self.page_size
 
+    def _table(self, held, places: int, width: int):
+        table = np.zeros((places, width), np.int32)  # (a page that was given back is not followed)
+        for row, h in zip(table, held):
+            row[:len(h[0])] = np.maximum(h[0], 0)
+        return table
+
     def _to(self, array, dtype):
         return torch.as_tensor(np.asarray(array), dtype=dtype).to(self.dev, non_blocking=True)
 
@@ -138,11 +181,43 @@ class PagedDecoder:
         with self._grown(requests, counts) as (held, before):
             return self._prompt(flat, counts, held, before)
 
+    def verify(self, requests, tokens):
+        """The next tokens[i] (one or more) of each requests[i], drafted by whatever means: logits
+        [all tokens, vocab] (FP32) of every one of them, one request's after the other's, as `step`
+        would answer them one at a time.  `rewind` takes back the ones that were wrong."""
+        tokens = [np.asarray(t.cpu() if torch.is_tensor(t) else t, np.int64).reshape(-1) for t in tokens]
+        if len(tokens) != len(requests) or any(not len(t) for t in tokens):
+            _refuse("Paged decoder: one or more tokens for every request")
+        flat = self._vocabulary(np.concatenate(tokens)) if tokens else None
+        counts = [len(t) for t in tokens]
+        with self._grown(requests, counts) as (held, before):
+            return self._chunk(flat, counts, held, before, None)
+
+    def _chunk(self, flat, counts, held, before, last):
+        """New tokens through the pages."""
+        slots, positions, starts = self._rows(counts, held, before)
+        table = self._to(self._table(held, len(held), max(len(h[0]) for h in held)), torch.int32)
+        lengths = self._to([h[1] for h in held], torch.int32)
+
+        def attention(cache, q, k, v, rotary):
+            q = cache.append(q, k, v, slots, rotary)
+            return cache.attend_chunk(q, starts, table, lengths, window=self.window, sinks=self.sinks)
+
+        return self._forward(self._to(flat, torch.int64), positions, attention, last)
+
+    def _rows(self, counts, held, before):
+        """Slots and positions of new rows, and where each request's begin."""
+        return (self._to(np.concatenate([self._slots(h[0], b, h[1]) for h, b in zip(held, before)]), torch.int64),
+                self._to(np.concatenate([np.arange(b, h[1]) for h, b in zip(held, before)]), torch.float32),
+                self._to(np.concatenate([[0], np.cumsum(counts)]), torch.int32))
+
     def _prompt(self, flat, counts, held, before):
         ends = np.cumsum(counts)
-        slots = self._to(np.concatenate([self._slots(h[0], b, h[1]) for h, b in zip(held, before)]), torch.int64)
-        positions = self._to(np.concatenate([np.arange(b, h[1]) for h, b in zip(held, before)]), torch.float32)
-        starts = self._to(np.concatenate([[0], ends]), torch.int32)
+        last = self._to(ends - 1, torch.int64)
+        if self.window is not None or self.caches[0].k_scales is None:
+            return self._chunk(flat, counts, held, before, last)
+        # 8- and 4-bit pages: a chunk sees its own rows as they are, and the rows of earlier calls as they are stored
+        slots, positions, starts = self._rows(counts, held, before)
         earlier = None
         if any(before):
             # keys of a request: the rows of earlier calls from the pages, then this call's own as they are
@@ -153,7 +228,8 @@ class PagedDecoder:
             earlier = (self._to(np.concatenate(rows), torch.int64), self._to(np.concatenate(new), torch.int64),
                        self._to(np.concatenate([[0], key_ends]), torch.int32))
 
-        def attention(cache, q, k, v):
+        def attention(cache, q, k, v, rotary):
+            q, k, v = self._rope(q.float(), rotary), self._rope(k.float(), rotary), v.float()
             cache.write(k, v, slots)
             q, k, v = q.to(self.dtype), k.to(self.dtype), v.to(self.dtype)
             if earlier is None:
@@ -162,7 +238,7 @@ class PagedDecoder:
             all_k[earlier[1]], all_v[earlier[1]] = k, v
             return prompt_attention(q, all_k, all_v, starts, key_starts=earlier[2])
 
-        return self._forward(self._to(flat, torch.int64), positions, attention, self._to(ends - 1, torch.int64))
+        return self._forward(self._to(flat, torch.int64), positions, attention, last)
 
     def step(self, requests, tokens):
         """One token of each request: logits [requests, vocab] (FP32).  Replays a CUDA graph that is
@@ -185,10 +261,7 @@ class PagedDecoder:
             row = np.full(places, rest, np.float32 if buffer.is_floating_point() else np.int64)
             row[:n] = values
             buffer.copy_(torch.as_tensor(row).to(buffer.dtype))
-        table = np.zeros((places, width), np.int32)
-        for row, h in zip(table, held):
-            row[:len(h[0])] = h[0]
-        inputs[-1].copy_(torch.as_tensor(table))
+        inputs[-1].copy_(torch.as_tensor(self._table(held, places, width)))
         graph.replay()
         return logits[:n].clone()
 
@@ -199,9 +272,11 @@ class PagedDecoder:
             self._to(np.full(batch, -1), torch.int64), self._to(np.zeros(batch), torch.int32),
             self._to(np.zeros((batch, width)), torch.int32))
 
-        def attention(cache, q, k, v):
-            cache.write(k, v, slots)
-            return cache.attend(q.to(self.dtype), table, lengths)
+        def attention(cache, q, k, v, rotary):
+            q = cache.append(q, k, v, slots, rotary)
+            if self.window is None:
+                return cache.attend(q, table, lengths)
+            return cache.attend(q, table, lengths, window=self.window, sinks=self.sinks)
 
         # once beside the recording, for what is set up at first calls: no row is written, none is read
         self._side.wait_stream(torch.cuda.current_stream(self.dev))
@@ -216,14 +291,34 @@ class PagedDecoder:
             del self._steps[next(iter(self._steps))]
         return graph, inputs, logits
 
-    def generate(self, prompts, count: int):
+    def generate(self, prompts, count: int, **choice):
         """Greedy: count tokens after each of prompts (sequences of tokens), as an int64 array
-        [prompts, count].  Its requests are closed before it returns."""
+        [prompts, count].  choice: what is put on the logits before each token is chosen, as
+        `adjust_logits` takes it (repetition, presence, frequency, bias_ids, bias, mask; the history is
+        a request's prompt and what it was answered).  Its requests are closed before it returns."""
         requests = [self.open() for _ in prompts]
+        history = None
+        if any(choice.get(name) is not None for name in ("repetition", "presence", "frequency")):
+            lengths = [len(p) for p in prompts]
+            row = np.full((len(prompts), max(lengths, default=0) + max(count, 0)), -1, np.int64)
+            for r, p in zip(row, prompts):
+                r[:len(p)] = p.cpu() if torch.is_tensor(p) else p
+            history = self._to(row, torch.int64)
+            at = torch.as_tensor(lengths, device=self.dev)[:, None]
+
+        def chosen(logits):
+            if choice:
+                adjust_logits(logits, history, out=logits, **choice)
+            token = logits.argmax(-1)
+            if history is not None and count > 0:  # (places past the answers hold -1: they are left out)
+                history.scatter_(1, at + len(out), token[:, None])
+            return token
+
+        out = []
         try:
-            out = [self.prompt(requests, prompts).argmax(-1)]
+            out.append(chosen(self.prompt(requests, prompts)))
             while len(out) < count:
-                out.append(self.step(requests, out[-1]).argmax(-1))
+                out.append(chosen(self.step(requests, out[-1])))
             return torch.stack(out[:count], 1).cpu().numpy() if count > 0 else np.zeros((len(prompts), 0), np.int64)
         finally:
             for r in requests:
@@ -237,23 +332,21 @@ class PagedDecoder:
     def _norm(self, x, w):
         return F.rms_norm(x, (self.g.hidden,), w, self.g.rms_eps).to(self.dtype)
 
-    def _rope(self, x, cos, sin):
-        half = self.g.head_dim // 2
-        a, b = x[..., :half], x[..., half:]
+    def _rope(self, x, rotary):
+        cos, sin = rotary[:, None].chunk(2, -1)
+        a, b = x.chunk(2, -1)
         return torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
 
     def _forward(self, tokens, positions, attention, last):
         g = self.g
         qw, kvw = g.q_heads * g.head_dim, g.kv_heads * g.head_dim
-        angle = positions[:, None, None] * self.inv_freq
-        cos, sin = angle.cos(), angle.sin()
+        angle = positions[:, None] * self.inv_freq
+        rotary = torch.cat([angle.cos(), angle.sin()], -1)
         h = self.emb[tokens].float()
         for lw, cache in zip(self.layers, self.caches):
-            qkv = F.linear(self._norm(h, lw["ln1"]), lw["qkv"], lw["qkv_b"]).float()
-            q = self._rope(qkv[:, :qw].unflatten(1, (g.q_heads, g.head_dim)), cos, sin)
-            k = self._rope(qkv[:, qw:qw + kvw].unflatten(1, (g.kv_heads, g.head_dim)), cos, sin)
-            v = qkv[:, qw + kvw:].unflatten(1, (g.kv_heads, g.head_dim))
-            h = h + F.linear(attention(cache, q, k, v).flatten(1), lw["o"]).float()
+            qkv = F.linear(self._norm(h, lw["ln1"]), lw["qkv"], lw["qkv_b"])
+            q, k, v = (x.unflatten(1, (-1, g.head_dim)) for x in qkv.split((qw, kvw, kvw), 1))
+            h = h + F.linear(attention(cache, q, k, v, rotary).flatten(1), lw["o"]).float()
             gate, up = F.linear(self._norm(h, lw["ln2"]), lw["gate_up"]).chunk(2, -1)
             h = h + F.linear(F.silu(gate) * up, lw["down"]).float()
         if last is not None:
