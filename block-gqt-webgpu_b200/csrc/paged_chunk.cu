@@ -1,5 +1,19 @@
 // Attention of a chunk of new tokens of every request over the pages of a cache, all of them or a window and the first
-// few: which kernel takes a call.
+// few: which kernel takes a call, by the columns - rows x query heads of a KV head - that its requests have on average.
+//
+// Few columns: the kernel of one token per request with 8 or 16 columns, a request's rows in blocks of as many.  It
+// reads a request's pages once for each block.  Many: the one on the fifth-generation tensor cores, which reads them once for up
+// to 256 columns (512 at head dim 64), at the price of starting and joining larger pieces.  Measured, in us (few, many):
+//     32 requests of 500 to 16000 tokens, 32 / 8 heads of 128, 16 columns: 16 bits 163, 124; 8 bits 154, 177; 4 bits 159, 234
+//                                                             20 columns: 16 bits 310, 125; 8 bits 272, 176; 4 bits 310, 232
+//     the same, 14 / 2 heads of 64, 28 columns: 43, 61; 8 bits 42, 82; 4 bits 47, 76; 35 columns: 73, 61; 70, 82; 74, 77
+//     the same, 9 / 3 heads of 64, 24 columns: 80, 69
+//     one request of 30000 tokens, 20 columns of 128: 59, 40; 28 of 64: 29, 44; eight of 200 to 2000, 20 of 128: 26, 33; 28 of
+//     64: 15, 28
+// At head dim 64 a page is half as long, and a second block finds it in L2; hence 32 columns there and 16 at 128.
+// (In between 16-bit pages of many long requests would be better off with the other kernel, those of few worse.)
+// 8 columns or 16: 32 requests as above, heads of 128, 8 columns 139 and 153 us (8 bits 109 and 143), 12 columns 263 and 158 (194
+// and 147).
 #include "paged_attention_impl.cuh"
 
 namespace bgtq {
@@ -22,7 +36,7 @@ size_t chunk_workspace(const PageView &c, uint32_t) {
 cudaError_t launch_chunk(const ChunkArgs &args, cudaStream_t s) {
     ChunkArgs a = args;
     if (a.window >= (uint64_t)a.width << a.c.page_shift) a.window = 0;  // all tokens that the table holds
-    if (a.q_tokens * a.group > 16ull * a.batch) return launch_paged_prompt(a, s);
+    if (a.q_tokens * a.group > (a.c.dim == 64 ? 32ull : 16ull) * a.batch) return launch_paged_prompt(a, s);
     switch (a.c.format) {
         case BGTQ_PAGES_F16: return by_shape<F_F16>(a, s);
         case BGTQ_PAGES_BF16: return by_shape<F_BF16>(a, s);

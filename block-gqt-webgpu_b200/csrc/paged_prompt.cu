@@ -76,7 +76,7 @@ struct Plan {
     static constexpr uint32_t kRawTile = kKeys * kRow, kRawScale = kKeys * kGroups * 2;
     // (the two tiles, the scales of both, and those of the K tile's tokens' values)
     static constexpr uint32_t kRawStage = 2 * kRawTile + 3 * kRawScale, kRawStages = kCodes ? (D == 128 ? 2 : 4) : 0;
-    static constexpr int kUpTile = F == F_INT8 ? 7 : 10, kUpKeys = kOwn ? 0 : kUpTile;  // log2 of what a tile's largest scale goes to
+    static constexpr int kUpTile = F == F_INT8 ? 7 : 10;  // log2 of what a tile's largest scale goes to
     // What softmax has to know of the K tile in a stage is kept until that tile's logits are done with, which is sure
     // when the load warp has gone all stages and the logits' lead further.
     static constexpr uint32_t kMeta = kRawStages + kStages + kBufs <= 8 ? 8 : 16;
@@ -89,7 +89,7 @@ struct Plan {
     static constexpr uint32_t kBadPages = kAbout + (kCodes ? kMeta * 16 : 0);              // [kMeta] pieces without a page: K, V
     static constexpr uint32_t kItems = kBadPages + kMeta * 4;      // [kDeal] Item
     static constexpr uint32_t kBars = kItems + kDeal * 64;
-    static constexpr uint32_t kBarCount = 3 * kStages + 2 * kRawStages + 3 * kTiles + 3 * kTiles * kBufs + 2 * kDeal + 2;
+    static constexpr uint32_t kBarCount = 3 * kStages + 2 * kRawStages + 4 * kTiles + 3 * kTiles * kBufs + 2 * kDeal + 2;
     static constexpr uint32_t kWords = kBars + 8 * kBarCount;      // tensor memory base, stop, bad-value flags
     static constexpr uint32_t kTotal = kWords + 32 + 1024;         // and the slack to align the base
     static_assert(kTotal <= 232448, "shared memory of a CTA");
@@ -161,12 +161,12 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
     const uint32_t bars = base + P::kBars;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     // a stage is full, free, or (raw) to be looked through first; a raw stage is full, free; of each row tile: its queries
-    // are there, are turned, are read; of each buffer of logits: they are there (and what was asked of the tensor cores
+    // are there, are turned, are read, and its part of an item's outputs is written; of each buffer of logits: they are there (and what was asked of the tensor cores
     // before them is done), the probabilities are, the last product from it is done; of each item: it is dealt, it is given
     // back
     constexpr uint32_t B_FULL = 0, B_FREE = P::kStages, B_RAW = 2 * P::kStages, B_CODES = 3 * P::kStages,
                        B_TURNED = B_CODES + P::kRawStages, B_QFULL = B_TURNED + P::kRawStages, B_QREADY = B_QFULL + NT,
-                       B_QFREE = B_QREADY + NT, B_S = B_QFREE + NT, B_P = B_S + NT * NB, B_O = B_P + NT * NB,
+                       B_QFREE = B_QREADY + NT, B_PART = B_QFREE + NT, B_S = B_PART + NT, B_P = B_S + NT * NB, B_O = B_P + NT * NB,
                        B_ITEM = B_O + NT * NB, B_TAKEN = B_ITEM + kDeal, B_END = B_TAKEN + kDeal;
     constexpr uint32_t W_LOAD = 4 * NT, W_MMA = W_LOAD + 1, W_ENDS = W_LOAD + 3;  // the warps past softmax
     const uint32_t per = kRows / a.group;  // rows of the request in a tile
@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             bar_init(bar(B_QFULL + i), 1);
             bar_init(bar(B_QREADY + i), 4);
             bar_init(bar(B_QFREE + i), 1);
+            bar_init(bar(B_PART + i), 4);
         }
         for (uint32_t i = 0; i < NT * NB; ++i) {
             bar_init(bar(B_S + i), 1);
@@ -266,10 +267,10 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
         // ---- softmax: thread = row of tile t ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kSoft));
         const int t = (int)warp >> 2;
-        const uint32_t row = threadIdx.x & 127u, p = row / a.group, g = row % a.group;
+        const uint32_t row = threadIdx.x & 127u, p = row / a.group;
         const uint32_t lanes = (warp & 3u) * 32u << 16;
         const uint32_t to = tmem + lanes + P::kColO + t * D;
-        uint32_t phase = 0, phase_o = 0;  // a bit for each buffer of logits
+        uint32_t phase = 0, phase_o = 0;  // a bit for each buffer of logits, and one for parts
         uint32_t q_phase = 0, stage_no = 0;
         // the tokens k0 .. k0 + 63 that a row at position `at` sees, a bit each
         auto mask_of = [&](int32_t at, int32_t keys, int32_t k0) -> uint64_t {
@@ -509,68 +510,87 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
                 if (!fine) break;
                 tc_after();
-                const uint32_t flagged = bad_flag[n % kDeal];
+                const uint32_t flagged = __shfl_sync(0xffffffffu, bad_flag[n % kDeal], 0);
                 // what outputs are multiplied by to be relative to the probabilities' maximum
                 const float back = !kCodes ? 1.0f : unit == -INFINITY ? 0.0f : ex2(unit - ref - kUpCodes - P::kUpTile);
-                // infinities and NaN among the values of the dimensions from d0 on that this row sees in tiles that were
-                // looked through, added to what the other tokens came to, which may be an infinity or a NaN of their own
-                auto overlay = [&](uint32_t *o, int d0, auto width) {
-                    constexpr int kW = decltype(width)::value;
+                // infinities and NaN among the values that this row sees in tiles that were looked through, added to
+                // what the other tokens came to, which may be an infinity or a NaN of their own
+                if (flagged) {
 #pragma unroll 1
-                    for (int32_t j = 0; j < sp.tiles; ++j) {
-                        const int32_t k0 = first_of(it, j);
-                        if (plain(it, k0)) continue;
-                        uint64_t m = live ? mask_of(at, it.keys, k0) : 0;
+                    for (int d0 = 0; d0 < D && sp.tiles; d0 += 16) {
+                        uint32_t o[16];
+                        tm_load16(to + d0, o);
+                        tc_wait_ld();
 #pragma unroll 1
-                        for (; m; m &= m - 1) {
-                            const uint32_t k = (uint32_t)k0 + __ffsll((long long)m) - 1;
-                            const int32_t page = __ldg(a.table + (int64_t)it.seq * a.table_stride + (k >> a.c.page_shift));
-                            if ((uint32_t)page >= a.c.pages) continue;
-                            const uint64_t r = ((uint64_t)page * a.c.heads + it.head << a.c.page_shift) + (k & (a.c.page_size - 1));
-                            if constexpr (kCodes) {
-                                const uint32_t sc = __ldg(a.c.vs + r * P::kGroups + (P::kGroups == 1 ? 0 : d0 / 32));
-                                if ((sc & 0x7f80u) == 0x7f80u)
+                        for (int32_t j = 0; j < sp.tiles; ++j) {
+                            const int32_t k0 = first_of(it, j);
+                            if (plain(it, k0)) continue;
+                            uint64_t m = live ? mask_of(at, it.keys, k0) : 0;
+#pragma unroll 1
+                            for (; m; m &= m - 1) {
+                                const uint32_t k = (uint32_t)k0 + __ffsll((long long)m) - 1;
+                                const int32_t page = __ldg(a.table + (int64_t)it.seq * a.table_stride + (k >> a.c.page_shift));
+                                if ((uint32_t)page >= a.c.pages) continue;
+                                const uint64_t r = ((uint64_t)page * a.c.heads + it.head << a.c.page_shift) + (k & (a.c.page_size - 1));
+                                if constexpr (kCodes) {
+                                    const uint32_t sc = __ldg(a.c.vs + r * P::kGroups + (P::kGroups == 1 ? 0 : d0 / 32));
+                                    if ((sc & 0x7f80u) == 0x7f80u)
 #pragma unroll
-                                    for (int i = 0; i < kW; ++i) o[i] = 0x7fc00000u;
-                            } else {
-                                constexpr uint32_t E = QBF ? 0x7f80u : 0x7c00u;
-                                const uint16_t *v = reinterpret_cast<const uint16_t *>(a.c.v) + r * D + d0;
+                                        for (int i = 0; i < 16; ++i) o[i] = 0x7fc00000u;
+                                } else {
+                                    constexpr uint32_t E = QBF ? 0x7f80u : 0x7c00u;
+                                    const uint16_t *v = reinterpret_cast<const uint16_t *>(a.c.v) + r * D + d0;
 #pragma unroll
-                                for (int i = 0; i < kW; ++i) {
-                                    const uint32_t y = __ldg(v + i);
-                                    if ((y & E) != E) continue;
-                                    const float z = QBF ? from_bf16(y) : __half2float(__ushort_as_half((unsigned short)y));
-                                    o[i] = __float_as_uint(__uint_as_float(o[i]) + z);
+                                    for (int i = 0; i < 16; ++i) {
+                                        const uint32_t y = __ldg(v + i);
+                                        if ((y & E) != E) continue;
+                                        const float z = QBF ? from_bf16(y) : __half2float(__ushort_as_half((unsigned short)y));
+                                        o[i] = __float_as_uint(__uint_as_float(o[i]) + z);
+                                    }
                                 }
                             }
                         }
+                        __syncwarp();
+                        tm_store16(to + d0, o);
+                        tc_wait_st();
                     }
-                };
-                // Parts of an item go to the workspace, [warp][dimension, maximum, sum][lane], and the warp that
-                // is the last of its kind to finish joins them, in the order of the CTAs.
+                }
+                // Parts of an item go to the workspace, [32 rows][dimension, maximum, sum][row].  The CTA that is the last
+                // to finish its part joins them, in the order of the CTAs, each warp of a row tile a quarter of the
+                // dimensions of all its rows: however few rows there are, four warps have loads under way.
                 const bool whole = it.parts == 1;
-                float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters) +
-                               (uint64_t)warp * (D + 2) * 32 + lane;
-                constexpr uint64_t kSlot = (uint64_t)4 * NT * (D + 2) * 32;
-                auto part_of = [&](int32_t c) { return parts + (2ull * c + (c == it.part ? 1 : 0)) * kSlot; };
+                constexpr uint64_t kBlock = (uint64_t)(D + 2) * 32, kSlot = 4 * NT * kBlock;
+                float *parts = reinterpret_cast<float *>(static_cast<unsigned char *>(a.workspace) + a.counters) + (uint64_t)(4 * t) * kBlock + lane;
+                auto part_of = [&](int32_t c, uint32_t block) { return parts + (2ull * c + (c == it.part ? 1 : 0)) * kSlot + block * kBlock; };
+                // blocks of 32 rows that are this warp's to write, and its runs of kW dimensions
+                constexpr int kW = P::kTurn, kL = kW / 8;
+                static_assert(D == 4 * kW);
+                uint32_t block = warp & 3u, block_end = block + 1;
+                int run = 0, run_end = D / kW;
                 if (!whole) {
-                    float *mine = part_of((int32_t)blockIdx.x);
-                    __stcg(mine + D * 32, sp.tiles ? ref : -INFINITY);
-                    __stcg(mine + (D + 1) * 32, sp.tiles ? sum : 0.0f);
+                    const uint32_t blocks = ((uint32_t)sp.count * a.group + 31) / 32;
+                    if (block < blocks) {
+                        float *mine = part_of((int32_t)blockIdx.x, block);
+                        __stcg(mine + D * 32, sp.tiles ? ref : -INFINITY);
+                        __stcg(mine + (D + 1) * 32, sp.tiles ? sum : 0.0f);
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16] = {};
-                        if (sp.tiles) {
-                            tm_load16(to + 16 * c, o);
-                            tc_wait_ld();
-                            if (flagged) overlay(o, 16 * c, std::integral_constant<int, 16>());
-                        }
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16] = {};
+                            if (sp.tiles) {
+                                tm_load16(to + 16 * c, o);
+                                tc_wait_ld();
+                            }
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]) * back);
+                            for (int i = 0; i < 16; ++i) __stcg(mine + (16 * c + i) * 32, __uint_as_float(o[i]) * back);
+                        }
+                        tc_before();
+                        __threadfence();
                     }
-                    tc_before();
-                    __threadfence();
                     __syncwarp();
+                    if (lane == 0) bar_arrive(bar(B_PART + t));
+                    if (!(fine = all_wait(bar(B_PART + t), phase >> 8 & 1u))) break;
+                    phase ^= 1u << 8;
+                    __threadfence();
                     uint32_t *counter = static_cast<uint32_t *>(a.workspace) + (uint64_t)it.part * 4 * NT + warp;
                     uint32_t before = 0;
                     if (lane == 0) {
@@ -582,106 +602,87 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                         continue;
                     }
                     __threadfence();
-                    ref = -INFINITY, sum = 0.0f;
-                    const int32_t after = it.part + it.parts;
-                    for (int32_t c = it.part; c < after; c += kJoin) {
-                        float m[kJoin], l[kJoin];
-#pragma unroll
-                        for (int b = 0; b < kJoin; ++b) {
-                            m[b] = c + b < after ? __ldcg(part_of(c + b) + D * 32) : -INFINITY;
-                            l[b] = c + b < after ? __ldcg(part_of(c + b) + (D + 1) * 32) : 0.0f;
-                        }
-                        float top = ref;
-#pragma unroll
-                        for (int b = 0; b < kJoin; ++b) top = max_nan(top, m[b]);
-                        const float from = top == -INFINITY ? 0.0f : top;
-                        sum *= ex2(ref - from);
-#pragma unroll
-                        for (int b = 0; b < kJoin; ++b) sum = fmaf(ex2(m[b] - from), l[b], sum);
-                        ref = top;
-                    }
+                    run = (int)block, run_end = run + 1;
+                    block = 0, block_end = blocks;
                 }
-                const bool none = at < 0 || it.keys == 0;
-                const float ref0 = ref == -INFINITY ? 0.0f : ref;
-                const float inv = none || sum == 0.0f ? 0.0f : whole ? back / sum : 1.0f / sum;  // (0: every logit is -infinity)
-                // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
-                constexpr int kW = P::kTurn, kL = kW / 8;
-                unsigned char *turn = sm + P::kOut + warp * 64 * kW;
                 const int64_t first_row = (int64_t)(it.token + t * (int32_t)per) * a.q_heads + it.head * a.group;
-                int32_t to_row[kL];  // of the rows that this lane writes for, from first_row on; -1 for none
-#pragma unroll
-                for (int i = 0; i < kL; ++i) {
-                    const uint32_t tr = (warp & 3u) * 32 + (32 / kL) * i + lane / kL, rp = tr / a.group;
-                    to_row[i] = rp < (uint32_t)sp.count ? (int32_t)(rp * a.q_heads + tr % a.group) : -1;
-                }
+                unsigned char *turn = sm + P::kOut + warp * 64 * kW;
                 // 16-byte chunk c of row r: a phase of eight lanes meets 128 different bytes, writing and reading
                 auto chunk = [&](uint32_t r, uint32_t c) { return turn + r * 2 * kW + ((c ^ r / (8 / kL) % kL) << 4); };
 #pragma unroll 1
-                for (int c = 0; c < D / kW; ++c) {
-                    uint32_t o[kW];
-#pragma unroll
-                    for (int i = 0; i < kW; ++i) o[i] = 0;
-                    if (!whole) {
-                        const int32_t after = it.part + it.parts;
-                        for (int32_t q = it.part; q < after; q += kJoin) {  // their loads in flight together
-                            float f[kJoin], y[kJoin][kW];
-#pragma unroll
-                            for (int b = 0; b < kJoin; ++b) {
-                                const float *from = part_of(q + b);
-                                f[b] = q + b < after ? __ldcg(from + D * 32) : -INFINITY;
-#pragma unroll
-                                for (int i = 0; i < kW; ++i) y[b][i] = q + b < after ? __ldcg(from + (kW * c + i) * 32) : 0.0f;
-                            }
-#pragma unroll
-                            for (int b = 0; b < kJoin; ++b) {
-                                const float e = ex2(f[b] - ref0);  // 0 for a part of no tile that this row sees
-#pragma unroll
-                                for (int i = 0; i < kW; ++i) o[i] = __float_as_uint(fmaf(e, y[b][i], __uint_as_float(o[i])));
-                            }
-                        }
-                    } else if (sp.tiles) {
-                        if constexpr (kW == 32) tm_load(to + kW * c, o);
-                        else tm_load16(to + kW * c, o);
-                        tc_wait_ld();
-                    }
-                    if (none) {
-#pragma unroll
-                        for (int i = 0; i < kW; ++i) o[i] = 0;
-                    }
-                    if (whole && flagged) overlay(o, kW * c, std::integral_constant<int, kW>());
-                    if (a.dtype == BGTQ_BF16) {
-#pragma unroll
-                        for (int i = 0; i < kL; ++i) {
-                            uint4 v;
-                            v.x = pack<true>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-                            v.y = pack<true>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-                            v.z = pack<true>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-                            v.w = pack<true>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(chunk(lane, i)) = v;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kL; ++i) {
-                            uint4 v;
-                            v.x = pack<false>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-                            v.y = pack<false>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-                            v.z = pack<false>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-                            v.w = pack<false>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(chunk(lane, i)) = v;
-                        }
-                    }
-                    __syncwarp();
+                for (; block < block_end; ++block) {
+                    const uint32_t own = 32 * block + lane, own_p = own / a.group;  // this thread's row
+                    const bool none = it.place + t * (int32_t)per + (int32_t)own_p < 0 || it.keys == 0;
+                    // kW dimensions at a time, turned through shared memory so that kL lanes write 16 kL bytes of a row
+                    int32_t to_row[kL];  // of the rows that this lane writes for, from first_row on; -1 for none
 #pragma unroll
                     for (int i = 0; i < kL; ++i) {
-                        const uint4 v = *reinterpret_cast<uint4 *>(chunk((32 / kL) * i + lane / kL, lane % kL));
-                        if (to_row[i] >= 0)
-                            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (first_row + to_row[i]) * D + kW * c +
-                                                       8 * (lane % kL)) = v;
+                        const uint32_t tr = 32 * block + (32 / kL) * i + lane / kL, rp = tr / a.group;
+                        to_row[i] = rp < (uint32_t)sp.count ? (int32_t)(rp * a.q_heads + tr % a.group) : -1;
                     }
-                    __syncwarp();
+#pragma unroll 1
+                    for (int c = run; c < run_end; ++c) {
+                        uint32_t o[kW];
+#pragma unroll
+                        for (int i = 0; i < kW; ++i) o[i] = 0;
+                        if (!whole) {
+                            ref = -INFINITY, sum = 0.0f;
+                            const int32_t after = it.part + it.parts;
+#pragma unroll 1
+                            for (int32_t q = it.part; q < after; q += kJoin) {  // their loads in flight together
+                                float m[kJoin], l[kJoin], y[kJoin][kW];
+#pragma unroll
+                                for (int b = 0; b < kJoin; ++b) {
+                                    const float *from = part_of(q + b, block);
+                                    m[b] = q + b < after ? __ldcg(from + D * 32) : -INFINITY;
+                                    l[b] = q + b < after ? __ldcg(from + (D + 1) * 32) : 0.0f;
+#pragma unroll
+                                    for (int i = 0; i < kW; ++i) y[b][i] = q + b < after ? __ldcg(from + (kW * c + i) * 32) : 0.0f;
+                                }
+                                float top = ref;
+#pragma unroll
+                                for (int b = 0; b < kJoin; ++b) top = max_nan(top, m[b]);
+                                const float to_top = top == -INFINITY ? 0.0f : top, f = ex2(ref - to_top);
+                                sum *= f;
+#pragma unroll
+                                for (int i = 0; i < kW; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+#pragma unroll
+                                for (int b = 0; b < kJoin; ++b) {
+                                    const float e = ex2(m[b] - to_top);  // 0 for a part of no tile that this row sees
+                                    sum = fmaf(e, l[b], sum);
+#pragma unroll
+                                    for (int i = 0; i < kW; ++i) o[i] = __float_as_uint(fmaf(e, y[b][i], __uint_as_float(o[i])));
+                                }
+                                ref = top;
+                            }
+                        } else if (sp.tiles) {
+                            if constexpr (kW == 32) tm_load(to + kW * c, o);
+                            else tm_load16(to + kW * c, o);
+                            tc_wait_ld();
+                        }
+                        if (none) {
+#pragma unroll
+                            for (int i = 0; i < kW; ++i) o[i] = 0;
+                        }
+                        const float inv = none || sum == 0.0f ? 0.0f : whole ? back / sum : 1.0f / sum;  // (0: every logit is -infinity)
+#pragma unroll
+                        for (int i = 0; i < kL; ++i) {
+                            auto two = [&](int k) { return pack<QBF>(__uint_as_float(o[8 * i + k]) * inv, __uint_as_float(o[8 * i + k + 1]) * inv); };
+                            *reinterpret_cast<uint4 *>(chunk(lane, i)) = make_uint4(two(0), two(2), two(4), two(6));
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < kL; ++i) {
+                            const uint4 v = *reinterpret_cast<uint4 *>(chunk((32 / kL) * i + lane / kL, lane % kL));
+                            if (to_row[i] >= 0)
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (first_row + to_row[i]) * D + kW * c +
+                                                           8 * (lane % kL)) = v;
+                        }
+                        __syncwarp();
+                    }
+                    if (run == 0 && own_p < (uint32_t)sp.count && a.lse)
+                        a.lse[first_row + (int64_t)own_p * a.q_heads + own % a.group] = none ? -INFINITY : (ref - (kCodes ? 0.0f : kUp<BF>) + __log2f(sum)) * kLn2;
                 }
-                if (live && a.lse)
-                    a.lse[first_row + (int64_t)p * a.q_heads + g] = none ? -INFINITY : (ref - (kCodes ? 0.0f : kUp<BF>) + __log2f(sum)) * kLn2;
                 tc_before();
             }
             if (!fine) break;
@@ -1222,7 +1223,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             auto weigh = [&](const uint16_t *keys, const uint16_t *values, const Sizes &zk, const Sizes &zv, uint32_t meta, uint32_t rows) {
                 if (lane == 0) {
                     About &about = reinterpret_cast<About *>(sm + P::kAbout)[meta];
-                    about.mul = __uint_as_float((zk.top - P::kUpKeys) << 23) * a.scale;
+                    about.mul = __uint_as_float((zk.top - (P::kOwn ? 0 : P::kUpTile)) << 23) * a.scale;
                     about.top = (float)zv.top - 127.0f;
                     about.each = (zk.apart() ? 1u : 0u) | (zv.apart() ? 2u : 0u);
                 }
