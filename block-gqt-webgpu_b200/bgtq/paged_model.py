@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .model import ModelGeometry
-from .serving import PagedCache, adjust_logits, prompt_attention, _refuse
+from .serving import PagedCache, adjust_logits, prompt_attention, _per_row, _refuse
 
 
 _RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width, both rounded up
@@ -304,6 +304,9 @@ class PagedDecoder:
             for r, p in zip(row, prompts):
                 r[:len(p)] = p.cpu() if torch.is_tensor(p) else p
             history = self._to(row, torch.int64)
+            # (numbers are filled in once, not for every token)
+            choice.update({name: _per_row(choice[name], len(prompts), history.device, name)
+                           for name in ("repetition", "presence", "frequency") if choice.get(name) is not None})
             at = torch.as_tensor(lengths, device=self.dev)[:, None]
 
         def chosen(logits):

@@ -52,8 +52,12 @@ def _recording(device) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
+# torch.cuda.current_stream(device).cuda_stream without the objects in between, which are a microsecond of a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
 
 
 class PagedCache:
@@ -414,10 +418,8 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
 
 
 def _per_row(x, batch: int, device, name: str):
-    """A penalty as float32 [batch]: a tensor as it is, a number filled in; None stays."""
-    if x is None:
-        return None
-    if not torch.is_tensor(x):
+    """A penalty as float32 [batch]: a tensor as it is, a number filled in."""
+    if not isinstance(x, torch.Tensor):
         if not -float("inf") < x < float("inf") or name == "repetition" and x <= 0.0:
             _refuse(f"Logits: {name} must be finite" + (" and positive" if name == "repetition" else ""))
         return torch.full((batch,), float(x), dtype=torch.float32, device=device)
@@ -467,8 +469,12 @@ def adjust_logits(logits, tokens=None, lengths=None, repetition=None, presence=N
         _refuse("Logits: lengths must be a contiguous int32 tensor [batch] on the logits' device, with tokens")
     if tokens is None and not repetition is presence is frequency is None:
         _refuse("Logits: penalties need tokens")
-    repetition, presence, frequency = (_per_row(x, batch, on, n) for x, n in (
-        (repetition, "repetition"), (presence, "presence"), (frequency, "frequency")))
+    if repetition is not None:
+        repetition = _per_row(repetition, batch, on, "repetition")
+    if presence is not None:
+        presence = _per_row(presence, batch, on, "presence")
+    if frequency is not None:
+        frequency = _per_row(frequency, batch, on, "frequency")
     bias_stride = mask_stride = entries = 0
     if (bias is None) != (bias_ids is None):
         _refuse("Logits: bias and bias_ids come together")
@@ -492,8 +498,11 @@ def adjust_logits(logits, tokens=None, lengths=None, repetition=None, presence=N
     p = _lib.LogitsDesc(on.index, dtype, batch, vocab, logits.data_ptr(), logits.stride(0),
                         None if tokens is None else tokens.data_ptr(), tokens_stride, width,
                         8 if tokens is not None and tokens.dtype == torch.int64 else 4,
-                        *(None if t is None else t.data_ptr()
-                          for t in (lengths, repetition, presence, frequency, bias_ids, bias)),
+                        None if lengths is None else lengths.data_ptr(),
+                        None if repetition is None else repetition.data_ptr(),
+                        None if presence is None else presence.data_ptr(),
+                        None if frequency is None else frequency.data_ptr(),
+                        None if bias_ids is None else bias_ids.data_ptr(), None if bias is None else bias.data_ptr(),
                         bias_stride, entries, None if mask is None else mask.data_ptr(), mask_stride, out.data_ptr(),
                         out.stride(0))
     status = _lib.lib().bgtq_adjust_logits(C.byref(p), _stream(on.index))
