@@ -35,10 +35,20 @@ namespace bgtq {
 namespace {
 
 constexpr uint32_t kDeal = 4;            // items dealt ahead
-constexpr int64_t kItemCost = 384;       // what an item costs beside its keys, in keys: queries, outputs, joining
-constexpr int32_t kWhole = 1024;         // items of no more keys are not split
-constexpr int64_t kPiece = 512;          // keys that make a CTA worth its while where items are few and long
-constexpr int kJoin = 2;                 // parts of an item that are joined at a time
+// What an item costs beside its keys, in keys: queries, outputs, joining.  (None: 20 requests of 1 to 700 rows after up to
+// 9000, 32 / 8 heads of 128, 271 us for 146, one of 500 rows after 4000, 14 / 2 heads of 64 in 8 bits, 76 for 58; 192: 167 and
+// 58, 640: 156 and 60.)
+constexpr int64_t kItemCost = 384;
+// Items of no more keys are not split: joining costs as much as they do, less where rows are few.  kWholeFew is for
+// requests of up to 64 columns - rows x query heads of a KV head.  (700 rows of one request, 32 / 8 heads of 128, 25 us, with
+// 512 for all 34; 12 prompts of 1 to 2047 rows 86 us, with 1536 92.  Few: 32 x 5 rows after 500 to 16000 in 8 bits 167 us
+// with 256, 180 with 1024; 8 x 8 rows after 200 to 2000, 14 / 2 heads of 64, 21.6 and 29.8, 32 / 8 of 128 22.6 and 32.4; 128 does
+// what 256 does.)
+constexpr int32_t kWhole = 1024, kWholeFew = 256;
+// Keys that make a CTA worth its while where items are few and long.  (8 x 8 rows after 200 to 2000 in 8 bits of 64
+// dimensions: 35 us with 256, 39 with 512, 48 with 1024; 8 after 30000, 14 / 2 heads of 64: 51, 44, 38.)
+constexpr int64_t kPiece = 512;
+constexpr int kJoin = 2;                 // parts of an item that are joined at a time (1: 8 rows after 30000 as above 58 us for 44)
 constexpr float kLazy = 8.0f;            // log2 of the growth of a maximum that is left standing
 template <bool BF> constexpr float kUp = BF ? 0.0f : 15.0f - kLazy;  // log2 of what probabilities are multiplied by
 // Over 8- and 4-bit pages (powers of two, as logarithms): how far a tile's largest probability x value scale may pass the
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             // ---- the deal ----
             // An item's price is its tokens, as its last row sees them, and kItemCost; items stand in order - requests, KV
             // heads, blocks - on a line as long as their prices, unit j of one at kItemCost + 64 j of its stretch, and the
-            // line is cut into equal ranges, one a CTA, none shorter than a tile.  An item of up to kWhole tokens is the
+            // line is cut into equal ranges, one a CTA, none shorter than a tile.  An item of up to kWhole (or kWholeFew) tokens is the
             // CTA's in whose range it begins.  With a window no item is priced above `most`, which holds its units.
             const int32_t block = (int32_t)(a.tiles * per);
             const int64_t most = a.window ? (int64_t)a.window + block + ((int64_t)(a.sinks + 63u) & ~63ll) + 2 * kKeys : (int64_t)1 << 40;
@@ -753,21 +763,22 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
             };
             int64_t total = __shfl_sync(0xffffffffu, own_upto, 31);
             uint32_t blocks = (uint32_t)mine.blocks;
-            auto longest_of = [&](const Seq &q) { return q.blocks ? (int32_t)min((int64_t)q.nk, min(most, (int64_t)0x7fffffff)) : 0; };
-            int32_t longest = longest_of(mine);
+            auto whole_of = [&](const Seq &q) { return (int64_t)q.nq * a.group <= 64 ? kWholeFew : kWhole; };
+            auto splits = [&](const Seq &q) { return q.blocks && min((int64_t)q.nk, most) > whole_of(q); };
+            bool split = splits(mine);
             if (a.batch > 32) {
                 int64_t rest = 0;
                 for (uint32_t s = lane + 32; s < a.batch; s += 32) {
                     const Seq q = load_seq(s);
                     rest += a.c.heads * price(q, q.blocks);
                     blocks += (uint32_t)q.blocks;
-                    longest = max(longest, longest_of(q));
+                    split |= splits(q);
                 }
                 total += __shfl_sync(0xffffffffu, scan(rest), 31);
             }
             const int64_t all = (int64_t)__reduce_add_sync(0xffffffffu, blocks) * a.c.heads;
             int64_t ctas = min((int64_t)gridDim.x, max((int64_t)1, total / kKeys));
-            if (__reduce_max_sync(0xffffffffu, longest) > kWhole) ctas = min(ctas, max(all, total / kPiece));
+            if (__any_sync(0xffffffffu, split)) ctas = min(ctas, max(all, total / kPiece));
             bool some = total > 0 && ctas > 0 && (int64_t)blockIdx.x < ctas;
             const int64_t each = some ? quotient(total, ctas) : 1, over = some ? total - each * ctas : 0;
             const int64_t start = blockIdx.x * each + min((int64_t)blockIdx.x, over);
@@ -825,7 +836,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const int32_t gap = lo / kKeys - sunk, units = max(1, (hi + kKeys - 1) / kKeys - gap);
                     const int64_t from = at + kItemCost;
                     int32_t one, two;
-                    if (keys <= kWhole) {  // where it begins
+                    if (keys <= whole_of(sq)) {  // where it begins
                         one = 0;
                         two = at >= start ? units : 0;
                     } else {
@@ -1375,11 +1386,13 @@ cudaError_t run(const ChunkArgs &args, int sms, uint32_t tiles, cudaStream_t s) 
 template <int F, bool QBF>
 cudaError_t by_shape(const ChunkArgs &a, int sms, cudaStream_t s) {
     // The row tiles of an item share its K and V loads and keep the softmax warps busy: as many as possible, while
-    // that makes half as many items as there are SMs.
+    // that makes a sixth as many items as there are SMs.  (Splitting keys is no dearer than splitting rows: 500 rows
+    // after 8000, 32 / 8 heads of 128, 79 us, and 102 with half as many items as SMs; two of 1000 after 4000 to 8000, 14 / 2 heads
+    // of 64 in 8 bits, 104 and 149.  An eighth, or a sixteenth: 700 rows of 64 dimensions without earlier tokens 28.6 us for 23.8.)
     const uint32_t per = kRows / a.group;
     auto items = [&](uint32_t tiles) { return a.c.heads * ((a.q_tokens + tiles * per - 1) / (tiles * per) + a.batch - 1); };
     uint32_t tiles = a.c.dim == 64 ? 4 : 2;
-    while (tiles > 1 && 2 * items(tiles) <= (uint64_t)sms) tiles /= 2;
+    while (tiles > 1 && 6 * items(tiles) <= (uint64_t)sms) tiles /= 2;
     if (a.c.dim == 128) return run<128, 2, F, QBF>(a, sms, tiles, s);
     return run<64, 4, F, QBF>(a, sms, tiles, s);
 }
