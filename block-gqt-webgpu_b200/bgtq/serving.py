@@ -165,7 +165,7 @@ class PagedCache:
         three are float16, bfloat16 or float32, of any strides with a contiguous last dimension.
         Dimension i < dim / 2 is rotated with dimension i + dim / 2 by the token's row of ``rotary``
         [rows, dim] (float32: dim / 2 cosines, then sines), row positions[t] (int64) or, without
-        positions, row t.  Negative slots are padding: nothing is stored of them.  A token whose
+        positions, row t.  Negative slots are padding: nothing is stored of them; others come once in a call.  A token whose
         position is outside the table is not stored and its results are zeros.
         Returns the queries, as dtype (default: q's own), with ``keys`` also the keys."""
         self._check_slots(slots)
@@ -450,7 +450,8 @@ def adjust_logits(logits, tokens=None, lengths=None, repetition=None, presence=N
     int64), negative ones left out.  Penalties are numbers or float32 [batch]; repetition is positive.  bias_ids (int32) and bias
     (float32) are [batch, n] or, for all rows alike, [1, n]; mask (int32, the bits of 32 tokens a word) [batch,
     ceil(vocab / 32)] or [1, ...].  Token ids past the vocabulary are left out and set bit 4 of `device_status`, lengths
-    outside 0 .. width are cut and set bit 8.  Returns the result, a new tensor or ``out`` (which may be logits)."""
+    outside 0 .. width are cut and set bit 8.  Returns the result, a new tensor or ``out``, which may be the logits
+    themselves and else shares no memory with them."""
     if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1 or logits.stride(1) != 1 and logits.shape[1] > 1:
         _refuse("Logits: logits must be a CUDA tensor [batch, vocab] with a contiguous last dimension")
     batch, vocab = logits.shape

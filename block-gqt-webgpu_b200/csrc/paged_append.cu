@@ -3,6 +3,11 @@
 //     y = x w / sqrt(mean(x^2) + eps),   (y_i, y_{i + D/2}) -> (y_i c_i - y_{i + D/2} s_i, y_{i + D/2} c_i + y_i s_i)
 // Rows that become codes are computed in pairs of FP32 numbers (a norm's factor in 64 bits) and rounded to FP32 once: a code is
 // a step function of its row, and so is the same whatever order sums and products are taken in.  All else is FP32.
+//
+// A row is D / 16 threads, each with two runs of eight dimensions that are rotated into each other: no shared memory, a norm's
+// sum and a row's largest by shuffles.  16384 tokens, 32 / 8 heads of 128 from BF16: into 16 bits 75 us, 5.4 TB/s; into 8 bits
+// 79; into 4 bits with norms 102, where the pairs of numbers and the packing of codes issue as long as the loads take.  A
+// token of one request takes 2.5 us, next to nothing of which is work.
 #include <type_traits>
 
 #include "paged_rows.cuh"

@@ -1,5 +1,11 @@
 // Attention of one new token per request, or of a few, over the pages of a cache:
-//     out = sum_t softmax_t(scale q.k_t) v_t  over the request's first `length` tokens.
+//     out = sum_t softmax_t(scale q.k_t) v_t  over the request's first `length` tokens;
+// of chunks (C) row i of n sees those up to its position, length - n + i, with a window the last and the first few of them.
+// Chunks are the same with (row, query head) pairs for query heads: a block of 8 or 16 of them shares its units, which have
+// a gap where no row's window reaches, and what a unit's edge hides from some of its columns is masked, a value that is
+// not finite there taken out of the product and added for the columns that see it.  (64 requests of one row, a window of 2048, 14 / 2
+// heads of 64: 25 us; the same tokens without a window 24, with the code for one token alone 22.  Bound by latency: the batch of 32
+// takes 15.)
 //
 // What bounds it is the one pass over K and V: 2 row_bytes a token and KV head, against 2 D
 // multiply-adds for each query head, so the work is laid out for the memory system.  128 requests

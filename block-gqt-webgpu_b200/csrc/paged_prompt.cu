@@ -16,17 +16,26 @@
 //               row that does not see it would turn into a NaN, is taken out; the rows that see it look the tile
 //               through once more, in the pages, when they are written
 //   codes       (8- and 4-bit pages) codes and scales are loaded as they are, and warps of their own turn a tile into
-//               FP16 operands ahead of the products: codes x scales over a power of two of the tile's largest scale, which
-//               multiplies the tile's logits as the scale of all logits does, and its probabilities as an addend of their
-//               exponents, so that softmax does no more than over 16-bit pages.  A key stays exact, so that
-//               logits are FP32's: 4-bit codes x scales have 11 bits, 8-bit ones have 15, of which a second operand
-//               holds the last four, multiplied by the same queries into the same logits.  (BF16 queries go to FP16
-//               over a power of two of their row, which loses what is below 2^-38 of the row's largest.)  A value in 8 bits is
-//               rounded to 11 bits, a sixteenth of the step that its code was rounded to.  Where the scales of a
-//               tile are more than 2^16 apart, as next to rows of 1e30, powers of two of each token take their place
-//               and multiply each logit, or each probability.  Probabilities x value scales are taken relative to
-//               the row's largest so far, in steps of at least 2^kRoom, so that values of any size whose weight is next
-//               to nothing leave the others as they are; what is rounded away is 2^-34 of the largest
+//               FP16 operands ahead of the products.  A key stays exact, so that logits are FP32's: 4-bit codes x scales
+//               over a power of two of the tile's largest scale have 11 bits; 8-bit ones have 15, of which at head dim 64 a
+//               second operand holds the last four, multiplied by the same queries into the same logits; at 128, where
+//               tensor time is what there is least of, 8-bit codes stay plain and softmax multiplies each key's logits
+//               by its scale.  The tile's power multiplies its logits as the scale of all logits does, and its
+//               probabilities as an addend of their exponents, so that softmax does no more than over 16-bit pages.
+//               (BF16 queries go to FP16 over a power of two of their row, which loses what is below 2^-38 of the row's
+//               largest.)  A value in 8 bits is rounded to 11 bits, a sixteenth of the step that its code was rounded
+//               to.  Where the scales of a tile are more than 2^16 apart, as next to rows of 1e30, powers of two of each
+//               token take their place and multiply each logit, or each probability.  Probabilities x value scales are
+//               taken relative to the row's largest so far, in steps of at least 2^kRoom, so that values of any size
+//               whose weight is next to nothing leave the others as they are; what is rounded away is 2^-34 of the
+//               largest
+//
+// What bounds it.  Many rows: the tensor cores and, at head dim 64, the exponentials of softmax: four chunks of 1024 rows after
+// 6000 to 8192 tokens, 32 / 8 heads of 128 in 16 bits, 445 us, 1140 TFLOP/s; two of 2048 after 24000 to 30000, 14 / 2 heads of
+// 64, 470 us, 876 TFLOP/s.  Over codes the warps that turn them and the code they share the instruction caches with:
+// the first in 8 bits 600 us, in 4 bits 686; the second in 8 bits 630 (96 registers of softmax's warps and the keys' second
+// operand).  Few rows: 32 requests of 5 rows after 500 to 16000 tokens, 32 / 8 heads of 128, 125 us, 4.8 TB/s; in 8
+// bits 167 us, 1.9 TB/s.  Few tokens: 20 to 45 us of the deal, the first pages' way through the table, and the join.
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -66,7 +75,9 @@ struct Plan {
     static constexpr uint32_t kBufs = NT == 4 ? 1 : 2;             // of logits, for each row tile
     static constexpr uint32_t kKeys = 64;                          // of a K or V tile
     static constexpr uint32_t kColO = kTiles * kBufs * kKeys;      // the first column of the outputs
-    static constexpr uint32_t kEnds = kCodes ? (NT == 4 ? 5 : 9) : 1;  // warps that look at, or turn, tiles
+    // Warps that look at, or turn, tiles; over codes the first sees to their scales.  (Two chunks of 2048 after 24000 to 30000, 14 / 2
+    // heads of 64 in 8 bits, one that turns 1189 us, four 630.)
+    static constexpr uint32_t kEnds = kCodes ? (NT == 4 ? 5 : 9) : 1;
     static constexpr uint32_t kThreads = 128 * NT + 32 * (3 + kEnds);
     // Registers after the hand-over, of softmax's warps and of the others: what the launch has, in all.
     static constexpr uint32_t kSoft = NT == 4 ? (kCodes ? 96 : 104) : kCodes ? 128 : 216, kRest = NT == 4 ? (kCodes ? 48 : 64) : 72;
@@ -171,9 +182,9 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
     const uint32_t bars = base + P::kBars;
     auto bar = [&](uint32_t i) { return bars + 8u * i; };
     // a stage is full, free, or (raw) to be looked through first; a raw stage is full, free; of each row tile: its queries
-    // are there, are turned, are read, and its part of an item's outputs is written; of each buffer of logits: they are there (and what was asked of the tensor cores
-    // before them is done), the probabilities are, the last product from it is done; of each item: it is dealt, it is given
-    // back
+    // are there, are turned, are read, its part of an item's outputs is written; of each buffer of logits: they are there (and
+    // what was asked of the tensor cores before them is done), the probabilities are, the last product from it is done; of
+    // each item: it is dealt, it is given back
     constexpr uint32_t B_FULL = 0, B_FREE = P::kStages, B_RAW = 2 * P::kStages, B_CODES = 3 * P::kStages,
                        B_TURNED = B_CODES + P::kRawStages, B_QFULL = B_TURNED + P::kRawStages, B_QREADY = B_QFULL + NT,
                        B_QFREE = B_QREADY + NT, B_PART = B_QFREE + NT, B_S = B_PART + NT, B_P = B_S + NT * NB, B_O = B_P + NT * NB,

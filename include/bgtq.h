@@ -522,8 +522,9 @@ bgtq_status bgtq_paged_attend(const bgtq_paged_cache *c, const void *q, bgtq_dty
  *             first and the second half of the token's row of `rotary`
  * and keys and values are stored at the token's slot as bgtq_paged_write stores rows, queries (and, where k_out is
  * given, keys) written to dense outputs.  Element (t, h, i) of q is at q[t * q_token_stride + h * q_head_stride + i]
- * of dtype (F16, BF16 or F32), k and v the same.  Rows of 8- and 4-bit pages are normed and rotated in 64 bits and
- * rounded to FP32 once before they are quantised, so their codes are the formula's; all else is FP32.  A negative
+ * of dtype (F16, BF16 or F32), k and v the same.  Rows of 8- and 4-bit pages are normed and rotated in more than
+ * FP32 (pairs of FP32 numbers, a norm's sum in 64 bits) and rounded to FP32 once before they are quantised, so their
+ * codes are the formula's; all else is FP32.  A negative
  * slot is padding: its outputs are written, its rows are not stored.  Slots of one call are distinct.  A slot past the
  * last page is not stored; a token whose position is outside the table is not stored and its outputs are zeros; both
  * set a bit of the device status word. */
@@ -622,11 +623,11 @@ bgtq_status bgtq_prompt_attend(const bgtq_prompt *p, void *stream);
  * each step where its arguments are given (null arrays and a repetition of 1, a presence and a frequency of 0 leave x as
  * it is), and is rounded to dtype once.  Token ids are int32 or int64 (id_bytes 4 or 8); negative ones are padding, ones
  * past the vocabulary are left out and set a bit of the device status word, as does a length below 0 or past width,
- * which is cut.  out may be logits. */
+ * which is cut.  out is logits itself or shares no memory with it. */
 typedef struct bgtq_logits {
     int device;
     bgtq_dtype dtype;       /* F16, BF16 or F32 */
-    uint32_t batch, vocab;
+    uint32_t batch, vocab;  /* at most 65535; 1 to 2^31 - 65537 */
     const void *logits;     /* [batch][vocab], rows logits_stride elements apart */
     int64_t logits_stride;
     const void *tokens;     /* [batch][width] ids, rows tokens_stride elements apart, or null */
