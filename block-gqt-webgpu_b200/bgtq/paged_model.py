@@ -25,6 +25,7 @@ from .model import ModelGeometry
 from .serving import PagedCache, adjust_logits, prompt_attention, _per_row, _refuse
 
 
+_PENALTIES = ("repetition", "presence", "frequency")
 _RECORDED = 16  # steps that a decoder keeps recorded, by requests and table width, both rounded up
 
 
@@ -296,18 +297,21 @@ class PagedDecoder:
         [prompts, count].  choice: what is put on the logits before each token is chosen, as
         `adjust_logits` takes it (repetition, presence, frequency, bias_ids, bias, mask; the history is
         a request's prompt and what it was answered).  Its requests are closed before it returns."""
-        requests = [self.open() for _ in prompts]
+        penalties = [name for name in _PENALTIES if choice.get(name) is not None]
+        if set(choice) - {*_PENALTIES, "bias_ids", "bias", "mask"}:
+            _refuse(f"Paged decoder: choice is of {', '.join(_PENALTIES)}, bias_ids, bias and mask")
         history = None
-        if any(choice.get(name) is not None for name in ("repetition", "presence", "frequency")):
-            lengths = [len(p) for p in prompts]
-            row = np.full((len(prompts), max(lengths, default=0) + max(count, 0)), -1, np.int64)
-            for r, p in zip(row, prompts):
-                r[:len(p)] = p.cpu() if torch.is_tensor(p) else p
+        if penalties:
+            texts = [np.asarray(p.cpu() if torch.is_tensor(p) else p, np.int64).reshape(-1) for p in prompts]
+            lengths = [len(p) for p in texts]
+            row = np.full((len(texts), max(lengths, default=0) + max(count, 0)), -1, np.int64)
+            for r, p in zip(row, texts):
+                r[:len(p)] = p
             history = self._to(row, torch.int64)
             # (numbers are filled in once, not for every token)
-            choice.update({name: _per_row(choice[name], len(prompts), history.device, name)
-                           for name in ("repetition", "presence", "frequency") if choice.get(name) is not None})
+            choice.update({name: _per_row(choice[name], len(texts), history.device, name) for name in penalties})
             at = torch.as_tensor(lengths, device=self.dev)[:, None]
+        requests = [self.open() for _ in prompts]
 
         def chosen(logits):
             if choice:

@@ -176,6 +176,19 @@ def test_generate_with_penalties_biases_and_a_mask(cuda):
     assert dec.generate(prompts[:1], 0, presence=1.0).shape == (1, 0) and dec.free_pages == 16
 
 
+def test_generate_refuses_before_it_opens_requests(cuda):
+    import torch
+    from bgtq import PagedDecoder
+    g = SMALL["llama"]
+    dec = PagedDecoder(weights_of(g, "f16"), g, pages=4, page_size=16, dtype=torch.float16)
+    for kw in (dict(repetition=0.0), dict(presence=math.nan), dict(frequency=torch.zeros(3, device="cuda")), dict(out=1), dict(lengths=1),
+               dict(tokens=1), dict(temperature=1.0), dict(bias=torch.zeros(1, 1, device="cuda")), dict(mask=torch.zeros(1, 1, device="cuda"))):
+        with pytest.raises(_lib.RangeError):
+            dec.generate([[1, 2]], 2, **kw)
+        assert not dec._held and dec.free_pages == 4
+    assert (dec.generate([np.array([[1, 2, 3]])], 3, frequency=0.0) == dec.generate([[1, 2, 3]], 3)).all()
+
+
 def test_refusals(cuda):
     import torch
     from bgtq import PagedDecoder
