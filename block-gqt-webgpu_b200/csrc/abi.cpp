@@ -63,9 +63,18 @@ uint32_t *device_status_word(int device) {
     if (device < 0 || device >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(g_status_mu);
     if (!g_status[device]) {
+        // A process's first call may be one that is being captured: what makes the word is not part of the graph.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
         void *p = nullptr;
-        if (cudaMalloc(&p, sizeof(uint32_t)) != cudaSuccess) return nullptr;
-        cudaMemset(p, 0, sizeof(uint32_t));
+        cudaStream_t side = nullptr;
+        const bool made = cudaMalloc(&p, sizeof(uint32_t)) == cudaSuccess &&
+                          cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking) == cudaSuccess &&
+                          cudaMemsetAsync(p, 0, sizeof(uint32_t), side) == cudaSuccess && cudaStreamSynchronize(side) == cudaSuccess;
+        if (side) cudaStreamDestroy(side);
+        if (!made && p) cudaFree(p);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!made) return nullptr;
         g_status[device] = static_cast<uint32_t *>(p);
     }
     return g_status[device];
