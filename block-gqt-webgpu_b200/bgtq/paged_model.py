@@ -101,7 +101,7 @@ class PagedDecoder:
         keep = -(-length // self.page_size)
         if length and -1 in pages[self._first(length) // self.page_size:keep]:
             _refuse("Paged decoder: pages of tokens that would be seen again have been given back")
-        self._free += pages[keep:][::-1]
+        self._free += [p for p in pages[keep:][::-1] if p >= 0]
         held[0], held[1] = pages[:keep], length
 
     def _first(self, length: int) -> int:
