@@ -108,13 +108,14 @@ class PagedDecoder:
         """The first token that the next one sees, but for sinks."""
         return 0 if self.window is None else max(0, length - self.window + 1)
 
-    def _release(self, held) -> None:
-        """Gives back the pages of tokens that no later one sees (-1 stands for them from then on)."""
+    def _unseen(self, held):
+        """Places of the pages of tokens that no later one sees, in order (those given back before lie in front of them)."""
         pages, length = held
-        for i in range(-(-self.sinks // self.page_size), min(self._first(length) // self.page_size, len(pages))):
-            if pages[i] >= 0:
-                self._free.append(pages[i])
-                pages[i] = -1
+        first, end = -(-self.sinks // self.page_size), min(self._first(length) // self.page_size, len(pages))
+        at = end
+        while at > first and pages[at - 1] >= 0:
+            at -= 1
+        return range(at, end)
 
     def length(self, request: int) -> int:
         """Tokens of a request whose rows the pages hold."""
@@ -131,20 +132,24 @@ class PagedDecoder:
 
     @contextlib.contextmanager
     def _grown(self, requests, counts):
-        """Pages for counts[i] more tokens of requests[i], all of them or a refusal: what each holds now and
-        its length before.  A body that fails has written no rows to count on, so it leaves lengths and
-        pages as they were."""
+        """Pages for counts[i] more tokens of requests[i], all of them or a refusal, which changes nothing: what
+        each holds now and its length before.  Pages that their later tokens do not see are given back (-1 stands
+        for them from then on).  A body that fails has written no rows to count on, so it leaves lengths and pages
+        as they were; but of the pages given back, those that the call took again have lost their rows, and stay
+        free.  They are the last that a call takes."""
         requests = requests.tolist() if hasattr(requests, "tolist") else list(requests)
         if not requests or len(set(requests)) < len(requests):
             _refuse("Paged decoder: requests must be one or more, each once")
         held = [self._request(r) for r in requests]
-        if self.window is not None:
-            for h in held:
-                self._release(h)
+        back = [(h[0], i, h[0][i]) for h in held for i in self._unseen(h)] if self.window is not None else []
         need = [-(-(h[1] + n) // self.page_size) - len(h[0]) for h, n in zip(held, counts)]
-        if sum(need) > len(self._free):
-            _refuse(f"Paged decoder: {sum(need)} pages wanted, {len(self._free)} free")
+        if sum(need) > len(self._free) + len(back):
+            _refuse(f"Paged decoder: {sum(need)} pages wanted, {len(self._free) + len(back)} free")
         before = [h[1] for h in held]
+        for pages, i, _ in back:
+            pages[i] = -1
+        kept = back[max(0, sum(need) - len(self._free)):]
+        self._free[:0] = [page for _, _, page in back[::-1]]
         for h, n, more in zip(held, counts, need):
             h[0] += [self._free.pop() for _ in range(more)]
             h[1] += n
@@ -155,6 +160,9 @@ class PagedDecoder:
                 self._free += h[0][len(h[0]) - more:][::-1]
                 del h[0][len(h[0]) - more:]
                 h[1] = start
+            for pages, i, page in kept:
+                pages[i] = page
+            del self._free[:len(kept)]
             raise
 
     def _slots(self, pages, first: int, upto: int):

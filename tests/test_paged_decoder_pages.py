@@ -57,3 +57,56 @@ def test_a_rewind_to_tokens_that_have_gone_is_refused():
     assert (dec._held[a][0], dec._free) == was and dec.length(a) == 360
     dec.rewind(a, 355)
     every_page_once(dec, 14)
+
+
+def state(dec):
+    return {r: (list(h[0]), h[1]) for r, h in dec._held.items()}, list(dec._free)
+
+
+def test_a_refused_call_changes_nothing():
+    """A call of too many tokens, and what a rewind takes back after it."""
+    dec = books(14, 50, 4)
+    a, b = dec.open(), dec.open()
+    grow(dec, a, 80)
+    was = state(dec)
+    for requests, counts in (([a], [400]), ([b, a], [1, 400])):
+        with pytest.raises(_lib.RangeError, match="pages wanted, 9 free"):
+            with dec._grown(requests, counts):
+                pass
+        assert state(dec) == was
+    dec.rewind(a, 60)
+    assert dec.length(a) == 60
+    every_page_once(dec, 14)
+
+
+@pytest.mark.parametrize("free", [0, 1, 2, 6])
+@pytest.mark.parametrize("count,taken", [(1, 1), (16, 1), (17, 2), (32, 2)])
+def test_a_call_that_fails_gives_back_what_it_took(free, count, taken):
+    """Of 7 pages the second and the third are behind the window: the last that a call takes, and, where it did not,
+    the request's again when it fails."""
+    dec = books(7 + free, 50, 4)
+    a = dec.open()
+    grow(dec, a, 112)
+    was, free_was = state(dec)
+    with pytest.raises(MemoryError):
+        with dec._grown([a], [count]) as (held, before):
+            assert before == [112] and held[0][0][1:3] == [-1, -1] and len(held[0][0]) == 7 + taken
+            raise MemoryError("made by the test")
+    every_page_once(dec, 7 + free)
+    lost = max(0, taken - free)
+    pages = dec._held[a][0]
+    assert dec.length(a) == 112 and len(dec._free) == free + lost and pages[1:3].count(-1) == lost
+    assert pages[:1] + pages[3:] == was[a][0][:1] + was[a][0][3:]
+    if not lost:
+        assert state(dec) == (was, free_was)
+    grow(dec, a, 10)
+    every_page_once(dec, 7 + free)
+
+
+def test_a_request_still_grows_past_the_pool():
+    dec = books(6, 50, 4)
+    a = dec.open()
+    for _ in range(40):
+        grow(dec, a, 16)
+        every_page_once(dec, 6)
+    assert dec.length(a) == 640
