@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .model import ModelGeometry
-from .serving import PagedCache, adjust_logits, prompt_attention, _per_row, _refuse
+from .serving import PagedCache, adjust_logits, prompt_attention, _Workspaces, _per_row, _refuse
 
 
 _PENALTIES = ("repetition", "presence", "frequency")
@@ -55,8 +55,11 @@ class PagedDecoder:
         self.dtype, self.page_size = dtype, int(page_size)
         self.dev = torch.device("cuda", device)
         self.caches = [PagedCache(g.kv_heads, g.head_dim, pages, page_size, format, device) for _ in range(g.layers)]
-        for c in self.caches[1:]:  # the layers follow each other on one stream: one workspace serves all
-            c._workspace = self.caches[0]._workspace
+        # The layers follow each other on one stream: one workspace serves all.  It is the decoder's own, for chunks too:
+        # torch hands the recording stream's handle to others as well, and recorded steps are replayed on any.
+        work = _Workspaces()
+        for c in self.caches:
+            c._workspace, c._chunk_work = self.caches[0]._workspace, work
         w = {k: v.detach().to(self.dev, dtype) for k, v in weights.items()}  # (attention has no gradient)
         self.emb, self.final_norm = w["model.embed_tokens.weight"], w["model.norm.weight"].float()
         self.layers = []

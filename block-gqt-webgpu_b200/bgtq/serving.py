@@ -16,13 +16,14 @@ Indices that only the GPU sees (slots, page tables, lengths, starts) are checked
 lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
 length or starts).
 
-Attention keeps a workspace for every stream that it has been called on.  A CUDA graph
+Attention keeps a workspace for every stream that it has been called on (`PagedDecoder` has workspaces of its own).  A CUDA graph
 recorded on such a stream uses that one, so it is not replayed at the same time as calls there or
 other graphs that were recorded there; recorded on a stream without one, it has its own.
 """
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 
 import torch
 
@@ -58,6 +59,19 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
+
+
+class _Workspaces(dict):
+    """(device, head dim, stream): (address, bytes, tensor).  `_ready_again` finds them all."""
+    made = weakref.WeakSet()
+    __hash__, __eq__ = object.__hash__, object.__eq__
+
+    def __init__(self):
+        super().__init__()
+        _Workspaces.made.add(self)
+
+
+_prompt_work, _chunk_work = _Workspaces(), _Workspaces()
 
 
 class PagedCache:
@@ -108,7 +122,7 @@ class PagedCache:
                                                               for t in (self.k_scales, self.v_scales)))
         self._ref = C.byref(self._desc)
         self._on = self.k.device
-        self._workspace = {}
+        self._workspace, self._chunk_work = {}, _chunk_work
         library = _lib.lib()
         self._write, self._read = library.bgtq_paged_write, library.bgtq_paged_read
         self._attend = library.bgtq_paged_attend
@@ -310,7 +324,7 @@ class PagedCache:
         sums = q.new_empty((tokens, heads), dtype=torch.float32) if lse else None
         q, q0, q1 = _even(q)
         st = _stream(self.device)
-        work = _chunk_work.get((self.device, self.dim, st)) or _chunk_workspace(self, heads, st)
+        work = self._chunk_work.get((self.device, self.dim, st)) or _chunk_workspace(self, heads, st)
         p = _lib.ChunkDesc(_DTYPE[dtype], batch, heads, tokens, q.data_ptr(), q0, q1,
                            None if starts is None else starts.data_ptr(), table.data_ptr(), table.stride(0),
                            table.shape[1], lengths.data_ptr(), 0.0 if scale is None else max(scale, _LEAST_SCALE),
@@ -319,9 +333,6 @@ class PagedCache:
         if status:
             _lib.check(status)
         return (out, sums) if lse else out
-
-
-_prompt_work, _chunk_work = {}, {}
 
 
 def _prompt_workspace(device, dim: int, stream: int):
@@ -335,12 +346,12 @@ def _prompt_workspace(device, dim: int, stream: int):
 
 
 def _chunk_workspace(cache, heads: int, stream: int):
-    """The same for chunks over pages: one for all caches of a device and head dim."""
+    """The same for chunks over pages: one for all caches of a device and head dim, but for a decoder's."""
     need = C.c_size_t()
     _lib.call("bgtq_paged_chunk_workspace", cache._ref, heads, C.byref(need))
     work = _room(need.value, cache._on)
     if not _recording(cache._on):
-        _chunk_work[cache.device, cache.dim, stream] = work
+        cache._chunk_work[cache.device, cache.dim, stream] = work
     return work
 
 
@@ -348,9 +359,10 @@ def _ready_again(device: int):
     """Zeroes the counters of the device's prompt and chunk workspaces: a call whose wait ran out ends without its
     joins.  (One-token attention waits for nothing, and a graph's own workspace is zeroed by its replays.)"""
     torch.cuda.synchronize(device)
-    for (on, _, _), work in (*_prompt_work.items(), *_chunk_work.items()):
-        if on == device:
-            work[2][:_lib.WORKSPACE_ZEROED].zero_()
+    for works in list(_Workspaces.made):
+        for (on, _, _), work in list(works.items()):
+            if on == device:
+                work[2][:_lib.WORKSPACE_ZEROED].zero_()
     torch.cuda.synchronize(device)
 
 
