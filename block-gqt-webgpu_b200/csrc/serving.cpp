@@ -317,7 +317,7 @@ bgtq_status bgtq_adjust_logits(const bgtq_logits *p, void *stream) {
     a.bias_ids = p->entries ? p->bias_ids : nullptr;
     a.bias = p->entries ? p->bias : nullptr;
     a.bias_stride = p->bias_stride;
-    a.entries = p->entries;
+    a.entries = p->bias ? p->entries : 0;  // (without biases their number says nothing)
     a.mask = p->mask;
     a.mask_stride = p->mask_stride;
     a.out = p->out;
