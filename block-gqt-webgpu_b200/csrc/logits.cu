@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, kResident) logits_kernel(const Logit
         if (a.presence) p = __ldg(a.presence + b);
         if (a.frequency) f = __ldg(a.frequency + b);
     }
+    if (a.lengths && !a.tokens && blockIdx.x == 0 && threadIdx.x == 0 && __ldg(a.lengths + b)) atomicOr(a.status, kStatusBadExtent);
     int32_t bias_id = -1;
     float bias = 0.0f;
     auto entry = [&](uint32_t j) {

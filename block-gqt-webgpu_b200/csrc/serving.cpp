@@ -310,7 +310,7 @@ bgtq_status bgtq_adjust_logits(const bgtq_logits *p, void *stream) {
     a.tokens_stride = p->tokens_stride;
     a.width = p->width;
     a.id_bytes = p->id_bytes;
-    a.lengths = p->lengths;
+    a.lengths = p->tokens || !p->width ? p->lengths : nullptr;  // (of an empty history they are looked over)
     a.repetition = p->repetition;
     a.presence = p->presence;
     a.frequency = p->frequency;
