@@ -432,9 +432,10 @@ def prompt_attention(q, k, v, starts, key_starts=None, causal: bool = True, scal
 def _per_row(x, batch: int, device, name: str):
     """A penalty as float32 [batch]: a tensor as it is, a number filled in."""
     if not isinstance(x, torch.Tensor):
+        x = C.c_float(x).value  # what FP32 makes of it: infinity and zero among it
         if not -float("inf") < x < float("inf") or name == "repetition" and x <= 0.0:
-            _refuse(f"Logits: {name} must be finite" + (" and positive" if name == "repetition" else ""))
-        return torch.full((batch,), float(x), dtype=torch.float32, device=device)
+            _refuse(f"Logits: {name} must be finite" + (" and positive" if name == "repetition" else "") + " in FP32")
+        return torch.full((batch,), x, dtype=torch.float32, device=device)
     if x.shape != (batch,) or x.dtype != torch.float32 or x.device != device or not x.is_contiguous():
         _refuse(f"Logits: {name} must be a number or a contiguous float32 tensor [batch] on the logits' device")
     return x
