@@ -412,8 +412,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const std::conditio
             const uint32_t t0 = place_of(pre, pre_unit) * T, kh = pair_of(pre) / blocks_of(pre);
             const int32_t page = __shfl_sync(0xffffffffu, pages_now, (used << span_shift) + (lane & (span - 1)));
             const bool asked = lane < span && t0 + (lane << shift) < (uint32_t)pre.len;
-            const uint32_t bad = __ballot_sync(0xffffffffu, asked && (uint32_t)page >= a.c.pages);
-            if (bad && lane == 0) atomicOr(a.status, kStatusBadSlot);
+            // chunks: a page of a unit between the first tokens and the window is absent, whatever the table says of it
+            bool hidden = false;
+            if constexpr (C) {
+                const uint32_t from = t0 + (lane << shift);
+                hidden = a.window && from >= a.sinks && (int64_t)from + (1 << shift) <= (int64_t)pre.len - pre.n - a.window + 1;
+            }
+            const bool missing = asked && (uint32_t)page >= a.c.pages;
+            if (__any_sync(0xffffffffu, missing && !hidden) && lane == 0) atomicOr(a.status, kStatusBadSlot);
+            const uint32_t bad = __ballot_sync(0xffffffffu, missing || (asked && hidden));
             if (lane == 0) flags[warp * 4 + stage] = bad;
             const uint32_t dst = ring_at + stage * S::kStage;
             const int32_t left = pre.len - (int32_t)t0;

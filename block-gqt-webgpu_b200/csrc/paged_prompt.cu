@@ -940,18 +940,22 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const int32_t token = token_of(k);
                     return token < it.keys ? __ldg(a.table + (int64_t)it.seq * a.table_stride + (token >> a.c.page_shift)) : -1;
                 };
+                // A piece between the first tokens and the window of the item's first row is absent, whatever the table says of it.
+                const int32_t shown = a.window ? (int32_t)max((int64_t)-1, (int64_t)it.place - a.window + 1 - piece_rows) : -1;
                 int32_t page = tiles ? page_of(0) : 0;
                 auto load = [&](int32_t k) {
                     const int32_t ahead = k + 1 < tiles + lead ? page_of(k + 1) : 0;
                     const int32_t token = token_of(k);
-                    const bool there = (uint32_t)page < a.c.pages;
+                    const bool hidden = token <= shown && (uint32_t)token >= a.sinks;
+                    const bool there = (uint32_t)page < a.c.pages && !hidden;
                     const uint32_t bad = __ballot_sync(0xffffffffu, token < it.keys && !there);
+                    const bool wrong = __any_sync(0xffffffffu, token < it.keys && !there && !hidden);
                     if (!(fine = fine && all_wait(bar((kCodes ? B_TURNED : B_FREE) + slot), free_phase))) return;
                     const bool values = k >= lead, keys = k < tiles;
                     const bool look = !kCodes && values && !plain(it, first_of(it, k - lead));
                     const uint32_t on = bar((kCodes ? B_CODES : look ? B_RAW : B_FULL) + slot), bit = 1u << slot;
                     if (lane == 0) {
-                        if (bad) atomicOr(a.status, kStatusBadSlot);
+                        if (wrong) atomicOr(a.status, kStatusBadSlot);
                         bad_pages[stage_no % P::kMeta] = (bad >> 8 & 15u) | (bad & 15u) << 4;
                         bar_expect(on, kCodes ? (values ? P::kRawTile + P::kRawScale : 0u) + (keys ? P::kRawTile + 2 * P::kRawScale : 0u)
                                               : (values ? P::kTile : 0u) + (keys ? P::kTile : 0u));
