@@ -23,9 +23,11 @@
 //               by its scale.  The tile's power multiplies its logits as the scale of all logits does, and its
 //               probabilities as an addend of their exponents, so that softmax does no more than over 16-bit pages.
 //               (BF16 queries go to FP16 over a power of two of their row, which loses what is below 2^-38 of the row's
-//               largest.)  A value in 8 bits is rounded to 11 bits, a sixteenth of the step that its code was rounded
-//               to (an FP16 output's error 3.5e-4 of its norm, 2.1e-4 in FP32 throughout; a second operand for values
-//               would be a third more products, a factor for each token in softmax took 785 us for 625).  Where the scales of a tile are more than 2^16 apart, as next to rows of 1e30, powers of two of each
+//               largest.)  A value in 8 bits is exact as well: its code by the power of two of its scale is an operand, and
+//               the scale's mantissa multiplies the probability before that is rounded (an FP16 output's error 2.8e-4 of
+//               its norm, 2.1e-4 in FP32 throughout; products of code and scale rounded to FP16 3.5e-4, and 4 % less time:
+//               600 us for 624 and 630 for 655 of the cases below, 168 for 183 of few rows).  Where the scales of a tile are
+//               more than 2^16 apart, as next to rows of 1e30, powers of two of each
 //               token take their place and multiply each logit, or each probability.  Probabilities x value scales are
 //               taken relative to the row's largest so far, in steps of at least 2^kRoom, so that values of any size
 //               whose weight is next to nothing leave the others as they are; what is rounded away is 2^-34 of the
@@ -34,9 +36,10 @@
 // What bounds it.  Many rows: the tensor cores and, at head dim 64, the exponentials of softmax: four chunks of 1024 rows after
 // 6000 to 8192 tokens, 32 / 8 heads of 128 in 16 bits, 445 us, 1140 TFLOP/s; two of 2048 after 24000 to 30000, 14 / 2 heads of
 // 64, 470 us, 876 TFLOP/s.  Over codes the warps that turn them and the code they share the instruction caches with:
-// the first in 8 bits 600 us, in 4 bits 686; the second in 8 bits 630 (96 registers of softmax's warps and the keys' second
-// operand).  Few rows: 32 requests of 5 rows after 500 to 16000 tokens, 32 / 8 heads of 128, 125 us, 4.8 TB/s; in 8
-// bits 167 us, 1.9 TB/s.  Few tokens: 20 to 45 us of the deal, the first pages' way through the table, and the join.
+// the first in 8 bits 624 us, in 4 bits 668; the second in 8 bits 655 (96 registers of softmax's warps and the keys' second
+// operand).  Few rows: 32 requests of 5 rows after 500 to 16000 tokens, 32 / 8 heads of 128, 117 us, 5.2 TB/s; in 8
+// bits 183 us, 1.7 TB/s, in 4 bits 219: the time is that of turning one stage of 64 tokens, 1.3 to 1.5 us with few rows and
+// with many, which is mostly latency, since all turning warps work on one stage at a time.  Few tokens: 20 to 45 us of the deal, the first pages' way through the table, and the join.
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -83,8 +86,8 @@ struct Plan {
     // Registers after the hand-over, of softmax's warps and of the others: what the launch has, in all.
     static constexpr uint32_t kSoft = NT == 4 ? (kCodes ? 96 : 104) : kCodes ? 128 : 216, kRest = NT == 4 ? (kCodes ? 48 : 64) : 72;
     // Exponentials of 16 on the FMA pipe.  (Their code is long, and beside the code that turns codes the caches of
-    // instructions do not hold it: four chunks of 1024 after 8192, 32 / 8 heads of 128, with none 587 us in 8 bits and 662 in
-    // 4, with 6 of 16 612 and 714.)
+    // instructions do not hold it: four chunks of 1024 after 8192, 32 / 8 heads of 128, with none 4 % less time in 8 bits and
+    // 7 % less in 4 than with 6 of 16.)
     static constexpr int kFma = D == 64 ? 2 : kCodes ? 0 : 6;
     static constexpr uint32_t kChunks = D / 64;                    // 64-dimension columns of a tile
     static constexpr uint32_t kQChunk = kRows * 128, kQTile = kChunks * kQChunk;  // bytes: rows of 64 elements
@@ -105,9 +108,10 @@ struct Plan {
     static constexpr uint32_t kQ = 0, kRing = kTiles * kQTile, kRaw = kRing + kStages * kStageBytes;
     static constexpr int kTurn = NT == 4 ? 16 : 32;                // dimensions of an output row stored at a time
     static constexpr uint32_t kOut = kRaw + kRawStages * kRawStage;                     // [softmax warps][32 rows][kTurn] outputs
-    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn;                 // [kMeta][2][kKeys] what logits, and, as
-                                                                                        // logarithms, probabilities are multiplied by
-    static constexpr uint32_t kAbout = kScales + (kCodes ? kMeta * 2 * kKeys * 4 : 0);     // [kMeta] About
+    // [kMeta][kBy][kKeys] what logits, and, as logarithms, probabilities are multiplied by; in 8 bits what probabilities are
+    // multiplied by besides, the scales' mantissas
+    static constexpr uint32_t kScales = kOut + 4 * kTiles * 64 * kTurn, kBy = F == F_INT8 ? 3 : 2;
+    static constexpr uint32_t kAbout = kScales + (kCodes ? kMeta * kBy * kKeys * 4 : 0);   // [kMeta] About
     static constexpr uint32_t kBadPages = kAbout + (kCodes ? kMeta * 16 : 0);              // [kMeta] pieces without a page: K, V
     static constexpr uint32_t kItems = kBadPages + kMeta * 4;      // [kDeal] Item
     static constexpr uint32_t kBars = kItems + kDeal * 64;
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 tc_wait_ld();
                 float *s = reinterpret_cast<float *>(x);
                 if (kCodes && (P::kOwn || each & 1u)) {
-                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (2 * kKeys / 4);
+                    const float4 *by = reinterpret_cast<const float4 *>(sm + P::kScales) + meta * (P::kBy * kKeys / 4);
 #pragma unroll
                     for (int i = 0; i < kKeys; i += 4) {
                         const float4 f = by[i / 4];
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                             sum *= j == 0 ? 1.0f : ex2(ref - top);
                             ref = top;
                         }
-                        const float *logs = reinterpret_cast<const float *>(sm + P::kScales) + (meta * 2 + 1) * kKeys;
+                        const float *logs = reinterpret_cast<const float *>(sm + P::kScales) + (meta * P::kBy + 1) * kKeys;
                         float peak = top + largest;
                         // (seldom, and so short loops over tensor memory: unrolled over registers, their code costs what kFma says)
                         if (each & 2u) {
@@ -504,11 +508,17 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 const float from = ref == -INFINITY ? 0.0f : kCodes ? unit - largest - kUpCodes : ref - kUp<BF>;
                 float2 total = make_float2(0.0f, 0.0f);
                 const float2 mul2 = make_float2(mul, mul), from2 = make_float2(-from, -from);
+                const float4 *mantissas = reinterpret_cast<const float4 *>(sm + P::kScales) + (meta * P::kBy + 2) * (kKeys / 4);
+                float4 four = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
 #pragma unroll
                 for (int i = 0; i < kKeys; i += 2) {
                     const float2 v = __ffma2_rn(make_float2(s[i], s[i + 1]), mul2, from2);
-                    const float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
+                    float2 e = i % 16 < P::kFma ? ex2_fma(v) : make_float2(ex2(v.x), ex2(v.y));
                     total = __fadd2_rn(total, e);
+                    if constexpr (F == F_INT8) {
+                        if (i % 4 == 0) four = mantissas[i / 4];
+                        e = __fmul2_rn(e, i % 4 ? make_float2(four.z, four.w) : make_float2(four.x, four.y));
+                    }
                     x[i / 2] = pack<BF>(e.x, e.y);
                 }
                 sum = kCodes ? fmaf(total.x + total.y, give, sum) : sum + (total.x + total.y);
@@ -1214,9 +1224,16 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 }
                 return max(big >> 7, 27u);
             };
+            // 8-bit values: probabilities take the mantissa of a scale that has one (not zero, infinity, NaN or below 2^-126),
+            // values the rest, so that no bit of a value is rounded away
+            auto mantissa = [](uint32_t scale) {
+                const uint32_t e = scale >> 7 & 255u;
+                return e - 1u < 254u ? from_bf16(0x3f80u | (scale & 0x7fu)) : 1.0f;
+            };
             // what codes are multiplied by, twice: their scale over the power of two of the tile or the token, times 2^kUpTile
-            auto factor = [&](const uint16_t *scales, uint32_t r, uint32_t c, const Sizes &z, bool there) {
-                const uint32_t scale = scales[r * G + (G == 1 ? 0 : c)];
+            auto factor = [&](const uint16_t *scales, uint32_t r, uint32_t c, const Sizes &z, bool there, auto of_values) {
+                uint32_t scale = scales[r * G + (G == 1 ? 0 : c)];
+                if (F == F_INT8 && decltype(of_values)::value && (scale >> 7 & 255u) - 1u < 254u) scale &= 0xff80u;
                 uint32_t e = z.top;
                 float f = from_bf16(scale);
                 if (z.apart()) {
@@ -1254,15 +1271,26 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     about.top = (float)zv.top - 127.0f;
                     about.each = (zk.apart() ? 1u : 0u) | (zv.apart() ? 2u : 0u);
                 }
-                float *by = reinterpret_cast<float *>(sm + P::kScales) + meta * 2 * kKeys;
-                if (P::kOwn || zk.apart())  // over the tile's largest
-                    for (uint32_t r = lane; r < P::kKeys; r += 32) {
-                        if constexpr (F == F_INT8) by[r] = from_bf16(keys[r]) * __uint_as_float((254 - zk.top) << 23);
-                        else by[r] = ex2((float)largest(keys + r * G) - (float)zk.top);
+                float *by = reinterpret_cast<float *>(sm + P::kScales) + meta * P::kBy * kKeys;
+                if constexpr (F == F_INT8) {
+                    const uint32_t two = reinterpret_cast<const uint32_t *>(values)[lane];
+                    reinterpret_cast<float2 *>(by + 2 * kKeys)[lane] = make_float2(mantissa(two & 0xffffu), mantissa(two >> 16));
+                }
+                if (P::kOwn || zk.apart()) {  // over the tile's largest
+                    if constexpr (F == F_INT8) {
+                        const uint32_t two = reinterpret_cast<const uint32_t *>(keys)[lane];
+                        reinterpret_cast<float2 *>(by)[lane] = __fmul2_rn(make_float2(from_bf16(two & 0xffffu), __uint_as_float(two & 0xffff0000u)),
+                                                                          make_float2(__uint_as_float((254 - zk.top) << 23), __uint_as_float((254 - zk.top) << 23)));
+                    } else {
+                        for (uint32_t r = lane; r < P::kKeys; r += 32) by[r] = ex2((float)largest(keys + r * G) - (float)zk.top);
                     }
+                }
                 if (zv.apart())  // (logarithms; what has no scale has no weight, or no values)
                     for (uint32_t r = lane; r < P::kKeys; r += 32) {
-                        if constexpr (F == F_INT8) by[kKeys + r] = r < rows && (values[r] & 0x7f80u) != 0x7f80u && values[r] ? __log2f(from_bf16(values[r])) : -150.0f;
+                        if constexpr (F == F_INT8) {
+                            const uint32_t s = values[r], e = s >> 7 & 255u;
+                            by[kKeys + r] = r >= rows || e == 255u || !s ? -150.0f : e ? (float)e - 127.0f : __log2f(from_bf16(s));
+                        }
                         else by[kKeys + r] = r < rows ? (float)largest(values + r * G) - 127.0f : -150.0f;
                     }
             };
@@ -1272,7 +1300,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                 uint32_t s2[kEach];
             };
             // (of values in a tile that is looked through, what has a NaN for a scale is zero)
-            auto fetch = [&](Batch &b, const uint4 *codes, const uint16_t *scales, uint32_t rows, uint32_t bad, bool look) {
+            auto fetch = [&](Batch &b, const uint4 *codes, const uint16_t *scales, uint32_t rows, uint32_t bad, bool look, auto of_values) {
 #pragma unroll
                 for (uint32_t q = 0; q < kEach; ++q) b.codes[q] = codes[row * kPer + place_of(q)];
                 const Sizes z = sizes(scales, rows, bad);
@@ -1287,7 +1315,7 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     const uint32_t c = place_of(q);
                     const bool nan = look && there && (scales[row * G + (G == 1 ? 0 : c)] & 0x7f80u) == 0x7f80u;
                     found |= nan;
-                    b.s2[q] = factor(scales, row, c, z, there && !nan);
+                    b.s2[q] = factor(scales, row, c, z, there && !nan, of_values);
                 }
                 return found;
             };
@@ -1309,13 +1337,13 @@ __global__ void __launch_bounds__(Plan<D, NT, F>::kThreads, 1) chunk_kernel(cons
                     Batch of_keys, of_values;
                     if (turns && values) {
                         const int32_t k0 = first_of(it, k - lead);
-                        if (fetch(of_values, codes, scales, (uint32_t)min(kKeys, it.keys - k0), bad >> 4, !plain(it, k0))) bad_flag[n % kDeal] = 1;
+                        if (fetch(of_values, codes, scales, (uint32_t)min(kKeys, it.keys - k0), bad >> 4, !plain(it, k0), std::true_type())) bad_flag[n % kDeal] = 1;
                     }
                     if (turns && keys) {
                         if constexpr (P::kOwn) {  // (codes as they are)
 #pragma unroll
                             for (uint32_t q = 0; q < kEach; ++q) of_keys.codes[q] = codes[P::kRawTile / 16 + row * kPer + place_of(q)], of_keys.s2[q] = 0;
-                        } else fetch(of_keys, codes + P::kRawTile / 16, scales + kNext, key_rows, bad & 15u, false);
+                        } else fetch(of_keys, codes + P::kRawTile / 16, scales + kNext, key_rows, bad & 15u, false, std::false_type());
                     }
                     if (weighs && keys)
                         weigh(scales + kNext, scales + 2 * kNext, sizes(scales + kNext, key_rows, bad & 15u), sizes(scales + 2 * kNext, key_rows, bad & 15u),
