@@ -18,6 +18,7 @@ bgtq_status refuse(const std::string &msg) {
 }
 bgtq_status launched(cudaError_t e, const char *what) {
     if (e == cudaSuccess) return BGTQ_OK;
+    cudaGetLastError();  // (what the runtime still holds would be taken for the next launch's)
     set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
     return BGTQ_ECUDA;
 }

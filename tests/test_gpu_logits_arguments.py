@@ -1,4 +1,4 @@
-"""adjust_logits at the C ABI: arguments that stand beside a null array."""
+"""The serving operators at the C ABI: arguments that stand beside a null array, and a call after one that failed."""
 import ctypes as C
 
 import pytest
@@ -30,3 +30,20 @@ def test_a_number_of_biases_without_biases_says_nothing(cuda, entries):
     want = x.clone()
     want[:, 0] -= 1
     assert torch.equal(got, want)
+
+
+def test_a_call_after_one_on_a_device_that_is_not_there(cuda):
+    """The error is the call's own."""
+    import torch
+    from bgtq import PagedCache
+    assert torch.cuda.device_count() < 60
+    x, cache = randn(1, 3, 500), PagedCache(1, 64, 4, 16, "f16")
+    rows, at = randn(2, 20, 1, 64), torch.arange(20, device="cuda")
+    want = cache.append(rows, rows, rows, at, randn(3, 20, 64))
+    q, table, lengths = randn(4, 1, 1, 64, dtype="f16"), torch.arange(2, dtype=torch.int32, device="cuda")[None], torch.tensor([20], dtype=torch.int32, device="cuda")
+    for call in (lambda: put(x, torch.empty_like(x)), lambda: cache.append(rows, rows, rows, at, randn(3, 20, 64)),
+                 lambda: cache.attend_chunk(q, None, table, lengths), lambda: cache.attend(q, table, lengths), lambda: cache.read(at)):
+        with pytest.raises(_lib.DeviceError):
+            put(x, torch.empty_like(x), device=61)
+        call()
+    assert torch.equal(cache.append(rows, rows, rows, at, randn(3, 20, 64)), want)
