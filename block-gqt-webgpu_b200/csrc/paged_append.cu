@@ -5,8 +5,8 @@
 // a step function of its row, and so is the same whatever order sums and products are taken in.  All else is FP32.
 //
 // A row is D / 16 threads, each with two runs of eight dimensions that are rotated into each other: no shared memory, a norm's
-// sum and a row's largest by shuffles.  16384 tokens, 32 / 8 heads of 128 from BF16: into 16 bits 75 us, 5.4 TB/s; into 8 bits
-// 79; into 4 bits with norms 102, where the pairs of numbers and the packing of codes issue as long as the loads take.  A
+// sum and a row's largest by shuffles.  16384 tokens, 32 / 8 heads of 128 from BF16: into 16 bits 76 us, 5.3 TB/s, with norms 90;
+// into 8 bits 80, with norms 109; into 4 bits 80, with norms 103, where the pairs of numbers issue as long as the loads take.  A
 // step of 16 requests, 9 / 3 heads of 64, takes 2.5 us, next to nothing of which is work.
 #include <type_traits>
 
