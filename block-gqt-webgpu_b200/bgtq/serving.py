@@ -16,9 +16,10 @@ Indices that only the GPU sees (slots, page tables, lengths, starts) are checked
 lies outside the cache is left out and sets a bit of `device_status` (4: slot or page, 8:
 length or starts).
 
-Attention keeps a workspace for every stream that it has been called on (`PagedDecoder` has workspaces of its own).  A CUDA graph
-recorded on such a stream uses that one, so it is not replayed at the same time as calls there or
-other graphs that were recorded there; recorded on a stream without one, it has its own.
+Attention keeps a workspace for every stream that it has been called on (`PagedDecoder` has workspaces
+of its own).  A CUDA graph recorded on such a stream uses that one, so it is not replayed at the same
+time as calls there or other graphs that were recorded there; recorded on a stream without one, it
+has its own.
 """
 from __future__ import annotations
 

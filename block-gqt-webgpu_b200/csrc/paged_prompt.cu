@@ -39,7 +39,8 @@
 // the first in 8 bits 624 us, in 4 bits 668; the second in 8 bits 655 (96 registers of softmax's warps and the keys' second
 // operand).  Few rows: 32 requests of 5 rows after 500 to 16000 tokens, 32 / 8 heads of 128, 117 us, 5.2 TB/s; in 8
 // bits 183 us, 1.7 TB/s, in 4 bits 219: the time is that of turning one stage of 64 tokens, 1.3 to 1.5 us with few rows and
-// with many, which is mostly latency, since all turning warps work on one stage at a time.  Few tokens: 20 to 45 us of the deal, the first pages' way through the table, and the join.
+// with many, which is mostly latency, since all turning warps work on one stage at a time.  Few tokens: 20 to 45 us of the
+// deal, the first pages' way through the table, and the join.
 #include <type_traits>
 
 #include "tcgen05.cuh"

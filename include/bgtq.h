@@ -554,8 +554,8 @@ bgtq_status bgtq_paged_append(const bgtq_paged_cache *c, const bgtq_append *p, v
  * t < sinks.  A row that sees nothing gives zeros and -inf; query rows that no request holds are not written.  Starts
  * that fall or pass q_tokens set a status bit and their request is skipped.  dtype, table, lengths, scale, out and lse
  * are bgtq_paged_attend's; of the table only entries of tokens that a row sees are followed (others may be read, and
- * need only be readable: they may hold any number).  An infinity among the values of 16-bit pages gives infinity to rows that see it, or NaN where
- * its probability is below what 16 bits hold.  Pointers to q and out are 16-byte aligned, q's strides positive
+ * need only be readable: they may hold any number).  An infinity among the values of 16-bit pages gives infinity to
+ * rows that see it, or NaN where its probability is below what 16 bits hold.  Pointers to q and out are 16-byte aligned, q's strides positive
  * multiples of 8 elements; q_heads / kv_heads <= 128. */
 typedef struct bgtq_chunk {
     bgtq_dtype dtype;
@@ -633,7 +633,7 @@ typedef struct bgtq_logits {
     const void *tokens;     /* [batch][width] ids, rows tokens_stride elements apart, or null */
     int64_t tokens_stride;
     uint32_t width, id_bytes;
-    const int32_t *lengths; /* [batch], or null: width */
+    const int32_t *lengths; /* [batch], or null: width (beside null tokens with a width, not looked at) */
     const float *repetition, *presence, *frequency; /* [batch], or null: 1, 0, 0 */
     const int32_t *bias_ids; /* [batch][entries], rows bias_stride elements apart (0: one row for all), or null */
     const float *bias;
