@@ -555,8 +555,8 @@ bgtq_status bgtq_paged_append(const bgtq_paged_cache *c, const bgtq_append *p, v
  * that fall or pass q_tokens set a status bit and their request is skipped.  dtype, table, lengths, scale, out and lse
  * are bgtq_paged_attend's; of the table only entries of tokens that a row sees are followed (others may be read, and
  * need only be readable: they may hold any number).  An infinity among the values of 16-bit pages gives infinity to
- * rows that see it, or NaN where its probability is below what 16 bits hold.  Pointers to q and out are 16-byte aligned, q's strides positive
- * multiples of 8 elements; q_heads / kv_heads <= 128. */
+ * rows that see it, or NaN where its probability is below what 16 bits hold.  Pointers to q and out are 16-byte aligned,
+ * q's strides positive multiples of 8 elements; q_heads / kv_heads <= 128. */
 typedef struct bgtq_chunk {
     bgtq_dtype dtype;
     uint32_t batch, q_heads;
